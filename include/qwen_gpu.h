@@ -168,6 +168,145 @@ int qg_moe_forward_residual(float *h, int *ids, float *weights, unsigned char *f
                             float *xn_out, float *out, int tokens, const qg_moe_layer *layer,
                             void *workspace, size_t workspace_bytes);
 
+/* ---- a speculative step over a paged cache: per-head norms and rotation,
+ * attention, softmax, draft verification, page management.  Additions beside
+ * qg_norm, qg_matmul and qg_moe_forward: with them the rows of one target
+ * batch (qwen.c:748-768: the last accepted token and its drafts) pass through
+ * a layer's attention and the drafts are accepted on the device, so a whole
+ * step can be captured into a graph.
+ *
+ * Conventions.  Device pointers of the current device; int arrays are read on
+ * the device at launch order, so one captured graph serves every step.  What
+ * the host can see is checked before anything is launched (invalid-value
+ * code); what only the device can see is bounded there: a page entry outside
+ * [0, pages) holds nothing, a length is taken as 0..table_pages * page_tokens,
+ * the rows of a sequence as at most max_rows inside [0, rows), and a parent
+ * that is not an earlier row of its sequence as none.  Nothing outside the
+ * given buffers is read or written. */
+
+/* Keys and values of `sequences` sequences in pages of page_tokens tokens.
+ * Position t of sequence s lies in page table[s][t / page_tokens] at token
+ * t % page_tokens.  A page may be held by several sequences (qg_kv_fork). */
+typedef struct {
+    void *k, *v;                /* [layers][pages][kv_heads][page_tokens][head_dim], 16-byte aligned */
+    int type;                   /* 0 F32, 1 F16, 30 BF16 */
+    int layers, pages, kv_heads; /* kv_heads 1..128 */
+    int page_tokens;            /* a power of two, 8..1024 */
+    int head_dim;               /* 64, 128 or 256 */
+    int *refs;                  /* [pages] table entries that hold each page, 0 = free; page calls only, else NULL */
+    int *table;                 /* [sequences][table_pages] page or -1 */
+    int *length;                /* [sequences] tokens held */
+    int sequences, table_pages; /* 1..1024 sequences; table_pages * page_tokens <= 2^28 */
+} qg_kv_cache;
+
+/* The rows of one batch: sequence s of the cache has rows start[s] ..
+ * start[s+1]-1 of the activations (none is allowed), row i of them takes the
+ * cache position length[s] + i.  parent NULL: each row follows the one before
+ * it (a chain, a prompt chunk).  Else parent[r] is the place in its sequence
+ * of the row that row r continues, -1 for none, and max_rows is at most 64. */
+typedef struct {
+    int rows, max_rows;         /* rows 1..65536; rows of one sequence at most max_rows */
+    const int *start;           /* [sequences + 1], ascending */
+    const int *parent;          /* [rows] or NULL */
+} qg_kv_batch;
+
+/* Query, key and value rows as a projection wrote them: head h of row t of q
+ * starts at q + t * q_row + h * q_head (floats); k and v likewise.  Pointers
+ * 16-byte aligned, strides multiples of 4. */
+typedef struct {
+    const float *q, *k, *v;
+    int64_t q_row, q_head, k_row, k_head, v_row, v_head;
+    int rows, q_heads, kv_heads, head_dim; /* head_dim 64, 128 or 256; heads 1..1024 */
+    const float *q_norm, *k_norm; /* [head_dim] RMS-norm weights, or NULL: that side is not normalised */
+    float eps;
+    int rope_dims;              /* leading dimensions rotated: a multiple of 8, 0..head_dim */
+    int interleaved;            /* pairs (2i, 2i+1); 0: (i, i + rope_dims/2) */
+    const double *freq;         /* [rope_dims/2] radians per position (theta^(-2i/rope_dims), or a scaled form) */
+    const int *position;        /* [rows], or NULL: length[s] + the row's depth below its root in the batch */
+} qg_qk_rows;
+
+/* Per-head RMS norm (as qg_norm) and rotation of q and k, in one pass; q_out
+ * [rows][q_heads][head_dim], k_out [rows][kv_heads][head_dim] fp32 (k_out may
+ * be NULL).  With a cache, k (normed, rotated) and v are rounded to its type
+ * and stored at their positions of `layer`; a row whose position has no page
+ * is not stored.  Without a cache, batch is NULL, v is ignored and position is
+ * needed where rope_dims > 0.  Angles are formed in 64 bits.  An output may be its own
+ * input where both have the same layout; otherwise they must not overlap.
+ * Rows of no sequence are left as they were. */
+int qg_qk_norm_rope(float *q_out, float *k_out, const qg_qk_rows *in, const qg_kv_cache *cache, int layer,
+                    const qg_kv_batch *batch);
+
+/* Attention of the batch's rows over the cache: row i of sequence s sees the
+ * length[s] cached tokens, itself and the rows it descends from (all stored
+ * before the call).  out, q [rows][q_heads][head_dim] fp32, q_heads a multiple
+ * of kv_heads up to 128 times as many, both 16-byte aligned; no overlap.
+ * Scores, statistics and sums are held in fp32; the products run on the matrix
+ * cores with queries and probabilities in planes of the cache's type that
+ * together carry at least 22 bits.  A row that sees no token (or none with a
+ * score above -infinity) is 0.  Rows of no sequence are left as they were. */
+size_t qg_tree_attention_workspace_bytes(const qg_kv_cache *cache, const qg_kv_batch *batch, int q_heads);
+int qg_tree_attention(float *out, const float *q, int q_heads, float scale, const qg_kv_cache *cache, int layer,
+                      const qg_kv_batch *batch, void *workspace, size_t workspace_bytes);
+
+/* out = softmax(x / temperature) of each row of [rows][cols]; out may be x.
+ * temperature 0: 1 at the lowest index of the largest value.  -infinity gives
+ * 0; a row of nothing but -infinity is 0; a row with NaN or +infinity is NaN.
+ * rows 1..65536, cols 1..2^24; 4-byte aligned. */
+size_t qg_softmax_workspace_bytes(int rows, int cols);
+int qg_softmax(float *out, const float *x, int rows, int cols, float temperature, void *workspace, size_t workspace_bytes);
+
+/* Verification of drafts by rejection sampling; the accepted tokens are
+ * distributed as the target's.  Row 0 of a sequence is its last accepted
+ * token, each further row a draft, token[r], of the row it continues
+ * (qg_kv_batch; max_rows <= 64).  p [rows][cols]: the target's probabilities
+ * after each row.  q [rows][cols]: the probabilities that a row's drafts were
+ * drawn from (independently), or NULL: each draft was chosen, not drawn.
+ * From row 0 the drafts of the current row are tried in order: with a = 0 and
+ * B = 1, draft x is accepted if u[r] q(x) B < p(x) - a q(x) and becomes the
+ * current row, else a += B, B = sum_i max(p_i - a q_i, 0).  (With q NULL:
+ * if u[r] B < p(x), else B -= p(x) and p(x) counts as 0.)  At a row
+ * without an accepted draft the last token is the first i with
+ * sum_{j<=i} w_j > u_last[s] sum_j w_j, w = max(p - a q, 0), or p where that
+ * sum is not positive; -1 where p has none either.  Products and sums in 64 bits.
+ * u, u_last in [0, 1).  Outputs: count[s] = accepted rows with row 0 (0 for a
+ * sequence without rows); path[s][0..count-1] their places; tokens_out[s]
+ * [0..count-1] the accepted tokens and the last one; -1 behind them
+ * ([sequences][max_rows] both).  A token outside [0, cols) is never accepted. */
+size_t qg_verify_workspace_bytes(int sequences, int cols);
+int qg_verify_drafts(int *tokens_out, int *path, int *count, const float *p, const float *q, const int *token,
+                     const float *u, const float *u_last, int cols, int sequences, const qg_kv_batch *batch,
+                     void *workspace, size_t workspace_bytes);
+
+/* Pages.  Calls that change tables take one stream at a time; each result is
+ * the same on every run.  qg_kv_workspace_bytes serves fork (of up to
+ * `sequences` pairs) and reserve. */
+size_t qg_kv_workspace_bytes(const qg_kv_cache *cache);
+/* Room for the batch's rows behind each sequence's tokens: pages are taken in
+ * ascending order, for the sequences in order.  A held page that would be
+ * written and that another sequence holds too is replaced, its tokens copied
+ * (every layer); of several sequences of the batch that share a page no other holds, the
+ * first keeps it.  status[s]: 0; 1 there are not enough free pages for the batch
+ * (nothing is taken for any of its sequences); 2 the sequence's table is too
+ * short (nothing is taken for it, the others are served). */
+int qg_kv_reserve(const qg_kv_cache *cache, const qg_kv_batch *batch, int *status, void *workspace, size_t workspace_bytes);
+/* For each pair i < n: sequence dst[i] lets go of its pages and shares those
+ * of src[i]'s tokens; its length is src[i]'s.  Sources are read as before the
+ * call; of several pairs with one dst the last counts; a pair with dst == src
+ * or an index out of range is left out.  n 1..sequences. */
+int qg_kv_fork(const qg_kv_cache *cache, const int *dst, const int *src, int n, void *workspace, size_t workspace_bytes);
+/* length[s] = min(length[s], new_length[s]) (new_length NULL: as it is), and
+ * the pages behind it are let go; 0 frees a sequence. */
+int qg_kv_truncate(const qg_kv_cache *cache, const int *new_length);
+/* The accepted rows (qg_verify_drafts' path and count) move to the front: the
+ * token at length[s] + path[s][i] goes to length[s] + i, in every layer, and
+ * new_length[s] = length[s] + count[s] (new_length may be the cache's length).
+ * A path is followed while it ascends inside its sequence's rows. */
+int qg_kv_compact(const qg_kv_cache *cache, const qg_kv_batch *batch, const int *path, const int *count, int *new_length);
+/* Pages dst[i] = copies of pages src[i] in every layer, i < n <= 4096.  A
+ * pair whose destination is among the sources or comes again later is left
+ * out, as is one with an index out of range. */
+int qg_kv_copy_pages(const qg_kv_cache *cache, const int *dst, const int *src, int n);
+
 /* CPU handoff of the flag-2 tokens (replaces the whole-batch reads of
  * qwen.c:665-666 and the write of qwen.c:672).  Device arrays; async on the
  * calling thread's stream.  pack: count[0] = number of tokens with

@@ -19,7 +19,8 @@ PKG = Path(__file__).resolve().parent
 ROOT = PKG.parent
 CSRC = PKG / "csrc"
 LIBDIR = PKG / "lib"
-HIP_SOURCES = ["qg_runtime.hip", "qg_ops.hip", "qg_moe.hip", "qg_decode.hip", "qg_prefill.hip", "nb_synth.hip"]
+HIP_SOURCES = ["qg_runtime.hip", "qg_ops.hip", "qg_moe.hip", "qg_decode.hip", "qg_prefill.hip", "qg_spec.hip", "qg_kv.hip",
+               "qg_attention.hip", "nb_synth.hip"]
 HOST_SOURCES = ["moe_host.c", "qwen_moe.c"]
 ARCH = os.environ.get("NEBULA_OFFLOAD_ARCH", "gfx950")
 

@@ -1,0 +1,374 @@
+// Pages of the cache (qg_kv_* of include/qwen_gpu.h): reserve with copy on
+// write, fork, truncate, the move of accepted rows, page copies.  All counts
+// live on the device and every call is a fixed number of kernels without a
+// host read, so a step that forks, reserves and compacts can be captured.
+// Which page is taken never depends on the order in which workgroups run: free
+// pages are those with no holder, taken in ascending order.
+#include "qg_kv.h"
+
+int qg_kv_check(const qg_kv_cache *c, bool pages, KvView *v) {
+    if (!c || !c->k || !c->v || !c->table || !c->length || (pages && !c->refs)) return hipErrorInvalidValue;
+    if ((((uintptr_t)c->k | (uintptr_t)c->v) & 15) || (((uintptr_t)c->table | (uintptr_t)c->length | (uintptr_t)c->refs) & 3))
+        return hipErrorInvalidValue;
+    if (c->type != QT_F32 && c->type != QT_F16 && c->type != QT_BF16) return hipErrorInvalidValue;
+    if (c->layers < 1 || c->pages < 1 || c->kv_heads < 1 || c->kv_heads > 128) return hipErrorInvalidValue;
+    if (c->head_dim != 64 && c->head_dim != 128 && c->head_dim != 256) return hipErrorInvalidValue;
+    if (c->page_tokens < 8 || c->page_tokens > 1024 || (c->page_tokens & (c->page_tokens - 1))) return hipErrorInvalidValue;
+    if (c->sequences < 1 || c->sequences > QG_MAX_SEQUENCES || c->table_pages < 1) return hipErrorInvalidValue;
+    if ((int64_t)c->table_pages * c->page_tokens > 1LL << 28) return hipErrorInvalidValue;
+    const size_t size = (size_t)c->kv_heads * c->page_tokens * c->head_dim * (c->type == QT_F32 ? 4 : 2);
+    if ((size_t)c->layers > (((size_t)1 << 46) / size) / (size_t)c->pages) return hipErrorInvalidValue;
+    if (v) {
+        int shift = 0;
+        while (1 << shift < c->page_tokens) shift++;
+        *v = KvView{(uint8_t *)c->k, (uint8_t *)c->v, c->refs, c->table, c->length, c->type, c->layers, c->pages, c->kv_heads, shift,
+                    c->head_dim, c->sequences, c->table_pages};
+    }
+    return hipSuccess;
+}
+
+int qg_batch_check(const qg_kv_batch *b, bool tree, BatchView *v) {
+    if (!b || !b->start || ((uintptr_t)b->start & 3) || ((uintptr_t)b->parent & 3)) return hipErrorInvalidValue;
+    if (b->rows < 1 || b->rows > QG_MAX_ROWS || b->max_rows < 1 || b->max_rows > b->rows) return hipErrorInvalidValue;
+    if ((tree || b->parent) && b->max_rows > QG_MAX_TREE) return hipErrorInvalidValue;
+    if (v) *v = BatchView{b->start, b->parent, b->rows, b->max_rows};
+    return hipSuccess;
+}
+
+namespace {
+
+QG_DEV void let_go(const KvView &c, int page) {
+    if ((unsigned)page < (unsigned)c.pages) atomicSub(&c.refs[page], 1);
+}
+
+__global__ __launch_bounds__(256) void kv_truncate_kernel(KvView c, const int *new_length) {
+    const int s = blockIdx.x;
+    int n = kv_length(c, s);
+    if (new_length) n = min(n, max(new_length[s], 0));
+    const int keep = (n + (1 << c.shift) - 1) >> c.shift;
+    int *row = c.table + (size_t)s * c.table_pages;
+    for (int j = keep + threadIdx.x; j < c.table_pages; j += 256) {
+        const int page = row[j];
+        if (page != -1) { let_go(c, page); row[j] = -1; }
+    }
+    __syncthreads();  // every thread has read the length
+    if (threadIdx.x == 0) c.length[s] = n;
+}
+
+// Fork, first half: pair i's source row as it is before the call, and one more
+// holder for each of its pages.  ws: [n][table_pages + 2] (use, length, pages).
+__global__ __launch_bounds__(256) void kv_fork_stage_kernel(KvView c, const int *dst, const int *src, int n, int *ws) {
+    const int i = blockIdx.x, d = dst[i], from = src[i];
+    int *at = ws + (size_t)i * (c.table_pages + 2);
+    bool bad = (unsigned)d >= (unsigned)c.sequences || (unsigned)from >= (unsigned)c.sequences || d == from;
+    for (int j = i + 1 + threadIdx.x; j < n; j += 256)
+        bad |= dst[j] == d && (unsigned)src[j] < (unsigned)c.sequences && src[j] != d;
+    bad = __syncthreads_or(bad);
+    if (threadIdx.x == 0) at[0] = !bad;
+    if (bad) return;
+    const int len = kv_length(c, from), keep = (len + (1 << c.shift) - 1) >> c.shift;
+    if (threadIdx.x == 0) at[1] = len;
+    for (int j = threadIdx.x; j < c.table_pages; j += 256) {
+        int page = j < keep ? c.table[(size_t)from * c.table_pages + j] : -1;
+        if ((unsigned)page >= (unsigned)c.pages) page = -1;
+        if (page >= 0) atomicAdd(&c.refs[page], 1);
+        at[2 + j] = page;
+    }
+}
+// Second half: the destination lets go of its own pages and takes the staged ones.
+__global__ __launch_bounds__(256) void kv_fork_kernel(KvView c, const int *dst, const int *ws) {
+    const int *at = ws + (size_t)blockIdx.x * (c.table_pages + 2);
+    if (!at[0]) return;
+    const int d = dst[blockIdx.x];
+    int *row = c.table + (size_t)d * c.table_pages;
+    for (int j = threadIdx.x; j < c.table_pages; j += 256) {
+        let_go(c, row[j]);
+        row[j] = at[2 + j];
+    }
+    if (threadIdx.x == 0) c.length[d] = at[1];
+}
+
+// Inclusive sum over the 1024 threads of a workgroup; s_sum[16] is scratch.
+QG_DEV int block_scan(int v, int *s_sum, int &total) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+        const int u = __shfl_up(v, d);
+        if (lane >= d) v += u;
+    }
+    __syncthreads();
+    if (lane == 63) s_sum[wave] = v;
+    __syncthreads();
+    int before = 0;
+    total = 0;
+#pragma unroll
+    for (int w = 0; w < 16; w++) {
+        const int x = s_sum[w];
+        if (w < wave) before += x;
+        total += x;
+    }
+    return v + before;
+}
+
+// Reserve, one workgroup (its sums run over all sequences and over the free
+// pages in order); a wave per sequence looks at its entries.  An entry needs a
+// page if it is empty, or if its page is held elsewhere too.  The second kind
+// is marked in the table as -2 - page while the sequences are counted, so that
+// every sequence judges by the holders before the call.  Pages are taken for
+// the whole batch or not at all: a sequence may keep a shared page only because
+// the others get copies of theirs.
+// ws: copies [sequences][2] for kv_cow_kernel, then the free pages found.
+__global__ __launch_bounds__(1024) void kv_reserve_kernel(KvView c, BatchView b, int *status, int *ws) {
+    __shared__ int s_len[QG_MAX_SEQUENCES], s_rows[QG_MAX_SEQUENCES], s_page[QG_MAX_SEQUENCES], s_need[QG_MAX_SEQUENCES], s_sum[16];
+    __shared__ int s_found;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, P = 1 << c.shift;
+    int *copies = ws, *free_pages = ws + 2 * c.sequences;
+    // each sequence's rows, and the page with room behind its tokens
+    int st = 0, mine = -1;
+    if (tid < c.sequences) {
+        int first, rows;
+        batch_rows(b, tid, first, rows);
+        const int len = kv_length(c, tid);
+        if (rows > kv_capacity(c) - len) { st = 2; rows = 0; }
+        if (rows && (len & (P - 1))) mine = kv_page(c, tid, len);
+        s_len[tid] = len;
+        s_rows[tid] = rows;
+        s_page[tid] = mine;
+    }
+    __syncthreads();
+    // of the batch's sequences that share a page no other holds, the first keeps it
+    bool copied = false;
+    if (mine >= 0) {
+        const int held = c.refs[mine];
+        if (held > 1) {
+            int same = 0;
+            bool before = false;
+            for (int j = 0; j < c.sequences; j++)
+                if (s_page[j] == mine) { same++; before |= j < tid; }
+            copied = before || same < held;
+        }
+    }
+    __syncthreads();
+    if (tid < c.sequences) s_page[tid] = copied;
+    __syncthreads();
+    for (int s = wave; s < c.sequences; s += 16) {
+        const int len = s_len[s], rows = s_rows[s], here = len >> c.shift, end = rows ? (len + rows + P - 1) >> c.shift : here;
+        int need = 0;
+        for (int j0 = here; j0 < end; j0 += 64) {
+            const int j = j0 + lane;
+            bool take = false;
+            if (j < end) {
+                int *entry = c.table + (size_t)s * c.table_pages + j;
+                const int page = *entry;
+                const bool none = (unsigned)page >= (unsigned)c.pages;
+                take = none || (j == here && (len & (P - 1)) ? s_page[s] != 0 : c.refs[page] > 1);
+                if (take) *entry = none ? -1 : -2 - page;
+            }
+            need += __popcll(__ballot(take));
+        }
+        if (lane == 0) s_need[s] = need;
+    }
+    __syncthreads();
+    int total;
+    const int need = tid < c.sequences ? s_need[tid] : 0;
+    const int upto = block_scan(need, s_sum, total);
+    // the first `total` free pages in ascending order, 16 of the pool per thread and round
+    int found = 0;
+    for (int p0 = 0; p0 < c.pages && found < total; p0 += 16384) {
+        unsigned mask = 0;
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+            const int p = p0 + tid * 16 + i;
+            if (p < c.pages && c.refs[p] == 0) mask |= 1u << i;
+        }
+        int sum;
+        int at = found + block_scan(__popc(mask), s_sum, sum) - __popc(mask);
+        for (; mask && at < total; mask &= mask - 1) free_pages[at++] = p0 + tid * 16 + __ffs(mask) - 1;
+        found += sum;
+    }
+    if (tid < c.sequences) {
+        if (s_rows[tid] && total > found) st = 1;
+        status[tid] = st;
+        copies[2 * tid] = copies[2 * tid + 1] = -1;
+        s_page[tid] = upto - need;  // the sequence's first page in the list
+    }
+    __syncthreads();  // free_pages and copies written above are read or written by other waves below
+    for (int s = wave; s < c.sequences; s += 16) {
+        if (!s_need[s]) continue;
+        const int len = s_len[s], here = len >> c.shift, end = (len + s_rows[s] + P - 1) >> c.shift;
+        int from = s_page[s];
+        const bool served = total <= found;
+        for (int j0 = here; j0 < end; j0 += 64) {
+            const int j = j0 + lane;
+            int *entry = c.table + (size_t)s * c.table_pages + j;
+            const int mark = j < end ? *entry : 0;
+            const bool take = mark < 0;
+            const unsigned long long all = __ballot(take);
+            if (take && served) {
+                const int page = free_pages[from + __popcll(all & ((1ULL << lane) - 1))];
+                *entry = page;
+                c.refs[page] = 1;
+                if (mark < -1) {
+                    atomicSub(&c.refs[-2 - mark], 1);
+                    if (j == here && (len & (P - 1))) { copies[2 * s] = -2 - mark; copies[2 * s + 1] = page; }
+                }
+            } else if (take && mark < -1) {
+                *entry = -2 - mark;
+            }
+            from += __popcll(all);
+        }
+    }
+}
+
+// One layer's page, k (blockIdx.z even) or v, in 16-byte pieces.
+QG_DEV void copy_page(const KvView &c, int dst, int src, int layer, bool v, int part, int parts) {
+    const size_t bytes = ((size_t)c.heads << c.shift) * c.dim * (c.type == QT_F32 ? 4 : 2);
+    uint8_t *base = (v ? c.v : c.k) + (size_t)layer * c.pages * bytes;
+    const uint4 *from = (const uint4 *)(base + src * bytes);
+    uint4 *to = (uint4 *)(base + dst * bytes);
+    for (size_t i = (size_t)part * 256 + threadIdx.x; i < bytes / 16; i += (size_t)parts * 256) to[i] = from[i];
+}
+__global__ __launch_bounds__(256) void kv_cow_kernel(KvView c, const int *copies) {
+    const int src = copies[2 * blockIdx.x], dst = copies[2 * blockIdx.x + 1];
+    if (src < 0) return;
+    for (int i = blockIdx.z; i < 2 * c.layers; i += gridDim.z) copy_page(c, dst, src, i >> 1, i & 1, blockIdx.y, gridDim.y);
+}
+__global__ __launch_bounds__(256) void kv_copy_pages_kernel(KvView c, const int *dst, const int *src, int n) {
+    const int i = blockIdx.x, d = dst[i], s = src[i];
+    bool bad = (unsigned)d >= (unsigned)c.pages || (unsigned)s >= (unsigned)c.pages;
+    for (int j = threadIdx.x; j < n; j += 256) bad |= src[j] == d || (j > i && dst[j] == d);
+    if (__syncthreads_or(bad)) return;
+    for (int k = blockIdx.z; k < 2 * c.layers; k += gridDim.z) copy_page(c, d, s, k >> 1, k & 1, blockIdx.y, gridDim.y);
+}
+
+// The accepted rows of a sequence move to the front of its new rows.  A thread
+// owns one 16-byte column of one head, layer and side and carries it through
+// all moves, so no two threads meet; a path ascends, so row i never lands
+// where a later one starts, and eight rows may be read before the first is written.
+// new_length NULL: written by kv_length_kernel, where the workgroups of a
+// sequence read the lengths that it replaces.
+QG_DEV int path_rows(const BatchView &b, const int *path, const int *count, int s, int lane, int &p) {
+    int first, n;
+    batch_rows(b, s, first, n);
+    const int keep = min(max(count[s], 0), n);
+    p = lane < keep ? path[(size_t)s * b.max_rows + lane] : -1;
+    const int before = __shfl_up(p, 1);
+    const bool ok = lane < keep && p < n && p > (lane ? before : -1);
+    const unsigned long long fault = ~__ballot(ok);
+    return fault ? __ffsll(fault) - 1 : 64;
+}
+__global__ __launch_bounds__(64) void kv_length_kernel(KvView c, BatchView b, const int *path, const int *count, int *new_length) {
+    int p;
+    const int upto = path_rows(b, path, count, blockIdx.x, threadIdx.x, p), len = kv_length(c, blockIdx.x);
+    if (threadIdx.x == 0) new_length[blockIdx.x] = len + upto;
+}
+__global__ __launch_bounds__(256) void kv_compact_kernel(KvView c, BatchView b, const int *path, const int *count, int *new_length) {
+    __shared__ size_t s_from[QG_MAX_TREE], s_to[QG_MAX_TREE];
+    __shared__ int s_moves;
+    const int s = blockIdx.y, lane = threadIdx.x & 63, es = c.type == QT_F32 ? 4 : 2;
+    if (threadIdx.x < 64) {
+        const int len = kv_length(c, s);
+        int p;
+        const int upto = path_rows(b, path, count, s, lane, p);
+        const bool move = lane < upto && p != lane;
+        const int from = move ? kv_page(c, s, len + p) : -1, to = move ? kv_page(c, s, len + lane) : -1;
+        const int slot = (1 << c.shift) - 1;
+        const bool both = from >= 0 && to >= 0;
+        const unsigned long long all = __ballot(both);
+        if (both) {
+            const int at = __popcll(all & ((1ULL << lane) - 1));
+            s_from[at] = kv_at(c, 0, from, 0, (len + p) & slot) * es;
+            s_to[at] = kv_at(c, 0, to, 0, (len + lane) & slot) * es;
+        }
+        if (lane == 0) {
+            s_moves = __popcll(all);
+            if (blockIdx.x == 0 && new_length) new_length[s] = len + upto;
+        }
+    }
+    __syncthreads();
+    const int moves = s_moves;
+    if (!moves) return;
+    const int pieces = c.dim * es / 16;
+    const size_t layer = (((size_t)c.pages * c.heads) << c.shift) * c.dim * es, head = ((size_t)c.dim << c.shift) * es;
+    const int all = 2 * c.layers * c.heads * pieces;
+    for (int i = blockIdx.x * 256 + threadIdx.x; i < all; i += gridDim.x * 256) {
+        const int piece = i % pieces, h = i / pieces % c.heads, l = i / pieces / c.heads;
+        uint8_t *base = (l & 1 ? c.v : c.k) + (l >> 1) * layer + h * head + piece * 16;
+        for (int m0 = 0; m0 < moves; m0 += 8) {
+            uint4 x[8];
+#pragma unroll
+            for (int m = 0; m < 8; m++) x[m] = *(const uint4 *)(base + s_from[min(m0 + m, moves - 1)]);
+#pragma unroll
+            for (int m = 0; m < 8; m++)
+                if (m0 + m < moves) *(uint4 *)(base + s_to[m0 + m]) = x[m];
+        }
+    }
+}
+
+size_t page_parts(const KvView &c) {  // workgroups per page, layer and side: 16 pieces of 16 bytes per thread
+    const size_t bytes = ((size_t)c.heads << c.shift) * c.dim * (c.type == QT_F32 ? 4 : 2);
+    const size_t n = (bytes / 16 + 4095) / 4096;
+    return n < 64 ? n : 64;
+}
+unsigned layer_parts(const KvView &c) { return 2 * c.layers < 4096 ? 2 * c.layers : 4096; }
+}  // namespace
+
+extern "C" {
+
+size_t qg_kv_workspace_bytes(const qg_kv_cache *cache) {
+    if (qg_kv_check(cache, false, nullptr)) return 0;
+    const size_t fork = (size_t)cache->sequences * (cache->table_pages + 2), reserve = 2 * (size_t)cache->sequences + cache->pages;
+    return 4 * (fork > reserve ? fork : reserve);
+}
+
+int qg_kv_reserve(const qg_kv_cache *cache, const qg_kv_batch *batch, int *status, void *ws, size_t ws_bytes) {
+    KvView c;
+    BatchView b;
+    if (qg_kv_check(cache, true, &c) || qg_batch_check(batch, false, &b)) return hipErrorInvalidValue;
+    if (!status || !ws || (((uintptr_t)status | (uintptr_t)ws) & 3) || ws_bytes < qg_kv_workspace_bytes(cache)) return hipErrorInvalidValue;
+    kv_reserve_kernel<<<1, 1024, 0, qg_stream()>>>(c, b, status, (int *)ws);
+    kv_cow_kernel<<<dim3(c.sequences, (unsigned)page_parts(c), layer_parts(c)), 256, 0, qg_stream()>>>(c, (const int *)ws);
+    return hipGetLastError();
+}
+
+int qg_kv_fork(const qg_kv_cache *cache, const int *dst, const int *src, int n, void *ws, size_t ws_bytes) {
+    KvView c;
+    if (qg_kv_check(cache, true, &c)) return hipErrorInvalidValue;
+    if (!dst || !src || n < 1 || n > c.sequences || !ws || ws_bytes < qg_kv_workspace_bytes(cache) ||
+        (((uintptr_t)dst | (uintptr_t)src | (uintptr_t)ws) & 3))
+        return hipErrorInvalidValue;
+    kv_fork_stage_kernel<<<n, 256, 0, qg_stream()>>>(c, dst, src, n, (int *)ws);
+    kv_fork_kernel<<<n, 256, 0, qg_stream()>>>(c, dst, (const int *)ws);
+    return hipGetLastError();
+}
+
+int qg_kv_truncate(const qg_kv_cache *cache, const int *new_length) {
+    KvView c;
+    if (qg_kv_check(cache, true, &c) || ((uintptr_t)new_length & 3)) return hipErrorInvalidValue;
+    kv_truncate_kernel<<<c.sequences, 256, 0, qg_stream()>>>(c, new_length);
+    return hipGetLastError();
+}
+
+int qg_kv_compact(const qg_kv_cache *cache, const qg_kv_batch *batch, const int *path, const int *count, int *new_length) {
+    KvView c;
+    BatchView b;
+    if (qg_kv_check(cache, false, &c) || qg_batch_check(batch, true, &b)) return hipErrorInvalidValue;
+    if (!path || !count || !new_length || (((uintptr_t)path | (uintptr_t)count | (uintptr_t)new_length) & 3)) return hipErrorInvalidValue;
+    const bool own = new_length == cache->length;
+    if (!own && qg_overlap(new_length, 4 * (size_t)c.sequences, cache->length, 4 * (size_t)c.sequences)) return hipErrorInvalidValue;
+    const long all = 2L * c.layers * c.heads * (c.dim * (c.type == QT_F32 ? 4 : 2) / 16), blocks = (all + 255) / 256;
+    kv_compact_kernel<<<dim3((unsigned)(blocks < 1024 ? blocks : 1024), c.sequences), 256, 0, qg_stream()>>>(c, b, path, count,
+                                                                                                          own ? nullptr : new_length);
+    if (own) kv_length_kernel<<<c.sequences, 64, 0, qg_stream()>>>(c, b, path, count, new_length);
+    return hipGetLastError();
+}
+
+int qg_kv_copy_pages(const qg_kv_cache *cache, const int *dst, const int *src, int n) {
+    KvView c;
+    if (qg_kv_check(cache, false, &c)) return hipErrorInvalidValue;
+    if (!dst || !src || n < 1 || n > 4096 || (((uintptr_t)dst | (uintptr_t)src) & 3)) return hipErrorInvalidValue;
+    kv_copy_pages_kernel<<<dim3(n, (unsigned)page_parts(c), layer_parts(c)), 256, 0, qg_stream()>>>(c, dst, src, n);
+    return hipGetLastError();
+}
+
+}  // extern "C"

@@ -41,6 +41,12 @@ SIGNATURES = {
     "synth_matrix": ([P, I, U64, U64, I, I, F], I), "synth_experts": ([P, I, U64, I, I, I, I, F], I), "prefill_int8_dense": ([I], I),
     "moe_handoff_pack": ([P, P, P, P, P, P, P, P, P, I, I], I), "moe_handoff_merge": ([P, P, P, P, I, I], I),
     "moe_handoff_notify": ([P, P], I), "host_alloc": ([Z], P), "host_free": ([P], None),
+    "qk_norm_rope": ([P, P, P, P, I, P], I), "tree_attention_workspace_bytes": ([P, P, I], Z),
+    "tree_attention": ([P, P, I, F, P, I, P, P, Z], I), "softmax_workspace_bytes": ([I, I], Z),
+    "softmax": ([P, P, I, I, F, P, Z], I), "verify_workspace_bytes": ([I, I], Z),
+    "verify_drafts": ([P, P, P, P, P, P, P, P, I, I, P, P, Z], I), "kv_workspace_bytes": ([P], Z),
+    "kv_reserve": ([P, P, P, P, Z], I), "kv_fork": ([P, P, P, I, P, Z], I), "kv_truncate": ([P, P], I),
+    "kv_compact": ([P, P, P, P, P], I), "kv_copy_pages": ([P, P, P, I], I),
 }
 
 # nm_cpu_moe_fn of include/nebula_moe.h: (ctx, out, x, ids, weights, tokens) -> 0 on success
@@ -100,6 +106,24 @@ class MoeLayer(C.Structure):
                 ("gate_type", I), ("up_type", I), ("down_type", I),
                 ("sh_gate", P), ("sh_up", P), ("sh_down", P), ("sh_gate_type", I), ("sh_up_type", I), ("sh_down_type", I),
                 ("sh_gate_inp", P), ("resident", P), ("threshold", D64), ("router_bias", P)]
+
+
+class KvCache(C.Structure):
+    """qg_kv_cache of include/qwen_gpu.h."""
+    _fields_ = [("k", P), ("v", P), ("type", I), ("layers", I), ("pages", I), ("kv_heads", I), ("page_tokens", I), ("head_dim", I),
+                ("refs", P), ("table", P), ("length", P), ("sequences", I), ("table_pages", I)]
+
+
+class KvBatch(C.Structure):
+    """qg_kv_batch of include/qwen_gpu.h."""
+    _fields_ = [("rows", I), ("max_rows", I), ("start", P), ("parent", P)]
+
+
+class QkRows(C.Structure):
+    """qg_qk_rows of include/qwen_gpu.h."""
+    _fields_ = [("q", P), ("k", P), ("v", P)] + [(n, C.c_int64) for n in ("q_row", "q_head", "k_row", "k_head", "v_row", "v_head")] + [
+        ("rows", I), ("q_heads", I), ("kv_heads", I), ("head_dim", I), ("q_norm", P), ("k_norm", P), ("eps", F),
+        ("rope_dims", I), ("interleaved", I), ("freq", P), ("position", P)]
 
 
 _LIB = None

@@ -1,0 +1,231 @@
+"""qg_tree_attention against a 64-bit statement of it (spec_oracle.attention)."""
+import ctypes as C
+import sys
+
+import numpy as np
+import pytest
+
+import spec_oracle as O
+from nebula_amd import qg
+from nebula_amd.qg import Device, call
+from spec_oracle import BF16, F16, F32, Batch, Cache
+
+pytestmark = pytest.mark.gpu
+
+
+def say(*a):
+    print(*a, flush=True, file=sys.stderr)
+
+
+def store(cache, batch, rng, layer=0, scale=1.0):
+    """The batch's own rows, in the host copy."""
+    for row, s, place in batch.places():
+        cache.put(layer, s, int(cache.length[s]) + place, *(scale * rng.standard_normal((2, cache.H, cache.D))))
+    cache.upload()
+
+
+def attend(cache, batch, q, scale, layer=0, sentinel=np.nan):
+    dq = Device(q)
+    out = Device(np.full(q.shape, sentinel, np.float32))
+    n = qg.lib().qg_tree_attention_workspace_bytes(cache.ref, batch.ref, q.shape[1])
+    assert n
+    ws = Device(np.full(n, 0xff, np.uint8))  # NaN: nothing of a workspace counts that was not written
+    say(f"attention q{q.shape} type={cache.typ} page={cache.P} lengths={list(cache.length)[:8]} rows={batch.rows} tree={batch.parent is not None}")
+    call("tree_attention", out.p, dq.p, q.shape[1], scale, cache.ref, layer, batch.ref, ws.p, n)
+    return out.get()
+
+
+def check(cache, batch, q, scale, layer=0):
+    got = attend(cache, batch, q, scale, layer)
+    want, tol, done = O.attention(cache, batch, q, scale, layer)
+    assert np.isnan(got[~done]).all()
+    bad = ~(np.abs(got - want) <= tol) & done[:, None, None]
+    assert not bad.any(), (np.argwhere(bad)[:5], np.nanmax(np.abs(got - want) / np.maximum(tol, 1e-30)))
+    return got
+
+
+@pytest.mark.parametrize("typ", [F16, BF16, F32])
+@pytest.mark.parametrize("dim,heads,group,page", [(64, 1, 1, 8), (64, 2, 8, 16), (128, 2, 5, 64), (128, 1, 16, 32), (256, 2, 4, 16), (128, 4, 3, 1024)])
+@pytest.mark.parametrize("tree", [False, True])
+def test_attention_shapes(qgl, typ, dim, heads, group, page, tree):
+    rng = np.random.default_rng(dim + group + page + typ)
+    counts, lengths = [1, 5, 0, 17, 2], [0, 31, 8, 100, 257]
+    cache = Cache(rng, lengths, counts, typ=typ, layers=2, kv_heads=heads, page=page, dim=dim)
+    batch = Batch(counts, [O.random_tree(rng, n) if n else [] for n in counts] if tree else None, rows=sum(counts) + 3)
+    store(cache, batch, rng, layer=1)
+    q = rng.standard_normal((batch.rows, heads * group, dim)).astype(np.float32)
+    check(cache, batch, q, dim ** -0.5, layer=1)
+
+
+@pytest.mark.parametrize("typ", [F16, BF16, F32])
+@pytest.mark.parametrize("length", [0, 1, 7, 8, 31, 32, 33, 63, 64, 127, 128, 129, 1000, 4099])
+def test_attention_one_row(qgl, typ, length):
+    rng = np.random.default_rng(length)
+    cache = Cache(rng, [length], [1], typ=typ, kv_heads=2, page=32, dim=64)
+    batch = Batch([1])
+    store(cache, batch, rng)
+    check(cache, batch, rng.standard_normal((1, 10, 64)).astype(np.float32), 0.125)
+
+
+@pytest.mark.parametrize("typ,dim", [(F16, 128), (BF16, 64), (F32, 64), (BF16, 256)])
+@pytest.mark.parametrize("rows,length", [(64, 0), (64, 77), (33, 2000), (2, 5000)])
+def test_attention_trees(qgl, typ, dim, rows, length):
+    rng = np.random.default_rng(rows + length)
+    for width in (1, 3, 64):
+        cache = Cache(rng, [length], [rows], typ=typ, kv_heads=1, page=16, dim=dim)
+        batch = Batch([rows], [O.random_tree(rng, rows, width)])
+        store(cache, batch, rng)
+        check(cache, batch, rng.standard_normal((rows, 4, dim)).astype(np.float32), dim ** -0.5)
+
+
+@pytest.mark.parametrize("typ", [F16, BF16, F32])
+def test_attention_prompt_chunk(qgl, typ):
+    """A chain longer than a tree may be: a prompt chunk behind cached tokens, and one at the start."""
+    rng = np.random.default_rng(5)
+    counts, lengths = [130, 300, 3], [65, 0, 200]
+    cache = Cache(rng, lengths, counts, typ=typ, kv_heads=2, page=32, dim=64)
+    batch = Batch(counts)
+    store(cache, batch, rng)
+    check(cache, batch, rng.standard_normal((batch.rows, 6, 64)).astype(np.float32), 0.125)
+
+
+@pytest.mark.parametrize("typ", [F16, BF16, F32])
+def test_attention_many_ragged_sequences(qgl, typ):
+    rng = np.random.default_rng(6)
+    counts = [int(x) for x in rng.integers(0, 4, 130)]
+    lengths = [int(x) for x in rng.integers(0, 90, 129)] + [3000]
+    cache = Cache(rng, lengths, counts, typ=typ, kv_heads=1, page=16, dim=64)
+    batch = Batch(counts, max_rows=3)
+    store(cache, batch, rng)
+    check(cache, batch, rng.standard_normal((batch.rows, 4, 64)).astype(np.float32), 0.125)
+
+
+@pytest.mark.parametrize("typ", [F16, BF16, F32])
+def test_attention_holes_and_bad_entries(qgl, typ):
+    """Table entries that are no pages hold nothing; a row that sees nothing is zero; lengths and row starts outside
+    their range are cut."""
+    rng = np.random.default_rng(7)
+    counts, lengths = [3, 4, 5, 2], [60, 40, 50, 0]
+    cache = Cache(rng, lengths, counts, typ=typ, kv_heads=2, page=16, dim=64)
+    batch = Batch(counts, [O.random_tree(rng, n) for n in counts])
+    store(cache, batch, rng)
+    cache.table[0, 1], cache.table[1, 0], cache.table[1, 1] = cache.pages, -7, 0x7fffffff
+    cache.table[2, :] = -1
+    cache.upload()
+    q = rng.standard_normal((batch.rows, 4, 64)).astype(np.float32)
+    got = check(cache, batch, q, 0.125)
+    assert (got[7:12] == 0).all()
+    # a length beyond the table is the table's; one below zero is none
+    cache.table[2, :] = cache.table[0, 2]
+    cache.length[:] = [1 << 30, -5, -(1 << 31), cache.width * cache.P + 1]
+    cache.upload()
+    got = attend(cache, batch, q, 0.125)
+    assert (got[3:7] == 0).all()  # neither cached tokens nor a page of their own
+    # starts that run backwards or beyond the rows
+    batch.dstart.set(np.array([5, -3, 900, 2, 1 << 30], np.int32))
+    cache.dlength.set(np.array(lengths, np.int32))
+    attend(cache, batch, q, 0.125)
+
+
+@pytest.mark.parametrize("typ", [F16, BF16, F32])
+def test_attention_masked_nonfinite(qgl, typ):
+    """NaN and infinities in keys and values reach the rows that see them and no others; behind the last token, in
+    free pages and in unused slots (all NaN here) they reach none."""
+    rng = np.random.default_rng(8)
+    rows, length = 9, 70
+    cache = Cache(rng, [length], [rows], typ=typ, kv_heads=1, page=16, dim=64)
+    parents = [-1, 0, 0, 1, 1, 2, 2, 5, 5]
+    batch = Batch([rows], [parents])
+    store(cache, batch, rng)
+    for t, what in ((length + 3, np.nan), (length + 6, np.inf)):
+        p = cache.page_of(0, t)
+        cache.v[0, p, 0, t % 16, 5] = O.encode([what], typ)[0]
+        cache.k[0, p, 0, t % 16, 9] = O.encode([np.nan if t == length + 3 else 0], typ)[0]
+    cache.upload()
+    q = rng.standard_normal((rows, 3, 64)).astype(np.float32)
+    got = attend(cache, batch, q, 0.125)
+    want, tol, done = O.attention(cache, batch, q, 0.125)
+    for r in range(rows):
+        if r == 3:
+            assert np.isnan(got[r]).all()
+        elif r == 6:
+            assert (got[r, :, 5] == np.inf).all()
+            keep = np.arange(64) != 5
+            assert np.all(np.abs(got[r][:, keep] - want[r][:, keep]) <= tol[r][:, keep])
+        else:
+            assert np.all(np.abs(got[r] - want[r]) <= tol[r]), r
+
+
+@pytest.mark.parametrize("typ", [F16, BF16, F32])
+def test_attention_score_range(qgl, typ):
+    """Scores far apart and large, queries of very different sizes, keys of the lowest value and scores of minus infinity."""
+    rng = np.random.default_rng(9)
+    cache = Cache(rng, [300, 90], [4, 2], typ=typ, kv_heads=1, page=32, dim=128)
+    batch = Batch([4, 2])
+    store(cache, batch, rng)
+    q = rng.standard_normal((6, 4, 128)).astype(np.float32)
+    q[0] *= 30
+    q[1] *= 1e-6
+    q[2, 1] = 0
+    q[3, 0, :64] *= 1e-8
+    check(cache, batch, q, 128 ** -0.5)
+    # the largest score comes late and is far above the others
+    for t in (250, 299):
+        cache.put(0, 0, t, np.full((1, 128), 3.0), np.full((1, 128), 1.0))
+    q[0] = np.abs(q[0]) * 0.2
+    cache.upload()
+    check(cache, batch, q, 128 ** -0.5)
+    # rows whose every score is minus infinity are zero; one finite score takes all
+    q[4:] = 0
+    q[4:, :, 0] = 1.0
+    p, low = cache.page_of, O.encode([-np.inf], typ)[0]
+    for t in range(92):
+        cache.k[0, p(1, t), 0, t % 32] = 0
+        if t != 40:
+            cache.k[0, p(1, t), 0, t % 32, 0] = low
+    cache.upload()
+    got = attend(cache, batch, q, 1.0)
+    want = cache.token(cache.v, 0, 1, 40)[0]
+    np.testing.assert_array_equal(got[4:], np.broadcast_to(want.astype(np.float32), (2, 4, 128)))
+    cache.k[0, p(1, 40), 0, 40 % 32, 0] = low
+    cache.upload()
+    assert (attend(cache, batch, q, 1.0)[4:] == 0).all()
+
+
+def test_attention_far_offsets(qgl):
+    """A layer behind more than 4 GiB of others: offsets beyond 32 bits."""
+    rng = np.random.default_rng(10)
+    layers, heads, dim, page = 40, 8, 128, 64
+    cache = Cache(rng, [200], [2], typ=F16, kv_heads=heads, page=page, dim=dim, spare=0)
+    pages = 1024
+    bytes_layer = pages * heads * page * dim * 2
+    big = [Device.__new__(Device) for _ in range(2)]
+    for d in big:
+        d.x, d.p = np.zeros(1, np.uint8), qg.lib().qg_alloc(layers * bytes_layer)
+        assert d.p
+    batch = Batch([2])
+    store(cache, batch, rng)
+    layer, first = layers - 1, pages - cache.pages
+    for d, host in zip(big, (cache.k, cache.v)):
+        at = d.p + layer * bytes_layer + first * heads * page * dim * 2
+        call("write", at, np.ascontiguousarray(host).ctypes.data, host.nbytes)
+    desc = qg.KvCache.from_buffer_copy(cache.desc)
+    table = Device(np.where(cache.table >= 0, cache.table + first, -1).astype(np.int32))
+    desc.k, desc.v, desc.layers, desc.pages, desc.table = big[0].p, big[1].p, layers, pages, table.p
+    q = rng.standard_normal((2, heads * 2, dim)).astype(np.float32)
+    want, tol, _ = O.attention(cache, batch, q, dim ** -0.5)
+    cache.ref = C.byref(desc)
+    got = attend(cache, batch, q, dim ** -0.5, layer)
+    assert np.all(np.abs(got - want) <= tol)
+
+
+@pytest.mark.parametrize("typ", [F16, BF16, F32])
+def test_attention_long_context_split(qgl, typ):
+    """A long cache beside short ones, so that its work is split and joined; the same answer twice, bit for bit."""
+    rng = np.random.default_rng(11)
+    cache = Cache(rng, [20000, 3, 500], [5, 5, 1], typ=typ, kv_heads=1, page=64, dim=64)
+    batch = Batch([5, 5, 1], [O.random_tree(rng, n) for n in (5, 5, 1)])
+    store(cache, batch, rng)
+    q = rng.standard_normal((11, 6, 64)).astype(np.float32)
+    a = check(cache, batch, q, 0.125)
+    np.testing.assert_array_equal(a, attend(cache, batch, q, 0.125))

@@ -1,0 +1,272 @@
+"""qg_kv_reserve / fork / truncate / compact / copy_pages against a model of the
+same rules in Python: tables, holders, lengths and every byte of the pages."""
+import sys
+
+import numpy as np
+import pytest
+
+import spec_oracle as O
+from nebula_amd import qg
+from nebula_amd.qg import Device, call
+from spec_oracle import BF16, F16, F32, Batch, Cache
+
+pytestmark = pytest.mark.gpu
+
+
+def say(*a):
+    print(*a, flush=True, file=sys.stderr)
+
+
+class Model:
+    """The rules, one sequence and one page at a time, on the host copy of a cache."""
+
+    def __init__(self, c):
+        self.c = c
+
+    def _let_go(self, p):
+        if 0 <= p < self.c.pages:
+            self.c.refs[p] -= 1
+
+    def truncate(self, new=None):
+        c = self.c
+        for s in range(c.B):
+            n = int(min(max(c.length[s], 0), c.width * c.P))
+            n = n if new is None else min(n, max(int(new[s]), 0))
+            for j in range(-(-n // c.P), c.width):
+                self._let_go(c.table[s, j])
+                c.table[s, j] = -1
+            c.length[s] = n
+
+    def fork(self, dst, src):
+        c, table, length = self.c, self.c.table.copy(), self.c.length.copy()
+        ok = [0 <= d < c.B and 0 <= s < c.B and d != s for d, s in zip(dst, src)]
+        for i, (d, s) in enumerate(zip(dst, src)):
+            if not ok[i] or any(ok[j] and dst[j] == d for j in range(i + 1, len(dst))):
+                continue
+            for p in c.table[d]:
+                self._let_go(p)
+            keep = -(-int(length[s]) // c.P)
+            row = np.where((np.arange(c.width) < keep) & (table[s] >= 0) & (table[s] < c.pages), table[s], -1)
+            for p in row[row >= 0]:
+                c.refs[p] += 1
+            c.table[d], c.length[d] = row, length[s]
+
+    def reserve(self, counts):
+        c = self.c
+        status, need, copies = np.zeros(c.B, np.int32), [], []
+        live = [s for s in range(c.B) if counts[s] and c.length[s] + counts[s] <= c.width * c.P]
+        for s in range(c.B):
+            if counts[s] and s not in live:
+                status[s] = 2
+        page = {s: c.page_of(s, int(c.length[s])) for s in live if c.length[s] % c.P}
+        for s in live:
+            L, here = int(c.length[s]), int(c.length[s]) // c.P
+            for j in range(here, -(-(L + counts[s]) // c.P)):
+                p = int(c.table[s, j])
+                if not 0 <= p < c.pages:
+                    need.append((s, j, -1))
+                elif j == here and s in page:
+                    same = [t for t in page if page[t] == p]
+                    if c.refs[p] > 1 and (same[0] != s or len(same) < c.refs[p]):
+                        need.append((s, j, p))
+                elif c.refs[p] > 1:
+                    need.append((s, j, p))
+        free = [p for p in range(c.pages) if c.refs[p] == 0]
+        if len(need) > len(free):
+            status[live] = 1
+            return status
+        for (s, j, old), p in zip(need, free):
+            if old >= 0:
+                c.refs[old] -= 1
+                if j == int(c.length[s]) // c.P and s in page:
+                    copies.append((p, old))
+            c.table[s, j] = p
+            c.refs[p] = 1
+        for p, old in copies:
+            c.k[:, p], c.v[:, p] = c.k[:, old], c.v[:, old]
+        return status
+
+    def compact(self, batch, path, count):
+        c, new = self.c, c_length(self.c)
+        for s in range(c.B):
+            n, L = int(batch.start[s + 1] - batch.start[s]), int(c.length[s])
+            before, kept = -1, 0
+            for i in range(min(max(int(count[s]), 0), n)):
+                p = int(path[s, i])
+                if not before < p < n:
+                    break
+                before, kept = p, kept + 1
+                a, b = c.page_of(s, L + p), c.page_of(s, L + i)
+                if p != i and a >= 0 and b >= 0:
+                    for pool in (c.k, c.v):
+                        pool[:, b, :, (L + i) % c.P] = pool[:, a, :, (L + p) % c.P]
+            new[s] += kept
+        return new
+
+
+def c_length(c):
+    return c.length.copy()
+
+
+def same(c, pools=True):
+    np.testing.assert_array_equal(c.dtable.get(), c.table)
+    np.testing.assert_array_equal(c.drefs.get(), c.refs)
+    np.testing.assert_array_equal(c.dlength.get(), c.length)
+    held = np.bincount(c.table[(c.table >= 0) & (c.table < c.pages)], minlength=c.pages)
+    np.testing.assert_array_equal(held, c.refs)
+    if pools:
+        np.testing.assert_array_equal(c.dk.get().view(np.uint8), c.k.view(np.uint8))
+        np.testing.assert_array_equal(c.dv.get().view(np.uint8), c.v.view(np.uint8))
+
+
+def workspace(c):
+    n = qg.lib().qg_kv_workspace_bytes(c.ref)
+    return Device(np.full(n, 0xff, np.uint8)), n
+
+
+def reserve(c, counts):
+    batch, status, (ws, n) = Batch(counts), Device(np.full(c.B, 9, np.int32)), workspace(c)
+    say(f"reserve {counts[:8]}")
+    call("kv_reserve", c.ref, batch.ref, status.p, ws.p, n)
+    return status.get()
+
+
+def fork(c, dst, src):
+    d, s, (ws, n) = Device(np.array(dst, np.int32)), Device(np.array(src, np.int32)), workspace(c)
+    say(f"fork {dst[:8]} from {src[:8]}")
+    call("kv_fork", c.ref, d.p, s.p, len(dst), ws.p, n)
+
+
+def truncate(c, new=None):
+    d = Device(np.array(new, np.int32)) if new is not None else None
+    say(f"truncate {new and new[:8]}")
+    call("kv_truncate", c.ref, d.p if d else None)
+
+
+@pytest.mark.parametrize("typ,page,dim,heads,layers", [(F16, 8, 64, 1, 1), (BF16, 32, 128, 3, 2), (F32, 16, 64, 2, 5), (F16, 256, 256, 1, 1)])
+def test_pages_random_walk(qgl, typ, page, dim, heads, layers):
+    """Forks, reserves, truncations and compactions in random order, with sequences that share pages, run out of pages
+    and outgrow their table."""
+    rng = np.random.default_rng(page + dim)
+    B = 7
+    c = Cache(rng, [5 * page // 2, 3, 0, page, 0, 2 * page + 1, 0], [0] * B, typ=typ, layers=layers, kv_heads=heads, page=page, dim=dim,
+              spare=9, table_pages=6)
+    m = Model(c)
+    for step in range(40):
+        kind = rng.integers(0, 4)
+        if kind == 0:
+            n = int(rng.integers(1, B + 1))
+            dst, src = (rng.integers(-1, B + 1, n).tolist() for _ in range(2))
+            fork(c, dst, src)
+            m.fork(dst, src)
+        elif kind == 1:
+            counts = rng.integers(0, page + 3, B).tolist()
+            counts[int(rng.integers(0, B))] = int(rng.integers(0, 3 * page))
+            if sum(counts):
+                np.testing.assert_array_equal(reserve(c, counts), m.reserve(counts))
+        elif kind == 2:
+            new = rng.integers(-1, 4 * page, B).tolist() if rng.random() < 0.8 else None
+            truncate(c, new)
+            m.truncate(new)
+        else:
+            counts = rng.integers(0, 18, B).tolist()
+            counts[0] = max(counts[0], 1)
+            status = m.reserve(counts)
+            np.testing.assert_array_equal(reserve(c, counts), status)
+            counts = [0 if s else n for s, n in zip(status, counts)]
+            if not sum(counts):
+                continue
+            batch = Batch(counts)
+            path = np.full((B, batch.max_rows), -1, np.int32)
+            count = np.zeros(B, np.int32)
+            for s, n in enumerate(counts):
+                count[s] = rng.integers(0, n + 1)
+                path[s, :count[s]] = np.sort(rng.choice(n, count[s], replace=False)) if n else []
+            dp, dc = Device(path), Device(count)
+            say("compact", count.tolist())
+            call("kv_compact", c.ref, batch.ref, dp.p, dc.p, c.dlength.p)
+            c.length = m.compact(batch, path, count)
+        same(c)
+
+
+def test_compact_all_moves(qgl):
+    """Paths of every shape: identity, far jumps, overlapping moves across pages, faults; the lengths kept apart."""
+    rng = np.random.default_rng(1)
+    for page in (8, 64):
+        counts = [64, 64, 17, 5, 9, 1, 0, 30]
+        c = Cache(rng, [3, 0, 100, 7, 8, 0, 5, 33], counts, typ=BF16, layers=3, kv_heads=2, page=page, dim=64)
+        batch = Batch(counts)
+        for row, s, place in batch.places():
+            for layer in range(3):
+                c.put(layer, s, int(c.length[s]) + place, *rng.standard_normal((2, 2, 64)))
+        if page == 8:  # a hole among the moved rows
+            c.refs[c.table[7, 4]] = 0
+            c.table[7, 4] = -1
+        c.upload()
+        path = np.full((8, 64), -1, np.int32)
+        path[0], path[1, :63] = np.arange(64), np.arange(1, 64)
+        path[2, :4], path[3, :5] = (0, 9, 10, 16), (0, 2, 2, 3, 4)   # the second repeats a row
+        path[4, :3], path[5, 0] = (0, 9, 1), 0                      # and this one leaves its sequence
+        path[6, :2], path[7, :10] = (0, 1), np.arange(10) * 3
+        count = np.array([64, 63, 4, 5, 3, 1, 2, 1000], np.int32)
+        dp, dc, out = Device(path), Device(count), Device(np.zeros(8, np.int32))
+        want = Model(c).compact(batch, path, count)
+        say(f"compact page={page}")
+        call("kv_compact", c.ref, batch.ref, dp.p, dc.p, out.p)
+        np.testing.assert_array_equal(out.get(), want)
+        same(c)
+
+
+def test_copy_pages(qgl):
+    rng = np.random.default_rng(2)
+    c = Cache(rng, [100], [0], typ=F16, layers=4, kv_heads=3, page=16, dim=64, spare=12)
+    for pool in (c.k, c.v):
+        pool[:] = rng.standard_normal(pool.shape)
+    c.upload()
+    dst, src = [9, 10, 11, 9, 3, -1, 12, 200], [1, 2, 1, 4, 5, 1, 200, 1]
+    # 9 comes twice (the last counts); 3 is a source below? it is not: copied; bad indexes are left out
+    dst += [13, 5]
+    src += [6, 7]       # 5 is a source of the pair above, so it is not written
+    for d, s, ok in zip(dst, src, (0, 1, 1, 1, 1, 0, 0, 0, 1, 0)):
+        if ok:
+            c.k[:, d], c.v[:, d] = c.k[:, s], c.v[:, s]
+    dd, ds = Device(np.array(dst, np.int32)), Device(np.array(src, np.int32))
+    say("copy pages")
+    call("kv_copy_pages", c.ref, dd.p, ds.p, len(dst))
+    np.testing.assert_array_equal(c.dk.get().view(np.uint16), c.k.view(np.uint16))
+    np.testing.assert_array_equal(c.dv.get().view(np.uint16), c.v.view(np.uint16))
+
+
+def test_reserve_many_sequences(qgl):
+    """1024 sequences over 40000 pages, some shared, some rows long: the pages come in order."""
+    rng = np.random.default_rng(3)
+    B = 1024
+    lengths = rng.integers(0, 60, B).tolist()
+    c = Cache(rng, lengths, [0] * B, typ=F16, kv_heads=1, page=8, dim=64, spare=30000, table_pages=300, fill=False)
+    c.k[:], c.v[:] = 0, 0
+    c.upload()
+    m = Model(c)
+    dst, src = rng.permutation(B)[:200].tolist(), rng.integers(0, B, 200).tolist()
+    fork(c, dst, src)
+    m.fork(dst, src)
+    counts = rng.integers(0, 20, B).tolist()
+    counts[5], counts[900] = 2000, 2399
+    np.testing.assert_array_equal(reserve(c, counts), m.reserve(counts))
+    same(c, pools=False)
+
+
+def test_reserve_keeps_forks_apart(qgl):
+    """Two sequences of different lengths in one page: neither's tokens change when both are written behind."""
+    rng = np.random.default_rng(4)
+    c = Cache(rng, [14, 0, 0], [0, 0, 0], typ=F32, kv_heads=1, page=16, dim=64, spare=3, table_pages=2)
+    fork(c, [1], [0])
+    truncate(c, [14, 10, 0])
+    m = Model(c)
+    m.fork([1], [0])
+    m.truncate([14, 10, 0])
+    same(c)
+    # only the shorter one is written: it must not lose the other's tokens; then no page is left for both
+    np.testing.assert_array_equal(reserve(c, [0, 2, 0]), m.reserve([0, 2, 0]))
+    same(c)
+    np.testing.assert_array_equal(reserve(c, [16, 20, 16]), m.reserve([16, 20, 16]))
+    same(c)
