@@ -1,63 +1,658 @@
 // Attention of a batch's rows over the paged cache (qg_tree_attention of
 // include/qwen_gpu.h).
+//
+// o = sum_j p_j v_j / sum_j p_j, p_j = exp(scale q.k_j - m), in one pass over the
+// keys with a running m.  A kv head's rows (its group's heads of every row of the
+// batch, in groups of 16 RT) share one read of its keys and values.  Keys are
+// split over workgroups (the number follows from the lengths, on the device),
+// over a workgroup's waves and within a wave into tiles of 32 (16 for F32); the
+// parts are joined in shared memory, and by a second kernel where a sequence has
+// more than one workgroup.
+//
+// A wave needs nothing of the others while it walks: keys and values go from
+// memory to its registers.  Scores are formed transposed, S^T = K Q^T (keys the
+// rows of the product), so that a lane ends with the scores of 8 consecutive
+// keys of one query row, which is what the second product, O^T = V^T P^T, wants
+// of it as an operand; for V^T a lane holds 8 keys x D/16 dimensions as they lie
+// in memory and pairs them with byte permutes.  Neither product moves a value
+// between lanes.
+//
+// Precision: q and p enter as planes that the 16-bit cores multiply exactly with
+// the cache's values: two fp16 planes (22 bits; q scaled by a power of two per
+// row), three bf16 planes (24 bits); an F32 cache uses the fp32 cores.
 #include "qg_kv.h"
 
 namespace {
 
-// One wave per row and head: a lane scores one key of 64 at a time; the output's
-// dimensions lie across the lanes.
-template <int TYPE, int D>
-__global__ __launch_bounds__(64) void attention_row_kernel(float *out, const float *q, int q_heads, float scale, KvView c, int layer, BatchView b) {
-    __shared__ float s_q[D];
-    const int row = blockIdx.x, head = blockIdx.y, lane = threadIdx.x, kv = head / (q_heads / c.heads);
-    int first, n;
-    const int s = batch_sequence(b, c.sequences, row, lane, first, n);
-    if (s < 0) return;
-    const int place = row - first, len = kv_length(c, s);
-    const unsigned long long seen = b.parent ? __shfl(tree_ancestors(b.parent + first, n, lane), place) : 0;
-    const float *qr = q + ((size_t)row * q_heads + head) * D;
-    for (int d = lane; d < D; d += 64) s_q[d] = qr[d] * scale;
-    __syncthreads();
-    float m = -__builtin_inff(), l = 0.0f, o[D / 64];
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+
+constexpr float P_BASE = 6.0f;  // p is held times 2^6: m may lag by 8 below the fp16 range's end
+constexpr float M_LAG = 8.0f;   // a new maximum counts once it is 2^8 above the old
+
+struct AttnArgs {
+    float *out;
+    const float *q;
+    float *part_o;   // [slots][row group][D]
+    float2 *part_ml; // [slots][row group]
+    int *odd;        // [rows][q_heads]: 1 where attention_join_kernel has to take the row up again
+    float scale;     // times log2 e
+    int q_heads, group, layer, target, slots;
+};
+
+// How the work is cut, the same in every wave of both kernels.  Sequence s has
+// `groups` row groups and `keys` keys; its keys are cut into parts of `chunk`,
+// chosen so that about `target` workgroups have work.
+struct Plan {
+    int s, first, n, len, groups, parts, chunk, part, z, h;  // of one unit
+    size_t slot;  // of part 0, row group 0, head 0 of the sequence
+};
+constexpr int CHUNK = 128;  // keys per workgroup, at least and in steps of
+
+// A lane's sequence: its rows, tokens and row groups.
+struct PlanLane { int first, n, len, groups; };
+template <int RG>
+QG_DEV PlanLane plan_lane(const KvView &c, const BatchView &b, const AttnArgs &A, int s) {
+    PlanLane x{0, 0, 0, 0};
+    if (s < c.sequences) {
+        batch_rows(b, s, x.first, x.n);
+        x.len = kv_length(c, s);
+        x.groups = (x.n * A.group + RG - 1) / RG;
+    }
+    return x;
+}
+
+// `mine`: the lane's sequence among the first 64, read once.  `unit` 0.. asks for a
+// unit of this workgroup's XCD, -1 for sequence `want`.  Units run through the
+// sequences (parts x heads x row groups), and an XCD takes a run of them, so that
+// row groups with the same keys meet in its L2.  False if there is no such unit.
+template <int RG>
+QG_DEV bool plan_find(const KvView &c, const BatchView &b, const AttnArgs &A, int lane, int block, int want, Plan &p) {
+    const PlanLane mine = plan_lane<RG>(c, b, A, lane);
+    float total = (float)mine.groups * (float)(mine.len + mine.n);
+    for (int s = lane + 64; s < c.sequences; s += 64) {
+        const PlanLane x = plan_lane<RG>(c, b, A, s);
+        total += (float)x.groups * (float)(x.len + x.n);
+    }
+    total = qg_row_sum(total);
+    total += __shfl_xor(total, 16);
+    total += __shfl_xor(total, 32);
+    // the sum's roundings are covered: A.slots holds what a chunk this long can give
+    const float even = total * (float)c.heads * 1.0001f / (float)A.target;
+    const int chunk = ((int)fminf(even, (float)(1 << 28)) / CHUNK + 1) * CHUNK;
+    auto scan = [&](int s0, PlanLane &x, int &parts, int &upto, int &upto_slots) {
+        x = s0 ? plan_lane<RG>(c, b, A, s0 + lane) : mine;
+        parts = x.n ? (x.len + x.n - 1) / chunk + 1 : 0;
+        upto = parts * x.groups * c.heads;
+        upto_slots = parts > 1 ? upto : 0;
 #pragma unroll
-    for (int i = 0; i < D / 64; i++) o[i] = 0.0f;
+        for (int d = 1; d < 64; d *= 2) {
+            const int u = __shfl_up(upto, d), e = __shfl_up(upto_slots, d);
+            if (lane >= d) { upto += u; upto_slots += e; }
+        }
+    };
+    PlanLane x;
+    int parts, upto, upto_slots, units = 0;
+    if (want < 0) {
+        for (int s0 = 0; s0 < c.sequences; s0 += 64) {
+            scan(s0, x, parts, upto, upto_slots);
+            units += __shfl(upto, 63);
+        }
+        const int per = (units + 7) / 8;
+        if (block >> 3 >= per) return false;
+        want = -1 - ((block & 7) * per + (block >> 3));
+        if (-1 - want >= units) return false;
+    }
+    const int unit = want < 0 ? -1 - want : -1;
+    int before = 0;
+    size_t slots = 0;
+    for (int s0 = 0; s0 < c.sequences; s0 += 64) {
+        if (s0 || unit < 0 || c.sequences > 64) scan(s0, x, parts, upto, upto_slots);
+        const int own = parts * x.groups * c.heads, own_slots = parts > 1 ? own : 0;
+        const unsigned long long here = unit < 0 ? (want >= s0 && want < s0 + 64 ? 1ULL << (want - s0) : 0)
+                                                 : __ballot(unit < before + upto && unit >= before + upto - own);
+        if (here) {
+            const int l = __builtin_ctzll(here);
+            p.s = s0 + l;
+            p.first = __shfl(x.first, l);
+            p.n = __shfl(x.n, l);
+            p.len = __shfl(x.len, l);
+            p.groups = __shfl(x.groups, l);
+            p.parts = __shfl(parts, l);
+            p.slot = slots + __shfl(upto_slots - own_slots, l);
+            if (unit >= 0) {
+                const int rest = unit - (before + __shfl(upto - own, l));
+                p.part = rest / (p.groups * c.heads);
+                p.h = rest / p.groups % c.heads;
+                p.z = rest % p.groups;
+            }
+            p.chunk = chunk;
+            return true;
+        }
+        before += __shfl(upto, 63);
+        slots += __shfl(upto_slots, 63);
+    }
+    return false;
+}
+
+// v_perm of two words into (a.lo, b.lo) or (a.hi, b.hi)
+QG_DEV uint32_t pair_lo(uint32_t a, uint32_t b) { return __builtin_amdgcn_perm(b, a, 0x05040100u); }
+QG_DEV uint32_t pair_hi(uint32_t a, uint32_t b) { return __builtin_amdgcn_perm(b, a, 0x07060302u); }
+
+// Eight floats as the planes of an operand: their sum is the value (bf16, exactly) or
+// within 2^-22 of it (fp16).
+template <int TYPE> struct Planes;
+template <> struct Planes<QT_F16> {
+    static constexpr int N = 2;
+    uint4 p[2];
+    __device__ __forceinline__ explicit Planes(const float (&x)[8]) {
+        uint32_t hi[4], lo[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            hi[i] = cvt2(x[2 * i], x[2 * i + 1]);
+            const qg_half2 h = __builtin_bit_cast(qg_half2, hi[i]);
+            lo[i] = cvt2(__builtin_fmaf((float)h[0], -1.0f, x[2 * i]), __builtin_fmaf((float)h[1], -1.0f, x[2 * i + 1]));
+        }
+        p[0] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+        p[1] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+    }
+    static __device__ __forceinline__ uint32_t cvt2(float a, float b) { return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(a, b)); }
+    static __device__ __forceinline__ qg_f4 mul(uint4 a, uint4 b, qg_f4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(qg_half8, a), __builtin_bit_cast(qg_half8, b), c, 0, 0, 0);
+    }
+};
+template <> struct Planes<QT_BF16> {
+    static constexpr int N = 3;
+    uint4 p[3];
+    __device__ __forceinline__ explicit Planes(const float (&x)[8]) {
+        uint32_t w[3][4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            float a = x[2 * i], b = x[2 * i + 1];
+#pragma unroll
+            for (int k = 0; k < 3; k++) {
+                const uint32_t ua = __float_as_uint(a), ub = __float_as_uint(b);
+                w[k][i] = pair_hi(ua, ub);
+                a -= __uint_as_float(ua & 0xffff0000u);
+                b -= __uint_as_float(ub & 0xffff0000u);
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < 3; k++) p[k] = make_uint4(w[k][0], w[k][1], w[k][2], w[k][3]);
+    }
+    static __device__ __forceinline__ qg_f4 mul(uint4 a, uint4 b, qg_f4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    }
+};
+
+// A tile's keys and values in a wave's registers and their products, by the cache's
+// type.  Lane l: n = l % 16, g = l / 16.  KEYS keys per tile, E of them (E g .. E g +
+// E - 1) in a lane's scores and values; DL = D/16 dimensions (DL n ..) in its values.
+template <int TYPE, int D>
+struct Tile {
+    static constexpr int KEYS = 32, E = 8, DL = D / 16, S = D / 32, PL = Planes<TYPE>::N, ES = 2;
+    uint4 k[2][S];
+    uint32_t v[8][DL / 2];
+    // the key (of the tile) whose row a lane loads as the first operand's row n of sub-tile j
+    static __device__ __forceinline__ int key_of(int n, int j) { return 8 * (n >> 2) + (n & 3) + 4 * j; }
+    // at: byte offset of key 8 (n / 4)'s row; the next keys follow
+    __device__ __forceinline__ void load_k(const uint8_t *at, int n, int g) {
+#pragma unroll
+        for (int j = 0; j < 2; j++)
+#pragma unroll
+            for (int s = 0; s < S; s++) k[j][s] = *(const uint4 *)(at + ((n & 3) + 4 * j) * (D * 2) + s * 64 + g * 16);
+    }
+    __device__ __forceinline__ void load_v(const uint8_t *at, int n) {
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            const uint8_t *p = at + e * (D * 2) + n * (DL * 2);
+            if constexpr (DL == 4) {
+                const uint2 x = *(const uint2 *)p;
+                v[e][0] = x.x; v[e][1] = x.y;
+            } else {
+#pragma unroll
+                for (int w = 0; w < DL / 8; w++) {
+                    const uint4 x = *(const uint4 *)(p + 16 * w);
+                    v[e][4 * w] = x.x; v[e][4 * w + 1] = x.y; v[e][4 * w + 2] = x.z; v[e][4 * w + 3] = x.w;
+                }
+            }
+        }
+    }
+    __device__ __forceinline__ void drop_v(int e) {
+#pragma unroll
+        for (int w = 0; w < DL / 2; w++) v[e][w] = 0;
+    }
+    // q fragments: [s][plane][lane] of 16 bytes
+    static constexpr int Q_BYTES = S * PL * 1024;
+    static __device__ __forceinline__ void put_q(uint8_t *frag, int n, int d0, const float (&x)[8], int first) {
+        const Planes<TYPE> p(x);
+#pragma unroll
+        for (int k = 0; k < PL; k++) {
+            uint8_t *to = frag + (((d0 >> 5) * PL + k) * 64 + ((d0 >> 3) & 3) * 16 + n) * 16;
+            if constexpr (DL == 4) *(uint2 *)(to + (d0 & 4) * 2) = make_uint2(p.p[k].x, p.p[k].y);
+            else *(uint4 *)to = p.p[k];
+        }
+    }
+    __device__ __forceinline__ void scores(const uint8_t *frag, int lane, float (&z)[8]) const {
+        qg_f4 a[2] = {};
+#pragma unroll
+        for (int s = 0; s < S; s++)
+#pragma unroll
+            for (int p = 0; p < PL; p++) {
+                const uint4 q = *(const uint4 *)(frag + ((s * PL + p) * 64 + lane) * 16);
+#pragma unroll
+                for (int j = 0; j < 2; j++) a[j] = Planes<TYPE>::mul(k[j][s], q, a[j]);
+            }
+#pragma unroll
+        for (int i = 0; i < 4; i++) { z[i] = a[0][i]; z[4 + i] = a[1][i]; }
+    }
+    template <int RT>
+    __device__ __forceinline__ void outputs(const float (&p)[RT][8], qg_f4 (&o)[RT][DL]) const {
+        uint4 w[RT][PL];
+#pragma unroll
+        for (int r = 0; r < RT; r++) {
+            const Planes<TYPE> x(p[r]);
+#pragma unroll
+            for (int k = 0; k < PL; k++) w[r][k] = x.p[k];
+        }
+#pragma unroll
+        for (int t = 0; t < DL; t++) {
+            uint32_t u[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) u[i] = t & 1 ? pair_hi(v[2 * i][t / 2], v[2 * i + 1][t / 2]) : pair_lo(v[2 * i][t / 2], v[2 * i + 1][t / 2]);
+            const uint4 a = make_uint4(u[0], u[1], u[2], u[3]);
+#pragma unroll
+            for (int r = 0; r < RT; r++)
+#pragma unroll
+                for (int k = 0; k < PL; k++) o[r][t] = Planes<TYPE>::mul(a, w[r][k], o[r][t]);
+        }
+    }
+};
+template <int D>
+struct Tile<QT_F32, D> {
+    static constexpr int KEYS = 16, E = 4, DL = D / 16, S = D / 16, ES = 4;
+    float4 k[S];
+    float v[4][DL];
+    __device__ __forceinline__ void load_k(const uint8_t *at, int n, int g) {
+#pragma unroll
+        for (int s = 0; s < S; s++) k[s] = *(const float4 *)(at + (n & 3) * (D * 4) + s * 64 + g * 16);
+    }
+    __device__ __forceinline__ void load_v(const uint8_t *at, int n) {
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+#pragma unroll
+            for (int w = 0; w < DL / 4; w++) {
+                const float4 x = *(const float4 *)(at + e * (D * 4) + n * (DL * 4) + 16 * w);
+                v[e][4 * w] = x.x; v[e][4 * w + 1] = x.y; v[e][4 * w + 2] = x.z; v[e][4 * w + 3] = x.w;
+            }
+    }
+    __device__ __forceinline__ void drop_v(int e) {
+#pragma unroll
+        for (int w = 0; w < DL; w++) v[e][w] = 0.0f;
+    }
+    static constexpr int Q_BYTES = S * 1024;
+    static __device__ __forceinline__ void put_q(uint8_t *frag, int n, int d0, const float (&x)[8], int count) {
+#pragma unroll
+        for (int i = 0; i < 8; i += 4)
+            if (i < count) {
+                const int d = d0 + i;
+                *(float4 *)(frag + ((d >> 4) * 64 + ((d >> 2) & 3) * 16 + n) * 16) = make_float4(x[i], x[i + 1], x[i + 2], x[i + 3]);
+            }
+    }
+    __device__ __forceinline__ void scores(const uint8_t *frag, int lane, float (&z)[4]) const {
+        qg_f4 a = {};
+#pragma unroll
+        for (int s = 0; s < S; s++) {
+            const float4 q = *(const float4 *)(frag + (s * 64 + lane) * 16);
+            a = __builtin_amdgcn_mfma_f32_16x16x4f32(k[s].x, q.x, a, 0, 0, 0);
+            a = __builtin_amdgcn_mfma_f32_16x16x4f32(k[s].y, q.y, a, 0, 0, 0);
+            a = __builtin_amdgcn_mfma_f32_16x16x4f32(k[s].z, q.z, a, 0, 0, 0);
+            a = __builtin_amdgcn_mfma_f32_16x16x4f32(k[s].w, q.w, a, 0, 0, 0);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; i++) z[i] = a[i];
+    }
+    template <int RT>
+    __device__ __forceinline__ void outputs(const float (&p)[RT][4], qg_f4 (&o)[RT][DL]) const {
+#pragma unroll
+        for (int t = 0; t < DL; t++)
+#pragma unroll
+            for (int r = 0; r < RT; r++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) o[r][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[e][t], p[r][e], o[r][t], 0, 0, 0);
+    }
+};
+
+// Sums that are no numbers under a weight that is one.  The planes' products make
+// NaN of an infinite value (0 x inf, inf - inf), and a value that is no number
+// reaches the rows of its tile that do not see it (0 x NaN); such rows are taken
+// up again, key by key.
+QG_DEV bool odd_sums(float a, float b, float weight) { return !__builtin_isfinite(a + b) && __builtin_isfinite(weight); }
+
+QG_DEV unsigned first_bits(int n, int most) { return (1u << min(max(n, 0), most)) - 1u; }
+
+template <int TYPE, int D, int RT, int NW>
+__global__ __launch_bounds__(64 * NW) void attention_kernel(AttnArgs A, KvView c, BatchView b) {
+    typedef Tile<TYPE, D> T;
+    constexpr int RG = 16 * RT, E = T::E, DL = T::DL, KEYS = T::KEYS, JOIN = NW * 16 * (D + 4) * 4;
+    __shared__ __attribute__((aligned(16))) uint8_t s_mem[RT * T::Q_BYTES > JOIN ? RT * T::Q_BYTES : JOIN];
+    __shared__ float s_m[NW][RG], s_l[NW][RG], s_back[RG];
+    __shared__ unsigned long long s_seen[QG_MAX_TREE];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = lane & 15, g = lane >> 4;
+    Plan p;
+    if (!plan_find<RG>(c, b, A, lane, blockIdx.x, -1, p)) return;
+    const int row0 = p.z * RG, rows = p.n * A.group;  // this group's first row, all rows of the head
+
+    // this unit's keys, and the first one that some row of the group may not see
+    const int last_t = min(row0 + RG - 1, rows - 1) / A.group, begin = p.part * p.chunk;
+    const int end = min(begin + p.chunk, p.len + (b.parent ? p.n : last_t + 1)), open = p.len + (b.parent ? 0 : row0 / A.group + 1);
+    const size_t page_bytes = ((size_t)c.heads << c.shift) * D * T::ES;
+    const uint8_t *kbase = c.k + (((size_t)A.layer * c.pages * c.heads + p.h) << c.shift) * D * T::ES;
+    const uint8_t *vbase = c.v + (((size_t)A.layer * c.pages * c.heads + p.h) << c.shift) * D * T::ES;
+    const int slot_mask = (1 << c.shift) - 1;
+    // a run of E keys from position pos, aligned to E: inside one page
+    auto run = [&](const uint8_t *base, int page, int pos) { return base + (size_t)max(page, 0) * page_bytes + (size_t)((pos & slot_mask) * (D * T::ES)); };
+    // the first tile's keys and values, and the second's pages, are on their way while the queries are laid out
+    T tile;
+    int t0 = begin + wave * KEYS, kpos = t0 + E * (n >> 2), vpos = t0 + E * g;
+    int kpage = kv_page(c, p.s, kpos), vpage = kv_page(c, p.s, vpos);
+    int kpage1 = kv_page(c, p.s, kpos + NW * KEYS), vpage1 = kv_page(c, p.s, vpos + NW * KEYS);
+    if (t0 < end) {
+        tile.load_k(run(kbase, kpage, kpos), n, g);
+        tile.load_v(run(vbase, vpage, vpos), n);
+    }
+
+    // the rows' queries, in planes and in the order of the products' operand; the
+    // power of two that a row was scaled by (fp16 planes) comes off the scores
+    for (int r0 = wave * 4; r0 < RG; r0 += NW * 4) {
+        const int r = r0 + g, at = row0 + r;
+        const bool live = at < rows;
+        const float *src = A.q + ((size_t)(p.first + at / A.group) * A.q_heads + p.h * A.group + at % A.group) * D + n * DL;
+        float x[DL];
+#pragma unroll
+        for (int i = 0; i < DL; i += 4) {
+            const float4 y = live ? *(const float4 *)(src + i) : make_float4(0, 0, 0, 0);
+            x[i] = y.x * A.scale; x[i + 1] = y.y * A.scale; x[i + 2] = y.z * A.scale; x[i + 3] = y.w * A.scale;
+        }
+        float back = 1.0f;
+        if constexpr (TYPE == QT_F16) {
+            float top = 0.0f;
+#pragma unroll
+            for (int i = 0; i < DL; i++) top = fmaxf(top, fabsf(x[i]));
+            top = qg_row_max(top);
+            // 2^e with top 2^e in [2^13, 2^14): fp16's whole precision for what matters of the row
+            const int e = min(max(127 + 13 - (int)(__float_as_uint(top) >> 23) + 0, -126), 126);
+            if (top > 0.0f && top < __builtin_inff()) {
+                const float f = __uint_as_float((uint32_t)(e + 127) << 23);
+                back = __uint_as_float((uint32_t)(127 - e) << 23);
+#pragma unroll
+                for (int i = 0; i < DL; i++) x[i] *= f;
+            }
+        }
+        if (n == 0) s_back[r] = back;
+        if (n == 0 && live && p.parts == 1) A.odd[(size_t)(p.first + at / A.group) * A.q_heads + p.h * A.group + at % A.group] = 0;
+        uint8_t *frag = s_mem + (r >> 4) * T::Q_BYTES;
+#pragma unroll
+        for (int i = 0; i < DL; i += 8) {
+            float y[8];
+#pragma unroll
+            for (int j = 0; j < 8; j++) y[j] = i + j < DL ? x[(i + j) % DL] : 0.0f;
+            T::put_q(frag, r & 15, n * DL + i, y, DL - i);
+        }
+    }
+    if (b.parent && wave == 0) s_seen[lane] = tree_ancestors(b.parent + p.first, p.n, lane);
+    __syncthreads();
+
+    qg_f4 o[RT][DL];
+    float m[RT], l[RT], back[RT];
+#pragma unroll
+    for (int r = 0; r < RT; r++) back[r] = TYPE == QT_F16 ? s_back[16 * r + n] : 1.0f;
+#pragma unroll
+    for (int r = 0; r < RT; r++) {
+        m[r] = -__builtin_inff();
+        l[r] = 0.0f;
+#pragma unroll
+        for (int t = 0; t < DL; t++) o[r][t] = qg_f4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+    for (; t0 < end; t0 += NW * KEYS) {
+        float z[RT][E];
+#pragma unroll
+        for (int r = 0; r < RT; r++) {
+            tile.scores(s_mem + r * T::Q_BYTES, lane, z[r]);
+            __builtin_amdgcn_sched_barrier(0);  // one row tile's queries in registers at a time
+        }
+        // the next tile's keys, whose pages are known, and the pages of the one after it
+        const int here = vpage, here_pos = vpos;
+        const bool more = t0 + NW * KEYS < end;
+        kpos += NW * KEYS;
+        vpos += NW * KEYS;
+        vpage = vpage1;
+        if (more) {
+            tile.load_k(run(kbase, kpage1, kpos), n, g);
+            kpage1 = kv_page(c, p.s, kpos + NW * KEYS);
+            vpage1 = kv_page(c, p.s, vpos + NW * KEYS);
+        }
+        unsigned vis[RT];
+#pragma unroll
+        for (int r = 0; r < RT; r++) vis[r] = (1u << E) - 1;
+        if (t0 + KEYS > open || !__all(here >= 0)) {
+#pragma unroll
+            for (int e = 0; e < E; e++)
+                if (here < 0 || here_pos + e >= end) tile.drop_v(e);
+#pragma unroll
+            for (int r = 0; r < RT; r++) {
+                // bit e: key here_pos + e, below the row's prefix or among the rows that it descends from
+                const int t = (row0 + 16 * r + n) / A.group, prefix = b.parent ? p.len : p.len + t + 1, k = here_pos - p.len;
+                unsigned seen = first_bits(prefix - here_pos, E);
+                if (b.parent && t < p.n && k < 64 && k > -E) seen |= (unsigned)(k < 0 ? s_seen[t] << -k : s_seen[t] >> k);
+                vis[r] = here < 0 ? 0 : seen & first_bits(end - here_pos, E);
+            }
+        }
+        // scores to weights: the maximum is renewed only where it moves by more than M_LAG
+#pragma unroll
+        for (int r = 0; r < RT; r++) {
+            float top = -__builtin_inff();
+#pragma unroll
+            for (int e = 0; e < E; e++) {
+                z[r][e] = vis[r] >> e & 1 ? z[r][e] * back[r] : -__builtin_inff();
+                top = fmaxf(top, z[r][e]);
+            }
+            if (__any(top > m[r] + M_LAG)) {
+                top = fmaxf(top, __shfl_xor(top, 16));
+                top = fmaxf(top, __shfl_xor(top, 32));
+                const float next = fmaxf(m[r], top);
+                const float a = next == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f(m[r] - next);
+                m[r] = next;
+                l[r] *= a;
+#pragma unroll
+                for (int t = 0; t < DL; t++) o[r][t] *= a;
+            }
+            const float base = m[r] == -__builtin_inff() ? 0.0f : m[r] - P_BASE;
+#pragma unroll
+            for (int e = 0; e < E; e++) {
+                z[r][e] = __builtin_amdgcn_exp2f(z[r][e] - base);
+                l[r] += z[r][e];
+            }
+        }
+        tile.template outputs<RT>(z, o);
+        if (more) tile.load_v(run(vbase, vpage, vpos), n);
+    }
+
+    // the waves' parts are joined row tile by row tile
+#pragma unroll
+    for (int r = 0; r < RT; r++) {
+        l[r] += __shfl_xor(l[r], 16);
+        l[r] += __shfl_xor(l[r], 32);
+        if (g == 0) { s_m[wave][16 * r + n] = m[r]; s_l[wave][16 * r + n] = l[r]; }
+    }
+    __syncthreads();  // the queries' fragments are done with
+    float *join = (float *)s_mem;
+#pragma unroll
+    for (int r = 0; r < RT; r++) {
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+#pragma unroll
+            for (int t = 0; t < DL; t += 4)
+                *(float4 *)(join + (wave * 16 + n) * (D + 4) + DL * (4 * g + i) + t) =
+                    make_float4(o[r][t][i], o[r][t + 1][i], o[r][t + 2][i], o[r][t + 3][i]);
+        __syncthreads();
+        for (int x = tid; x < 16 * D / 4; x += 64 * NW) {
+            const int row = x / (D / 4), d = x % (D / 4) * 4, at = row0 + 16 * r + row;
+            if (at >= rows) continue;
+            float top = -__builtin_inff(), sum = 0.0f;
+#pragma unroll
+            for (int w = 0; w < NW; w++) top = fmaxf(top, s_m[w][16 * r + row]);
+            float4 y = make_float4(0, 0, 0, 0);
+#pragma unroll
+            for (int w = 0; w < NW; w++) {
+                const float mw = s_m[w][16 * r + row];
+                if (mw == -__builtin_inff() && s_l[w][16 * r + row] == 0.0f) continue;
+                const float f = mw == top ? 1.0f : __builtin_amdgcn_exp2f(mw - top);
+                const float4 u = *(const float4 *)(join + (w * 16 + row) * (D + 4) + d);
+                sum = __builtin_fmaf(f, s_l[w][16 * r + row], sum);
+                y.x = __builtin_fmaf(f, u.x, y.x);
+                y.y = __builtin_fmaf(f, u.y, y.y);
+                y.z = __builtin_fmaf(f, u.z, y.z);
+                y.w = __builtin_fmaf(f, u.w, y.w);
+            }
+            if (p.parts == 1) {
+                const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+                const size_t to = (size_t)(p.first + at / A.group) * A.q_heads + p.h * A.group + at % A.group;
+                *(float4 *)(A.out + to * D + d) = make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv);
+                if (odd_sums(y.x, y.y, sum) || odd_sums(y.z, y.w, sum)) A.odd[to] = 1;
+            } else {
+                const size_t slot = p.slot + ((size_t)p.part * c.heads + p.h) * p.groups + p.z;
+                if (slot < (size_t)A.slots) {
+                    *(float4 *)(A.part_o + (slot * RG + 16 * r + row) * D + d) = y;
+                    if (d == 0) A.part_ml[slot * RG + 16 * r + row] = make_float2(top, sum);
+                }
+            }
+        }
+        __syncthreads();
+    }
+}
+
+// One row and head, key by key: a lane scores one of 64 keys at a time, the
+// output's dimensions lie across the lanes.
+template <int TYPE, int D>
+QG_DEV void attend_row(const AttnArgs &A, const KvView &c, const BatchView &b, int s, int first, int n, int row, int head, int lane, float *s_q) {
+    constexpr int V = D / 64;
+    const int place = row - first, len = kv_length(c, s), kv = head / A.group;
+    const unsigned long long seen = b.parent ? __shfl(tree_ancestors(b.parent + first, n, lane), place) : 0;
+    const float *q = A.q + ((size_t)row * A.q_heads + head) * D;
+    for (int d = lane; d < D; d += 64) s_q[d] = q[d] * A.scale;
+    __syncthreads();
+    float m = -__builtin_inff(), l = 0.0f, o[V];
+#pragma unroll
+    for (int i = 0; i < V; i++) o[i] = 0.0f;
     const int end = len + (b.parent ? n : place + 1);
     for (int t0 = 0; t0 < end; t0 += 64) {
         const int t = t0 + lane, page = t < end ? kv_page(c, s, t) : -1;
         const bool visible = page >= 0 && (t < len || !b.parent || (seen >> (t - len) & 1));
-        float sc = -__builtin_inff();
-        const size_t at = kv_at(c, layer, max(page, 0), kv, t & ((1 << c.shift) - 1));
+        const size_t at = kv_at(c, A.layer, max(page, 0), kv, t & ((1 << c.shift) - 1));
+        float z = -__builtin_inff();
         if (visible) {
-            sc = 0.0f;
-            for (int d = 0; d < D; d++) sc = __builtin_fmaf(s_q[d], kv_load<TYPE>(c.k, at + d), sc);
+            z = 0.0f;
+            for (int d = 0; d < D; d++) z = __builtin_fmaf(s_q[d], kv_load<TYPE>(c.k, at + d), z);
         }
-        float top = m;
-        for (int i = 0; i < 64; i++) { const float x = __shfl(sc, i); top = x != x || x > top ? x : top; }
-        if (top == -__builtin_inff()) continue;
-        const float a = expf(m - top), pr = visible ? expf(sc - top) : 0.0f;
+        const float top = fmaxf(m, qg_wave_max(z));
+        const float a = top == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f(m - top);
+        const float p = visible ? __builtin_amdgcn_exp2f(z - (top == -__builtin_inff() ? 0.0f : top)) : 0.0f;
         m = top;
-        l = l * a + qg_sum_lanes<64>(pr);
+        l = l * a + qg_sum_lanes<64>(p);
 #pragma unroll
-        for (int i = 0; i < D / 64; i++) o[i] *= a;
+        for (int i = 0; i < V; i++) o[i] *= a;
         for (unsigned long long left = __ballot(visible); left; left &= left - 1) {
             const int k = __builtin_ctzll(left);
-            const float w = __shfl(pr, k);
-            const size_t vat = __shfl((unsigned long long)at, k);
+            const float w = __shfl(p, k);
+            const size_t v = __shfl((unsigned long long)at, k);
 #pragma unroll
-            for (int i = 0; i < D / 64; i++) o[i] = __builtin_fmaf(w, kv_load<TYPE>(c.v, vat + lane + 64 * i), o[i]);
+            for (int i = 0; i < V; i++) o[i] = __builtin_fmaf(w, kv_load<TYPE>(c.v, v + lane * V + i), o[i]);
         }
     }
 #pragma unroll
-    for (int i = 0; i < D / 64; i++) out[((size_t)row * q_heads + head) * D + lane + 64 * i] = l == 0.0f ? 0.0f : o[i] / l;
+    for (int i = 0; i < V; i++) A.out[((size_t)row * A.q_heads + head) * D + lane * V + i] = l == 0.0f ? 0.0f : o[i] / l;
 }
 
-template <int TYPE>
-void launch_rows(float *out, const float *q, int q_heads, float scale, const KvView &c, int layer, const BatchView &b, hipStream_t s) {
-    const dim3 grid(b.rows, q_heads);
-    if (c.dim == 64) attention_row_kernel<TYPE, 64><<<grid, 64, 0, s>>>(out, q, q_heads, scale, c, layer, b);
-    else if (c.dim == 128) attention_row_kernel<TYPE, 128><<<grid, 64, 0, s>>>(out, q, q_heads, scale, c, layer, b);
-    else attention_row_kernel<TYPE, 256><<<grid, 64, 0, s>>>(out, q, q_heads, scale, c, layer, b);
+// A wave per row and head: joins the parts of sequences that were cut, and takes
+// up odd rows again.
+template <int TYPE, int D, int RG>
+__global__ __launch_bounds__(64) void attention_join_kernel(AttnArgs A, KvView c, BatchView b) {
+    constexpr int V = D / 64;
+    __shared__ float s_q[D];
+    const int row = blockIdx.x, head = blockIdx.y, lane = threadIdx.x;
+    int first, n;
+    const int s = batch_sequence(b, c.sequences, row, lane, first, n);
+    if (s < 0) return;
+    Plan p;
+    if (!plan_find<RG>(c, b, A, lane, 0, s, p)) return;
+    if (p.parts < 2) {
+        if (A.odd[(size_t)row * A.q_heads + head]) attend_row<TYPE, D>(A, c, b, s, first, n, row, head, lane, s_q);
+        return;
+    }
+    const int h = head / A.group, at = (row - first) * A.group + head % A.group;
+    const size_t step = (size_t)c.heads * p.groups, slot0 = p.slot + (size_t)h * p.groups + at / RG;
+    if (slot0 + (p.parts - 1) * step >= (size_t)A.slots) return;
+    const float2 *ml = A.part_ml + slot0 * RG + at % RG;
+    float top = -__builtin_inff();
+    for (int i = lane; i < p.parts; i += 64) top = fmaxf(top, ml[i * step * RG].x);
+    top = qg_wave_max(top);
+    float sum = 0.0f, y[V];
+#pragma unroll
+    for (int v = 0; v < V; v++) y[v] = 0.0f;
+    const float *po = A.part_o + (slot0 * RG + at % RG) * D + lane * V;
+#pragma unroll 4
+    for (int i = 0; i < p.parts; i++) {
+        const float2 x = ml[i * step * RG];
+        if (x.x == -__builtin_inff() && x.y == 0.0f) continue;
+        const float f = x.x == top ? 1.0f : __builtin_amdgcn_exp2f(x.x - top);
+        sum = __builtin_fmaf(f, x.y, sum);
+#pragma unroll
+        for (int v = 0; v < V; v++) y[v] = __builtin_fmaf(f, po[i * step * RG * D + v], y[v]);
+    }
+    bool odd = false;
+#pragma unroll
+    for (int v = 0; v < V; v++) odd |= odd_sums(y[v], 0.0f, sum);
+    if (__any(odd)) {
+        attend_row<TYPE, D>(A, c, b, s, first, n, row, head, lane, s_q);
+        return;
+    }
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+#pragma unroll
+    for (int v = 0; v < V; v++) A.out[((size_t)row * A.q_heads + head) * D + lane * V + v] = y[v] * inv;
 }
+
+// Row tiles per wave: as few row groups as the registers allow, and no more tiles than those need.
+int row_tiles(int dim, long rows) {
+    const long most = dim == 256 ? 2 : 4, groups = (rows + 16 * most - 1) / (16 * most);
+    return (int)((rows + 16 * groups - 1) / (16 * groups));
+}
+constexpr int WAVES = 4;
+
+template <int TYPE, int D, int RT>
+void launch(const AttnArgs &A, const KvView &c, const BatchView &b, hipStream_t s) {
+    const long groups = (long)b.rows * A.group / (16 * RT) + c.sequences;  // of all sequences: each rounds up
+    const long units = A.target + groups * c.heads + 8;
+    attention_kernel<TYPE, D, RT, WAVES><<<(unsigned)((units + 7) / 8 * 8), 64 * WAVES, 0, s>>>(A, c, b);
+    attention_join_kernel<TYPE, D, 16 * RT><<<dim3(b.rows, A.q_heads), 64, 0, s>>>(A, c, b);
+}
+template <int TYPE, int D>
+void launch_rt(int rt, const AttnArgs &A, const KvView &c, const BatchView &b, hipStream_t s) {
+    if (rt == 1) launch<TYPE, D, 1>(A, c, b, s);
+    else if (rt == 2) launch<TYPE, D, 2>(A, c, b, s);
+    else if constexpr (D != 256) rt == 3 ? launch<TYPE, D, 3>(A, c, b, s) : launch<TYPE, D, 4>(A, c, b, s);
+}
+template <int TYPE>
+void launch_dim(int rt, const AttnArgs &A, const KvView &c, const BatchView &b, hipStream_t s) {
+    if (c.dim == 64) launch_rt<TYPE, 64>(rt, A, c, b, s);
+    else if (c.dim == 128) launch_rt<TYPE, 128>(rt, A, c, b, s);
+    else launch_rt<TYPE, 256>(rt, A, c, b, s);
+}
+
+// Workgroups that the plan aims at, and the partial results that can come of it:
+// a cut sequence has fewer parts than twice its keys / chunk, and the chunk is at
+// least all sequences' keys x row groups x heads / target.
+constexpr int TARGET = 512;
+constexpr size_t SLOTS = 2 * TARGET;
 }  // namespace
 
 extern "C" {
@@ -65,7 +660,9 @@ extern "C" {
 size_t qg_tree_attention_workspace_bytes(const qg_kv_cache *cache, const qg_kv_batch *batch, int q_heads) {
     if (qg_kv_check(cache, false, nullptr) || qg_batch_check(batch, false, nullptr)) return 0;
     if (q_heads < 1 || q_heads % cache->kv_heads || q_heads / cache->kv_heads > 128) return 0;
-    return 16;
+    const int group = q_heads / cache->kv_heads;
+    const int rg = 16 * row_tiles(cache->head_dim, (long)batch->max_rows * group);
+    return SLOTS * rg * (4 * (size_t)cache->head_dim + sizeof(float2)) + 4 * (size_t)batch->rows * q_heads;
 }
 
 int qg_tree_attention(float *out, const float *q, int q_heads, float scale, const qg_kv_cache *cache, int layer,
@@ -78,9 +675,13 @@ int qg_tree_attention(float *out, const float *q, int q_heads, float scale, cons
     if (layer < 0 || layer >= c.layers || !__builtin_isfinite(scale)) return hipErrorInvalidValue;
     const size_t bytes = 4 * (size_t)b.rows * q_heads * c.dim;
     if (qg_overlap(out, bytes, q, bytes) || qg_overlap(ws, need, q, bytes) || qg_overlap(ws, need, out, bytes)) return hipErrorInvalidValue;
-    if (c.type == QT_F32) launch_rows<QT_F32>(out, q, q_heads, scale, c, layer, b, qg_stream());
-    else if (c.type == QT_F16) launch_rows<QT_F16>(out, q, q_heads, scale, c, layer, b, qg_stream());
-    else launch_rows<QT_BF16>(out, q, q_heads, scale, c, layer, b, qg_stream());
+    const int group = q_heads / c.heads, rt = row_tiles(c.dim, (long)b.max_rows * group);
+    float *part_o = (float *)ws;
+    float2 *part_ml = (float2 *)(part_o + SLOTS * 16 * rt * c.dim);
+    const AttnArgs A{out, q, part_o, part_ml, (int *)(part_ml + SLOTS * 16 * rt), scale * 1.44269504088896341f, q_heads, group, layer, TARGET, (int)SLOTS};
+    if (c.type == QT_F32) launch_dim<QT_F32>(rt, A, c, b, qg_stream());
+    else if (c.type == QT_F16) launch_dim<QT_F16>(rt, A, c, b, qg_stream());
+    else launch_dim<QT_BF16>(rt, A, c, b, qg_stream());
     return hipGetLastError();
 }
 
