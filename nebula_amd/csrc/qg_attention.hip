@@ -36,12 +36,12 @@ struct AttnArgs {
     float2 *part_ml; // [slots][row group]
     int *odd;        // [rows][q_heads]: 1 where attention_join_kernel has to take the row up again
     float scale;     // times log2 e
-    int q_heads, group, layer, target, slots;
+    int q_heads, group, layer, resident, slots;  // resident: workgroups that run at once
 };
 
 // How the work is cut, the same in every wave of both kernels.  Sequence s has
 // `groups` row groups and `keys` keys; its keys are cut into parts of `chunk`,
-// chosen so that about `target` workgroups have work.
+// chosen so that about as many workgroups have work as run at once.
 struct Plan {
     int s, first, n, len, groups, parts, chunk, part, z, h;  // of one unit
     size_t slot;  // of part 0, row group 0, head 0 of the sequence
@@ -68,17 +68,29 @@ QG_DEV PlanLane plan_lane(const KvView &c, const BatchView &b, const AttnArgs &A
 template <int RG>
 QG_DEV bool plan_find(const KvView &c, const BatchView &b, const AttnArgs &A, int lane, int block, int want, Plan &p) {
     const PlanLane mine = plan_lane<RG>(c, b, A, lane);
-    float total = (float)mine.groups * (float)(mine.len + mine.n);
-    for (int s = lane + 64; s < c.sequences; s += 64) {
-        const PlanLane x = plan_lane<RG>(c, b, A, s);
-        total += (float)x.groups * (float)(x.len + x.n);
+    // a sum over all sequences of what `f` says of each
+    auto over = [&](auto f) {
+        float v = f(mine);
+        for (int s = lane + 64; s < c.sequences; s += 64) v += f(plan_lane<RG>(c, b, A, s));
+        v = qg_row_sum(v);
+        float x = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 64; i += 16) x += __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), i));
+        return x * (float)c.heads;
+    };
+    // One round of resident workgroups, each with one unit: a second round for a few
+    // units would cost as much as the first.  Where the row groups alone fill half
+    // the card, two rounds' worth of shorter units instead.
+    const float least = over([](const PlanLane &x) { return (float)x.groups; });
+    const float room = 2.0f * least > (float)A.resident ? 2.0f * (float)A.resident : (float)A.resident;
+    // 1.0001: above the sum whatever its roundings, so that the slots suffice
+    const float even = 1.0001f * over([](const PlanLane &x) { return (float)x.groups * (float)(x.len + x.n); }) / room;
+    int chunk = ((int)fminf(even, (float)(1 << 28)) / CHUNK + 1) * CHUNK;
+    for (int i = 0; i < 4; i++) {  // the parts round up: longer ones until they fit
+        const float units = over([&](const PlanLane &x) { return x.n ? (float)(((x.len + x.n - 1) / chunk + 1) * x.groups) : 0.0f; });
+        if (units <= room || least >= room) break;
+        chunk = max((int)fminf((float)chunk * units / room, (float)(1 << 28)) / CHUNK, chunk / CHUNK) * CHUNK + CHUNK;
     }
-    total = qg_row_sum(total);
-    total += __shfl_xor(total, 16);
-    total += __shfl_xor(total, 32);
-    // the sum's roundings are covered: A.slots holds what a chunk this long can give
-    const float even = total * (float)c.heads * 1.0001f / (float)A.target;
-    const int chunk = ((int)fminf(even, (float)(1 << 28)) / CHUNK + 1) * CHUNK;
     auto scan = [&](int s0, PlanLane &x, int &parts, int &upto, int &upto_slots) {
         x = s0 ? plan_lane<RG>(c, b, A, s0 + lane) : mine;
         parts = x.n ? (x.len + x.n - 1) / chunk + 1 : 0;
@@ -95,7 +107,7 @@ QG_DEV bool plan_find(const KvView &c, const BatchView &b, const AttnArgs &A, in
     if (want < 0) {
         for (int s0 = 0; s0 < c.sequences; s0 += 64) {
             scan(s0, x, parts, upto, upto_slots);
-            units += __shfl(upto, 63);
+            units += __builtin_amdgcn_readlane(upto, 63);
         }
         const int per = (units + 7) / 8;
         if (block >> 3 >= per) return false;
@@ -113,14 +125,14 @@ QG_DEV bool plan_find(const KvView &c, const BatchView &b, const AttnArgs &A, in
         if (here) {
             const int l = __builtin_ctzll(here);
             p.s = s0 + l;
-            p.first = __shfl(x.first, l);
-            p.n = __shfl(x.n, l);
-            p.len = __shfl(x.len, l);
-            p.groups = __shfl(x.groups, l);
-            p.parts = __shfl(parts, l);
-            p.slot = slots + __shfl(upto_slots - own_slots, l);
+            p.first = __builtin_amdgcn_readlane(x.first, l);
+            p.n = __builtin_amdgcn_readlane(x.n, l);
+            p.len = __builtin_amdgcn_readlane(x.len, l);
+            p.groups = __builtin_amdgcn_readlane(x.groups, l);
+            p.parts = __builtin_amdgcn_readlane(parts, l);
+            p.slot = slots + __builtin_amdgcn_readlane(upto_slots - own_slots, l);
             if (unit >= 0) {
-                const int rest = unit - (before + __shfl(upto - own, l));
+                const int rest = unit - (before + __builtin_amdgcn_readlane(upto - own, l));
                 p.part = rest / (p.groups * c.heads);
                 p.h = rest / p.groups % c.heads;
                 p.z = rest % p.groups;
@@ -128,8 +140,8 @@ QG_DEV bool plan_find(const KvView &c, const BatchView &b, const AttnArgs &A, in
             p.chunk = chunk;
             return true;
         }
-        before += __shfl(upto, 63);
-        slots += __shfl(upto_slots, 63);
+        before += __builtin_amdgcn_readlane(upto, 63);
+        slots += __builtin_amdgcn_readlane(upto_slots, 63);
     }
     return false;
 }
@@ -149,8 +161,11 @@ template <> struct Planes<QT_F16> {
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             hi[i] = cvt2(x[2 * i], x[2 * i + 1]);
-            const qg_half2 h = __builtin_bit_cast(qg_half2, hi[i]);
-            lo[i] = cvt2(__builtin_fmaf((float)h[0], -1.0f, x[2 * i]), __builtin_fmaf((float)h[1], -1.0f, x[2 * i + 1]));
+            // x - hi in one instruction each
+            float a, b;
+            asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(a) : "v"(hi[i]), "v"(x[2 * i]));
+            asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(b) : "v"(hi[i]), "v"(x[2 * i + 1]));
+            lo[i] = cvt2(a, b);
         }
         p[0] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
         p[1] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
@@ -331,7 +346,7 @@ QG_DEV bool odd_sums(float a, float b, float weight) { return !__builtin_isfinit
 QG_DEV unsigned first_bits(int n, int most) { return (1u << min(max(n, 0), most)) - 1u; }
 
 template <int TYPE, int D, int RT, int NW>
-__global__ __launch_bounds__(64 * NW) void attention_kernel(AttnArgs A, KvView c, BatchView b) {
+__global__ __launch_bounds__(64 * NW, (D / 64) * RT <= 6 ? 2 : 1) void attention_kernel(AttnArgs A, KvView c, BatchView b) {
     typedef Tile<TYPE, D> T;
     constexpr int RG = 16 * RT, E = T::E, DL = T::DL, KEYS = T::KEYS, JOIN = NW * 16 * (D + 4) * 4;
     __shared__ __attribute__((aligned(16))) uint8_t s_mem[RT * T::Q_BYTES > JOIN ? RT * T::Q_BYTES : JOIN];
@@ -431,9 +446,6 @@ __global__ __launch_bounds__(64 * NW) void attention_kernel(AttnArgs A, KvView c
             kpage1 = kv_page(c, p.s, kpos + NW * KEYS);
             vpage1 = kv_page(c, p.s, vpos + NW * KEYS);
         }
-        unsigned vis[RT];
-#pragma unroll
-        for (int r = 0; r < RT; r++) vis[r] = (1u << E) - 1;
         if (t0 + KEYS > open || !__all(here >= 0)) {
 #pragma unroll
             for (int e = 0; e < E; e++)
@@ -444,18 +456,18 @@ __global__ __launch_bounds__(64 * NW) void attention_kernel(AttnArgs A, KvView c
                 const int t = (row0 + 16 * r + n) / A.group, prefix = b.parent ? p.len : p.len + t + 1, k = here_pos - p.len;
                 unsigned seen = first_bits(prefix - here_pos, E);
                 if (b.parent && t < p.n && k < 64 && k > -E) seen |= (unsigned)(k < 0 ? s_seen[t] << -k : s_seen[t] >> k);
-                vis[r] = here < 0 ? 0 : seen & first_bits(end - here_pos, E);
+                seen = here < 0 ? 0 : seen & first_bits(end - here_pos, E);
+#pragma unroll
+                for (int e = 0; e < E; e++) z[r][e] = seen >> e & 1 ? z[r][e] : -__builtin_inff();
             }
         }
         // scores to weights: the maximum is renewed only where it moves by more than M_LAG
 #pragma unroll
         for (int r = 0; r < RT; r++) {
-            float top = -__builtin_inff();
+            float top = z[r][0];
 #pragma unroll
-            for (int e = 0; e < E; e++) {
-                z[r][e] = vis[r] >> e & 1 ? z[r][e] * back[r] : -__builtin_inff();
-                top = fmaxf(top, z[r][e]);
-            }
+            for (int e = 1; e < E; e++) top = fmaxf(top, z[r][e]);
+            top *= back[r];
             if (__any(top > m[r] + M_LAG)) {
                 top = fmaxf(top, __shfl_xor(top, 16));
                 top = fmaxf(top, __shfl_xor(top, 32));
@@ -469,7 +481,7 @@ __global__ __launch_bounds__(64 * NW) void attention_kernel(AttnArgs A, KvView c
             const float base = m[r] == -__builtin_inff() ? 0.0f : m[r] - P_BASE;
 #pragma unroll
             for (int e = 0; e < E; e++) {
-                z[r][e] = __builtin_amdgcn_exp2f(z[r][e] - base);
+                z[r][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(z[r][e], back[r], -base));
                 l[r] += z[r][e];
             }
         }
@@ -631,7 +643,7 @@ constexpr int WAVES = 4;
 template <int TYPE, int D, int RT>
 void launch(const AttnArgs &A, const KvView &c, const BatchView &b, hipStream_t s) {
     const long groups = (long)b.rows * A.group / (16 * RT) + c.sequences;  // of all sequences: each rounds up
-    const long units = A.target + groups * c.heads + 8;
+    const long units = 2 * A.resident + groups * c.heads + 8;
     attention_kernel<TYPE, D, RT, WAVES><<<(unsigned)((units + 7) / 8 * 8), 64 * WAVES, 0, s>>>(A, c, b);
     attention_join_kernel<TYPE, D, 16 * RT><<<dim3(b.rows, A.q_heads), 64, 0, s>>>(A, c, b);
 }
@@ -648,11 +660,16 @@ void launch_dim(int rt, const AttnArgs &A, const KvView &c, const BatchView &b, 
     else launch_rt<TYPE, 256>(rt, A, c, b, s);
 }
 
-// Workgroups that the plan aims at, and the partial results that can come of it:
-// a cut sequence has fewer parts than twice its keys / chunk, and the chunk is at
-// least all sequences' keys x row groups x heads / target.
-constexpr int TARGET = 512;
-constexpr size_t SLOTS = 2 * TARGET;
+// Workgroups that run at once: a wave per SIMD each, so what the registers allow
+// (in 64-dimension row tiles: 1 takes 104 registers, 2 up to 154, 6 up to 256).
+int resident(int dim, int rt) {
+    const int w = dim / 64 * rt;
+    return qg_cu_count() * (w == 1 ? 4 : w == 2 ? 3 : w <= 6 ? 2 : 1);
+}
+// Partial results that the plan can ask for: a cut sequence has fewer parts than
+// twice its keys / chunk, and the chunk is at least all sequences' keys x row
+// groups x heads / two rounds.
+size_t slots(int dim, int rt) { return 4 * (size_t)resident(dim, rt); }
 }  // namespace
 
 extern "C" {
@@ -661,8 +678,8 @@ size_t qg_tree_attention_workspace_bytes(const qg_kv_cache *cache, const qg_kv_b
     if (qg_kv_check(cache, false, nullptr) || qg_batch_check(batch, false, nullptr)) return 0;
     if (q_heads < 1 || q_heads % cache->kv_heads || q_heads / cache->kv_heads > 128) return 0;
     const int group = q_heads / cache->kv_heads;
-    const int rg = 16 * row_tiles(cache->head_dim, (long)batch->max_rows * group);
-    return SLOTS * rg * (4 * (size_t)cache->head_dim + sizeof(float2)) + 4 * (size_t)batch->rows * q_heads;
+    const int rt = row_tiles(cache->head_dim, (long)batch->max_rows * group);
+    return slots(cache->head_dim, rt) * 16 * rt * (4 * (size_t)cache->head_dim + sizeof(float2)) + 4 * (size_t)batch->rows * q_heads;
 }
 
 int qg_tree_attention(float *out, const float *q, int q_heads, float scale, const qg_kv_cache *cache, int layer,
@@ -677,8 +694,10 @@ int qg_tree_attention(float *out, const float *q, int q_heads, float scale, cons
     if (qg_overlap(out, bytes, q, bytes) || qg_overlap(ws, need, q, bytes) || qg_overlap(ws, need, out, bytes)) return hipErrorInvalidValue;
     const int group = q_heads / c.heads, rt = row_tiles(c.dim, (long)b.max_rows * group);
     float *part_o = (float *)ws;
-    float2 *part_ml = (float2 *)(part_o + SLOTS * 16 * rt * c.dim);
-    const AttnArgs A{out, q, part_o, part_ml, (int *)(part_ml + SLOTS * 16 * rt), scale * 1.44269504088896341f, q_heads, group, layer, TARGET, (int)SLOTS};
+    const size_t parts = slots(c.dim, rt) * 16 * rt;
+    float2 *part_ml = (float2 *)(part_o + parts * c.dim);
+    const AttnArgs A{out, q, part_o, part_ml, (int *)(part_ml + parts), scale * 1.44269504088896341f, q_heads, group, layer, resident(c.dim, rt),
+                     (int)slots(c.dim, rt)};
     if (c.type == QT_F32) launch_dim<QT_F32>(rt, A, c, b, qg_stream());
     else if (c.type == QT_F16) launch_dim<QT_F16>(rt, A, c, b, qg_stream());
     else launch_dim<QT_BF16>(rt, A, c, b, qg_stream());
