@@ -552,7 +552,7 @@ QG_DEV void attend_row(const AttnArgs &A, const KvView &c, const BatchView &b, i
     const unsigned long long seen = b.parent ? __shfl(tree_ancestors(b.parent + first, n, lane), place) : 0;
     const float *q = A.q + ((size_t)row * A.q_heads + head) * D;
     for (int d = lane; d < D; d += 64) s_q[d] = q[d] * A.scale;
-    __syncthreads();
+    __builtin_amdgcn_wave_barrier();  // one wave's own
     float m = -__builtin_inff(), l = 0.0f, o[V];
 #pragma unroll
     for (int i = 0; i < V; i++) o[i] = 0.0f;
@@ -585,57 +585,88 @@ QG_DEV void attend_row(const AttnArgs &A, const KvView &c, const BatchView &b, i
     for (int i = 0; i < V; i++) A.out[((size_t)row * A.q_heads + head) * D + lane * V + i] = l == 0.0f ? 0.0f : o[i] / l;
 }
 
-// A wave per row and head: joins the parts of sequences that were cut, and takes
-// up odd rows again.
+// A workgroup per row and head: joins the parts of sequences that were cut, and
+// takes up odd rows again.  A wave sums every fourth part; a lane holds the weight
+// of one part, so that the parts' loads wait for nothing.
+constexpr int JOIN_WAVES = 4;
 template <int TYPE, int D, int RG>
-__global__ __launch_bounds__(64) void attention_join_kernel(AttnArgs A, KvView c, BatchView b) {
+__global__ __launch_bounds__(64 * JOIN_WAVES) void attention_join_kernel(AttnArgs A, KvView c, BatchView b) {
     constexpr int V = D / 64;
-    __shared__ float s_q[D];
-    const int row = blockIdx.x, head = blockIdx.y, lane = threadIdx.x;
+    __shared__ float s_y[JOIN_WAVES][D], s_q[D];
+    __shared__ float2 s_w[JOIN_WAVES];
+    const int row = blockIdx.x, head = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     int first, n;
     const int s = batch_sequence(b, c.sequences, row, lane, first, n);
     if (s < 0) return;
     Plan p;
     if (!plan_find<RG>(c, b, A, lane, 0, s, p)) return;
-    if (p.parts < 2) {
-        if (A.odd[(size_t)row * A.q_heads + head]) attend_row<TYPE, D>(A, c, b, s, first, n, row, head, lane, s_q);
-        return;
+    bool odd = p.parts < 2 && A.odd[(size_t)row * A.q_heads + head];
+    if (p.parts > 1) {
+        const int h = head / A.group, at = (row - first) * A.group + head % A.group;
+        const size_t step = (size_t)c.heads * p.groups, slot0 = p.slot + (size_t)h * p.groups + at / RG;
+        if (slot0 + (p.parts - 1) * step >= (size_t)A.slots) return;
+        const float2 *ml = A.part_ml + slot0 * RG + at % RG;
+        const float *po = A.part_o + (slot0 * RG + at % RG) * D + lane * V;
+        float top = -__builtin_inff(), sum = 0.0f, y[V];
+#pragma unroll
+        for (int v = 0; v < V; v++) y[v] = 0.0f;
+        for (int i0 = wave; i0 < p.parts; i0 += 64 * JOIN_WAVES) {
+            const int mine = i0 + lane * JOIN_WAVES, count = min((p.parts - i0 + JOIN_WAVES - 1) / JOIN_WAVES, 64);
+            const float2 x = mine < p.parts ? ml[mine * step * RG] : make_float2(-__builtin_inff(), 0.0f);
+            const float next = fmaxf(top, qg_wave_max(x.x));
+            const float old = next == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f(top - next);
+            // a part without a key leaves nothing (its sums were not written)
+            const float f = x.x == -__builtin_inff() && x.y == 0.0f ? 0.0f : x.x == next ? 1.0f : __builtin_amdgcn_exp2f(x.x - next);
+            top = next;
+            sum = sum * old + qg_sum_lanes<64>(f == 0.0f ? 0.0f : f * x.y);
+#pragma unroll
+            for (int v = 0; v < V; v++) y[v] *= old;
+            for (int i = 0; i < count; i += 8) {
+                float u[8][V];
+#pragma unroll
+                for (int k = 0; k < 8; k++)
+#pragma unroll
+                    for (int v = 0; v < V; v++) u[k][v] = po[(i0 + min(i + k, count - 1) * JOIN_WAVES) * step * RG * D + v];
+#pragma unroll
+                for (int k = 0; k < 8; k++) {
+                    const float w = i + k < count ? __int_as_float(__builtin_amdgcn_readlane(__float_as_int(f), (i + k) & 63)) : 0.0f;
+#pragma unroll
+                    for (int v = 0; v < V; v++) y[v] = w == 0.0f ? y[v] : __builtin_fmaf(w, u[k][v], y[v]);
+                }
+            }
+        }
+#pragma unroll
+        for (int v = 0; v < V; v++) s_y[wave][lane * V + v] = y[v];
+        if (lane == 0) s_w[wave] = make_float2(top, sum);
+        __syncthreads();
+        const float all = fmaxf(fmaxf(s_w[0].x, s_w[1].x), fmaxf(s_w[2].x, s_w[3].x));
+        sum = 0.0f;
+#pragma unroll
+        for (int v = 0; v < V; v++) y[v] = 0.0f;
+#pragma unroll
+        for (int w = 0; w < JOIN_WAVES; w++) {
+            const float2 x = s_w[w];
+            if (x.x == -__builtin_inff() && x.y == 0.0f) continue;
+            const float f = x.x == all ? 1.0f : __builtin_amdgcn_exp2f(x.x - all);
+            sum = __builtin_fmaf(f, x.y, sum);
+#pragma unroll
+            for (int v = 0; v < V; v++) y[v] = __builtin_fmaf(f, s_y[w][lane * V + v], y[v]);
+        }
+#pragma unroll
+        for (int v = 0; v < V; v++) odd |= odd_sums(y[v], 0.0f, sum);
+        odd = __any(odd);
+        if (wave == 0 && !odd) {
+            const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+#pragma unroll
+            for (int v = 0; v < V; v++) A.out[((size_t)row * A.q_heads + head) * D + lane * V + v] = y[v] * inv;
+        }
     }
-    const int h = head / A.group, at = (row - first) * A.group + head % A.group;
-    const size_t step = (size_t)c.heads * p.groups, slot0 = p.slot + (size_t)h * p.groups + at / RG;
-    if (slot0 + (p.parts - 1) * step >= (size_t)A.slots) return;
-    const float2 *ml = A.part_ml + slot0 * RG + at % RG;
-    float top = -__builtin_inff();
-    for (int i = lane; i < p.parts; i += 64) top = fmaxf(top, ml[i * step * RG].x);
-    top = qg_wave_max(top);
-    float sum = 0.0f, y[V];
-#pragma unroll
-    for (int v = 0; v < V; v++) y[v] = 0.0f;
-    const float *po = A.part_o + (slot0 * RG + at % RG) * D + lane * V;
-#pragma unroll 4
-    for (int i = 0; i < p.parts; i++) {
-        const float2 x = ml[i * step * RG];
-        if (x.x == -__builtin_inff() && x.y == 0.0f) continue;
-        const float f = x.x == top ? 1.0f : __builtin_amdgcn_exp2f(x.x - top);
-        sum = __builtin_fmaf(f, x.y, sum);
-#pragma unroll
-        for (int v = 0; v < V; v++) y[v] = __builtin_fmaf(f, po[i * step * RG * D + v], y[v]);
-    }
-    bool odd = false;
-#pragma unroll
-    for (int v = 0; v < V; v++) odd |= odd_sums(y[v], 0.0f, sum);
-    if (__any(odd)) {
-        attend_row<TYPE, D>(A, c, b, s, first, n, row, head, lane, s_q);
-        return;
-    }
-    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-#pragma unroll
-    for (int v = 0; v < V; v++) A.out[((size_t)row * A.q_heads + head) * D + lane * V + v] = y[v] * inv;
+    if (odd && wave == 0) attend_row<TYPE, D>(A, c, b, s, first, n, row, head, lane, s_q);
 }
 
 // Row tiles per wave: as few row groups as the registers allow, and no more tiles than those need.
 int row_tiles(int dim, long rows) {
-    const long most = dim == 256 ? 2 : 4, groups = (rows + 16 * most - 1) / (16 * most);
+    const long most = dim == 256 ? 2 : dim == 128 ? 3 : 4, groups = (rows + 16 * most - 1) / (16 * most);
     return (int)((rows + 16 * groups - 1) / (16 * groups));
 }
 constexpr int WAVES = 4;
@@ -645,13 +676,16 @@ void launch(const AttnArgs &A, const KvView &c, const BatchView &b, hipStream_t 
     const long groups = (long)b.rows * A.group / (16 * RT) + c.sequences;  // of all sequences: each rounds up
     const long units = 2 * A.resident + groups * c.heads + 8;
     attention_kernel<TYPE, D, RT, WAVES><<<(unsigned)((units + 7) / 8 * 8), 64 * WAVES, 0, s>>>(A, c, b);
-    attention_join_kernel<TYPE, D, 16 * RT><<<dim3(b.rows, A.q_heads), 64, 0, s>>>(A, c, b);
+    attention_join_kernel<TYPE, D, 16 * RT><<<dim3(b.rows, A.q_heads), 64 * JOIN_WAVES, 0, s>>>(A, c, b);
 }
 template <int TYPE, int D>
 void launch_rt(int rt, const AttnArgs &A, const KvView &c, const BatchView &b, hipStream_t s) {
     if (rt == 1) launch<TYPE, D, 1>(A, c, b, s);
     else if (rt == 2) launch<TYPE, D, 2>(A, c, b, s);
-    else if constexpr (D != 256) rt == 3 ? launch<TYPE, D, 3>(A, c, b, s) : launch<TYPE, D, 4>(A, c, b, s);
+    else if constexpr (D != 256) {
+        if (rt == 3) launch<TYPE, D, 3>(A, c, b, s);
+        else if constexpr (D == 64) launch<TYPE, D, 4>(A, c, b, s);
+    }
 }
 template <int TYPE>
 void launch_dim(int rt, const AttnArgs &A, const KvView &c, const BatchView &b, hipStream_t s) {
