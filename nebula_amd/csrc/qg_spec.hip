@@ -29,11 +29,26 @@ QG_DEV void turn_of(double angle, float &s, float &c) {
     sincospif((float)(2.0 * r), &s, &c);
 }
 
-template <int D>
-__global__ __launch_bounds__(256) void qk_rope_kernel(RopeArgs A, KvView c, BatchView b, int layer) {
+// A wave takes U heads-per-wave of one row: the row's place, its angles' sines and
+// the loads of all its heads once.
+template <int D, int U>
+__global__ __launch_bounds__(256) void qk_rope_kernel(RopeArgs A, KvView c, BatchView b, int layer, int parts) {
     constexpr int LPH = D / 4, HPW = 64 / LPH;  // lanes per head, heads per wave
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, row = blockIdx.x;
-    const int d = (lane % LPH) * 4, h = (blockIdx.y * 4 + wave) * HPW + lane / LPH;
+    const int lane = threadIdx.x & 63, id = blockIdx.x * 4 + (threadIdx.x >> 6), row = id / parts;
+    if (row >= A.rows) return;
+    const int d = (lane % LPH) * 4, h0 = id % parts * (U * HPW) + lane / LPH, heads = A.q_heads + A.kv_heads * (A.cached ? 2 : 1);
+    // where head h of the row is read; 0, 1, 2: q, k, v
+    auto kind = [&](int h) { return h < A.q_heads ? 0 : h < A.q_heads + A.kv_heads ? 1 : 2; };
+    auto nth = [&](int h) { return h < A.q_heads ? h : h < A.q_heads + A.kv_heads ? h - A.q_heads : h - A.q_heads - A.kv_heads; };
+    float x[U][4];
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+        const int h = h0 + u * HPW, k = kind(h), i = nth(h);
+        const float *src = k == 0 ? A.q + row * A.q_row + i * A.q_head : k == 1 ? A.k + row * A.k_row + i * A.k_head
+                                                                              : A.v + row * A.v_row + i * A.v_head;
+        const float4 y = h < heads ? *(const float4 *)(src + d) : make_float4(0, 0, 0, 0);
+        x[u][0] = y.x; x[u][1] = y.y; x[u][2] = y.z; x[u][3] = y.w;
+    }
     int pos = 0, slot = -1, page = -1;
     if (A.cached) {
         int first, n;
@@ -48,286 +63,506 @@ __global__ __launch_bounds__(256) void qk_rope_kernel(RopeArgs A, KvView c, Batc
         slot = (len + place) & ((1 << c.shift) - 1);
     }
     if (A.position) pos = A.position[row];
-    const int kind = h < A.q_heads ? 0 : h < A.q_heads + A.kv_heads ? 1 : 2;
-    const int head = kind == 0 ? h : h - A.q_heads - (kind == 2 ? A.kv_heads : 0);
-    const bool live = h < A.q_heads + A.kv_heads * (A.cached ? 2 : 1);
-    const float *src = kind == 0 ? A.q + row * A.q_row + head * A.q_head : kind == 1 ? A.k + row * A.k_row + head * A.k_head
-                                                                                 : A.v + row * A.v_row + head * A.v_head;
-    float4 x4 = live ? *(const float4 *)(src + d) : make_float4(0, 0, 0, 0);
-    float x[4] = {x4.x, x4.y, x4.z, x4.w};
-    const float *w = kind == 0 ? A.q_norm : A.k_norm;
-    float ss = 0.0f;
+    // of a lane's four dimensions: their pairs' angles, and the lane that holds the other halves
+    const int half = A.rope / 2;
+    const bool low = d < half, turned = d < A.rope;
+    float sn[4], cs[4];
+    if (turned) {
+        const int f = A.interleaved ? d / 2 : low ? d : d - half;
 #pragma unroll
-    for (int i = 0; i < 4; i++) ss = __builtin_fmaf(x[i], x[i], ss);
-    ss = qg_row_sum(ss);
-    if (LPH >= 32) ss += __shfl_xor(ss, 16);
-    if (LPH >= 64) ss += __shfl_xor(ss, 32);
-    if (kind < 2 && w) {
-        const float scale = 1.0f / __builtin_sqrtf(ss / (float)D + A.eps);
-        const float4 w4 = *(const float4 *)(w + d);
-        x[0] = x[0] * scale * w4.x;
-        x[1] = x[1] * scale * w4.y;
-        x[2] = x[2] * scale * w4.z;
-        x[3] = x[3] * scale * w4.w;
+        for (int i = 0; i < 4; i++) {
+            if (A.interleaved && i >= 2) { sn[i] = cs[i] = 0.0f; continue; }
+            turn_of((double)pos * A.freq[f + i], sn[i], cs[i]);
+        }
     }
-    if (A.rope) {
-        const int half = A.rope / 2;
-        float y[4];
-        if (A.interleaved) {
-            const int f = min(d, A.rope - 4) / 2;
+    const int other = (lane + (low ? half / 4 : -(half / 4))) & 63;
 #pragma unroll
-            for (int i = 0; i < 2; i++) {
-                float sn, cs;
-                turn_of((double)pos * A.freq[f + i], sn, cs);
-                y[2 * i] = x[2 * i] * cs - x[2 * i + 1] * sn;
-                y[2 * i + 1] = x[2 * i + 1] * cs + x[2 * i] * sn;
+    for (int u = 0; u < U; u++) {
+        const int h = h0 + u * HPW, k = kind(h), i = nth(h);
+        const float *w = k == 0 ? A.q_norm : A.k_norm;
+        float ss = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 4; j++) ss = __builtin_fmaf(x[u][j], x[u][j], ss);
+        ss = qg_row_sum(ss);
+        if (LPH >= 32) ss += __shfl_xor(ss, 16);
+        if (LPH >= 64) ss += __shfl_xor(ss, 32);
+        if (k < 2 && w) {
+            const float scale = 1.0f / __builtin_sqrtf(ss / (float)D + A.eps);
+            const float4 w4 = *(const float4 *)(w + d);
+            x[u][0] = x[u][0] * scale * w4.x;
+            x[u][1] = x[u][1] * scale * w4.y;
+            x[u][2] = x[u][2] * scale * w4.z;
+            x[u][3] = x[u][3] * scale * w4.w;
+        }
+        if (A.rope) {
+            float y[4];
+            if (A.interleaved) {
+#pragma unroll
+                for (int j = 0; j < 4; j += 2) {
+                    y[j] = x[u][j] * cs[j / 2] - x[u][j + 1] * sn[j / 2];
+                    y[j + 1] = x[u][j + 1] * cs[j / 2] + x[u][j] * sn[j / 2];
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const float p = __shfl(x[u][j], other);
+                    y[j] = low ? x[u][j] * cs[j] - p * sn[j] : x[u][j] * cs[j] + p * sn[j];
+                }
             }
+            if (k < 2 && turned) {
+#pragma unroll
+                for (int j = 0; j < 4; j++) x[u][j] = y[j];
+            }
+        }
+        if (h >= heads) continue;
+        const float4 y = make_float4(x[u][0], x[u][1], x[u][2], x[u][3]);
+        if (k == 0) *(float4 *)(A.q_out + ((size_t)row * A.q_heads + i) * D + d) = y;
+        if (k == 1 && A.k_out) *(float4 *)(A.k_out + ((size_t)row * A.kv_heads + i) * D + d) = y;
+        if (k == 0 || page < 0) continue;
+        uint8_t *pool = k == 1 ? c.k : c.v;
+        const size_t at = kv_at(c, layer, page, i, slot) + d;
+        if (c.type == QT_F32) {
+            *(float4 *)((float *)pool + at) = y;
         } else {
-            const bool low = d < half;
-            const int other = lane + (low ? half / 4 : -(half / 4)), f = d < A.rope ? (low ? d : d - half) : 0;
+            uint32_t r[4];
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const float p = __shfl(x[i], other & 63);
-                float sn, cs;
-                turn_of((double)pos * A.freq[f + i], sn, cs);
-                y[i] = low ? x[i] * cs - p * sn : x[i] * cs + p * sn;
-            }
-        }
-        if (kind < 2 && d < A.rope) {
-#pragma unroll
-            for (int i = 0; i < 4; i++) x[i] = y[i];
+            for (int j = 0; j < 4; j++) r[j] = c.type == QT_F16 ? kv_f16(x[u][j]) : kv_bf16(x[u][j]);
+            *(uint2 *)((uint16_t *)pool + at) = make_uint2(r[0] | r[1] << 16, r[2] | r[3] << 16);
         }
     }
-    if (!live) return;
-    if (kind == 0) {
-        *(float4 *)(A.q_out + ((size_t)row * A.q_heads + head) * D + d) = make_float4(x[0], x[1], x[2], x[3]);
-        return;
-    }
-    if (kind == 1 && A.k_out) *(float4 *)(A.k_out + ((size_t)row * A.kv_heads + head) * D + d) = make_float4(x[0], x[1], x[2], x[3]);
-    if (page < 0) return;
-    uint8_t *pool = kind == 1 ? c.k : c.v;
-    const size_t at = kv_at(c, layer, page, head, slot) + d;
-    if (c.type == QT_F32) {
-        *(float4 *)((float *)pool + at) = make_float4(x[0], x[1], x[2], x[3]);
-    } else {
-        uint32_t r[4];
-#pragma unroll
-        for (int i = 0; i < 4; i++) r[i] = c.type == QT_F16 ? kv_f16(x[i]) : kv_bf16(x[i]);
-        *(uint2 *)((uint16_t *)pool + at) = make_uint2(r[0] | r[1] << 16, r[2] | r[3] << 16);
-    }
+}
+template <int D>
+void launch_rope(const RopeArgs &A, const KvView &c, const BatchView &b, int layer, hipStream_t s) {
+    const int units = (A.q_heads + A.kv_heads * (A.cached ? 2 : 1) + 256 / D - 1) / (256 / D);  // wavefuls of heads per row
+    const bool wide = (long)A.rows * units > 8192;
+    const int parts = wide ? (units + 4) / 5 : units;
+    const unsigned blocks = (unsigned)(((long)A.rows * parts + 3) / 4);
+    if (wide) qk_rope_kernel<D, 5><<<blocks, 256, 0, s>>>(A, c, b, layer, parts);
+    else qk_rope_kernel<D, 1><<<blocks, 256, 0, s>>>(A, c, b, layer, parts);
 }
 
 // ------------------------------------------------------------------------
-// Softmax of a row: e_i = exp((x_i - m) / T), out = e_i / sum e.
+// Softmax of a row: e_i = 2^((x_i - m) log2 e / T), out = e_i / sum e.  A NaN, or
+// an infinite m, makes the sum NaN and with it the row.  Loads and stores are
+// one float per lane, so that a row may start anywhere.
 // ------------------------------------------------------------------------
-constexpr int SM_THREADS = 1024;
 
-// The largest of two values; NaN if either is.
-QG_DEV float max_nan(float a, float b) { return a != a || a > b ? a : b; }
-
-// A workgroup's value by `op`, in every thread; s[16] is scratch.
-template <typename T, typename F>
+// A workgroup's value by `op`, in every thread; s holds one per wave.
+template <int THREADS, typename T, typename F>
 QG_DEV T block_all(T v, T *s, F op) {
 #pragma unroll
     for (int d = 1; d < 64; d *= 2) v = op(v, __shfl_xor(v, d));
+    if (THREADS == 64) return v;
     __syncthreads();
     if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = v;
     __syncthreads();
     v = s[0];
 #pragma unroll
-    for (int w = 1; w < SM_THREADS / 64; w++) v = op(v, s[w]);
+    for (int w = 1; w < THREADS / 64; w++) v = op(v, s[w]);
     return v;
 }
+struct Larger { __device__ __forceinline__ float operator()(float a, float b) const { return fmaxf(a, b); } };
+struct Added {
+    template <typename T> __device__ __forceinline__ T operator()(T a, T b) const { return a + b; }
+};
+struct Lower { __device__ __forceinline__ int operator()(int a, int b) const { return min(a, b); } };
+constexpr int SM_NAN = -1;  // in place of the index of a row's largest value
 
-__global__ __launch_bounds__(SM_THREADS) void softmax_row_kernel(float *out, const float *x, int cols, float inv) {
-    __shared__ float s_f[16];
-    __shared__ int s_i[16];
+// The lowest index of value m in x[0..n), SM_NAN if there is a NaN, n without
+// either; in every thread.
+template <int THREADS>
+QG_DEV int lowest_of(const float *x, int n, float m, int *s) {
+    int at = n;
+    for (int i = threadIdx.x; i < n; i += THREADS) {
+        const float v = x[i];
+        if (v != v) at = SM_NAN;
+        else if (v == m) at = min(at, i);
+    }
+    return block_all<THREADS>(at, s, Lower());
+}
+
+// A workgroup per row.  REGS values of a thread stay in registers and KEPT in
+// shared memory between the three passes (largest value, sum, output); what is
+// longer is read again.
+template <int THREADS, int REGS, int KEPT>
+__global__ __launch_bounds__(THREADS) void softmax_row_kernel(float *out, const float *x, int cols, float scale) {
+    __shared__ float s_x[KEPT ? KEPT * THREADS : 1], s_f[THREADS / 64];
+    __shared__ int s_i[THREADS / 64];
+    constexpr int HELD = (REGS + KEPT) * THREADS;
+    const int tid = threadIdx.x;
     const float *row = x + (size_t)blockIdx.x * cols;
     float *to = out + (size_t)blockIdx.x * cols;
-    float m = -__builtin_inff();
-    for (int i = threadIdx.x; i < cols; i += SM_THREADS) m = max_nan(row[i], m);
-    m = block_all(m, s_f, max_nan);
-    if (m == -__builtin_inff()) {
-        for (int i = threadIdx.x; i < cols; i += SM_THREADS) to[i] = 0.0f;
-        return;
+    const float none = -__builtin_inff();
+    float r[REGS], m = none;
+#pragma unroll
+    for (int k = 0; k < REGS; k++) r[k] = k * THREADS + tid < cols ? row[k * THREADS + tid] : none;
+#pragma unroll 8
+    for (int k = 0; k < KEPT; k++) {
+        const int i = (REGS + k) * THREADS + tid;
+        const float v = i < cols ? row[i] : none;
+        s_x[k * THREADS + tid] = v;
+        m = fmaxf(m, v);
     }
-    if (!__builtin_isfinite(m)) {
-        for (int i = threadIdx.x; i < cols; i += SM_THREADS) to[i] = __builtin_nanf("");
-        return;
-    }
-    if (inv == 0.0f) {  // temperature 0
-        int at = cols;
-        for (int i = cols - 1 - threadIdx.x; i >= 0; i -= SM_THREADS) if (row[i] == m) at = i;
-        at = block_all(at, s_i, [](int a, int b) { return min(a, b); });
-        for (int i = threadIdx.x; i < cols; i += SM_THREADS) to[i] = i == at ? 1.0f : 0.0f;
+    for (int i = HELD + tid; i < cols; i += THREADS) m = fmaxf(m, row[i]);
+#pragma unroll
+    for (int k = 0; k < REGS; k++) m = fmaxf(m, r[k]);
+    m = block_all<THREADS>(m, s_f, Larger());
+    if (scale == 0.0f || m == none) {  // temperature 0, or nothing above -infinity
+        const int at = lowest_of<THREADS>(row, cols, scale == 0.0f ? m : 0.0f, s_i);
+        const bool nan = at == SM_NAN || m == __builtin_inff();
+        __syncthreads();
+        for (int i = tid; i < cols; i += THREADS) to[i] = nan ? __builtin_nanf("") : m != none && i == at ? 1.0f : 0.0f;
         return;
     }
     float sum = 0.0f;
-    for (int i = threadIdx.x; i < cols; i += SM_THREADS) sum += expf((row[i] - m) * inv);
-    sum = block_all(sum, s_f, [](float a, float b) { return a + b; });
-    for (int i = threadIdx.x; i < cols; i += SM_THREADS) to[i] = expf((row[i] - m) * inv) / sum;
+#pragma unroll
+    for (int k = 0; k < REGS; k++) { r[k] = __builtin_amdgcn_exp2f((r[k] - m) * scale); sum += r[k]; }
+#pragma unroll 8
+    for (int k = 0; k < KEPT; k++) {
+        const float e = __builtin_amdgcn_exp2f((s_x[k * THREADS + tid] - m) * scale);
+        s_x[k * THREADS + tid] = e;
+        sum += e;
+    }
+    for (int i = HELD + tid; i < cols; i += THREADS) sum += __builtin_amdgcn_exp2f((row[i] - m) * scale);
+    const float inv = 1.0f / block_all<THREADS>(sum, s_f, Added());
+#pragma unroll
+    for (int k = 0; k < REGS; k++) if (k * THREADS + tid < cols) to[k * THREADS + tid] = r[k] * inv;
+#pragma unroll 8
+    for (int k = 0; k < KEPT; k++) {
+        const int i = (REGS + k) * THREADS + tid;
+        if (i < cols) to[i] = s_x[k * THREADS + tid] * inv;
+    }
+    for (int i = HELD + tid; i < cols; i += THREADS) to[i] = __builtin_amdgcn_exp2f((row[i] - m) * scale) * inv;
 }
 
-// ------------------------------------------------------------------------
-// Verification.  A workgroup per sequence.  After j rejections at a row the
-// target's distribution without the drafts' share is max(p_{j-1} - q, 0) / Z;
-// written out from the first that is max(p - a q, 0) / B with a += B at each
-// rejection, so every pass reads p and q alone and nothing is kept per token.
-// ------------------------------------------------------------------------
-constexpr int VF_TILE = 4 * SM_THREADS, VF_TILES = (1 << 24) / VF_TILE;
+// Few rows: pieces of SM_PIECE values, a workgroup each; first every piece's
+// largest value, its index and the sum, then every piece's outputs from the row's.
+constexpr int SM_THREADS = 256, SM_REGS = 16, SM_PIECE = SM_THREADS * SM_REGS;
+struct SoftPart { float m, sum; int at, pad; };
 
+template <bool LAST>
+__global__ __launch_bounds__(SM_THREADS) void softmax_piece_kernel(float *out, const float *x, int cols, float scale, SoftPart *parts) {
+    __shared__ float s_f[4];
+    __shared__ int s_i[4];
+    const int tid = threadIdx.x, c0 = blockIdx.x * SM_PIECE, n = min(SM_PIECE, cols - c0), pieces = gridDim.x;
+    const float *row = x + (size_t)blockIdx.y * cols + c0, none = -__builtin_inff();
+    parts += (size_t)blockIdx.y * pieces;
+    float r[SM_REGS], m = none, sum = 0.0f;
+#pragma unroll
+    for (int k = 0; k < SM_REGS; k++) r[k] = k * SM_THREADS + tid < n ? row[k * SM_THREADS + tid] : none;
+    if (!LAST) {
+#pragma unroll
+        for (int k = 0; k < SM_REGS; k++) m = fmaxf(m, r[k]);
+        m = block_all<SM_THREADS>(m, s_f, Larger());
+        int at = n;
+        if (scale == 0.0f || m == none) {
+            at = lowest_of<SM_THREADS>(row, n, scale == 0.0f ? m : 0.0f, s_i);
+        } else {
+#pragma unroll
+            for (int k = 0; k < SM_REGS; k++) sum += __builtin_amdgcn_exp2f((r[k] - m) * scale);
+            sum = block_all<SM_THREADS>(sum, s_f, Added());
+        }
+        if (tid == 0) parts[blockIdx.x] = SoftPart{m, sum, at == SM_NAN ? SM_NAN : c0 + at, 0};
+        return;
+    }
+    float *to = out + (size_t)blockIdx.y * cols + c0;
+    for (int i = tid; i < pieces; i += SM_THREADS) m = fmaxf(m, parts[i].m);
+    m = block_all<SM_THREADS>(m, s_f, Larger());
+    int at = 0x7fffffff;
+    for (int i = tid; i < pieces; i += SM_THREADS) {
+        const SoftPart p = parts[i];
+        if (p.at == SM_NAN) at = SM_NAN;
+        else if (p.m == m) at = min(at, p.at);
+        if (p.m != none) sum += p.sum * __builtin_amdgcn_exp2f((p.m - m) * scale);
+    }
+    sum = block_all<SM_THREADS>(sum, s_f, Added());
+    at = block_all<SM_THREADS>(at, s_i, Lower());
+    const bool nan = at == SM_NAN || m == __builtin_inff();
+    const float inv = 1.0f / sum;
+#pragma unroll
+    for (int k = 0; k < SM_REGS; k++) {
+        const int i = k * SM_THREADS + tid;
+        float y = __builtin_amdgcn_exp2f((r[k] - m) * scale) * inv;
+        if (scale == 0.0f || m == none) y = m != none && c0 + i == at ? 1.0f : 0.0f;
+        if (i < n) to[i] = nan ? __builtin_nanf("") : y;
+    }
+}
+// Pieces where the rows alone would not fill the card.
+bool softmax_pieces(int rows, int cols) { return rows < 128 && cols > SM_PIECE; }
+
+// ------------------------------------------------------------------------
+// Verification.  After j rejections at a row the target's distribution without
+// the drafts' share is max(p_{j-1} - q, 0) / Z; written out from the first, that
+// is max(p - a q, 0) / B with a += B at each rejection.  So a sum over the
+// vocabulary depends on (row, a) alone, and the walk is a sequence of such sums
+// with a little arithmetic between.  A sum is a launch over pieces of the
+// vocabulary, whose workgroups all take the walk to the next sum by themselves;
+// the last kernel draws the token.  A chain has one sum: it ends at its first
+// rejection.
+// ------------------------------------------------------------------------
+constexpr int VF_THREADS = 256, VF_REGS = 16, VF_PIECE = VF_THREADS * VF_REGS, VF_LAST = 1024;
+
+struct Walk;
 struct VerifyArgs {
     int *tokens_out, *path, *count;
     const float *p, *q, *u, *u_last;
     const int *token;
-    int cols;
+    int cols, pieces;
+    double *sums;            // [2][sequences][pieces], likewise
+    Walk *walks;             // [sequences][2], the last round's and this one's
 };
-// What is left of token i at a row: w = max(p - a q, 0), or p without the
-// rejected tokens drop[0..drops).
+// Where a sequence's walk stands: the accepted rows, the rejected drafts of the
+// current row, and what is left of its distribution.
+struct Walk {
+    unsigned long long taken, gone;
+    double a, mass;
+    int node, next, half, state;  // half: of sums, the one that holds this (row, a)'s
+};
+enum { WALK_SUM = 0, WALK_DRAW_SUM = 1, WALK_DRAW = 2 };  // needs a sum; needs one and then draws; draws
+
+// A sequence's drafts in shared memory: token, parent, number, and the
+// probabilities of each at the row that it continues.
+struct Drafts {
+    float p[QG_MAX_TREE], q[QG_MAX_TREE], u[QG_MAX_TREE];
+    int token[QG_MAX_TREE], up[QG_MAX_TREE];
+};
+QG_DEV void read_drafts(const VerifyArgs &A, const BatchView &b, int first, int n, Drafts &d) {
+    const int i = threadIdx.x;
+    if (i < n) {
+        const int r = first + i, x = A.token[r];
+        int up = b.parent ? tree_parent(b.parent[r], i) : i - 1;
+        if ((unsigned)x >= (unsigned)A.cols) up = -1;
+        d.token[i] = x;
+        d.up[i] = up;
+        d.u[i] = A.u[r];
+        const size_t at = (size_t)(first + max(up, 0)) * A.cols + x;
+        d.p[i] = up >= 0 ? A.p[at] : 0.0f;
+        d.q[i] = up >= 0 && A.q ? A.q[at] : 0.0f;
+    }
+    __syncthreads();
+}
+// Takes the walk on until a sum is needed or a token can be drawn (the same in
+// every thread).  summed: mass is the sum of what is left at (node, a).
+QG_DEV void walk_on(Walk &w, const Drafts &d, int n, bool sampled, bool summed) {
+    for (int i = w.next; i < n; i++) {
+        if (d.up[i] != w.node) continue;
+        const double u = (double)d.u[i];
+        double p = (double)d.p[i];
+        bool accept;
+        if (sampled) {
+            const double q = (double)d.q[i];
+            p -= w.a * q;
+            accept = u * q * w.mass < p;
+        } else {
+            for (unsigned long long g = w.gone; g; g &= g - 1)
+                if (d.token[__builtin_ctzll(g)] == d.token[i]) p = 0.0;
+            accept = u * w.mass < p;
+        }
+        summed = false;
+        if (accept) {
+            w.taken |= 1ULL << i;
+            w.node = i;
+            w.a = 0.0; w.mass = 1.0; w.gone = 0;
+        } else if (sampled) {
+            w.a += w.mass;
+            w.next = i + 1;
+            w.state = WALK_SUM;
+            return;
+        } else {
+            w.mass -= p > 0.0 ? p : 0.0;
+            w.gone |= 1ULL << i;
+        }
+    }
+    w.next = n;
+    w.state = summed ? WALK_DRAW : WALK_DRAW_SUM;
+}
+// What is left of token i at a row: max(p - a q, 0), or p without the rejected tokens.
 struct Left {
     const float *p, *q;
     double a;
-    const int *drop;
-    int drops;
+    unsigned long long gone;
+    const int *token;
+    __device__ __forceinline__ double of(float pi, float qi, int i) const {
+        double w = (double)pi;
+        if (q) w -= a * (double)qi;
+        else for (unsigned long long g = gone; g; g &= g - 1) w = token[__builtin_ctzll(g)] == i ? 0.0 : w;
+        return w > 0.0 ? w : 0.0;
+    }
+    __device__ __forceinline__ double at(int i) const { return of(p[i], q ? q[i] : 0.0f, i); }
 };
-QG_DEV double left_at(const Left &l, int i) {
-    double w = (double)l.p[i];
-    if (l.q) w -= l.a * (double)l.q[i];
-    else for (int k = 0; k < l.drops; k++) w = i == l.drop[k] ? 0.0 : w;
-    return w > 0.0 ? w : 0.0;
+QG_DEV Left left_of(const VerifyArgs &A, const Walk &w, const Drafts &d, int first) {
+    const size_t at = (size_t)(first + w.node) * A.cols;
+    return Left{A.p + at, A.q ? A.q + at : nullptr, w.a, w.gone, d.token};
 }
-// The sum of what is left, tile by tile (s_tile keeps the tiles' sums).
-QG_DEV double left_sum(const Left &l, int cols, double *s_red, double *s_tile) {
-    double total = 0.0;
-    for (int t = 0; t * VF_TILE < cols; t++) {
-        double v = 0.0;
+// The sum over a piece, in every thread of THREADS.
+template <int THREADS>
+QG_DEV double piece_sum(const Left &l, int c0, int n, double *s) {
+    constexpr int R = VF_PIECE / THREADS;
+    float p[R], q[R];
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-            const int i = t * VF_TILE + j * SM_THREADS + threadIdx.x;
-            if (i < cols) v += left_at(l, i);
-        }
-        v = block_all(v, s_red, [](double a, double b) { return a + b; });
-        if (threadIdx.x == 0) s_tile[t] = v;
-        total += v;
+    for (int k = 0; k < R; k++) {
+        const int i = k * THREADS + threadIdx.x;
+        p[k] = i < n ? l.p[c0 + i] : 0.0f;
+        q[k] = i < n && l.q ? l.q[c0 + i] : 0.0f;
     }
-    __syncthreads();
-    return total;
+    double v = 0.0;
+#pragma unroll
+    for (int k = 0; k < R; k++) v += l.of(p[k], q[k], c0 + k * THREADS + threadIdx.x);
+    return block_all<THREADS>(v, s, Added());
 }
-// The first token whose running sum passes goal (0 <= goal < total): its tile,
-// then its place there.  Only tokens with something left are taken, so sums that
-// round differently in the two steps cannot pick another.
-QG_DEV int left_pick(const Left &l, int cols, double goal, double *s_red, const double *s_tile, int *s_int) {
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, tiles = (cols + VF_TILE - 1) / VF_TILE;
-    double before = 0.0;
-    int tile = -1;
-    double at = 0.0;
-    for (int t = 0; t < tiles; t++) {  // the last tile with something in it, should none pass
-        const double v = s_tile[t];
-        if (v > 0.0) { tile = t; at = before; if (before + v > goal) break; }
-        before += v;
-    }
-    if (tile < 0) return -1;
-    int last = -1;
-    for (int j = 0; j < 4; j++) {
-        const int i = tile * VF_TILE + j * SM_THREADS + tid;
-        const double w = i < cols ? left_at(l, i) : 0.0;
-        double sum = w;
-#pragma unroll
-        for (int d = 1; d < 64; d *= 2) {
-            const double y = __shfl_up(sum, d);
-            if (lane >= d) sum += y;
-        }
-        __syncthreads();
-        if (lane == 63) s_red[wave] = sum;
-        if (tid < 2) s_int[tid] = tid ? -1 : 0x7fffffff;
-        __syncthreads();
-        double all = 0.0;
-        for (int k = 0; k < SM_THREADS / 64; k++) {
-            if (k == wave) sum += at + all;
-            all += s_red[k];
-        }
-        at += all;
-        if (w > 0.0) {
-            atomicMax(&s_int[1], i);
-            if (sum > goal) atomicMin(&s_int[0], i);
-        }
-        __syncthreads();
-        if (s_int[0] != 0x7fffffff) return s_int[0];
-        last = max(last, s_int[1]);
-    }
-    return last;
+// The sum over all pieces' sums, in every thread.
+template <int THREADS>
+QG_DEV double all_pieces(const double *sums, int pieces, double *s) {
+    double v = 0.0;
+    for (int i = threadIdx.x; i < pieces; i += THREADS) v += sums[i];
+    return block_all<THREADS>(v, s, Added());
 }
 
-__global__ __launch_bounds__(SM_THREADS) void verify_kernel(VerifyArgs A, BatchView b) {
-    __shared__ double s_red[16], s_tile[VF_TILES];
-    __shared__ float s_p[QG_MAX_TREE], s_q[QG_MAX_TREE], s_u[QG_MAX_TREE];
-    __shared__ int s_tok[QG_MAX_TREE], s_up[QG_MAX_TREE], s_drop[QG_MAX_TREE], s_int[2];
-    const int s = blockIdx.x, tid = threadIdx.x;
+// One sum: workgroup x of sequence y takes the walk to its next sum and adds its
+// piece of it.  round 0 starts the walk.
+__global__ __launch_bounds__(VF_THREADS) void verify_sum_kernel(VerifyArgs A, BatchView b, int round) {
+    __shared__ Drafts d;
+    __shared__ double s_red[4];
+    const int s = blockIdx.y;
+    int first, n;
+    batch_rows(b, s, first, n);
+    if (n == 0) return;
+    Walk w{1, 0, 0.0, 1.0, 0, 1, 0, WALK_SUM};
+    if (round) {
+        w = A.walks[s * 2 + ((round - 1) & 1)];
+        if (w.state != WALK_SUM) {  // decided: the next kernel finds it where it looks
+            if (blockIdx.x == 0 && threadIdx.x == 0) A.walks[s * 2 + (round & 1)] = w;
+            return;
+        }
+        w.mass = all_pieces<VF_THREADS>(A.sums + ((size_t)w.half * gridDim.y + s) * A.pieces, A.pieces, s_red);
+    }
+    read_drafts(A, b, first, n, d);
+    walk_on(w, d, n, A.q != nullptr, round > 0);
+    if (w.state != WALK_DRAW) {
+        w.half = round & 1;
+        const int c0 = blockIdx.x * VF_PIECE;
+        const double v = piece_sum<VF_THREADS>(left_of(A, w, d, first), c0, min(VF_PIECE, A.cols - c0), s_red);
+        if (threadIdx.x == 0) A.sums[((size_t)w.half * gridDim.y + s) * A.pieces + blockIdx.x] = v;
+    }
+    if (blockIdx.x == 0 && threadIdx.x == 0) A.walks[s * 2 + (round & 1)] = w;
+}
+
+// The rest of the walk and the last token, a workgroup per sequence.
+__global__ __launch_bounds__(VF_LAST) void verify_draw_kernel(VerifyArgs A, BatchView b, int rounds) {
+    __shared__ Drafts d;
+    __shared__ double s_red[16];
+    __shared__ int s_int[2];
+    const int s = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     int first, n;
     batch_rows(b, s, first, n);
     int *tokens = A.tokens_out + (size_t)s * b.max_rows, *path = A.path + (size_t)s * b.max_rows;
-    if (tid < b.max_rows) tokens[tid] = path[tid] = -1;
     if (n == 0) {
+        if (tid < b.max_rows) tokens[tid] = path[tid] = -1;
         if (tid == 0) A.count[s] = 0;
         return;
     }
-    if (tid < n) {
-        const int r = first + tid, x = A.token[r];
-        int up = b.parent ? tree_parent(b.parent[r], tid) : tid - 1;
-        if ((unsigned)x >= (unsigned)A.cols) up = -1;
-        s_tok[tid] = x;
-        s_up[tid] = up;
-        s_u[tid] = A.u[r];
-        const size_t at = (size_t)(first + max(up, 0)) * A.cols + x;
-        s_p[tid] = up >= 0 ? A.p[at] : 0.0f;
-        s_q[tid] = up >= 0 && A.q ? A.q[at] : 0.0f;
-    }
-    __syncthreads();
-    int node = 0, kept = 0, drops = 0;
-    double a = 0.0, mass = 1.0;
-    if (tid == 0) path[0] = 0;
-    for (int i = 1; i < n; i++) {  // the same walk in every thread
-        if (s_up[i] != node) continue;
-        const double u = (double)s_u[i];
-        double p = (double)s_p[i];
-        bool accept;
-        if (A.q) {
-            const double q = (double)s_q[i];
-            p -= a * q;
-            accept = u * q * mass < p;
-        } else {
-            for (int k = 0; k < drops; k++) if (s_drop[k] == s_tok[i]) p = 0.0;
-            accept = u * mass < p;
+    Walk w = A.walks[s * 2 + ((rounds - 1) & 1)];
+    double *sums = A.sums + ((size_t)w.half * gridDim.x + s) * A.pieces;
+    read_drafts(A, b, first, n, d);
+    auto sum_of = [&](const Left &l) {  // by this workgroup alone
+        __syncthreads();
+        for (int k = 0; k < A.pieces; k++) {
+            const int c0 = k * VF_PIECE;
+            const double v = piece_sum<VF_LAST>(l, c0, min(VF_PIECE, A.cols - c0), s_red);
+            if (tid == 0) sums[k] = v;
         }
-        if (accept) {
-            if (tid == 0) { tokens[kept] = s_tok[i]; path[kept + 1] = i; }
-            kept++;
-            node = i;
-            a = 0.0; mass = 1.0; drops = 0;
-            continue;
-        }
-        if (A.q) {
-            a += mass;
-            const size_t at = (size_t)(first + node) * A.cols;
-            mass = left_sum(Left{A.p + at, A.q + at, a, nullptr, 0}, A.cols, s_red, s_tile);
-        } else {
-            mass -= p > 0.0 ? p : 0.0;
-            __syncthreads();
-            if (tid == 0) s_drop[drops] = s_tok[i];
-            drops++;
-            __syncthreads();
-        }
+        __threadfence_block();
+        __syncthreads();
+        return all_pieces<VF_LAST>(sums, A.pieces, s_red);
+    };
+    double total = all_pieces<VF_LAST>(sums, A.pieces, s_red);
+    while (w.state == WALK_SUM) {
+        w.mass = total;
+        walk_on(w, d, n, A.q != nullptr, true);
+        if (w.state != WALK_DRAW) total = sum_of(left_of(A, w, d, first));
     }
-    const size_t at = (size_t)(first + node) * A.cols;
-    Left l{A.p + at, A.q ? A.q + at : nullptr, a, s_drop, drops};
-    double total = left_sum(l, A.cols, s_red, s_tile);
-    if (!(total > 0.0)) {
-        l = Left{A.p + at, nullptr, 0.0, s_drop, 0};
-        total = left_sum(l, A.cols, s_red, s_tile);
+    Left l = left_of(A, w, d, first);
+    if (!(total > 0.0)) {  // nothing is left: the row's own distribution
+        l = Left{l.p, nullptr, 0.0, 0, d.token};
+        total = sum_of(l);
     }
-    const int pick = left_pick(l, A.cols, (double)A.u_last[s] * total, s_red, s_tile, s_int);
-    if (tid == 0) { tokens[kept] = pick; A.count[s] = kept + 1; }
+    // The piece in which the running sum passes the goal (the last one with something in it, should rounding keep it
+    // below), then the token there.  Only tokens with something left are taken, so that the two steps' roundings
+    // cannot pick another.
+    const double goal = (double)A.u_last[s] * total;
+    int pick = -1, piece = -1;
+    double at = 0.0, before = 0.0;
+    for (int k0 = 0; k0 < A.pieces; k0 += 64) {  // the same in every wave
+        const double v = k0 + lane < A.pieces ? sums[k0 + lane] : 0.0;
+        double upto = v;
+#pragma unroll
+        for (int x = 1; x < 64; x *= 2) {
+            const double y = __shfl_up(upto, x);
+            if (lane >= x) upto += y;
+        }
+        const unsigned long long some = __ballot(v > 0.0), pass = __ballot(v > 0.0 && before + upto > goal);
+        if (pass || some) {
+            const int k = pass ? __builtin_ctzll(pass) : 63 - __builtin_clzll(some);
+            piece = k0 + k;
+            at = before + __shfl(upto, k) - __shfl(v, k);
+        }
+        if (pass) break;
+        before += __shfl(upto, 63);
+    }
+    if (piece >= 0) {
+        double v[4], mine = 0.0;
+        const int i0 = piece * VF_PIECE + 4 * tid;  // four tokens in a row per thread
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            v[j] = i0 + j < A.cols ? l.at(i0 + j) : 0.0;
+            mine += v[j];
+        }
+        double upto = mine;
+#pragma unroll
+        for (int x = 1; x < 64; x *= 2) {
+            const double y = __shfl_up(upto, x);
+            if (lane >= x) upto += y;
+        }
+        __syncthreads();
+        if (lane == 63) s_red[wave] = upto;
+        if (tid < 2) s_int[tid] = tid ? -1 : 0x7fffffff;
+        __syncthreads();
+        double sum = at;
+        for (int k = 0; k < wave; k++) sum += s_red[k];
+        sum += upto - mine;
+        int first_past = 0x7fffffff, last = -1;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            sum += v[j];
+            if (v[j] > 0.0) {
+                last = i0 + j;
+                if (sum > goal && first_past == 0x7fffffff) first_past = i0 + j;
+            }
+        }
+        if (last >= 0) atomicMax(&s_int[1], last);
+        if (first_past != 0x7fffffff) atomicMin(&s_int[0], first_past);
+        __syncthreads();
+        pick = s_int[0] != 0x7fffffff ? s_int[0] : s_int[1];
+    }
+    // the accepted rows are an ascending path
+    const int kept = __popcll(w.taken);
+    if (tid < b.max_rows) {
+        int row = -1, said = -1;
+        unsigned long long rest = w.taken;
+        for (int k = 0; k < tid; k++) rest &= rest - 1;
+        if (tid < kept) {
+            row = __builtin_ctzll(rest);
+            rest &= rest - 1;
+            said = rest ? d.token[__builtin_ctzll(rest)] : pick;
+        }
+        path[tid] = row;
+        tokens[tid] = said;
+    }
+    if (tid == 0) A.count[s] = kept;
 }
+// Sums by launches over the whole card; a tree's later ones (each takes another
+// rejection with drafts left to try) are few and fall to the drawing workgroup.
+int verify_rounds(const BatchView &b, bool sampled) { return b.parent && sampled ? 4 : 1; }
 
 }  // namespace
 
@@ -371,17 +606,15 @@ int qg_qk_norm_rope(float *q_out, float *k_out, const qg_qk_rows *in, const qg_k
     const RopeArgs A{q_out, k_out, in->q, in->k, in->v, in->q_row, in->q_head, in->k_row, in->k_head, in->v_row, in->v_head,
                      in->q_norm, in->k_norm, in->freq, in->position, in->eps, in->rows, in->q_heads, in->kv_heads, in->rope_dims,
                      in->interleaved != 0, cache != nullptr};
-    const int heads = in->q_heads + in->kv_heads * (cache ? 2 : 1), per = 4 * (256 / D);
-    const dim3 grid(in->rows, (heads + per - 1) / per);
-    if (D == 64) qk_rope_kernel<64><<<grid, 256, 0, qg_stream()>>>(A, c, b, layer);
-    else if (D == 128) qk_rope_kernel<128><<<grid, 256, 0, qg_stream()>>>(A, c, b, layer);
-    else qk_rope_kernel<256><<<grid, 256, 0, qg_stream()>>>(A, c, b, layer);
+    if (D == 64) launch_rope<64>(A, c, b, layer, qg_stream());
+    else if (D == 128) launch_rope<128>(A, c, b, layer, qg_stream());
+    else launch_rope<256>(A, c, b, layer, qg_stream());
     return hipGetLastError();
 }
 
 size_t qg_softmax_workspace_bytes(int rows, int cols) {
     if (rows < 1 || rows > QG_MAX_ROWS || cols < 1 || cols > 1 << 24) return 0;
-    return 16;
+    return softmax_pieces(rows, cols) ? (size_t)rows * ((cols + SM_PIECE - 1) / SM_PIECE) * sizeof(SoftPart) : sizeof(SoftPart);
 }
 
 int qg_softmax(float *out, const float *x, int rows, int cols, float temperature, void *ws, size_t ws_bytes) {
@@ -389,14 +622,26 @@ int qg_softmax(float *out, const float *x, int rows, int cols, float temperature
     if (!need || !out || !x || !ws || ws_bytes < need || (((uintptr_t)out | (uintptr_t)x) & 3) || ((uintptr_t)ws & 15)) return hipErrorInvalidValue;
     if (!(temperature >= 0.0f) || !__builtin_isfinite(temperature)) return hipErrorInvalidValue;
     const size_t bytes = 4 * (size_t)rows * cols;
-    if (out != x && qg_overlap(out, bytes, x, bytes)) return hipErrorInvalidValue;
-    softmax_row_kernel<<<rows, SM_THREADS, 0, qg_stream()>>>(out, x, cols, temperature > 0.0f ? 1.0f / temperature : 0.0f);
+    if ((out != x && qg_overlap(out, bytes, x, bytes)) || qg_overlap(ws, need, x, bytes) || qg_overlap(ws, need, out, bytes)) return hipErrorInvalidValue;
+    // log2 e / T, finite and not 0, which stands for temperature 0
+    const float scale = temperature > 0.0f ? fminf(fmaxf(1.44269504088896341f / temperature, 1e-37f), 3e38f) : 0.0f;
+    if (softmax_pieces(rows, cols)) {
+        const dim3 grid((cols + SM_PIECE - 1) / SM_PIECE, rows);
+        softmax_piece_kernel<false><<<grid, SM_THREADS, 0, qg_stream()>>>(out, x, cols, scale, (SoftPart *)ws);
+        softmax_piece_kernel<true><<<grid, SM_THREADS, 0, qg_stream()>>>(out, x, cols, scale, (SoftPart *)ws);
+    } else if (cols <= 4096) {
+        softmax_row_kernel<256, 16, 0><<<rows, 256, 0, qg_stream()>>>(out, x, cols, scale);
+    } else if (cols <= 16384) {
+        softmax_row_kernel<1024, 16, 0><<<rows, 1024, 0, qg_stream()>>>(out, x, cols, scale);
+    } else {
+        softmax_row_kernel<1024, 96, 36><<<rows, 1024, 0, qg_stream()>>>(out, x, cols, scale);
+    }
     return hipGetLastError();
 }
 
 size_t qg_verify_workspace_bytes(int sequences, int cols) {
     if (sequences < 1 || sequences > QG_MAX_SEQUENCES || cols < 1 || cols > 1 << 24) return 0;
-    return 16;
+    return 2 * (size_t)sequences * (((size_t)cols + VF_PIECE - 1) / VF_PIECE * sizeof(double) + sizeof(Walk));
 }
 
 int qg_verify_drafts(int *tokens_out, int *path, int *count, const float *p, const float *q, const int *token, const float *u,
@@ -408,8 +653,11 @@ int qg_verify_drafts(int *tokens_out, int *path, int *count, const float *p, con
     if (((uintptr_t)tokens_out | (uintptr_t)path | (uintptr_t)count | (uintptr_t)p | (uintptr_t)q | (uintptr_t)token | (uintptr_t)u |
          (uintptr_t)u_last) & 3)
         return hipErrorInvalidValue;
-    const VerifyArgs A{tokens_out, path, count, p, q, u, u_last, token, cols};
-    verify_kernel<<<sequences, SM_THREADS, 0, qg_stream()>>>(A, b);
+    const int pieces = (cols + VF_PIECE - 1) / VF_PIECE, rounds = verify_rounds(b, q != nullptr);
+    Walk *walks = (Walk *)ws;
+    const VerifyArgs A{tokens_out, path, count, p, q, u, u_last, token, cols, pieces, (double *)(walks + 2 * sequences), walks};
+    for (int r = 0; r < rounds; r++) verify_sum_kernel<<<dim3(pieces, sequences), VF_THREADS, 0, qg_stream()>>>(A, b, r);
+    verify_draw_kernel<<<sequences, VF_LAST, 0, qg_stream()>>>(A, b, rounds);
     return hipGetLastError();
 }
 
