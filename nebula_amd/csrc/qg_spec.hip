@@ -300,16 +300,20 @@ bool softmax_pieces(int rows, int cols) { return rows < 128 && cols > SM_PIECE; 
 // the last kernel draws the token.  A chain has one sum: it ends at its first
 // rejection.
 // ------------------------------------------------------------------------
-constexpr int VF_THREADS = 256, VF_REGS = 16, VF_PIECE = VF_THREADS * VF_REGS, VF_LAST = 1024;
+constexpr int VF_THREADS = 256, VF_BLOCK = 4096, VF_LAST = 1024;
 
+// A draft, in the lane of its place: its token and parent, its number, and its
+// probabilities at the row that it continues.  Every wave holds them all.
+struct Draft { float p, q, u; int token, up; };
 struct Walk;
 struct VerifyArgs {
     int *tokens_out, *path, *count;
     const float *p, *q, *u, *u_last;
     const int *token;
-    int cols, pieces;
+    int cols, piece, pieces; // a piece: whole blocks of VF_BLOCK tokens
     double *sums;            // [2][sequences][pieces], likewise
     Walk *walks;             // [sequences][2], the last round's and this one's
+    Draft *drafts;           // [sequences][QG_MAX_TREE], as the first round read them
 };
 // Where a sequence's walk stands: the accepted rows, the rejected drafts of the
 // current row, and what is left of its distribution.
@@ -320,60 +324,63 @@ struct Walk {
 };
 enum { WALK_SUM = 0, WALK_DRAW_SUM = 1, WALK_DRAW = 2 };  // needs a sum; needs one and then draws; draws
 
-// A sequence's drafts in shared memory: token, parent, number, and the
-// probabilities of each at the row that it continues.
-struct Drafts {
-    float p[QG_MAX_TREE], q[QG_MAX_TREE], u[QG_MAX_TREE];
-    int token[QG_MAX_TREE], up[QG_MAX_TREE];
-};
-QG_DEV void read_drafts(const VerifyArgs &A, const BatchView &b, int first, int n, Drafts &d) {
-    const int i = threadIdx.x;
-    if (i < n) {
-        const int r = first + i, x = A.token[r];
-        int up = b.parent ? tree_parent(b.parent[r], i) : i - 1;
-        if ((unsigned)x >= (unsigned)A.cols) up = -1;
-        d.token[i] = x;
-        d.up[i] = up;
-        d.u[i] = A.u[r];
-        const size_t at = (size_t)(first + max(up, 0)) * A.cols + x;
-        d.p[i] = up >= 0 ? A.p[at] : 0.0f;
-        d.q[i] = up >= 0 && A.q ? A.q[at] : 0.0f;
+QG_DEV Draft read_draft(const VerifyArgs &A, const BatchView &b, int first, int n, int lane) {
+    Draft d{0.0f, 0.0f, 0.0f, 0, -1};
+    if (lane < n) {
+        const int r = first + lane;
+        d.token = A.token[r];
+        d.up = b.parent ? tree_parent(b.parent[r], lane) : lane - 1;
+        d.u = A.u[r];
+        if ((unsigned)d.token >= (unsigned)A.cols) d.up = -1;
+        if (d.up >= 0) {
+            const size_t at = (size_t)(first + d.up) * A.cols + d.token;
+            d.p = A.p[at];
+            if (A.q) d.q = A.q[at];
+        }
     }
-    __syncthreads();
+    return d;
 }
-// Takes the walk on until a sum is needed or a token can be drawn (the same in
-// every thread).  summed: mass is the sum of what is left at (node, a).
-QG_DEV void walk_on(Walk &w, const Drafts &d, int n, bool sampled, bool summed) {
-    for (int i = w.next; i < n; i++) {
-        if (d.up[i] != w.node) continue;
-        const double u = (double)d.u[i];
-        double p = (double)d.p[i];
-        bool accept;
-        if (sampled) {
-            const double q = (double)d.q[i];
-            p -= w.a * q;
-            accept = u * q * w.mass < p;
-        } else {
-            for (unsigned long long g = w.gone; g; g &= g - 1)
-                if (d.token[__builtin_ctzll(g)] == d.token[i]) p = 0.0;
-            accept = u * w.mass < p;
-        }
-        summed = false;
-        if (accept) {
-            w.taken |= 1ULL << i;
-            w.node = i;
-            w.a = 0.0; w.mass = 1.0; w.gone = 0;
-        } else if (sampled) {
-            w.a += w.mass;
+QG_DEV float lane_f(float x, int l) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), l)); }
+QG_DEV unsigned long long same_u64(unsigned long long x) {  // of a value that all lanes share: in scalar registers
+    return (unsigned long long)__builtin_amdgcn_readfirstlane((int)(x >> 32)) << 32 | (unsigned)__builtin_amdgcn_readfirstlane((int)x);
+}
+// Takes the walk on until a sum is needed or a token can be drawn, by a whole wave.
+// summed: mass is the sum of what is left at (node, a).
+QG_DEV void walk_on(Walk &w, const Draft &d, bool sampled, bool summed) {
+    for (;;) {
+        // the row's drafts that are still to be tried, in order
+        unsigned long long drafts = __ballot(d.up == w.node && (int)(threadIdx.x & 63) >= w.next);
+        bool moved = false;
+        for (; drafts && !moved; drafts &= drafts - 1) {
+            const int i = __builtin_ctzll(drafts);
+            const double u = (double)lane_f(d.u, i);
+            double p = (double)lane_f(d.p, i);
+            summed = false;
+            if (sampled) {
+                const double q = (double)lane_f(d.q, i);
+                p -= w.a * q;
+                moved = u * q * w.mass < p;
+            } else {
+                const int x = __builtin_amdgcn_readlane(d.token, i);
+                if (__ballot(d.token == x) & w.gone) p = 0.0;
+                moved = u * w.mass < p;
+            }
             w.next = i + 1;
-            w.state = WALK_SUM;
-            return;
-        } else {
-            w.mass -= p > 0.0 ? p : 0.0;
-            w.gone |= 1ULL << i;
+            if (moved) {
+                w.taken |= 1ULL << i;
+                w.node = i;
+                w.a = 0.0; w.mass = 1.0; w.gone = 0;
+            } else if (sampled) {
+                w.a += w.mass;
+                w.state = WALK_SUM;
+                return;
+            } else {
+                w.mass -= p > 0.0 ? p : 0.0;
+                w.gone |= 1ULL << i;
+            }
         }
+        if (!moved) break;
     }
-    w.next = n;
     w.state = summed ? WALK_DRAW : WALK_DRAW_SUM;
 }
 // What is left of token i at a row: max(p - a q, 0), or p without the rejected tokens.
@@ -381,67 +388,92 @@ struct Left {
     const float *p, *q;
     double a;
     unsigned long long gone;
-    const int *token;
+    int token;  // the lane's draft
     __device__ __forceinline__ double of(float pi, float qi, int i) const {
         double w = (double)pi;
         if (q) w -= a * (double)qi;
-        else for (unsigned long long g = gone; g; g &= g - 1) w = token[__builtin_ctzll(g)] == i ? 0.0 : w;
+        else for (unsigned long long g = gone; g; g &= g - 1) w = __builtin_amdgcn_readlane(token, __builtin_ctzll(g)) == i ? 0.0 : w;
         return w > 0.0 ? w : 0.0;
     }
     __device__ __forceinline__ double at(int i) const { return of(p[i], q ? q[i] : 0.0f, i); }
 };
-QG_DEV Left left_of(const VerifyArgs &A, const Walk &w, const Drafts &d, int first) {
+QG_DEV Left left_of(const VerifyArgs &A, const Walk &w, const Draft &d, int first) {
     const size_t at = (size_t)(first + w.node) * A.cols;
-    return Left{A.p + at, A.q ? A.q + at : nullptr, w.a, w.gone, d.token};
+    return Left{A.p + at, A.q ? A.q + at : nullptr, w.a, same_u64(w.gone), d.token};
 }
-// The sum over a piece, in every thread of THREADS.
+// The sum over tokens c0 .. end - 1, in every thread of THREADS.
 template <int THREADS>
-QG_DEV double piece_sum(const Left &l, int c0, int n, double *s) {
-    constexpr int R = VF_PIECE / THREADS;
-    float p[R], q[R];
+QG_DEV double piece_sum(const Left &l, int c0, int end, double *s) {
+    constexpr int R = VF_BLOCK / THREADS;
+    double v = 0.0;
+    for (; c0 + VF_BLOCK <= end; c0 += VF_BLOCK) {
+        const float *at = l.p + c0 + threadIdx.x, *by = (l.q ? l.q : l.p) + c0 + threadIdx.x;
+        float p[R], q[R];
 #pragma unroll
-    for (int k = 0; k < R; k++) {
-        const int i = k * THREADS + threadIdx.x;
-        p[k] = i < n ? l.p[c0 + i] : 0.0f;
-        q[k] = i < n && l.q ? l.q[c0 + i] : 0.0f;
+        for (int k = 0; k < R; k++) p[k] = at[k * THREADS];
+        if (l.q) {
+#pragma unroll
+            for (int k = 0; k < R; k++) q[k] = by[k * THREADS];
+        }
+#pragma unroll
+        for (int k = 0; k < R; k++) v += l.of(p[k], q[k], c0 + k * THREADS + threadIdx.x);
     }
-    double v = 0.0;
-#pragma unroll
-    for (int k = 0; k < R; k++) v += l.of(p[k], q[k], c0 + k * THREADS + threadIdx.x);
+    for (int i = c0 + threadIdx.x; i < end; i += THREADS) v += l.at(i);
     return block_all<THREADS>(v, s, Added());
 }
-// The sum over all pieces' sums, in every thread.
-template <int THREADS>
-QG_DEV double all_pieces(const double *sums, int pieces, double *s) {
-    double v = 0.0;
-    for (int i = threadIdx.x; i < pieces; i += THREADS) v += sums[i];
-    return block_all<THREADS>(v, s, Added());
+// The pieces' sums of the half that holds them, in order, 64 to a wave's lanes;
+// both halves are read before it is known which (the first 64 of each, `ahead`).
+struct Ahead { double v[2]; };
+QG_DEV Ahead pieces_ahead(const VerifyArgs &A, int sequences, int s, int lane) {
+    Ahead x;
+#pragma unroll
+    for (int h = 0; h < 2; h++) x.v[h] = lane < A.pieces ? A.sums[((size_t)h * sequences + s) * A.pieces + lane] : 0.0;
+    return x;
+}
+QG_DEV double wave_upto(double v, int lane) {  // inclusive sums over the lanes
+#pragma unroll
+    for (int x = 1; x < 64; x *= 2) {
+        const double y = __shfl_up(v, x);
+        if (lane >= x) v += y;
+    }
+    return v;
+}
+// Their sum, in every lane of every wave.
+QG_DEV double all_pieces(const double *sums, int pieces, double ahead, int lane) {
+    double total = 0.0;
+    for (int k0 = 0; k0 < pieces; k0 += 64)
+        total += __shfl(wave_upto(k0 == 0 ? ahead : k0 + lane < pieces ? sums[k0 + lane] : 0.0, lane), 63);
+    return total;
 }
 
 // One sum: workgroup x of sequence y takes the walk to its next sum and adds its
 // piece of it.  round 0 starts the walk.
 __global__ __launch_bounds__(VF_THREADS) void verify_sum_kernel(VerifyArgs A, BatchView b, int round) {
-    __shared__ Drafts d;
     __shared__ double s_red[4];
-    const int s = blockIdx.y;
+    const int s = blockIdx.y, lane = threadIdx.x & 63;
     int first, n;
     batch_rows(b, s, first, n);
     if (n == 0) return;
     Walk w{1, 0, 0.0, 1.0, 0, 1, 0, WALK_SUM};
+    Draft d;
     if (round) {
         w = A.walks[s * 2 + ((round - 1) & 1)];
         if (w.state != WALK_SUM) {  // decided: the next kernel finds it where it looks
             if (blockIdx.x == 0 && threadIdx.x == 0) A.walks[s * 2 + (round & 1)] = w;
             return;
         }
-        w.mass = all_pieces<VF_THREADS>(A.sums + ((size_t)w.half * gridDim.y + s) * A.pieces, A.pieces, s_red);
+        const Ahead x = pieces_ahead(A, gridDim.y, s, lane);
+        d = A.drafts[s * QG_MAX_TREE + lane];
+        w.mass = all_pieces(A.sums + ((size_t)w.half * gridDim.y + s) * A.pieces, A.pieces, w.half ? x.v[1] : x.v[0], lane);
+    } else {
+        d = read_draft(A, b, first, n, lane);
+        if (blockIdx.x == 0 && threadIdx.x < QG_MAX_TREE) A.drafts[s * QG_MAX_TREE + lane] = d;
     }
-    read_drafts(A, b, first, n, d);
-    walk_on(w, d, n, A.q != nullptr, round > 0);
+    walk_on(w, d, A.q != nullptr, round > 0);
     if (w.state != WALK_DRAW) {
         w.half = round & 1;
-        const int c0 = blockIdx.x * VF_PIECE;
-        const double v = piece_sum<VF_THREADS>(left_of(A, w, d, first), c0, min(VF_PIECE, A.cols - c0), s_red);
+        const int c0 = blockIdx.x * A.piece;
+        const double v = piece_sum<VF_THREADS>(left_of(A, w, d, first), c0, min(c0 + A.piece, A.cols), s_red);
         if (threadIdx.x == 0) A.sums[((size_t)w.half * gridDim.y + s) * A.pieces + blockIdx.x] = v;
     }
     if (blockIdx.x == 0 && threadIdx.x == 0) A.walks[s * 2 + (round & 1)] = w;
@@ -449,9 +481,8 @@ __global__ __launch_bounds__(VF_THREADS) void verify_sum_kernel(VerifyArgs A, Ba
 
 // The rest of the walk and the last token, a workgroup per sequence.
 __global__ __launch_bounds__(VF_LAST) void verify_draw_kernel(VerifyArgs A, BatchView b, int rounds) {
-    __shared__ Drafts d;
     __shared__ double s_red[16];
-    __shared__ int s_int[2];
+    __shared__ int2 s_got[VF_LAST / 64];
     const int s = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     int first, n;
     batch_rows(b, s, first, n);
@@ -461,29 +492,30 @@ __global__ __launch_bounds__(VF_LAST) void verify_draw_kernel(VerifyArgs A, Batc
         if (tid == 0) A.count[s] = 0;
         return;
     }
+    const Ahead x = pieces_ahead(A, gridDim.x, s, lane);
     Walk w = A.walks[s * 2 + ((rounds - 1) & 1)];
-    double *sums = A.sums + ((size_t)w.half * gridDim.x + s) * A.pieces;
-    read_drafts(A, b, first, n, d);
+    const Draft d = A.drafts[s * QG_MAX_TREE + lane];
+    double *sums = A.sums + ((size_t)w.half * gridDim.x + s) * A.pieces, ahead = (w.half ? x.v[1] : x.v[0]);
     auto sum_of = [&](const Left &l) {  // by this workgroup alone
         __syncthreads();
         for (int k = 0; k < A.pieces; k++) {
-            const int c0 = k * VF_PIECE;
-            const double v = piece_sum<VF_LAST>(l, c0, min(VF_PIECE, A.cols - c0), s_red);
+            const double v = piece_sum<VF_LAST>(l, k * A.piece, min((k + 1) * A.piece, A.cols), s_red);
             if (tid == 0) sums[k] = v;
         }
         __threadfence_block();
         __syncthreads();
-        return all_pieces<VF_LAST>(sums, A.pieces, s_red);
+        ahead = lane < A.pieces ? sums[lane] : 0.0;
+        return all_pieces(sums, A.pieces, ahead, lane);
     };
-    double total = all_pieces<VF_LAST>(sums, A.pieces, s_red);
+    double total = all_pieces(sums, A.pieces, ahead, lane);
     while (w.state == WALK_SUM) {
         w.mass = total;
-        walk_on(w, d, n, A.q != nullptr, true);
+        walk_on(w, d, A.q != nullptr, true);
         if (w.state != WALK_DRAW) total = sum_of(left_of(A, w, d, first));
     }
     Left l = left_of(A, w, d, first);
     if (!(total > 0.0)) {  // nothing is left: the row's own distribution
-        l = Left{l.p, nullptr, 0.0, 0, d.token};
+        l = Left{l.p, nullptr, 0.0, 0, 0};
         total = sum_of(l);
     }
     // The piece in which the running sum passes the goal (the last one with something in it, should rounding keep it
@@ -493,13 +525,7 @@ __global__ __launch_bounds__(VF_LAST) void verify_draw_kernel(VerifyArgs A, Batc
     int pick = -1, piece = -1;
     double at = 0.0, before = 0.0;
     for (int k0 = 0; k0 < A.pieces; k0 += 64) {  // the same in every wave
-        const double v = k0 + lane < A.pieces ? sums[k0 + lane] : 0.0;
-        double upto = v;
-#pragma unroll
-        for (int x = 1; x < 64; x *= 2) {
-            const double y = __shfl_up(upto, x);
-            if (lane >= x) upto += y;
-        }
+        const double v = k0 == 0 ? ahead : k0 + lane < A.pieces ? sums[k0 + lane] : 0.0, upto = wave_upto(v, lane);
         const unsigned long long some = __ballot(v > 0.0), pass = __ballot(v > 0.0 && before + upto > goal);
         if (pass || some) {
             const int k = pass ? __builtin_ctzll(pass) : 63 - __builtin_clzll(some);
@@ -509,56 +535,66 @@ __global__ __launch_bounds__(VF_LAST) void verify_draw_kernel(VerifyArgs A, Batc
         if (pass) break;
         before += __shfl(upto, 63);
     }
-    if (piece >= 0) {
+    bool found = false;
+    for (int c0 = piece * A.piece; piece >= 0 && !found && c0 < min((piece + 1) * A.piece, A.cols); c0 += VF_BLOCK) {
         double v[4], mine = 0.0;
-        const int i0 = piece * VF_PIECE + 4 * tid;  // four tokens in a row per thread
+        const int i0 = c0 + 4 * tid;  // four tokens in a row per thread
 #pragma unroll
         for (int j = 0; j < 4; j++) {
             v[j] = i0 + j < A.cols ? l.at(i0 + j) : 0.0;
             mine += v[j];
         }
-        double upto = mine;
-#pragma unroll
-        for (int x = 1; x < 64; x *= 2) {
-            const double y = __shfl_up(upto, x);
-            if (lane >= x) upto += y;
-        }
+        const double upto = wave_upto(mine, lane);
         __syncthreads();
         if (lane == 63) s_red[wave] = upto;
-        if (tid < 2) s_int[tid] = tid ? -1 : 0x7fffffff;
         __syncthreads();
-        double sum = at;
-        for (int k = 0; k < wave; k++) sum += s_red[k];
-        sum += upto - mine;
-        int first_past = 0x7fffffff, last = -1;
+        // each wave's first token past the goal, or its last one with something left
+        double sum = at + (upto - mine), block = 0.0;
+#pragma unroll
+        for (int k = 0; k < VF_LAST / 64; k++) {
+            const double x = s_red[k];
+            block += x;
+            if (k < wave) sum += x;
+        }
+        at += block;
+        int past = -1, last = -1;
 #pragma unroll
         for (int j = 0; j < 4; j++) {
             sum += v[j];
             if (v[j] > 0.0) {
                 last = i0 + j;
-                if (sum > goal && first_past == 0x7fffffff) first_past = i0 + j;
+                if (sum > goal && past < 0) past = i0 + j;
             }
         }
-        if (last >= 0) atomicMax(&s_int[1], last);
-        if (first_past != 0x7fffffff) atomicMin(&s_int[0], first_past);
+        const unsigned long long passes = __ballot(past >= 0), some = __ballot(last >= 0);
+        const int got = passes ? __shfl(past, __builtin_ctzll(passes)) : some ? __shfl(last, 63 - __builtin_clzll(some)) : -1;
+        if (lane == 0) s_got[wave] = make_int2(got, passes != 0);
         __syncthreads();
-        pick = s_int[0] != 0x7fffffff ? s_int[0] : s_int[1];
+        for (int k = 0; k < VF_LAST / 64 && !found; k++) {  // the first that passes, else the last one
+            const int2 x = s_got[k];
+            if (x.x >= 0) pick = x.x;
+            found = x.y;
+        }
     }
     // the accepted rows are an ascending path
     const int kept = __popcll(w.taken);
-    if (tid < b.max_rows) {
-        int row = -1, said = -1;
-        unsigned long long rest = w.taken;
-        for (int k = 0; k < tid; k++) rest &= rest - 1;
-        if (tid < kept) {
-            row = __builtin_ctzll(rest);
-            rest &= rest - 1;
-            said = rest ? d.token[__builtin_ctzll(rest)] : pick;
-        }
-        path[tid] = row;
-        tokens[tid] = said;
+    if (tid >= kept && tid < b.max_rows) path[tid] = tokens[tid] = -1;
+    if (tid < n && w.taken >> tid & 1) {
+        const int k = __popcll(w.taken & ((1ULL << tid) - 1));
+        path[k] = tid;
+        if (k) tokens[k - 1] = d.token;
     }
-    if (tid == 0) A.count[s] = kept;
+    if (tid == 0) {
+        tokens[kept - 1] = pick;
+        A.count[s] = kept;
+    }
+}
+// The tokens of a piece and their number: pieces of a block for few sequences, of
+// more for many, whose workgroups are enough and whose walks then cost less.
+struct Pieces { size_t x, y; };
+Pieces verify_pieces(int sequences, int cols) {
+    const size_t blocks = ((size_t)cols + VF_BLOCK - 1) / VF_BLOCK, per = (blocks * sequences + 2047) / 2048;
+    return Pieces{per * VF_BLOCK, (blocks + per - 1) / per};
 }
 // Sums by launches over the whole card; a tree's later ones (each takes another
 // rejection with drafts left to try) are few and fall to the drawing workgroup.
@@ -641,7 +677,8 @@ int qg_softmax(float *out, const float *x, int rows, int cols, float temperature
 
 size_t qg_verify_workspace_bytes(int sequences, int cols) {
     if (sequences < 1 || sequences > QG_MAX_SEQUENCES || cols < 1 || cols > 1 << 24) return 0;
-    return 2 * (size_t)sequences * (((size_t)cols + VF_PIECE - 1) / VF_PIECE * sizeof(double) + sizeof(Walk));
+    return 2 * (size_t)sequences * (verify_pieces(sequences, cols).y * sizeof(double) + sizeof(Walk)) +
+           (size_t)sequences * QG_MAX_TREE * sizeof(Draft);
 }
 
 int qg_verify_drafts(int *tokens_out, int *path, int *count, const float *p, const float *q, const int *token, const float *u,
@@ -653,10 +690,12 @@ int qg_verify_drafts(int *tokens_out, int *path, int *count, const float *p, con
     if (((uintptr_t)tokens_out | (uintptr_t)path | (uintptr_t)count | (uintptr_t)p | (uintptr_t)q | (uintptr_t)token | (uintptr_t)u |
          (uintptr_t)u_last) & 3)
         return hipErrorInvalidValue;
-    const int pieces = (cols + VF_PIECE - 1) / VF_PIECE, rounds = verify_rounds(b, q != nullptr);
+    const Pieces pieces = verify_pieces(sequences, cols);
+    const int rounds = verify_rounds(b, q != nullptr);
     Walk *walks = (Walk *)ws;
-    const VerifyArgs A{tokens_out, path, count, p, q, u, u_last, token, cols, pieces, (double *)(walks + 2 * sequences), walks};
-    for (int r = 0; r < rounds; r++) verify_sum_kernel<<<dim3(pieces, sequences), VF_THREADS, 0, qg_stream()>>>(A, b, r);
+    const VerifyArgs A{tokens_out, path, count, p, q, u, u_last, token, cols, (int)pieces.x, (int)pieces.y, (double *)(walks + 2 * sequences), walks,
+                       (Draft *)((double *)(walks + 2 * sequences) + 2 * (size_t)sequences * pieces.y)};
+    for (int r = 0; r < rounds; r++) verify_sum_kernel<<<dim3((unsigned)pieces.y, sequences), VF_THREADS, 0, qg_stream()>>>(A, b, r);
     verify_draw_kernel<<<sequences, VF_LAST, 0, qg_stream()>>>(A, b, rounds);
     return hipGetLastError();
 }
