@@ -181,6 +181,38 @@ QG_DEV int lowest_of(const float *x, int n, float m, int *s) {
     return block_all<THREADS>(at, s, Lower());
 }
 
+// N values of a thread, THREADS apart, from x[0..n) on: whole groups of G without
+// a bound per value, which would cost an address each.
+template <int THREADS, int N, int G, typename F>
+QG_DEV void read_spread(const float *x, int n, F put) {
+    const float *at = x + threadIdx.x;
+#pragma unroll
+    for (int k0 = 0; k0 < N; k0 += G) {
+        if ((k0 + G) * THREADS <= n) {
+#pragma unroll
+            for (int k = k0; k < k0 + G; k++) put(k, at[k * THREADS]);
+        } else {
+#pragma unroll
+            for (int k = k0; k < k0 + G; k++) put(k, k * THREADS + (int)threadIdx.x < n ? at[k * THREADS] : -__builtin_inff());
+        }
+    }
+}
+template <int THREADS, int N, int G, typename F>
+QG_DEV void write_spread(float *x, int n, F get) {
+    float *at = x + threadIdx.x;
+#pragma unroll
+    for (int k0 = 0; k0 < N; k0 += G) {
+        if ((k0 + G) * THREADS <= n) {
+#pragma unroll
+            for (int k = k0; k < k0 + G; k++) at[k * THREADS] = get(k);
+        } else {
+#pragma unroll
+            for (int k = k0; k < k0 + G; k++)
+                if (k * THREADS + (int)threadIdx.x < n) at[k * THREADS] = get(k);
+        }
+    }
+}
+
 // A workgroup per row.  REGS values of a thread stay in registers and KEPT in
 // shared memory between the three passes (largest value, sum, output); what is
 // longer is read again.
@@ -194,15 +226,12 @@ __global__ __launch_bounds__(THREADS) void softmax_row_kernel(float *out, const 
     float *to = out + (size_t)blockIdx.x * cols;
     const float none = -__builtin_inff();
     float r[REGS], m = none;
-#pragma unroll
-    for (int k = 0; k < REGS; k++) r[k] = k * THREADS + tid < cols ? row[k * THREADS + tid] : none;
-#pragma unroll 8
-    for (int k = 0; k < KEPT; k++) {
-        const int i = (REGS + k) * THREADS + tid;
-        const float v = i < cols ? row[i] : none;
-        s_x[k * THREADS + tid] = v;
-        m = fmaxf(m, v);
-    }
+    read_spread<THREADS, REGS, 8>(row, cols, [&](int k, float v) { r[k] = v; });
+    if constexpr (KEPT > 0)
+        read_spread<THREADS, KEPT, 4>(row + REGS * THREADS, cols - REGS * THREADS, [&](int k, float v) {
+            s_x[k * THREADS + tid] = v;
+            m = fmaxf(m, v);
+        });
     for (int i = HELD + tid; i < cols; i += THREADS) m = fmaxf(m, row[i]);
 #pragma unroll
     for (int k = 0; k < REGS; k++) m = fmaxf(m, r[k]);
@@ -225,13 +254,9 @@ __global__ __launch_bounds__(THREADS) void softmax_row_kernel(float *out, const 
     }
     for (int i = HELD + tid; i < cols; i += THREADS) sum += __builtin_amdgcn_exp2f((row[i] - m) * scale);
     const float inv = 1.0f / block_all<THREADS>(sum, s_f, Added());
-#pragma unroll
-    for (int k = 0; k < REGS; k++) if (k * THREADS + tid < cols) to[k * THREADS + tid] = r[k] * inv;
-#pragma unroll 8
-    for (int k = 0; k < KEPT; k++) {
-        const int i = (REGS + k) * THREADS + tid;
-        if (i < cols) to[i] = s_x[k * THREADS + tid] * inv;
-    }
+    write_spread<THREADS, REGS, 8>(to, cols, [&](int k) { return r[k] * inv; });
+    if constexpr (KEPT > 0)
+        write_spread<THREADS, KEPT, 4>(to + REGS * THREADS, cols - REGS * THREADS, [&](int k) { return s_x[k * THREADS + tid] * inv; });
     for (int i = HELD + tid; i < cols; i += THREADS) to[i] = __builtin_amdgcn_exp2f((row[i] - m) * scale) * inv;
 }
 
@@ -248,8 +273,7 @@ __global__ __launch_bounds__(SM_THREADS) void softmax_piece_kernel(float *out, c
     const float *row = x + (size_t)blockIdx.y * cols + c0, none = -__builtin_inff();
     parts += (size_t)blockIdx.y * pieces;
     float r[SM_REGS], m = none, sum = 0.0f;
-#pragma unroll
-    for (int k = 0; k < SM_REGS; k++) r[k] = k * SM_THREADS + tid < n ? row[k * SM_THREADS + tid] : none;
+    read_spread<SM_THREADS, SM_REGS, SM_REGS>(row, n, [&](int k, float v) { r[k] = v; });
     if (!LAST) {
 #pragma unroll
         for (int k = 0; k < SM_REGS; k++) m = fmaxf(m, r[k]);
@@ -279,13 +303,12 @@ __global__ __launch_bounds__(SM_THREADS) void softmax_piece_kernel(float *out, c
     at = block_all<SM_THREADS>(at, s_i, Lower());
     const bool nan = at == SM_NAN || m == __builtin_inff();
     const float inv = 1.0f / sum;
-#pragma unroll
-    for (int k = 0; k < SM_REGS; k++) {
-        const int i = k * SM_THREADS + tid;
+    const bool one = scale == 0.0f || m == none;
+    write_spread<SM_THREADS, SM_REGS, SM_REGS>(to, n, [&](int k) {
         float y = __builtin_amdgcn_exp2f((r[k] - m) * scale) * inv;
-        if (scale == 0.0f || m == none) y = m != none && c0 + i == at ? 1.0f : 0.0f;
-        if (i < n) to[i] = nan ? __builtin_nanf("") : y;
-    }
+        if (one) y = m != none && c0 + k * SM_THREADS + tid == at ? 1.0f : 0.0f;
+        return nan ? __builtin_nanf("") : y;
+    });
 }
 // Pieces where the rows alone would not fill the card.
 bool softmax_pieces(int rows, int cols) { return rows < 128 && cols > SM_PIECE; }
