@@ -111,18 +111,19 @@ QG_DEV int block_scan(int v, int *s_sum, int &total) {
 }
 
 // Reserve, one workgroup (its sums run over all sequences and over the free
-// pages in order); a wave per sequence looks at its entries.  An entry needs a
+// pages in order); 16 lanes look at a sequence's entries.  An entry needs a
 // page if it is empty, or if its page is held elsewhere too.  The second kind
 // is marked in the table as -2 - page while the sequences are counted, so that
 // every sequence judges by the holders before the call.  Pages are taken for
 // the whole batch or not at all: a sequence may keep a shared page only because
 // the others get copies of theirs.
-// ws: copies [sequences][2] for kv_cow_kernel, then the free pages found.
+// ws: the copies for kv_cow_kernel, number and (source, destination) pairs, then
+// the free pages found.
 __global__ __launch_bounds__(1024) void kv_reserve_kernel(KvView c, BatchView b, int *status, int *ws) {
     __shared__ int s_len[QG_MAX_SEQUENCES], s_rows[QG_MAX_SEQUENCES], s_page[QG_MAX_SEQUENCES], s_need[QG_MAX_SEQUENCES], s_sum[16];
-    __shared__ int s_found;
+    __shared__ int s_rank[QG_MAX_SEQUENCES];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, P = 1 << c.shift;
-    int *copies = ws, *free_pages = ws + 2 * c.sequences;
+    int *copies = ws + 2, *free_pages = copies + 2 * c.sequences;
     // each sequence's rows, and the page with room behind its tokens
     int st = 0, mine = -1;
     if (tid < c.sequences) {
@@ -151,11 +152,16 @@ __global__ __launch_bounds__(1024) void kv_reserve_kernel(KvView c, BatchView b,
     __syncthreads();
     if (tid < c.sequences) s_page[tid] = copied;
     __syncthreads();
-    for (int s = wave; s < c.sequences; s += 16) {
-        const int len = s_len[s], rows = s_rows[s], here = len >> c.shift, end = rows ? (len + rows + P - 1) >> c.shift : here;
+    // 16 lanes per sequence, four sequences per wave: what one waits for, all wait for
+    const int part = lane >> 4, l16 = lane & 15;
+    auto ours = [&](bool x) { return (unsigned)(__ballot(x) >> (16 * part)) & 0xffffu; };  // of the sequence's 16 lanes
+    for (int s0 = 0; s0 < c.sequences; s0 += 64) {
+        const int s = s0 + wave * 4 + part;
+        const bool live = s < c.sequences;
+        const int len = live ? s_len[s] : 0, rows = live ? s_rows[s] : 0, here = len >> c.shift;
+        const int end = rows ? (len + rows + P - 1) >> c.shift : here;
         int need = 0;
-        for (int j0 = here; j0 < end; j0 += 64) {
-            const int j = j0 + lane;
+        for (int j = here + l16; __any(j < end); j += 16) {
             bool take = false;
             if (j < end) {
                 int *entry = c.table + (size_t)s * c.table_pages + j;
@@ -164,9 +170,9 @@ __global__ __launch_bounds__(1024) void kv_reserve_kernel(KvView c, BatchView b,
                 take = none || (j == here && (len & (P - 1)) ? s_page[s] != 0 : c.refs[page] > 1);
                 if (take) *entry = none ? -1 : -2 - page;
             }
-            need += __popcll(__ballot(take));
+            need += __popc(ours(take));
         }
-        if (lane == 0) s_need[s] = need;
+        if (live && l16 == 0) s_need[s] = need;
     }
     __syncthreads();
     int total;
@@ -176,11 +182,11 @@ __global__ __launch_bounds__(1024) void kv_reserve_kernel(KvView c, BatchView b,
     int found = 0;
     for (int p0 = 0; p0 < c.pages && found < total; p0 += 16384) {
         unsigned mask = 0;
+        int held[16];
 #pragma unroll
-        for (int i = 0; i < 16; i++) {
-            const int p = p0 + tid * 16 + i;
-            if (p < c.pages && c.refs[p] == 0) mask |= 1u << i;
-        }
+        for (int i = 0; i < 16; i++) held[i] = c.refs[min(p0 + tid * 16 + i, c.pages - 1)];
+#pragma unroll
+        for (int i = 0; i < 16; i++) mask |= p0 + tid * 16 + i < c.pages && held[i] == 0 ? 1u << i : 0u;
         int sum;
         int at = found + block_scan(__popc(mask), s_sum, sum) - __popc(mask);
         for (; mask && at < total; mask &= mask - 1) free_pages[at++] = p0 + tid * 16 + __ffs(mask) - 1;
@@ -189,33 +195,37 @@ __global__ __launch_bounds__(1024) void kv_reserve_kernel(KvView c, BatchView b,
     if (tid < c.sequences) {
         if (s_rows[tid] && total > found) st = 1;
         status[tid] = st;
-        copies[2 * tid] = copies[2 * tid + 1] = -1;
         s_page[tid] = upto - need;  // the sequence's first page in the list
     }
+    // a copied page is its sequence's first
+    int n_copies;
+    const int rank = block_scan(copied, s_sum, n_copies);
+    if (tid < c.sequences) s_rank[tid] = rank - 1;
+    if (tid == 0) ws[0] = total <= found ? n_copies : 0;
     __syncthreads();  // free_pages and copies written above are read or written by other waves below
-    for (int s = wave; s < c.sequences; s += 16) {
-        if (!s_need[s]) continue;
-        const int len = s_len[s], here = len >> c.shift, end = (len + s_rows[s] + P - 1) >> c.shift;
-        int from = s_page[s];
-        const bool served = total <= found;
-        for (int j0 = here; j0 < end; j0 += 64) {
-            const int j = j0 + lane;
+    const bool served = total <= found;
+    for (int s0 = 0; s0 < c.sequences; s0 += 64) {
+        const int s = s0 + wave * 4 + part;
+        const bool live = s < c.sequences && s_need[s];
+        const int len = live ? s_len[s] : 0, here = len >> c.shift, end = live ? (len + s_rows[s] + P - 1) >> c.shift : here;
+        int from = live ? s_page[s] : 0;
+        for (int j = here + l16; __any(j < end); j += 16) {
             int *entry = c.table + (size_t)s * c.table_pages + j;
             const int mark = j < end ? *entry : 0;
             const bool take = mark < 0;
-            const unsigned long long all = __ballot(take);
+            const unsigned all = ours(take);
             if (take && served) {
-                const int page = free_pages[from + __popcll(all & ((1ULL << lane) - 1))];
+                const int page = free_pages[from + __popc(all & ((1u << l16) - 1))];
                 *entry = page;
                 c.refs[page] = 1;
                 if (mark < -1) {
                     atomicSub(&c.refs[-2 - mark], 1);
-                    if (j == here && (len & (P - 1))) { copies[2 * s] = -2 - mark; copies[2 * s + 1] = page; }
+                    if (j == here && (len & (P - 1))) { copies[2 * s_rank[s]] = -2 - mark; copies[2 * s_rank[s] + 1] = page; }
                 }
             } else if (take && mark < -1) {
                 *entry = -2 - mark;
             }
-            from += __popcll(all);
+            from += __popc(all);
         }
     }
 }
@@ -228,10 +238,13 @@ QG_DEV void copy_page(const KvView &c, int dst, int src, int layer, bool v, int 
     uint4 *to = (uint4 *)(base + dst * bytes);
     for (size_t i = (size_t)part * 256 + threadIdx.x; i < bytes / 16; i += (size_t)parts * 256) to[i] = from[i];
 }
-__global__ __launch_bounds__(256) void kv_cow_kernel(KvView c, const int *copies) {
-    const int src = copies[2 * blockIdx.x], dst = copies[2 * blockIdx.x + 1];
-    if (src < 0) return;
-    for (int i = blockIdx.z; i < 2 * c.layers; i += gridDim.z) copy_page(c, dst, src, i >> 1, i & 1, blockIdx.y, gridDim.y);
+__global__ __launch_bounds__(256) void kv_cow_kernel(KvView c, const int *ws, int parts) {
+    const int per = 2 * c.layers * parts;  // of one page: layers, k and v, parts
+    const long all = (long)ws[0] * per;
+    for (long i = blockIdx.x; i < all; i += gridDim.x) {
+        const int copy = (int)(i / per), x = (int)(i % per);
+        copy_page(c, ws[3 + 2 * copy], ws[2 + 2 * copy], x / parts >> 1, x / parts & 1, x % parts, parts);
+    }
 }
 __global__ __launch_bounds__(256) void kv_copy_pages_kernel(KvView c, const int *dst, const int *src, int n) {
     const int i = blockIdx.x, d = dst[i], s = src[i];
@@ -317,7 +330,7 @@ extern "C" {
 
 size_t qg_kv_workspace_bytes(const qg_kv_cache *cache) {
     if (qg_kv_check(cache, false, nullptr)) return 0;
-    const size_t fork = (size_t)cache->sequences * (cache->table_pages + 2), reserve = 2 * (size_t)cache->sequences + cache->pages;
+    const size_t fork = (size_t)cache->sequences * (cache->table_pages + 2), reserve = 2 + 2 * (size_t)cache->sequences + cache->pages;
     return 4 * (fork > reserve ? fork : reserve);
 }
 
@@ -327,7 +340,8 @@ int qg_kv_reserve(const qg_kv_cache *cache, const qg_kv_batch *batch, int *statu
     if (qg_kv_check(cache, true, &c) || qg_batch_check(batch, false, &b)) return hipErrorInvalidValue;
     if (!status || !ws || (((uintptr_t)status | (uintptr_t)ws) & 3) || ws_bytes < qg_kv_workspace_bytes(cache)) return hipErrorInvalidValue;
     kv_reserve_kernel<<<1, 1024, 0, qg_stream()>>>(c, b, status, (int *)ws);
-    kv_cow_kernel<<<dim3(c.sequences, (unsigned)page_parts(c), layer_parts(c)), 256, 0, qg_stream()>>>(c, (const int *)ws);
+    const long work = 2L * c.layers * page_parts(c) * c.sequences;
+    kv_cow_kernel<<<(unsigned)(work < 8192 ? work : 8192), 256, 0, qg_stream()>>>(c, (const int *)ws, (int)page_parts(c));
     return hipGetLastError();
 }
 
