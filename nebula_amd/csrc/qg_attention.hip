@@ -34,16 +34,20 @@ struct AttnArgs {
     const float *q;
     float *part_o;   // [slots][row group][D]
     float2 *part_ml; // [slots][row group]
-    int *odd;        // [rows][q_heads]: 1 where attention_join_kernel has to take the row up again
+    int4 *joins;     // [rows][q_heads]: what attention_join_kernel has to do, see Join
     float scale;     // times log2 e
-    int q_heads, group, layer, resident, slots;  // resident: workgroups that run at once
+    int q_heads, group, layer, resident, slots, run;  // resident: workgroups that run at once; run: see plan_find
+    unsigned group_inv;                          // 2^32 / group, rounded up
 };
 
-// How the work is cut, the same in every wave of both kernels.  Sequence s has
+// x / group for x < 2^24: the product is over by less than x / 2^32 < 1 / group.
+QG_DEV int by_group(const AttnArgs &A, int x) { return A.group == 1 ? x : (int)__umulhi((unsigned)x, A.group_inv); }
+
+// How the work is cut, the same in every wave.  Sequence s has
 // `groups` row groups and `keys` keys; its keys are cut into parts of `chunk`,
 // chosen so that about as many workgroups have work as run at once.
 struct Plan {
-    int s, first, n, len, groups, parts, chunk, part, z, h;  // of one unit
+    int s, first, n, len, groups, chunk, part, z, h;  // of one unit
     size_t slot;  // of part 0, row group 0, head 0 of the sequence
 };
 constexpr int CHUNK = 128;  // keys per workgroup, at least and in steps of
@@ -61,12 +65,13 @@ QG_DEV PlanLane plan_lane(const KvView &c, const BatchView &b, const AttnArgs &A
     return x;
 }
 
-// `mine`: the lane's sequence among the first 64, read once.  `unit` 0.. asks for a
-// unit of this workgroup's XCD, -1 for sequence `want`.  Units run through the
-// sequences (parts x heads x row groups), and an XCD takes a run of them, so that
-// row groups with the same keys meet in its L2.  False if there is no such unit.
+// The unit of a workgroup.  Units run through the sequences (parts x heads x row
+// groups) in runs that go to one XCD, so that row groups with the same keys meet
+// in its L2: an eighth of them all where they are alike (each XCD then gets as many
+// as it runs at once), sixteen and sixteen where a prompt's rows see more and more.
+// False if there is none.
 template <int RG>
-QG_DEV bool plan_find(const KvView &c, const BatchView &b, const AttnArgs &A, int lane, int block, int want, Plan &p) {
+QG_DEV bool plan_find(const KvView &c, const BatchView &b, const AttnArgs &A, int lane, int block, Plan &p) {
     const PlanLane mine = plan_lane<RG>(c, b, A, lane);
     // a sum over all sequences of what `f` says of each
     auto over = [&](auto f) {
@@ -79,16 +84,17 @@ QG_DEV bool plan_find(const KvView &c, const BatchView &b, const AttnArgs &A, in
         return x * (float)c.heads;
     };
     // One round of resident workgroups, each with one unit: a second round for a few
-    // units would cost as much as the first.  Where the row groups alone fill half
-    // the card, two rounds' worth of shorter units instead.
+    // units would cost as much as the first.  Where the row groups alone come to half
+    // a round, two rounds.
     const float least = over([](const PlanLane &x) { return (float)x.groups; });
-    const float room = 2.0f * least > (float)A.resident ? 2.0f * (float)A.resident : (float)A.resident;
+    const bool single = 2.0f * least <= (float)A.resident;
+    const float room = single ? (float)A.resident : 2.0f * (float)A.resident;
     // 1.0001: above the sum whatever its roundings, so that the slots suffice
     const float even = 1.0001f * over([](const PlanLane &x) { return (float)x.groups * (float)(x.len + x.n); }) / room;
     int chunk = ((int)fminf(even, (float)(1 << 28)) / CHUNK + 1) * CHUNK;
-    for (int i = 0; i < 4; i++) {  // the parts round up: longer ones until they fit
+    for (int i = 0; i < 4 && !A.run && least <= room; i++) {  // the parts round up: longer ones until they fit
         const float units = over([&](const PlanLane &x) { return x.n ? (float)(((x.len + x.n - 1) / chunk + 1) * x.groups) : 0.0f; });
-        if (units <= room || least >= room) break;
+        if (units <= room) break;
         chunk = max((int)fminf((float)chunk * units / room, (float)(1 << 28)) / CHUNK, chunk / CHUNK) * CHUNK + CHUNK;
     }
     auto scan = [&](int s0, PlanLane &x, int &parts, int &upto, int &upto_slots) {
@@ -104,24 +110,19 @@ QG_DEV bool plan_find(const KvView &c, const BatchView &b, const AttnArgs &A, in
     };
     PlanLane x;
     int parts, upto, upto_slots, units = 0;
-    if (want < 0) {
-        for (int s0 = 0; s0 < c.sequences; s0 += 64) {
-            scan(s0, x, parts, upto, upto_slots);
-            units += __builtin_amdgcn_readlane(upto, 63);
-        }
-        const int per = (units + 7) / 8;
-        if (block >> 3 >= per) return false;
-        want = -1 - ((block & 7) * per + (block >> 3));
-        if (-1 - want >= units) return false;
+    for (int s0 = 0; s0 < c.sequences; s0 += 64) {
+        scan(s0, x, parts, upto, upto_slots);
+        units += __builtin_amdgcn_readlane(upto, 63);
     }
-    const int unit = want < 0 ? -1 - want : -1;
+    const int run = A.run ? A.run : (units + 7) / 8, k = block >> 3;
+    const int unit = (k / run * 8 + (block & 7)) * run + k % run;
+    if (unit >= units) return false;
     int before = 0;
     size_t slots = 0;
     for (int s0 = 0; s0 < c.sequences; s0 += 64) {
-        if (s0 || unit < 0 || c.sequences > 64) scan(s0, x, parts, upto, upto_slots);
+        if (c.sequences > 64) scan(s0, x, parts, upto, upto_slots);
         const int own = parts * x.groups * c.heads, own_slots = parts > 1 ? own : 0;
-        const unsigned long long here = unit < 0 ? (want >= s0 && want < s0 + 64 ? 1ULL << (want - s0) : 0)
-                                                 : __ballot(unit < before + upto && unit >= before + upto - own);
+        const unsigned long long here = __ballot(unit < before + upto && unit >= before + upto - own);
         if (here) {
             const int l = __builtin_ctzll(here);
             p.s = s0 + l;
@@ -129,14 +130,11 @@ QG_DEV bool plan_find(const KvView &c, const BatchView &b, const AttnArgs &A, in
             p.n = __builtin_amdgcn_readlane(x.n, l);
             p.len = __builtin_amdgcn_readlane(x.len, l);
             p.groups = __builtin_amdgcn_readlane(x.groups, l);
-            p.parts = __builtin_amdgcn_readlane(parts, l);
             p.slot = slots + __builtin_amdgcn_readlane(upto_slots - own_slots, l);
-            if (unit >= 0) {
-                const int rest = unit - (before + __builtin_amdgcn_readlane(upto - own, l));
-                p.part = rest / (p.groups * c.heads);
-                p.h = rest / p.groups % c.heads;
-                p.z = rest % p.groups;
-            }
+            const int rest = unit - (before + __builtin_amdgcn_readlane(upto - own, l));
+            p.part = rest / (p.groups * c.heads);
+            p.h = rest / p.groups % c.heads;
+            p.z = p.groups - 1 - rest % p.groups;  // the last rows, which see the most, first
             p.chunk = chunk;
             return true;
         }
@@ -145,6 +143,10 @@ QG_DEV bool plan_find(const KvView &c, const BatchView &b, const AttnArgs &A, in
     }
     return false;
 }
+
+// What is left to do for a row and head: nothing (parts 1, odd 0), to join `parts`
+// partial results from `slot` on, `step` apart, or to take the row up again (odd 1).
+struct Join { int parts, slot, step, odd; };
 
 // v_perm of two words into (a.lo, b.lo) or (a.hi, b.hi)
 QG_DEV uint32_t pair_lo(uint32_t a, uint32_t b) { return __builtin_amdgcn_perm(b, a, 0x05040100u); }
@@ -354,12 +356,26 @@ __global__ __launch_bounds__(64 * NW, (D / 64) * RT <= 6 ? 2 : 1) void attention
     __shared__ unsigned long long s_seen[QG_MAX_TREE];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = lane & 15, g = lane >> 4;
     Plan p;
-    if (!plan_find<RG>(c, b, A, lane, blockIdx.x, -1, p)) return;
+    if (!plan_find<RG>(c, b, A, lane, blockIdx.x, p)) return;
     const int row0 = p.z * RG, rows = p.n * A.group;  // this group's first row, all rows of the head
-
-    // this unit's keys, and the first one that some row of the group may not see
-    const int last_t = min(row0 + RG - 1, rows - 1) / A.group, begin = p.part * p.chunk;
-    const int end = min(begin + p.chunk, p.len + (b.parent ? p.n : last_t + 1)), open = p.len + (b.parent ? 0 : row0 / A.group + 1);
+    // the group's keys, the first one that some row may not see, and this unit's
+    const int last_t = by_group(A, min(row0 + RG, rows) - 1), begin = p.part * p.chunk;
+    const int keys = p.len + (b.parent ? p.n : last_t + 1), open = p.len + (b.parent ? 0 : by_group(A, row0) + 1);
+    const int parts = (keys - 1) / p.chunk + 1, end = min(begin + p.chunk, keys);
+    if (p.part >= parts) return;  // rows that come before the sequence's last keys
+    // the queries first: what is read in front of them would have to arrive before them
+    float x[RG / (4 * NW)][DL];
+    size_t at_q[RG / (4 * NW)];  // the row and head, or -1
+#pragma unroll
+    for (int i = 0; i < RG / (4 * NW); i++) {
+        const int at = row0 + (i * NW + wave) * 4 + g, t = by_group(A, at);
+        at_q[i] = at < rows ? (size_t)(p.first + t) * A.q_heads + p.h * A.group + (at - t * A.group) : (size_t)-1;
+#pragma unroll
+        for (int d = 0; d < DL; d += 4) {
+            const float4 y = at < rows ? *(const float4 *)(A.q + at_q[i] * D + n * DL + d) : make_float4(0, 0, 0, 0);
+            x[i][d] = y.x; x[i][d + 1] = y.y; x[i][d + 2] = y.z; x[i][d + 3] = y.w;
+        }
+    }
     const size_t page_bytes = ((size_t)c.heads << c.shift) * D * T::ES;
     const uint8_t *kbase = c.k + (((size_t)A.layer * c.pages * c.heads + p.h) << c.shift) * D * T::ES;
     const uint8_t *vbase = c.v + (((size_t)A.layer * c.pages * c.heads + p.h) << c.shift) * D * T::ES;
@@ -378,40 +394,36 @@ __global__ __launch_bounds__(64 * NW, (D / 64) * RT <= 6 ? 2 : 1) void attention
 
     // the rows' queries, in planes and in the order of the products' operand; the
     // power of two that a row was scaled by (fp16 planes) comes off the scores
-    for (int r0 = wave * 4; r0 < RG; r0 += NW * 4) {
-        const int r = r0 + g, at = row0 + r;
-        const bool live = at < rows;
-        const float *src = A.q + ((size_t)(p.first + at / A.group) * A.q_heads + p.h * A.group + at % A.group) * D + n * DL;
-        float x[DL];
 #pragma unroll
-        for (int i = 0; i < DL; i += 4) {
-            const float4 y = live ? *(const float4 *)(src + i) : make_float4(0, 0, 0, 0);
-            x[i] = y.x * A.scale; x[i + 1] = y.y * A.scale; x[i + 2] = y.z * A.scale; x[i + 3] = y.w * A.scale;
-        }
+    for (int i = 0; i < RG / (4 * NW); i++) {
+        const int r = (i * NW + wave) * 4 + g;
+#pragma unroll
+        for (int d = 0; d < DL; d++) x[i][d] *= A.scale;
         float back = 1.0f;
         if constexpr (TYPE == QT_F16) {
             float top = 0.0f;
 #pragma unroll
-            for (int i = 0; i < DL; i++) top = fmaxf(top, fabsf(x[i]));
+            for (int d = 0; d < DL; d++) top = fmaxf(top, fabsf(x[i][d]));
             top = qg_row_max(top);
             // 2^e with top 2^e in [2^13, 2^14): fp16's whole precision for what matters of the row
-            const int e = min(max(127 + 13 - (int)(__float_as_uint(top) >> 23) + 0, -126), 126);
+            const int e = min(max(127 + 13 - (int)(__float_as_uint(top) >> 23), -126), 126);
             if (top > 0.0f && top < __builtin_inff()) {
                 const float f = __uint_as_float((uint32_t)(e + 127) << 23);
                 back = __uint_as_float((uint32_t)(127 - e) << 23);
 #pragma unroll
-                for (int i = 0; i < DL; i++) x[i] *= f;
+                for (int d = 0; d < DL; d++) x[i][d] *= f;
             }
         }
         if (n == 0) s_back[r] = back;
-        if (n == 0 && live && p.parts == 1) A.odd[(size_t)(p.first + at / A.group) * A.q_heads + p.h * A.group + at % A.group] = 0;
+        if (n == 0 && p.part == 0 && at_q[i] != (size_t)-1)
+            A.joins[at_q[i]] = make_int4(parts, (int)(p.slot + (size_t)p.h * p.groups + p.z), c.heads * p.groups, 0);
         uint8_t *frag = s_mem + (r >> 4) * T::Q_BYTES;
 #pragma unroll
-        for (int i = 0; i < DL; i += 8) {
+        for (int d = 0; d < DL; d += 8) {
             float y[8];
 #pragma unroll
-            for (int j = 0; j < 8; j++) y[j] = i + j < DL ? x[(i + j) % DL] : 0.0f;
-            T::put_q(frag, r & 15, n * DL + i, y, DL - i);
+            for (int j = 0; j < 8; j++) y[j] = d + j < DL ? x[i][(d + j) % DL] : 0.0f;
+            T::put_q(frag, r & 15, n * DL + d, y, DL - d);
         }
     }
     if (b.parent && wave == 0) s_seen[lane] = tree_ancestors(b.parent + p.first, p.n, lane);
@@ -453,7 +465,7 @@ __global__ __launch_bounds__(64 * NW, (D / 64) * RT <= 6 ? 2 : 1) void attention
 #pragma unroll
             for (int r = 0; r < RT; r++) {
                 // bit e: key here_pos + e, below the row's prefix or among the rows that it descends from
-                const int t = (row0 + 16 * r + n) / A.group, prefix = b.parent ? p.len : p.len + t + 1, k = here_pos - p.len;
+                const int t = by_group(A, row0 + 16 * r + n), prefix = b.parent ? p.len : p.len + t + 1, k = here_pos - p.len;
                 unsigned seen = first_bits(prefix - here_pos, E);
                 if (b.parent && t < p.n && k < 64 && k > -E) seen |= (unsigned)(k < 0 ? s_seen[t] << -k : s_seen[t] >> k);
                 seen = here < 0 ? 0 : seen & first_bits(end - here_pos, E);
@@ -489,14 +501,31 @@ __global__ __launch_bounds__(64 * NW, (D / 64) * RT <= 6 ? 2 : 1) void attention
         if (more) tile.load_v(run(vbase, vpage, vpos), n);
     }
 
-    // the waves' parts are joined row tile by row tile
+    // the waves' sums are joined row tile by row tile: their weights first
 #pragma unroll
     for (int r = 0; r < RT; r++) {
         l[r] += __shfl_xor(l[r], 16);
         l[r] += __shfl_xor(l[r], 32);
         if (g == 0) { s_m[wave][16 * r + n] = m[r]; s_l[wave][16 * r + n] = l[r]; }
     }
-    __syncthreads();  // the queries' fragments are done with
+    __syncthreads();  // the queries' fragments are done with, too
+    const size_t slot = p.slot + ((size_t)p.part * c.heads + p.h) * p.groups + p.z;
+    const bool fits = slot < (size_t)A.slots;
+    if (tid < RG) {
+        float top = -__builtin_inff(), sum = 0.0f;
+#pragma unroll
+        for (int w = 0; w < NW; w++) top = fmaxf(top, s_m[w][tid]);
+#pragma unroll
+        for (int w = 0; w < NW; w++) {
+            const float mw = s_m[w][tid], lw = s_l[w][tid];
+            // a wave without a visible key leaves nothing
+            const float f = mw == -__builtin_inff() && lw == 0.0f ? 0.0f : mw == top ? 1.0f : __builtin_amdgcn_exp2f(mw - top);
+            sum = f == 0.0f ? sum : __builtin_fmaf(f, lw, sum);
+            s_m[w][tid] = f;
+        }
+        s_l[0][tid] = sum;
+        if (parts > 1 && fits) A.part_ml[slot * RG + tid] = make_float2(top, sum);
+    }
     float *join = (float *)s_mem;
 #pragma unroll
     for (int r = 0; r < RT; r++) {
@@ -507,36 +536,30 @@ __global__ __launch_bounds__(64 * NW, (D / 64) * RT <= 6 ? 2 : 1) void attention
                 *(float4 *)(join + (wave * 16 + n) * (D + 4) + DL * (4 * g + i) + t) =
                     make_float4(o[r][t][i], o[r][t + 1][i], o[r][t + 2][i], o[r][t + 3][i]);
         __syncthreads();
-        for (int x = tid; x < 16 * D / 4; x += 64 * NW) {
-            const int row = x / (D / 4), d = x % (D / 4) * 4, at = row0 + 16 * r + row;
-            if (at >= rows) continue;
-            float top = -__builtin_inff(), sum = 0.0f;
 #pragma unroll
-            for (int w = 0; w < NW; w++) top = fmaxf(top, s_m[w][16 * r + row]);
+        for (int x0 = 0; x0 < 16 * D / 4; x0 += 64 * NW) {
+            const int x = x0 + tid, row = x / (D / 4), d = x % (D / 4) * 4, at = row0 + 16 * r + row;
+            if (16 * D / 4 < 64 * NW && x >= 16 * D / 4) break;
             float4 y = make_float4(0, 0, 0, 0);
 #pragma unroll
             for (int w = 0; w < NW; w++) {
-                const float mw = s_m[w][16 * r + row];
-                if (mw == -__builtin_inff() && s_l[w][16 * r + row] == 0.0f) continue;
-                const float f = mw == top ? 1.0f : __builtin_amdgcn_exp2f(mw - top);
+                const float f = s_m[w][16 * r + row];
                 const float4 u = *(const float4 *)(join + (w * 16 + row) * (D + 4) + d);
-                sum = __builtin_fmaf(f, s_l[w][16 * r + row], sum);
-                y.x = __builtin_fmaf(f, u.x, y.x);
-                y.y = __builtin_fmaf(f, u.y, y.y);
-                y.z = __builtin_fmaf(f, u.z, y.z);
-                y.w = __builtin_fmaf(f, u.w, y.w);
+                y.x = f == 0.0f ? y.x : __builtin_fmaf(f, u.x, y.x);
+                y.y = f == 0.0f ? y.y : __builtin_fmaf(f, u.y, y.y);
+                y.z = f == 0.0f ? y.z : __builtin_fmaf(f, u.z, y.z);
+                y.w = f == 0.0f ? y.w : __builtin_fmaf(f, u.w, y.w);
             }
-            if (p.parts == 1) {
+            if (at >= rows) continue;
+            const float sum = s_l[0][16 * r + row];
+            if (parts == 1) {
                 const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-                const size_t to = (size_t)(p.first + at / A.group) * A.q_heads + p.h * A.group + at % A.group;
+                const int t = by_group(A, at);
+                const size_t to = (size_t)(p.first + t) * A.q_heads + p.h * A.group + (at - t * A.group);
                 *(float4 *)(A.out + to * D + d) = make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv);
-                if (odd_sums(y.x, y.y, sum) || odd_sums(y.z, y.w, sum)) A.odd[to] = 1;
-            } else {
-                const size_t slot = p.slot + ((size_t)p.part * c.heads + p.h) * p.groups + p.z;
-                if (slot < (size_t)A.slots) {
-                    *(float4 *)(A.part_o + (slot * RG + 16 * r + row) * D + d) = y;
-                    if (d == 0) A.part_ml[slot * RG + 16 * r + row] = make_float2(top, sum);
-                }
+                if (odd_sums(y.x, y.y, sum) || odd_sums(y.z, y.w, sum)) A.joins[to].w = 1;
+            } else if (fits) {
+                *(float4 *)(A.part_o + (slot * RG + 16 * r + row) * D + d) = y;
             }
         }
         __syncthreads();
@@ -548,7 +571,7 @@ __global__ __launch_bounds__(64 * NW, (D / 64) * RT <= 6 ? 2 : 1) void attention
 template <int TYPE, int D>
 QG_DEV void attend_row(const AttnArgs &A, const KvView &c, const BatchView &b, int s, int first, int n, int row, int head, int lane, float *s_q) {
     constexpr int V = D / 64;
-    const int place = row - first, len = kv_length(c, s), kv = head / A.group;
+    const int place = row - first, len = kv_length(c, s), kv = by_group(A, head);
     const unsigned long long seen = b.parent ? __shfl(tree_ancestors(b.parent + first, n, lane), place) : 0;
     const float *q = A.q + ((size_t)row * A.q_heads + head) * D;
     for (int d = lane; d < D; d += 64) s_q[d] = q[d] * A.scale;
@@ -585,83 +608,108 @@ QG_DEV void attend_row(const AttnArgs &A, const KvView &c, const BatchView &b, i
     for (int i = 0; i < V; i++) A.out[((size_t)row * A.q_heads + head) * D + lane * V + i] = l == 0.0f ? 0.0f : o[i] / l;
 }
 
-// A workgroup per row and head: joins the parts of sequences that were cut, and
-// takes up odd rows again.  A wave sums every fourth part; a lane holds the weight
-// of one part, so that the parts' loads wait for nothing.
+// Joins the parts of sequences that were cut, and takes up odd rows again.  Few
+// rows and heads: a workgroup each, whose four waves take a quarter of the parts.
+// Many (a prompt chunk: few parts each): a wave each.
 constexpr int JOIN_WAVES = 4;
-template <int TYPE, int D, int RG>
-__global__ __launch_bounds__(64 * JOIN_WAVES) void attention_join_kernel(AttnArgs A, KvView c, BatchView b) {
+constexpr size_t JOIN_FEW = 4096;
+
+// Parts i0, i0 + by, .. of a row: their largest m, and sums under it.  A lane holds
+// the weight of one part, so that the parts' loads wait for nothing.
+template <int D, int RG>
+QG_DEV void join_parts(const AttnArgs &A, const Join &j, int in_group, int i0, int by, int lane, float &top, float &sum, float (&y)[D / 64]) {
     constexpr int V = D / 64;
-    __shared__ float s_y[JOIN_WAVES][D], s_q[D];
-    __shared__ float2 s_w[JOIN_WAVES];
-    const int row = blockIdx.x, head = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    int first, n;
-    const int s = batch_sequence(b, c.sequences, row, lane, first, n);
-    if (s < 0) return;
-    Plan p;
-    if (!plan_find<RG>(c, b, A, lane, 0, s, p)) return;
-    bool odd = p.parts < 2 && A.odd[(size_t)row * A.q_heads + head];
-    if (p.parts > 1) {
-        const int h = head / A.group, at = (row - first) * A.group + head % A.group;
-        const size_t step = (size_t)c.heads * p.groups, slot0 = p.slot + (size_t)h * p.groups + at / RG;
-        if (slot0 + (p.parts - 1) * step >= (size_t)A.slots) return;
-        const float2 *ml = A.part_ml + slot0 * RG + at % RG;
-        const float *po = A.part_o + (slot0 * RG + at % RG) * D + lane * V;
-        float top = -__builtin_inff(), sum = 0.0f, y[V];
+    const float2 *ml = A.part_ml + (size_t)j.slot * RG + in_group;
+    const float *po = A.part_o + ((size_t)j.slot * RG + in_group) * D + lane * V;
+    top = -__builtin_inff();
+    sum = 0.0f;
 #pragma unroll
-        for (int v = 0; v < V; v++) y[v] = 0.0f;
-        for (int i0 = wave; i0 < p.parts; i0 += 64 * JOIN_WAVES) {
-            const int mine = i0 + lane * JOIN_WAVES, count = min((p.parts - i0 + JOIN_WAVES - 1) / JOIN_WAVES, 64);
-            const float2 x = mine < p.parts ? ml[mine * step * RG] : make_float2(-__builtin_inff(), 0.0f);
-            const float next = fmaxf(top, qg_wave_max(x.x));
-            const float old = next == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f(top - next);
-            // a part without a key leaves nothing (its sums were not written)
-            const float f = x.x == -__builtin_inff() && x.y == 0.0f ? 0.0f : x.x == next ? 1.0f : __builtin_amdgcn_exp2f(x.x - next);
-            top = next;
-            sum = sum * old + qg_sum_lanes<64>(f == 0.0f ? 0.0f : f * x.y);
+    for (int v = 0; v < V; v++) y[v] = 0.0f;
+    for (; i0 < j.parts; i0 += 64 * by) {
+        const int mine = i0 + lane * by, count = min((j.parts - i0 + by - 1) / by, 64);
+        const float2 x = mine < j.parts ? ml[(size_t)mine * j.step * RG] : make_float2(-__builtin_inff(), 0.0f);
+        const float next = fmaxf(top, qg_wave_max(x.x));
+        const float old = next == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f(top - next);
+        // a part without a visible key leaves nothing
+        const float f = x.x == -__builtin_inff() && x.y == 0.0f ? 0.0f : x.x == next ? 1.0f : __builtin_amdgcn_exp2f(x.x - next);
+        top = next;
+        sum = sum * old + qg_sum_lanes<64>(f == 0.0f ? 0.0f : f * x.y);
 #pragma unroll
-            for (int v = 0; v < V; v++) y[v] *= old;
-            for (int i = 0; i < count; i += 8) {
-                float u[8][V];
+        for (int v = 0; v < V; v++) y[v] *= old;
+        for (int i = 0; i < count; i += 8) {
+            float u[8][V];
 #pragma unroll
-                for (int k = 0; k < 8; k++)
+            for (int k = 0; k < 8; k++) {
+                const float *from = po + (size_t)(i0 + min(i + k, count - 1) * by) * j.step * RG * D;
 #pragma unroll
-                    for (int v = 0; v < V; v++) u[k][v] = po[(i0 + min(i + k, count - 1) * JOIN_WAVES) * step * RG * D + v];
+                for (int v = 0; v < V; v++) u[k][v] = from[v];
+            }
 #pragma unroll
-                for (int k = 0; k < 8; k++) {
-                    const float w = i + k < count ? __int_as_float(__builtin_amdgcn_readlane(__float_as_int(f), (i + k) & 63)) : 0.0f;
+            for (int k = 0; k < 8; k++) {
+                const float w = i + k < count ? __int_as_float(__builtin_amdgcn_readlane(__float_as_int(f), (i + k) & 63)) : 0.0f;
 #pragma unroll
-                    for (int v = 0; v < V; v++) y[v] = w == 0.0f ? y[v] : __builtin_fmaf(w, u[k][v], y[v]);
-                }
+                for (int v = 0; v < V; v++) y[v] = w == 0.0f ? y[v] : __builtin_fmaf(w, u[k][v], y[v]);
             }
         }
-#pragma unroll
-        for (int v = 0; v < V; v++) s_y[wave][lane * V + v] = y[v];
-        if (lane == 0) s_w[wave] = make_float2(top, sum);
-        __syncthreads();
-        const float all = fmaxf(fmaxf(s_w[0].x, s_w[1].x), fmaxf(s_w[2].x, s_w[3].x));
-        sum = 0.0f;
-#pragma unroll
-        for (int v = 0; v < V; v++) y[v] = 0.0f;
-#pragma unroll
-        for (int w = 0; w < JOIN_WAVES; w++) {
-            const float2 x = s_w[w];
-            if (x.x == -__builtin_inff() && x.y == 0.0f) continue;
-            const float f = x.x == all ? 1.0f : __builtin_amdgcn_exp2f(x.x - all);
-            sum = __builtin_fmaf(f, x.y, sum);
-#pragma unroll
-            for (int v = 0; v < V; v++) y[v] = __builtin_fmaf(f, s_y[w][lane * V + v], y[v]);
-        }
-#pragma unroll
-        for (int v = 0; v < V; v++) odd |= odd_sums(y[v], 0.0f, sum);
-        odd = __any(odd);
-        if (wave == 0 && !odd) {
-            const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-#pragma unroll
-            for (int v = 0; v < V; v++) A.out[((size_t)row * A.q_heads + head) * D + lane * V + v] = y[v] * inv;
-        }
     }
-    if (odd && wave == 0) attend_row<TYPE, D>(A, c, b, s, first, n, row, head, lane, s_q);
+}
+// Divides and stores a joined row; true if it is odd.
+template <int D>
+QG_DEV bool join_done(const AttnArgs &A, size_t at, int lane, float sum, const float (&y)[D / 64]) {
+    bool odd = false;
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+#pragma unroll
+    for (int v = 0; v < D / 64; v++) {
+        odd |= odd_sums(y[v], 0.0f, sum);
+        A.out[at * D + lane * (D / 64) + v] = y[v] * inv;
+    }
+    return __any(odd);
+}
+template <int TYPE, int D, int RG, int EACH>
+__global__ __launch_bounds__(64 * JOIN_WAVES) void attention_join_kernel(AttnArgs A, KvView c, BatchView b) {
+    constexpr int V = D / 64;
+    __shared__ float s_y[JOIN_WAVES][D];
+    __shared__ float2 s_w[JOIN_WAVES];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const size_t at = EACH == 1 ? blockIdx.x : (size_t)blockIdx.x * EACH + wave;
+    if (at >= (size_t)b.rows * A.q_heads) return;
+    const int row = (int)(at / A.q_heads), head = (int)(at % A.q_heads);
+    const int4 x = A.joins[at];
+    const Join j{x.x, x.y, x.z, x.w};
+    int first, n;
+    const int s = batch_sequence(b, c.sequences, row, lane, first, n);
+    if (s < 0) return;  // nothing was written for it
+    bool odd = j.odd == 1;
+    if (j.parts > 1) {
+        if ((size_t)j.slot + (size_t)(j.parts - 1) * j.step >= (size_t)A.slots) return;
+        const int in_group = ((row - first) * A.group + (head - by_group(A, head) * A.group)) % RG;
+        float top, sum, y[V];
+        if (EACH > 1) {
+            join_parts<D, RG>(A, j, in_group, 0, 1, lane, top, sum, y);
+        } else {
+            join_parts<D, RG>(A, j, in_group, wave, JOIN_WAVES, lane, top, sum, y);
+#pragma unroll
+            for (int v = 0; v < V; v++) s_y[wave][lane * V + v] = y[v];
+            if (lane == 0) s_w[wave] = make_float2(top, sum);
+            __syncthreads();
+            if (wave) return;
+            const float most = fmaxf(fmaxf(s_w[0].x, s_w[1].x), fmaxf(s_w[2].x, s_w[3].x));
+            sum = 0.0f;
+#pragma unroll
+            for (int v = 0; v < V; v++) y[v] = 0.0f;
+#pragma unroll
+            for (int w = 0; w < JOIN_WAVES; w++) {
+                const float2 u = s_w[w];
+                if (u.x == -__builtin_inff() && u.y == 0.0f) continue;
+                const float f = u.x == most ? 1.0f : __builtin_amdgcn_exp2f(u.x - most);
+                sum = __builtin_fmaf(f, u.y, sum);
+#pragma unroll
+                for (int v = 0; v < V; v++) y[v] = __builtin_fmaf(f, s_y[w][lane * V + v], y[v]);
+            }
+        }
+        odd = join_done<D>(A, at, lane, sum, y);
+    }
+    if (odd && (EACH > 1 || wave == 0)) attend_row<TYPE, D>(A, c, b, s, first, n, row, head, lane, s_y[wave]);
 }
 
 // Row tiles per wave: as few row groups as the registers allow, and no more tiles than those need.
@@ -675,8 +723,10 @@ template <int TYPE, int D, int RT>
 void launch(const AttnArgs &A, const KvView &c, const BatchView &b, hipStream_t s) {
     const long groups = (long)b.rows * A.group / (16 * RT) + c.sequences;  // of all sequences: each rounds up
     const long units = 2 * A.resident + groups * c.heads + 8;
-    attention_kernel<TYPE, D, RT, WAVES><<<(unsigned)((units + 7) / 8 * 8), 64 * WAVES, 0, s>>>(A, c, b);
-    attention_join_kernel<TYPE, D, 16 * RT><<<dim3(b.rows, A.q_heads), 64 * JOIN_WAVES, 0, s>>>(A, c, b);
+    attention_kernel<TYPE, D, RT, WAVES><<<(unsigned)((units + 127) / 128 * 128), 64 * WAVES, 0, s>>>(A, c, b);
+    const size_t jobs = (size_t)b.rows * A.q_heads;
+    if (jobs > JOIN_FEW) attention_join_kernel<TYPE, D, 16 * RT, 4><<<(unsigned)((jobs + 3) / 4), 256, 0, s>>>(A, c, b);
+    else attention_join_kernel<TYPE, D, 16 * RT, 1><<<(unsigned)jobs, 256, 0, s>>>(A, c, b);
 }
 template <int TYPE, int D>
 void launch_rt(int rt, const AttnArgs &A, const KvView &c, const BatchView &b, hipStream_t s) {
@@ -713,7 +763,7 @@ size_t qg_tree_attention_workspace_bytes(const qg_kv_cache *cache, const qg_kv_b
     if (q_heads < 1 || q_heads % cache->kv_heads || q_heads / cache->kv_heads > 128) return 0;
     const int group = q_heads / cache->kv_heads;
     const int rt = row_tiles(cache->head_dim, (long)batch->max_rows * group);
-    return slots(cache->head_dim, rt) * 16 * rt * (4 * (size_t)cache->head_dim + sizeof(float2)) + 4 * (size_t)batch->rows * q_heads;
+    return slots(cache->head_dim, rt) * 16 * rt * (4 * (size_t)cache->head_dim + sizeof(float2)) + sizeof(int4) * (size_t)batch->rows * q_heads;
 }
 
 int qg_tree_attention(float *out, const float *q, int q_heads, float scale, const qg_kv_cache *cache, int layer,
@@ -728,10 +778,12 @@ int qg_tree_attention(float *out, const float *q, int q_heads, float scale, cons
     if (qg_overlap(out, bytes, q, bytes) || qg_overlap(ws, need, q, bytes) || qg_overlap(ws, need, out, bytes)) return hipErrorInvalidValue;
     const int group = q_heads / c.heads, rt = row_tiles(c.dim, (long)b.max_rows * group);
     float *part_o = (float *)ws;
+    const int run = !b.parent && b.max_rows > QG_MAX_TREE ? 16 : 0;
     const size_t parts = slots(c.dim, rt) * 16 * rt;
     float2 *part_ml = (float2 *)(part_o + parts * c.dim);
-    const AttnArgs A{out, q, part_o, part_ml, (int *)(part_ml + parts), scale * 1.44269504088896341f, q_heads, group, layer, resident(c.dim, rt),
-                     (int)slots(c.dim, rt)};
+    const AttnArgs A{out, q, part_o, part_ml, (int4 *)(part_ml + parts), scale * 1.44269504088896341f, q_heads, group, layer, resident(c.dim, rt),
+                     (int)slots(c.dim, rt), run,
+                     (unsigned)(((1ULL << 32) + group - 1) / group)};
     if (c.type == QT_F32) launch_dim<QT_F32>(rt, A, c, b, qg_stream());
     else if (c.type == QT_F16) launch_dim<QT_F16>(rt, A, c, b, qg_stream());
     else launch_dim<QT_BF16>(rt, A, c, b, qg_stream());
