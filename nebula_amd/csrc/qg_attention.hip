@@ -249,18 +249,37 @@ struct Tile {
             else *(uint4 *)to = p.p[k];
         }
     }
-    __device__ __forceinline__ void scores(const uint8_t *frag, int lane, float (&z)[8]) const {
-        qg_f4 a[2] = {};
+    // The row tiles' queries are read half a tile ahead of their products where
+    // registers are left for it (two fp16 planes: 16 x 17 rows x 98304 keys 656 -> 628
+    // us; three bf16 planes at 128 dimensions, or one row tile with a third wave per
+    // SIMD, lose more to the registers: 1 row x 98304 keys 33 -> 37).
+    template <int RT>
+    __device__ __forceinline__ void scores(const uint8_t *frag, int lane, float (&z)[RT][8]) const {
+        constexpr bool AHEAD = RT > 1 && (TYPE == QT_F16 || D == 256);
+        constexpr int H = S / 2 * PL;  // fragments of a half
+        uint4 q[2][H];
+        auto read = [&](int half, uint4 (&to)[H]) {
 #pragma unroll
-        for (int s = 0; s < S; s++)
+            for (int i = 0; i < H; i++) to[i] = *(const uint4 *)(frag + (size_t)half * (H * 1024) + i * 1024 + lane * 16);
+        };
+        if (AHEAD) read(0, q[0]);
 #pragma unroll
-            for (int p = 0; p < PL; p++) {
-                const uint4 q = *(const uint4 *)(frag + ((s * PL + p) * 64 + lane) * 16);
+        for (int r = 0; r < RT; r++) {
+            qg_f4 a[2] = {};
 #pragma unroll
-                for (int j = 0; j < 2; j++) a[j] = Planes<TYPE>::mul(k[j][s], q, a[j]);
+            for (int half = 0; half < 2; half++) {
+                if (!AHEAD) read(2 * r + half, q[half]);
+                else if (2 * r + half + 1 < 2 * RT) read(2 * r + half + 1, q[1 - half]);
+                if (AHEAD) __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int i = 0; i < H; i++)
+#pragma unroll
+                    for (int j = 0; j < 2; j++) a[j] = Planes<TYPE>::mul(k[j][half * (S / 2) + i / PL], q[half][i], a[j]);
+                if (AHEAD || half) __builtin_amdgcn_sched_barrier(0);  // one row tile's queries in registers at a time
             }
 #pragma unroll
-        for (int i = 0; i < 4; i++) { z[i] = a[0][i]; z[4 + i] = a[1][i]; }
+            for (int i = 0; i < 4; i++) { z[r][i] = a[0][i]; z[r][4 + i] = a[1][i]; }
+        }
     }
     template <int RT>
     __device__ __forceinline__ void outputs(const float (&p)[RT][8], qg_f4 (&o)[RT][DL]) const {
@@ -271,16 +290,23 @@ struct Tile {
 #pragma unroll
             for (int k = 0; k < PL; k++) w[r][k] = x.p[k];
         }
+        // two dimension tiles at a time: products that add to one sum lie apart
 #pragma unroll
-        for (int t = 0; t < DL; t++) {
-            uint32_t u[4];
+        for (int t = 0; t < DL; t += 2) {
+            uint4 a[2];
 #pragma unroll
-            for (int i = 0; i < 4; i++) u[i] = t & 1 ? pair_hi(v[2 * i][t / 2], v[2 * i + 1][t / 2]) : pair_lo(v[2 * i][t / 2], v[2 * i + 1][t / 2]);
-            const uint4 a = make_uint4(u[0], u[1], u[2], u[3]);
+            for (int h = 0; h < 2; h++) {
+                uint32_t u[4];
 #pragma unroll
-            for (int r = 0; r < RT; r++)
+                for (int i = 0; i < 4; i++) u[i] = h ? pair_hi(v[2 * i][t / 2], v[2 * i + 1][t / 2]) : pair_lo(v[2 * i][t / 2], v[2 * i + 1][t / 2]);
+                a[h] = make_uint4(u[0], u[1], u[2], u[3]);
+            }
 #pragma unroll
-                for (int k = 0; k < PL; k++) o[r][t] = Planes<TYPE>::mul(a, w[r][k], o[r][t]);
+            for (int k = 0; k < PL; k++)
+#pragma unroll
+                for (int r = 0; r < RT; r++)
+#pragma unroll
+                    for (int h = 0; h < 2; h++) o[r][t + h] = Planes<TYPE>::mul(a[h], w[r][k], o[r][t + h]);
         }
     }
 };
@@ -315,18 +341,23 @@ struct Tile<QT_F32, D> {
                 *(float4 *)(frag + ((d >> 4) * 64 + ((d >> 2) & 3) * 16 + n) * 16) = make_float4(x[i], x[i + 1], x[i + 2], x[i + 3]);
             }
     }
-    __device__ __forceinline__ void scores(const uint8_t *frag, int lane, float (&z)[4]) const {
-        qg_f4 a = {};
+    template <int RT>
+    __device__ __forceinline__ void scores(const uint8_t *frag, int lane, float (&z)[RT][4]) const {
 #pragma unroll
-        for (int s = 0; s < S; s++) {
-            const float4 q = *(const float4 *)(frag + (s * 64 + lane) * 16);
-            a = __builtin_amdgcn_mfma_f32_16x16x4f32(k[s].x, q.x, a, 0, 0, 0);
-            a = __builtin_amdgcn_mfma_f32_16x16x4f32(k[s].y, q.y, a, 0, 0, 0);
-            a = __builtin_amdgcn_mfma_f32_16x16x4f32(k[s].z, q.z, a, 0, 0, 0);
-            a = __builtin_amdgcn_mfma_f32_16x16x4f32(k[s].w, q.w, a, 0, 0, 0);
+        for (int r = 0; r < RT; r++) {
+            qg_f4 a = {};
+#pragma unroll
+            for (int s = 0; s < S; s++) {
+                const float4 q = *(const float4 *)(frag + ((r * S + s) * 64 + lane) * 16);
+                a = __builtin_amdgcn_mfma_f32_16x16x4f32(k[s].x, q.x, a, 0, 0, 0);
+                a = __builtin_amdgcn_mfma_f32_16x16x4f32(k[s].y, q.y, a, 0, 0, 0);
+                a = __builtin_amdgcn_mfma_f32_16x16x4f32(k[s].z, q.z, a, 0, 0, 0);
+                a = __builtin_amdgcn_mfma_f32_16x16x4f32(k[s].w, q.w, a, 0, 0, 0);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; i++) z[r][i] = a[i];
+            __builtin_amdgcn_sched_barrier(0);  // one row tile's queries in registers at a time
         }
-#pragma unroll
-        for (int i = 0; i < 4; i++) z[i] = a[i];
     }
     template <int RT>
     __device__ __forceinline__ void outputs(const float (&p)[RT][4], qg_f4 (&o)[RT][DL]) const {
@@ -346,6 +377,12 @@ struct Tile<QT_F32, D> {
 QG_DEV bool odd_sums(float a, float b, float weight) { return !__builtin_isfinite(a + b) && __builtin_isfinite(weight); }
 
 QG_DEV unsigned first_bits(int n, int most) { return (1u << min(max(n, 0), most)) - 1u; }
+
+// What a part's sums (under its largest score m, weights l) count under another
+// maximum; below zero for one without a visible key, whose sums may be anything.
+QG_DEV float part_weight(float m, float l, float top) {
+    return m == -__builtin_inff() && l == 0.0f ? -1.0f : m == top ? 1.0f : __builtin_amdgcn_exp2f(m - top);
+}
 
 template <int TYPE, int D, int RT, int NW>
 __global__ __launch_bounds__(64 * NW, (D / 64) * RT <= 6 ? 2 : 1) void attention_kernel(AttnArgs A, KvView c, BatchView b) {
@@ -442,11 +479,7 @@ __global__ __launch_bounds__(64 * NW, (D / 64) * RT <= 6 ? 2 : 1) void attention
     }
     for (; t0 < end; t0 += NW * KEYS) {
         float z[RT][E];
-#pragma unroll
-        for (int r = 0; r < RT; r++) {
-            tile.scores(s_mem + r * T::Q_BYTES, lane, z[r]);
-            __builtin_amdgcn_sched_barrier(0);  // one row tile's queries in registers at a time
-        }
+        tile.template scores<RT>(s_mem, lane, z);
         // the next tile's keys, whose pages are known, and the pages of the one after it
         const int here = vpage, here_pos = vpos;
         const bool more = t0 + NW * KEYS < end;
@@ -517,10 +550,8 @@ __global__ __launch_bounds__(64 * NW, (D / 64) * RT <= 6 ? 2 : 1) void attention
         for (int w = 0; w < NW; w++) top = fmaxf(top, s_m[w][tid]);
 #pragma unroll
         for (int w = 0; w < NW; w++) {
-            const float mw = s_m[w][tid], lw = s_l[w][tid];
-            // a wave without a visible key leaves nothing
-            const float f = mw == -__builtin_inff() && lw == 0.0f ? 0.0f : mw == top ? 1.0f : __builtin_amdgcn_exp2f(mw - top);
-            sum = f == 0.0f ? sum : __builtin_fmaf(f, lw, sum);
+            const float lw = s_l[w][tid], f = part_weight(s_m[w][tid], lw, top);
+            if (f >= 0.0f) sum = __builtin_fmaf(f, lw, sum);
             s_m[w][tid] = f;
         }
         s_l[0][tid] = sum;
@@ -545,10 +576,10 @@ __global__ __launch_bounds__(64 * NW, (D / 64) * RT <= 6 ? 2 : 1) void attention
             for (int w = 0; w < NW; w++) {
                 const float f = s_m[w][16 * r + row];
                 const float4 u = *(const float4 *)(join + (w * 16 + row) * (D + 4) + d);
-                y.x = f == 0.0f ? y.x : __builtin_fmaf(f, u.x, y.x);
-                y.y = f == 0.0f ? y.y : __builtin_fmaf(f, u.y, y.y);
-                y.z = f == 0.0f ? y.z : __builtin_fmaf(f, u.z, y.z);
-                y.w = f == 0.0f ? y.w : __builtin_fmaf(f, u.w, y.w);
+                y.x = f < 0.0f ? y.x : __builtin_fmaf(f, u.x, y.x);
+                y.y = f < 0.0f ? y.y : __builtin_fmaf(f, u.y, y.y);
+                y.z = f < 0.0f ? y.z : __builtin_fmaf(f, u.z, y.z);
+                y.w = f < 0.0f ? y.w : __builtin_fmaf(f, u.w, y.w);
             }
             if (at >= rows) continue;
             const float sum = s_l[0][16 * r + row];
@@ -630,10 +661,9 @@ QG_DEV void join_parts(const AttnArgs &A, const Join &j, int in_group, int i0, i
         const float2 x = mine < j.parts ? ml[(size_t)mine * j.step * RG] : make_float2(-__builtin_inff(), 0.0f);
         const float next = fmaxf(top, qg_wave_max(x.x));
         const float old = next == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f(top - next);
-        // a part without a visible key leaves nothing
-        const float f = x.x == -__builtin_inff() && x.y == 0.0f ? 0.0f : x.x == next ? 1.0f : __builtin_amdgcn_exp2f(x.x - next);
+        const float f = part_weight(x.x, x.y, next);
         top = next;
-        sum = sum * old + qg_sum_lanes<64>(f == 0.0f ? 0.0f : f * x.y);
+        sum = sum * old + qg_sum_lanes<64>(f < 0.0f ? 0.0f : f * x.y);
 #pragma unroll
         for (int v = 0; v < V; v++) y[v] *= old;
         for (int i = 0; i < count; i += 8) {
@@ -646,9 +676,9 @@ QG_DEV void join_parts(const AttnArgs &A, const Join &j, int in_group, int i0, i
             }
 #pragma unroll
             for (int k = 0; k < 8; k++) {
-                const float w = i + k < count ? __int_as_float(__builtin_amdgcn_readlane(__float_as_int(f), (i + k) & 63)) : 0.0f;
+                const float w = i + k < count ? __int_as_float(__builtin_amdgcn_readlane(__float_as_int(f), (i + k) & 63)) : -1.0f;
 #pragma unroll
-                for (int v = 0; v < V; v++) y[v] = w == 0.0f ? y[v] : __builtin_fmaf(w, u[k][v], y[v]);
+                for (int v = 0; v < V; v++) y[v] = w < 0.0f ? y[v] : __builtin_fmaf(w, u[k][v], y[v]);
             }
         }
     }
@@ -700,8 +730,8 @@ __global__ __launch_bounds__(64 * JOIN_WAVES) void attention_join_kernel(AttnArg
 #pragma unroll
             for (int w = 0; w < JOIN_WAVES; w++) {
                 const float2 u = s_w[w];
-                if (u.x == -__builtin_inff() && u.y == 0.0f) continue;
-                const float f = u.x == most ? 1.0f : __builtin_amdgcn_exp2f(u.x - most);
+                const float f = part_weight(u.x, u.y, most);
+                if (f < 0.0f) continue;
                 sum = __builtin_fmaf(f, u.y, sum);
 #pragma unroll
                 for (int v = 0; v < V; v++) y[v] = __builtin_fmaf(f, s_y[w][lane * V + v], y[v]);
