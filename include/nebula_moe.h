@@ -3,7 +3,8 @@
  *
  * It plays the role of the reference's moe()/shared_direct() and the
  * per-layer loop of qwen_target (qwen.c:714-735,759-762) for a stack of MoE
- * layers without attention: each layer is h <- h + MoE(RMSNorm(h)) (eps 1e-6,
+ * layers, with attention over a paged cache before each (nm_stack_verify) or
+ * without attention (nm_stack_forward): each layer is h <- h + MoE(RMSNorm(h)) (eps 1e-6,
  * unit weight, the norm of gpu.cu:204-214), one qg_moe_forward_residual call.  The whole stack for a token
  * count is captured once into a graph and replayed, the way qwen.c:726-734
  * captures the shared expert per batch size; unlike the reference no routing
@@ -36,6 +37,33 @@ int nm_stack_forward(nm_stack *s, int tokens, int use_graph);
  * ids [tokens][10], weights [tokens][10], MoE output [tokens][D]. */
 int nm_stack_record(nm_stack *s, int layer, const float **x, const int **ids, const float **weights, const float **out);
 const char *nm_last_error(void);
+
+/* Attention before each layer's MoE, over a paged cache whose layer l belongs
+ * to the stack's layer l (qg_kv_cache; its pages are the caller's,
+ * qg_kv_reserve).  Projections are qg_matmul weights; every q and k head is
+ * normalised and rotated by qg_qk_norm_rope. */
+typedef struct {
+    const void *qkv;                    /* [(q_heads + 2 kv_heads) head_dim][width]: q, k, v heads */
+    const void *out;                    /* [width][q_heads head_dim] */
+    int qkv_type, out_type;
+    const float *q_norm, *k_norm;       /* [head_dim] or NULL */
+} nm_attention_layer;
+typedef struct {
+    int q_heads, rope_dims, interleaved;
+    const double *freq;                 /* [rope_dims / 2], as qg_qk_rows */
+    float scale;                        /* of the scores */
+} nm_attention;
+/* Copies the descriptors (device pointers stay the caller's) and allocates the
+ * attention's buffers; once per stack.  cache->layers is the stack's. */
+int nm_stack_attend(nm_stack *s, const nm_attention_layer *layers, const nm_attention *attention, const qg_kv_cache *cache);
+/* All layers of the batch's rows (last accepted tokens and their drafts; at
+ * most the stack's max_tokens together) in the first rows of the hidden state:
+ * h <- h + Wo attention(RMSNorm(h)), h <- h + MoE(RMSNorm(h)) (eps 1e-6, unit
+ * weight).  Keys and values of the rows are stored behind the cached tokens;
+ * lengths do not change (qg_kv_compact does that once drafts are accepted).
+ * use_graph: captured on first use per number of rows and replayed while the
+ * batch's arrays stay where they are; what they hold may change. */
+int nm_stack_verify(nm_stack *s, const qg_kv_batch *batch, int use_graph);
 
 /* CPU handoff of one layer's flag-2 tokens (the hybrid path of
  * qwen.c:658-678, narrowed from the whole batch to the flagged tokens).

@@ -40,11 +40,32 @@ struct nm_stack {
     float *rec_x, *rec_out, *rec_w;
     int *rec_ids;
     void *graphs[NM_MAX_TOKENS + 1];
+    /* attention (nm_stack_attend) */
+    nm_attention attn;
+    nm_attention_layer *attn_layers;
+    qg_kv_cache cache;
+    float *x, *qkv, *q, *a;     /* normalised rows, projections, queries, attention rows */
+    void *attn_ws;
+    size_t attn_ws_bytes;
+    void *verify_graphs[NM_MAX_TOKENS + 1];
+    qg_kv_batch verify_batches[NM_MAX_TOKENS + 1];
 };
+
+static void attend_free(nm_stack *s) {
+    qg_free(s->x); qg_free(s->qkv); qg_free(s->q); qg_free(s->a); qg_free(s->attn_ws);
+    free(s->attn_layers);
+    s->x = s->qkv = s->q = s->a = NULL;
+    s->attn_ws = NULL;
+    s->attn_layers = NULL;
+}
 
 void nm_stack_destroy(nm_stack *s) {
     if (!s) return;
-    for (int i = 0; i <= NM_MAX_TOKENS; i++) if (s->graphs[i]) qg_graph_destroy(s->graphs[i]);
+    for (int i = 0; i <= NM_MAX_TOKENS; i++) {
+        if (s->graphs[i]) qg_graph_destroy(s->graphs[i]);
+        if (s->verify_graphs[i]) qg_graph_destroy(s->verify_graphs[i]);
+    }
+    attend_free(s);
     qg_free(s->h); qg_free(s->w); qg_free(s->ids); qg_free(s->ws);
     qg_free(s->rec_x); qg_free(s->rec_out); qg_free(s->rec_w); qg_free(s->rec_ids);
     free(s->layers);
@@ -115,6 +136,102 @@ int nm_stack_record(nm_stack *s, int layer, const float **x, const int **ids, co
     if (out) *out = s->rec_out + a * layer;
     if (ids) *ids = s->rec_ids + b * layer;
     if (weights) *weights = s->rec_w + b * layer;
+    return 0;
+}
+
+/* ---- attention before each layer's MoE ---- */
+int nm_stack_attend(nm_stack *s, const nm_attention_layer *layers, const nm_attention *attention, const qg_kv_cache *cache) {
+    if (!s || !layers || !attention || !cache) return fail("invalid attention arguments");
+    if (s->attn_layers) return fail("the stack has its attention");
+    if (cache->layers != s->n_layers) return fail("a cache of %d layers for a stack of %d", cache->layers, s->n_layers);
+    for (int l = 0; l < s->n_layers; l++)
+        if (!layers[l].qkv || !layers[l].out) return fail("layer %d without projections", l);
+    /* the largest batch of the stack, for the sizes; its pointers are not used */
+    const int T = s->max_tokens;
+    int none;
+    const qg_kv_batch most = {.rows = T, .max_rows = T, .start = &none};
+    const size_t ws = qg_tree_attention_workspace_bytes(cache, &most, attention->q_heads);
+    if (!ws) return fail("invalid attention or cache shape");
+    if (attention->rope_dims < 0 || attention->rope_dims > cache->head_dim || attention->rope_dims % 8 ||
+        (attention->rope_dims && !attention->freq))
+        return fail("invalid rotation");
+    const size_t qw = (size_t)attention->q_heads * cache->head_dim, kw = (size_t)cache->kv_heads * cache->head_dim;
+    s->attn_ws_bytes = 0;
+    /* fewer rows may take another shape of the kernel, with more partial results */
+    for (int rows = 1; rows <= T; rows++)
+        for (int most_rows = 1; most_rows <= rows; most_rows++) {
+            const qg_kv_batch b = {.rows = rows, .max_rows = most_rows, .start = &none};
+            const size_t n = qg_tree_attention_workspace_bytes(cache, &b, attention->q_heads);
+            if (n > s->attn_ws_bytes) s->attn_ws_bytes = n;
+        }
+    s->attn_layers = malloc(sizeof *layers * (size_t)s->n_layers);
+    s->x = qg_alloc((size_t)T * s->width * sizeof(float));
+    s->qkv = qg_alloc((size_t)T * (qw + 2 * kw) * sizeof(float));
+    s->q = qg_alloc((size_t)T * qw * sizeof(float));
+    s->a = qg_alloc((size_t)T * qw * sizeof(float));
+    s->attn_ws = qg_alloc(s->attn_ws_bytes);
+    if (!s->attn_layers || !s->x || !s->qkv || !s->q || !s->a || !s->attn_ws) {
+        attend_free(s);
+        return fail("attention allocation");
+    }
+    /* rows of no sequence have no attention: zeros, not what the memory held */
+    const int rc = qg_zero(s->a, (size_t)T * qw * sizeof(float));
+    if (rc || qg_sync()) {
+        attend_free(s);
+        return fail("initialise attention rows");
+    }
+    memcpy(s->attn_layers, layers, sizeof *layers * (size_t)s->n_layers);
+    s->attn = *attention;
+    s->cache = *cache;
+    return 0;
+}
+
+static int run_verify(nm_stack *s, const qg_kv_batch *batch) {
+    const int nt = batch->rows, D = s->width, hd = s->cache.head_dim, Hq = s->attn.q_heads, Hk = s->cache.kv_heads;
+    const int qw = Hq * hd, kw = Hk * hd, row = qw + 2 * kw;
+    for (int l = 0; l < s->n_layers; l++) {
+        const nm_attention_layer *L = &s->attn_layers[l];
+        const qg_qk_rows rows = {
+            .q = s->qkv, .k = s->qkv + qw, .v = s->qkv + qw + kw, .q_row = row, .q_head = hd, .k_row = row, .k_head = hd,
+            .v_row = row, .v_head = hd, .rows = nt, .q_heads = Hq, .kv_heads = Hk, .head_dim = hd, .q_norm = L->q_norm,
+            .k_norm = L->k_norm, .eps = 1e-6f, .rope_dims = s->attn.rope_dims, .interleaved = s->attn.interleaved,
+            .freq = s->attn.freq,
+        };
+        GPU(qg_norm(s->x, s->h, NULL, D, 1, nt, 0, 0, 1e-6f));
+        GPU(qg_matmul(s->qkv, L->qkv, L->qkv_type, row, D, s->x, nt));
+        GPU(qg_qk_norm_rope(s->q, NULL, &rows, &s->cache, l, batch));
+        GPU(qg_tree_attention(s->a, s->q, Hq, s->attn.scale, &s->cache, l, batch, s->attn_ws, s->attn_ws_bytes));
+        GPU(qg_matmul(s->x, L->out, L->out_type, D, qw, s->a, nt));
+        GPU(qg_binary(s->h, s->h, s->x, nt * D, 0));
+        const size_t act = (size_t)s->max_tokens * D, sel = (size_t)s->max_tokens * NM_TOP;
+        GPU(qg_moe_forward_residual(s->h, s->record ? s->rec_ids + sel * l : s->ids, s->record ? s->rec_w + sel * l : s->w, NULL, NULL,
+                                    s->record ? s->rec_x + act * l : NULL, s->record ? s->rec_out + act * l : NULL, nt, &s->layers[l],
+                                    s->ws, s->ws_bytes));
+    }
+    return 0;
+}
+
+int nm_stack_verify(nm_stack *s, const qg_kv_batch *batch, int use_graph) {
+    if (!s || !s->attn_layers || !batch) return fail("invalid verify arguments");
+    if (batch->rows < 1 || batch->rows > s->max_tokens) return fail("%d rows for a stack of %d tokens", batch->rows, s->max_tokens);
+    if (!batch->start || batch->max_rows < 1 || batch->max_rows > batch->rows) return fail("invalid batch");
+    if (!use_graph) return run_verify(s, batch);
+    void **g = &s->verify_graphs[batch->rows];
+    qg_kv_batch *b = &s->verify_batches[batch->rows];
+    if (*g && (b->max_rows != batch->max_rows || b->start != batch->start || b->parent != batch->parent)) {
+        /* the graph reads other arrays; it may still be running */
+        GPU(qg_sync());
+        qg_graph_destroy(*g);
+        *g = NULL;
+    }
+    if (!*g) {
+        GPU(qg_graph_begin(g));
+        if (run_verify(s, batch)) { qg_graph_destroy(*g); *g = NULL; return -1; }
+        const int end = qg_graph_end(*g);
+        if (end) { qg_graph_destroy(*g); *g = NULL; return fail("capture verify step: %s", qg_error(end)); }
+        *b = *batch;
+    }
+    GPU(qg_graph_launch(*g));
     return 0;
 }
 

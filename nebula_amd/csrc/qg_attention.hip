@@ -388,6 +388,9 @@ template <int TYPE, int D, int RT, int NW>
 __global__ __launch_bounds__(64 * NW, (D / 64) * RT <= 6 ? 2 : 1) void attention_kernel(AttnArgs A, KvView c, BatchView b) {
     typedef Tile<TYPE, D> T;
     constexpr int RG = 16 * RT, E = T::E, DL = T::DL, KEYS = T::KEYS, JOIN = NW * 16 * (D + 4) * 4;
+    // a wave in its products goes before one in its softmax (2048-row chunk at 256 dimensions 540 -> 502 us; at 64
+    // dimensions, where the softmax is most of the time, 204 -> 213: not there)
+    constexpr bool FIRST = D > 64;
     __shared__ __attribute__((aligned(16))) uint8_t s_mem[RT * T::Q_BYTES > JOIN ? RT * T::Q_BYTES : JOIN];
     __shared__ float s_m[NW][RG], s_l[NW][RG], s_back[RG];
     __shared__ unsigned long long s_seen[QG_MAX_TREE];
@@ -479,7 +482,9 @@ __global__ __launch_bounds__(64 * NW, (D / 64) * RT <= 6 ? 2 : 1) void attention
     }
     for (; t0 < end; t0 += NW * KEYS) {
         float z[RT][E];
+        if (FIRST) __builtin_amdgcn_s_setprio(1);
         tile.template scores<RT>(s_mem, lane, z);
+        if (FIRST) __builtin_amdgcn_s_setprio(0);
         // the next tile's keys, whose pages are known, and the pages of the one after it
         const int here = vpage, here_pos = vpos;
         const bool more = t0 + NW * KEYS < end;
@@ -530,7 +535,9 @@ __global__ __launch_bounds__(64 * NW, (D / 64) * RT <= 6 ? 2 : 1) void attention
                 l[r] += z[r][e];
             }
         }
+        if (FIRST) __builtin_amdgcn_s_setprio(1);
         tile.template outputs<RT>(z, o);
+        if (FIRST) __builtin_amdgcn_s_setprio(0);
         if (more) tile.load_v(run(vbase, vpage, vpos), n);
     }
 

@@ -58,6 +58,7 @@ HOST_SIGNATURES = {
     "handoff_scratch_bytes": ([I, I], Z),
     "moe_handoff": ([P, P, P, P, P, P, I, I, P, Z, CPU_MOE_FN, P, P], I),
     "handoff_reserve": ([I, I], I), "device_reads": ([], C.c_uint64),
+    "stack_attend": ([P, P, P, P], I), "stack_verify": ([P, P, I], I),
 }
 
 
@@ -106,6 +107,16 @@ class MoeLayer(C.Structure):
                 ("gate_type", I), ("up_type", I), ("down_type", I),
                 ("sh_gate", P), ("sh_up", P), ("sh_down", P), ("sh_gate_type", I), ("sh_up_type", I), ("sh_down_type", I),
                 ("sh_gate_inp", P), ("resident", P), ("threshold", D64), ("router_bias", P)]
+
+
+class AttentionLayer(C.Structure):
+    """nm_attention_layer of include/nebula_moe.h."""
+    _fields_ = [("qkv", P), ("out", P), ("qkv_type", I), ("out_type", I), ("q_norm", P), ("k_norm", P)]
+
+
+class Attention(C.Structure):
+    """nm_attention of include/nebula_moe.h."""
+    _fields_ = [("q_heads", I), ("rope_dims", I), ("interleaved", I), ("freq", P), ("scale", F)]
 
 
 class KvCache(C.Structure):
