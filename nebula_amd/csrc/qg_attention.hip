@@ -114,6 +114,7 @@ QG_DEV bool plan_find(const KvView &c, const BatchView &b, const AttnArgs &A, in
         scan(s0, x, parts, upto, upto_slots);
         units += __builtin_amdgcn_readlane(upto, 63);
     }
+    if (units <= 0) return false;
     const int run = A.run ? A.run : (units + 7) / 8, k = block >> 3;
     const int unit = (k / run * 8 + (block & 7)) * run + k % run;
     if (unit >= units) return false;
@@ -132,6 +133,7 @@ QG_DEV bool plan_find(const KvView &c, const BatchView &b, const AttnArgs &A, in
             p.groups = __builtin_amdgcn_readlane(x.groups, l);
             p.slot = slots + __builtin_amdgcn_readlane(upto_slots - own_slots, l);
             const int rest = unit - (before + __builtin_amdgcn_readlane(upto - own, l));
+            if (rest < 0 || rest >= __builtin_amdgcn_readlane(own, l)) return false;  // row starts that overlap, past 2^31 units
             p.part = rest / (p.groups * c.heads);
             p.h = rest / p.groups % c.heads;
             p.z = p.groups - 1 - rest % p.groups;  // the last rows, which see the most, first
@@ -146,7 +148,13 @@ QG_DEV bool plan_find(const KvView &c, const BatchView &b, const AttnArgs &A, in
 
 // What is left to do for a row and head: nothing (parts 1, odd 0), to join `parts`
 // partial results from `slot` on, `step` apart, or to take the row up again (odd 1).
-struct Join { int parts, slot, step, odd; };
+struct Join {
+    int parts, slot, step, odd;
+    // Inside the slots: not what the memory held where row starts that overlap leave a unit out.
+    __device__ bool inside(long slots) const {
+        return parts > 0 && parts <= slots && slot >= 0 && slot < slots && step > 0 && step <= slots && slot + (parts - 1L) * step < slots;
+    }
+};
 
 // v_perm of two words into (a.lo, b.lo) or (a.hi, b.hi)
 QG_DEV uint32_t pair_lo(uint32_t a, uint32_t b) { return __builtin_amdgcn_perm(b, a, 0x05040100u); }
@@ -718,7 +726,7 @@ __global__ __launch_bounds__(64 * JOIN_WAVES) void attention_join_kernel(AttnArg
     if (s < 0) return;  // nothing was written for it
     bool odd = j.odd == 1;
     if (j.parts > 1) {
-        if ((size_t)j.slot + (size_t)(j.parts - 1) * j.step >= (size_t)A.slots) return;
+        if (!j.inside(A.slots)) return;
         const int in_group = ((row - first) * A.group + (head - by_group(A, head) * A.group)) % RG;
         float top, sum, y[V];
         if (EACH > 1) {

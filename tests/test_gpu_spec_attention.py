@@ -229,3 +229,25 @@ def test_attention_long_context_split(qgl, typ):
     q = rng.standard_normal((11, 6, 64)).astype(np.float32)
     a = check(cache, batch, q, 0.125)
     np.testing.assert_array_equal(a, attend(cache, batch, q, 0.125))
+
+
+def test_attention_overlapping_starts(qgl):
+    """Row starts that run forwards and backwards give sequences the same rows, more of them than there is work for:
+    nothing outside the buffers is touched, and rows of no sequence stay."""
+    rng = np.random.default_rng(12)
+    B, N = 200, 40
+    cache = Cache(rng, [10] * B, [N] * B, typ=F16, kv_heads=1, page=32, dim=64, fill=False)
+    cache.k[:], cache.v[:] = 0.5, 0.25
+    cache.upload()
+    batch = Batch([0] * (B - 1) + [N], rows=N + 2, max_rows=N)
+    batch.dstart.set(np.array([0, N] * (B // 2) + [0], np.int32))
+    q = rng.standard_normal((N + 2, 8, 64)).astype(np.float32)
+    got = attend(cache, batch, q, 0.125)
+    assert np.isnan(got[N:]).all()
+
+
+def test_attention_without_rows(qgl):
+    """A batch none of whose rows belongs to a sequence."""
+    cache = Cache(np.random.default_rng(13), [10, 0], [0, 0], typ=F16, kv_heads=1, page=8, dim=64)
+    batch = Batch([0, 0], rows=4, max_rows=2)
+    assert np.isnan(attend(cache, batch, np.ones((4, 2, 64), np.float32), 0.125)).all()
