@@ -17,6 +17,14 @@
 // in memory and pairs them with byte permutes.  Neither product moves a value
 // between lanes.
 //
+// What bounds it (MI355X, fp16 cache, 16 heads over 2, 128 dimensions).  Up to 48 rows
+// of a head (one row group): memory, 16 sequences x 98304 keys 289 us with 2 rows
+// and 303 with 6, 5.3 to 5.6 TB/s.  More row groups share the reads in the L2 but each
+// adds its products and softmax: 451 us with 12 rows, 617 with 17 (the matrix cores
+// busy for a third of the time, the rest a wave's latencies with two waves per SIMD).
+// One sequence of 24576 keys, 17 rows: 31 us, of which 13 before the first product
+// and after the last.
+//
 // Precision: q and p enter as planes that the 16-bit cores multiply exactly with
 // the cache's values: two fp16 planes (22 bits; q scaled by a power of two per
 // row), three bf16 planes (24 bits); an F32 cache uses the fp32 cores.
@@ -656,9 +664,11 @@ QG_DEV void attend_row(const AttnArgs &A, const KvView &c, const BatchView &b, i
 
 // Joins the parts of sequences that were cut, and takes up odd rows again.  Few
 // rows and heads: a workgroup each, whose four waves take a quarter of the parts.
-// Many (a prompt chunk: few parts each): a wave each.
+// Many (then each has few parts): a wave each.  A chunk behind 2000 keys, whole call,
+// workgroup / wave each: 1024 rows and heads 25.5 / 26.1 us, 2048 31.5 / 29.7, 4096
+// 47.7 / 42.7; but one row of 16 heads over 98304 keys 30 / 54.
 constexpr int JOIN_WAVES = 4;
-constexpr size_t JOIN_FEW = 4096;
+constexpr size_t JOIN_FEW = 1024;
 
 // Parts i0, i0 + by, .. of a row: their largest m, and sums under it.  A lane holds
 // the weight of one part, so that the parts' loads wait for nothing.

@@ -30,7 +30,9 @@ QG_DEV void turn_of(double angle, float &s, float &c) {
 }
 
 // A wave takes U heads-per-wave of one row: the row's place, its angles' sines and
-// the loads of all its heads once.
+// the loads of all its heads once.  Bound by memory where rows are many (8192 rows
+// of 16 + 2 + 2 heads of 128: 35 us, 4.6 TB/s; with one head per wave 59), by the
+// launch and two dependent reads where they are few (one row 3.6 us).
 template <int D, int U>
 __global__ __launch_bounds__(256) void qk_rope_kernel(RopeArgs A, KvView c, BatchView b, int layer, int parts) {
     constexpr int LPH = D / 4, HPW = 64 / LPH;  // lanes per head, heads per wave
@@ -134,7 +136,7 @@ __global__ __launch_bounds__(256) void qk_rope_kernel(RopeArgs A, KvView c, Batc
 template <int D>
 void launch_rope(const RopeArgs &A, const KvView &c, const BatchView &b, int layer, hipStream_t s) {
     const int units = (A.q_heads + A.kv_heads * (A.cached ? 2 : 1) + 256 / D - 1) / (256 / D);  // wavefuls of heads per row
-    const bool wide = (long)A.rows * units > 8192;
+    const bool wide = (long)A.rows * units > 8192;  // more waves than the card holds: five times the work for each
     const int parts = wide ? (units + 4) / 5 : units;
     const unsigned blocks = (unsigned)(((long)A.rows * parts + 3) / 4);
     if (wide) qk_rope_kernel<D, 5><<<blocks, 256, 0, s>>>(A, c, b, layer, parts);
@@ -213,14 +215,15 @@ QG_DEV void write_spread(float *x, int n, F get) {
     }
 }
 
-// A workgroup per row.  REGS values of a thread stay in registers and KEPT in
-// shared memory between the three passes (largest value, sum, output); what is
-// longer is read again.
+// A workgroup per row of up to (REGS + KEPT) THREADS values: REGS values of a thread
+// stay in registers and KEPT in shared memory between the three passes (largest
+// value, sum, output).  96 + 36 values of 1024 threads are a CU's whole store: a row
+// of 135168 is read once and written once (1088 x 131072: 255 us, 4.5 TB/s; read
+// twice, with one value per thread and pass, 631).
 template <int THREADS, int REGS, int KEPT>
 __global__ __launch_bounds__(THREADS) void softmax_row_kernel(float *out, const float *x, int cols, float scale) {
     __shared__ float s_x[KEPT ? KEPT * THREADS : 1], s_f[THREADS / 64];
     __shared__ int s_i[THREADS / 64];
-    constexpr int HELD = (REGS + KEPT) * THREADS;
     const int tid = threadIdx.x;
     const float *row = x + (size_t)blockIdx.x * cols;
     float *to = out + (size_t)blockIdx.x * cols;
@@ -232,7 +235,6 @@ __global__ __launch_bounds__(THREADS) void softmax_row_kernel(float *out, const 
             s_x[k * THREADS + tid] = v;
             m = fmaxf(m, v);
         });
-    for (int i = HELD + tid; i < cols; i += THREADS) m = fmaxf(m, row[i]);
 #pragma unroll
     for (int k = 0; k < REGS; k++) m = fmaxf(m, r[k]);
     m = block_all<THREADS>(m, s_f, Larger());
@@ -252,16 +254,16 @@ __global__ __launch_bounds__(THREADS) void softmax_row_kernel(float *out, const 
         s_x[k * THREADS + tid] = e;
         sum += e;
     }
-    for (int i = HELD + tid; i < cols; i += THREADS) sum += __builtin_amdgcn_exp2f((row[i] - m) * scale);
     const float inv = 1.0f / block_all<THREADS>(sum, s_f, Added());
     write_spread<THREADS, REGS, 8>(to, cols, [&](int k) { return r[k] * inv; });
     if constexpr (KEPT > 0)
         write_spread<THREADS, KEPT, 4>(to + REGS * THREADS, cols - REGS * THREADS, [&](int k) { return s_x[k * THREADS + tid] * inv; });
-    for (int i = HELD + tid; i < cols; i += THREADS) to[i] = __builtin_amdgcn_exp2f((row[i] - m) * scale) * inv;
 }
 
 // Few rows: pieces of SM_PIECE values, a workgroup each; first every piece's
-// largest value, its index and the sum, then every piece's outputs from the row's.
+// largest value, its index and the sum, then every piece's outputs from the row's
+// (the second read is served by the caches).  17 x 151936: 3.6 + 5.0 us for 4.3 us of
+// memory traffic, each kernel a launch and two or three dependent reads.
 constexpr int SM_THREADS = 256, SM_REGS = 16, SM_PIECE = SM_THREADS * SM_REGS;
 struct SoftPart { float m, sum; int at, pad; };
 
@@ -269,9 +271,10 @@ template <bool LAST>
 __global__ __launch_bounds__(SM_THREADS) void softmax_piece_kernel(float *out, const float *x, int cols, float scale, SoftPart *parts) {
     __shared__ float s_f[4];
     __shared__ int s_i[4];
-    const int tid = threadIdx.x, c0 = blockIdx.x * SM_PIECE, n = min(SM_PIECE, cols - c0), pieces = gridDim.x;
-    const float *row = x + (size_t)blockIdx.y * cols + c0, none = -__builtin_inff();
-    parts += (size_t)blockIdx.y * pieces;
+    const int pieces = (cols + SM_PIECE - 1) / SM_PIECE, which = blockIdx.x / pieces, piece = blockIdx.x % pieces;
+    const int tid = threadIdx.x, c0 = piece * SM_PIECE, n = min(SM_PIECE, cols - c0);
+    const float *row = x + (size_t)which * cols + c0, none = -__builtin_inff();
+    parts += (size_t)which * pieces;
     float r[SM_REGS], m = none, sum = 0.0f;
     read_spread<SM_THREADS, SM_REGS, SM_REGS>(row, n, [&](int k, float v) { r[k] = v; });
     if (!LAST) {
@@ -286,10 +289,10 @@ __global__ __launch_bounds__(SM_THREADS) void softmax_piece_kernel(float *out, c
             for (int k = 0; k < SM_REGS; k++) sum += __builtin_amdgcn_exp2f((r[k] - m) * scale);
             sum = block_all<SM_THREADS>(sum, s_f, Added());
         }
-        if (tid == 0) parts[blockIdx.x] = SoftPart{m, sum, at == SM_NAN ? SM_NAN : c0 + at, 0};
+        if (tid == 0) parts[piece] = SoftPart{m, sum, at == SM_NAN ? SM_NAN : c0 + at, 0};
         return;
     }
-    float *to = out + (size_t)blockIdx.y * cols + c0;
+    float *to = out + (size_t)which * cols + c0;
     for (int i = tid; i < pieces; i += SM_THREADS) m = fmaxf(m, parts[i].m);
     m = block_all<SM_THREADS>(m, s_f, Larger());
     int at = 0x7fffffff;
@@ -310,8 +313,13 @@ __global__ __launch_bounds__(SM_THREADS) void softmax_piece_kernel(float *out, c
         return nan ? __builtin_nanf("") : y;
     });
 }
-// Pieces where the rows alone would not fill the card.
-bool softmax_pieces(int rows, int cols) { return rows < 128 && cols > SM_PIECE; }
+// Pieces for long rows: always where a row is longer than a workgroup holds (96 rows of
+// 200000: 38 us in pieces, 77 by rows; 512: 242 / 286), else while the rows are too
+// few to fill the card (131072 columns: 64 rows 16.9 / 24.8, 96 26.9 / 27.8, 128 33.5 /
+// 29.1; 70000: 64 11.3 / 20.3, 256 35.6 / 32.7).  Rows of up to 40960 are faster by
+// rows however few (1 row of 32000: 8.0 / 6.8; 8192: 7.9 / 5.1).
+constexpr int SM_SHORT = 40 * 1024, SM_HELD = (96 + 36) * 1024;
+bool softmax_pieces(int rows, int cols) { return cols > SM_HELD || (cols > SM_SHORT && (long)rows * cols < 13000000); }
 
 // ------------------------------------------------------------------------
 // Verification.  After j rejections at a row the target's distribution without
@@ -470,7 +478,9 @@ QG_DEV double all_pieces(const double *sums, int pieces, double ahead, int lane)
 }
 
 // One sum: workgroup x of sequence y takes the walk to its next sum and adds its
-// piece of it.  round 0 starts the walk.
+// piece of it.  round 0 starts the walk.  64 sequences x 131072 tokens: 14 us for the
+// first sum (67 MB, 4.7 TB/s), then 4 to 6 for what few sequences still need; one
+// sequence x 151936: 4 us, four dependent reads.
 __global__ __launch_bounds__(VF_THREADS) void verify_sum_kernel(VerifyArgs A, BatchView b, int round) {
     __shared__ double s_red[4];
     const int s = blockIdx.y, lane = threadIdx.x & 63;
@@ -621,6 +631,8 @@ Pieces verify_pieces(int sequences, int cols) {
 }
 // Sums by launches over the whole card; a tree's later ones (each takes another
 // rejection with drafts left to try) are few and fall to the drawing workgroup.
+// With 2 / 4 / 7: 64 trees of 17 rows x 131072 tokens 75 / 38 / 46 us, 16 of 33 x
+// 50000 40 / 31 / 39, one of 17 x 151936 15 / 19 / 26.
 int verify_rounds(const BatchView &b, bool sampled) { return b.parent && sampled ? 4 : 1; }
 
 }  // namespace
@@ -685,13 +697,15 @@ int qg_softmax(float *out, const float *x, int rows, int cols, float temperature
     // log2 e / T, finite and not 0, which stands for temperature 0
     const float scale = temperature > 0.0f ? fminf(fmaxf(1.44269504088896341f / temperature, 1e-37f), 3e38f) : 0.0f;
     if (softmax_pieces(rows, cols)) {
-        const dim3 grid((cols + SM_PIECE - 1) / SM_PIECE, rows);
+        const unsigned grid = (unsigned)((cols + SM_PIECE - 1) / SM_PIECE * rows);
         softmax_piece_kernel<false><<<grid, SM_THREADS, 0, qg_stream()>>>(out, x, cols, scale, (SoftPart *)ws);
         softmax_piece_kernel<true><<<grid, SM_THREADS, 0, qg_stream()>>>(out, x, cols, scale, (SoftPart *)ws);
     } else if (cols <= 4096) {
         softmax_row_kernel<256, 16, 0><<<rows, 256, 0, qg_stream()>>>(out, x, cols, scale);
     } else if (cols <= 16384) {
         softmax_row_kernel<1024, 16, 0><<<rows, 1024, 0, qg_stream()>>>(out, x, cols, scale);
+    } else if (cols <= SM_SHORT) {
+        softmax_row_kernel<1024, 40, 0><<<rows, 1024, 0, qg_stream()>>>(out, x, cols, scale);
     } else {
         softmax_row_kernel<1024, 96, 36><<<rows, 1024, 0, qg_stream()>>>(out, x, cols, scale);
     }

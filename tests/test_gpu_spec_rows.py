@@ -148,7 +148,7 @@ def softmax_oracle(x, T):
     return e / e.sum(-1, keepdims=True), tol
 
 
-@pytest.mark.parametrize("rows,cols", [(1, 1), (3, 2), (1, 63), (5, 1000), (2, 4097), (17, 32003), (1, 151936), (300, 1025), (2, 300001), (1000, 7), (130, 20011), (129, 140003)])
+@pytest.mark.parametrize("rows,cols", [(1, 1), (3, 2), (1, 63), (5, 1000), (2, 4097), (17, 32003), (1, 151936), (300, 1025), (2, 300001), (1000, 7), (130, 20011), (129, 140003), (3, 40960), (3, 40961), (200, 70001), (140, 131072)])
 @pytest.mark.parametrize("T", [0.7, 1.0, 30.0])
 def test_softmax(qgl, rows, cols, T):
     rng = np.random.default_rng(rows * 7 + cols)
@@ -161,7 +161,7 @@ def test_softmax(qgl, rows, cols, T):
         assert np.all(np.abs(got - want) <= tol * want + 2.0 ** -126), np.max(np.abs(got - want) / (tol * want + 2.0 ** -126))
 
 
-@pytest.mark.parametrize("rows,cols", [(6, 5), (6, 5000), (6, 131072), (600, 4100), (130, 20001), (129, 140003)])
+@pytest.mark.parametrize("rows,cols", [(6, 5), (6, 5000), (6, 131072), (600, 4100), (130, 20001), (129, 140003), (300, 50001)])
 def test_softmax_special_rows(qgl, rows, cols):
     rng = np.random.default_rng(cols)
     x = rng.standard_normal((rows, cols)).astype(np.float32)
@@ -181,7 +181,7 @@ def test_softmax_special_rows(qgl, rows, cols):
     assert np.all(np.abs(got[6:] - want) <= tol * want + 2.0 ** -126)
 
 
-@pytest.mark.parametrize("rows,cols", [(4, 1), (5, 4099), (2, 151937), (700, 1500), (128, 20001)])
+@pytest.mark.parametrize("rows,cols", [(4, 1), (5, 4099), (2, 151937), (700, 1500), (128, 20001), (300, 50001)])
 def test_softmax_greedy(qgl, rows, cols):
     """Temperature 0: one at the lowest index of the largest value."""
     rng = np.random.default_rng(cols)
