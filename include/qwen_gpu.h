@@ -243,7 +243,9 @@ int qg_qk_norm_rope(float *q_out, float *k_out, const qg_qk_rows *in, const qg_k
  * Scores, statistics and sums are held in fp32; the products run on the matrix
  * cores with queries and probabilities in planes of the cache's type that
  * together carry at least 22 bits.  A row that sees no token (or none with a
- * score above -infinity) is 0.  Rows of no sequence are left as they were. */
+ * score above -infinity) is 0.  Rows of no sequence are left as they were.
+ * rows x q_heads at most 2^25.  The workspace of a batch serves every batch of
+ * no more rows. */
 size_t qg_tree_attention_workspace_bytes(const qg_kv_cache *cache, const qg_kv_batch *batch, int q_heads);
 int qg_tree_attention(float *out, const float *q, int q_heads, float scale, const qg_kv_cache *cache, int layer,
                       const qg_kv_batch *batch, void *workspace, size_t workspace_bytes);
@@ -251,7 +253,7 @@ int qg_tree_attention(float *out, const float *q, int q_heads, float scale, cons
 /* out = softmax(x / temperature) of each row of [rows][cols]; out may be x.
  * temperature 0: 1 at the lowest index of the largest value.  -infinity gives
  * 0; a row of nothing but -infinity is 0; a row with NaN or +infinity is NaN.
- * rows 1..65536, cols 1..2^24; 4-byte aligned. */
+ * rows 1..65536, cols 1..2^24, at most 2^35 values; 4-byte aligned. */
 size_t qg_softmax_workspace_bytes(int rows, int cols);
 int qg_softmax(float *out, const float *x, int rows, int cols, float temperature, void *workspace, size_t workspace_bytes);
 

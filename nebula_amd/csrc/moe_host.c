@@ -156,14 +156,7 @@ int nm_stack_attend(nm_stack *s, const nm_attention_layer *layers, const nm_atte
         (attention->rope_dims && !attention->freq))
         return fail("invalid rotation");
     const size_t qw = (size_t)attention->q_heads * cache->head_dim, kw = (size_t)cache->kv_heads * cache->head_dim;
-    s->attn_ws_bytes = 0;
-    /* fewer rows may take another shape of the kernel, with more partial results */
-    for (int rows = 1; rows <= T; rows++)
-        for (int most_rows = 1; most_rows <= rows; most_rows++) {
-            const qg_kv_batch b = {.rows = rows, .max_rows = most_rows, .start = &none};
-            const size_t n = qg_tree_attention_workspace_bytes(cache, &b, attention->q_heads);
-            if (n > s->attn_ws_bytes) s->attn_ws_bytes = n;
-        }
+    s->attn_ws_bytes = ws;
     s->attn_layers = malloc(sizeof *layers * (size_t)s->n_layers);
     s->x = qg_alloc((size_t)T * s->width * sizeof(float));
     s->qkv = qg_alloc((size_t)T * (qw + 2 * kw) * sizeof(float));

@@ -768,8 +768,9 @@ __global__ __launch_bounds__(64 * JOIN_WAVES) void attention_join_kernel(AttnArg
 }
 
 // Row tiles per wave: as few row groups as the registers allow, and no more tiles than those need.
+constexpr int most_tiles(int dim) { return dim == 256 ? 2 : dim == 128 ? 3 : 4; }
 int row_tiles(int dim, long rows) {
-    const long most = dim == 256 ? 2 : dim == 128 ? 3 : 4, groups = (rows + 16 * most - 1) / (16 * most);
+    const long most = most_tiles(dim), groups = (rows + 16 * most - 1) / (16 * most);
     return (int)((rows + 16 * groups - 1) / (16 * groups));
 }
 constexpr int WAVES = 4;
@@ -809,6 +810,14 @@ int resident(int dim, int rt) {
 // twice its keys / chunk, and the chunk is at least all sequences' keys x row
 // groups x heads / two rounds.
 size_t slots(int dim, int rt) { return 4 * (size_t)resident(dim, rt); }
+// Rows of them: of the shape that needs the most, so that a workspace serves every
+// batch of no more rows.
+size_t part_rows(int dim) {
+    size_t most = 0;
+    for (int rt = 1; rt <= most_tiles(dim); rt++) most = most > slots(dim, rt) * 16 * rt ? most : slots(dim, rt) * 16 * rt;
+    return most;
+}
+constexpr long JOBS = 1L << 25;  // rows x heads: of the join kernel, a wave each, within 2^32 threads
 }  // namespace
 
 extern "C" {
@@ -816,9 +825,8 @@ extern "C" {
 size_t qg_tree_attention_workspace_bytes(const qg_kv_cache *cache, const qg_kv_batch *batch, int q_heads) {
     if (qg_kv_check(cache, false, nullptr) || qg_batch_check(batch, false, nullptr)) return 0;
     if (q_heads < 1 || q_heads % cache->kv_heads || q_heads / cache->kv_heads > 128) return 0;
-    const int group = q_heads / cache->kv_heads;
-    const int rt = row_tiles(cache->head_dim, (long)batch->max_rows * group);
-    return slots(cache->head_dim, rt) * 16 * rt * (4 * (size_t)cache->head_dim + sizeof(float2)) + sizeof(int4) * (size_t)batch->rows * q_heads;
+    if ((long)batch->rows * q_heads > JOBS) return 0;
+    return part_rows(cache->head_dim) * (4 * (size_t)cache->head_dim + sizeof(float2)) + sizeof(int4) * (size_t)batch->rows * q_heads;
 }
 
 int qg_tree_attention(float *out, const float *q, int q_heads, float scale, const qg_kv_cache *cache, int layer,

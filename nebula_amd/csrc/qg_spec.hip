@@ -684,7 +684,7 @@ int qg_qk_norm_rope(float *q_out, float *k_out, const qg_qk_rows *in, const qg_k
 }
 
 size_t qg_softmax_workspace_bytes(int rows, int cols) {
-    if (rows < 1 || rows > QG_MAX_ROWS || cols < 1 || cols > 1 << 24) return 0;
+    if (rows < 1 || rows > QG_MAX_ROWS || cols < 1 || cols > 1 << 24 || (long)rows * cols > 1L << 35) return 0;
     return softmax_pieces(rows, cols) ? (size_t)rows * ((cols + SM_PIECE - 1) / SM_PIECE) * sizeof(SoftPart) : sizeof(SoftPart);
 }
 

@@ -96,7 +96,14 @@ def test_refused_workspaces(lib):
     assert n and lib.qg_softmax(A, 2 * A, 3, 1000, 1.0, 22 * A, n - 1) == INVALID
     n = lib.qg_verify_workspace_bytes(3, 1000)
     assert n and lib.qg_verify_drafts(A, A, A, A, A, A, A, A, 1000, 3, ref(b), 22 * A, n - 1) == INVALID
-    for rows_, cols in ((0, 5), (5, 0), (65537, 5), (5, (1 << 24) + 1), (-1, -1)):
+    # a workspace serves every batch of no more rows; too many rows x heads for one launch are refused
+    sizes = [lib.qg_tree_attention_workspace_bytes(ref(cache(head_dim=128)), ref(batch(rows=64, max_rows=m)), 16) for m in range(1, 65)]
+    assert len(set(sizes)) == 1
+    assert all(0 < lib.qg_tree_attention_workspace_bytes(ref(c), ref(batch(rows=r, max_rows=1)), 4) <= n0
+               for n0 in [lib.qg_tree_attention_workspace_bytes(ref(c), ref(batch(rows=40, max_rows=40, parent=None)), 4)] for r in range(1, 41))
+    assert lib.qg_tree_attention_workspace_bytes(ref(c), ref(batch(rows=65536, max_rows=9)), 256) > 0
+    assert lib.qg_tree_attention_workspace_bytes(ref(cache(kv_heads=128)), ref(batch(rows=65536, max_rows=9)), 1024) == 0
+    for rows_, cols in ((0, 5), (5, 0), (65537, 5), (5, (1 << 24) + 1), (-1, -1), (4096, 1 << 24)):
         assert lib.qg_softmax_workspace_bytes(rows_, cols) == 0
     for seq, cols in ((0, 5), (1025, 5), (5, 0), (5, (1 << 24) + 1)):
         assert lib.qg_verify_workspace_bytes(seq, cols) == 0
