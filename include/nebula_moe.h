@@ -59,7 +59,7 @@ int nm_stack_attend(nm_stack *s, const nm_attention_layer *layers, const nm_atte
 /* All layers of the batch's rows (last accepted tokens and their drafts; at
  * most the stack's max_tokens together) in the first rows of the hidden state:
  * h <- h + Wo attention(RMSNorm(h)), h <- h + MoE(RMSNorm(h)) (eps 1e-6, unit
- * weight).  Keys and values of the rows are stored behind the cached tokens;
+ * weight); rows of no sequence take the MoE alone.  Keys and values of the rows are stored behind the cached tokens;
  * lengths do not change (qg_kv_compact does that once drafts are accepted).
  * use_graph: captured on first use per number of rows and replayed while the
  * batch's arrays stay where they are; what they hold may change. */

@@ -167,12 +167,6 @@ int nm_stack_attend(nm_stack *s, const nm_attention_layer *layers, const nm_atte
         attend_free(s);
         return fail("attention allocation");
     }
-    /* rows of no sequence have no attention: zeros, not what the memory held */
-    const int rc = qg_zero(s->a, (size_t)T * qw * sizeof(float));
-    if (rc || qg_sync()) {
-        attend_free(s);
-        return fail("initialise attention rows");
-    }
     memcpy(s->attn_layers, layers, sizeof *layers * (size_t)s->n_layers);
     s->attn = *attention;
     s->cache = *cache;
@@ -182,6 +176,8 @@ int nm_stack_attend(nm_stack *s, const nm_attention_layer *layers, const nm_atte
 static int run_verify(nm_stack *s, const qg_kv_batch *batch) {
     const int nt = batch->rows, D = s->width, hd = s->cache.head_dim, Hq = s->attn.q_heads, Hk = s->cache.kv_heads;
     const int qw = Hq * hd, kw = Hk * hd, row = qw + 2 * kw;
+    /* rows of no sequence have no attention: zeros, not what the last batch left there */
+    GPU(qg_zero(s->a, (size_t)nt * qw * sizeof(float)));
     for (int l = 0; l < s->n_layers; l++) {
         const nm_attention_layer *L = &s->attn_layers[l];
         const qg_qk_rows rows = {

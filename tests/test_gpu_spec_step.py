@@ -315,6 +315,35 @@ def test_stack_verify_other_batches(stack_parts):
         host.nm_stack_destroy(stack)
 
 
+def test_stack_verify_rows_of_no_sequence(stack_parts):
+    """Rows behind the last sequence take the MoE alone, whatever the batch before had in their places."""
+    rng = np.random.default_rng(11)
+    host = qg.host()
+    cache = Cache(np.random.default_rng(12), [50], [9], typ=F16, layers=LAYERS, kv_heads=HK, page=16, dim=HD)
+    stack = make_stack(stack_parts, cache, 9)
+    try:
+        h0 = rng.standard_normal((9, WIDTH)).astype(np.float32)
+        for counts, graph in (([9], 0), ([4], 0), ([9], 1), ([4], 1)):
+            batch = Batch(counts, max_rows=9, rows=9)
+            call("write", host.nm_stack_hidden(stack), h0.ctypes.data, h0.nbytes)
+            say(f"rows {counts} of 9, graph={graph}")
+            assert host.nm_stack_verify(stack, batch.ref, graph) == 0, host.nm_last_error()
+            call("sync")
+            got = np.empty_like(h0)
+            call("read", got.ctypes.data, host.nm_stack_hidden(stack), got.nbytes)
+            if counts == [4]:
+                call("write", host.nm_stack_hidden(stack), h0.ctypes.data, h0.nbytes)
+                assert host.nm_stack_forward(stack, 9, 0) == 0, host.nm_last_error()
+                call("sync")
+                alone = np.empty_like(h0)
+                call("read", alone.ctypes.data, host.nm_stack_hidden(stack), alone.nbytes)
+                # sums of a few thousand fp32 terms, in an order that other rows may change
+                np.testing.assert_allclose(got[4:], alone[4:], rtol=1e-4, atol=1e-4)
+                assert np.abs(got[:4] - alone[:4]).max() > 0.01
+    finally:
+        host.nm_stack_destroy(stack)
+
+
 def test_stack_attend_refusals(stack_parts):
     layers, qkv, out, norms, freq = stack_parts
     host = qg.host()
