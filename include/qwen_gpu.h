@@ -182,7 +182,9 @@ int qg_moe_forward_residual(float *h, int *ids, float *weights, unsigned char *f
  * [0, pages) holds nothing, a length is taken as 0..table_pages * page_tokens,
  * the rows of a sequence as at most max_rows inside [0, rows), and a parent
  * that is not an earlier row of its sequence as none.  Nothing outside the
- * given buffers is read or written. */
+ * given buffers is read or written.  A workspace belongs to one call until that
+ * has run: calls of one stream may share it, others (and graphs that may run at
+ * once) may not. */
 
 /* Keys and values of `sequences` sequences in pages of page_tokens tokens.
  * Position t of sequence s lies in page table[s][t / page_tokens] at token
@@ -190,7 +192,7 @@ int qg_moe_forward_residual(float *h, int *ids, float *weights, unsigned char *f
 typedef struct {
     void *k, *v;                /* [layers][pages][kv_heads][page_tokens][head_dim], 16-byte aligned */
     int type;                   /* 0 F32, 1 F16, 30 BF16 */
-    int layers, pages, kv_heads; /* kv_heads 1..128 */
+    int layers, pages, kv_heads; /* layers 1..65536, kv_heads 1..128 */
     int page_tokens;            /* a power of two, 8..1024 */
     int head_dim;               /* 64, 128 or 256 */
     int *refs;                  /* [pages] table entries that hold each page, 0 = free; page calls only, else NULL */
@@ -273,7 +275,7 @@ int qg_softmax(float *out, const float *x, int rows, int cols, float temperature
  * u, u_last in [0, 1).  Outputs: count[s] = accepted rows with row 0 (0 for a
  * sequence without rows); path[s][0..count-1] their places; tokens_out[s]
  * [0..count-1] the accepted tokens and the last one; -1 behind them
- * ([sequences][max_rows] both).  A token outside [0, cols) is never accepted. */
+ * ([sequences][max_rows] both; outputs, workspace, p and q do not overlap).  A token outside [0, cols) is never accepted. */
 size_t qg_verify_workspace_bytes(int sequences, int cols);
 int qg_verify_drafts(int *tokens_out, int *path, int *count, const float *p, const float *q, const int *token,
                      const float *u, const float *u_last, int cols, int sequences, const qg_kv_batch *batch,
@@ -297,7 +299,8 @@ int qg_kv_reserve(const qg_kv_cache *cache, const qg_kv_batch *batch, int *statu
  * or an index out of range is left out.  n 1..sequences. */
 int qg_kv_fork(const qg_kv_cache *cache, const int *dst, const int *src, int n, void *workspace, size_t workspace_bytes);
 /* length[s] = min(length[s], new_length[s]) (new_length NULL: as it is), and
- * the pages behind it are let go; 0 frees a sequence. */
+ * the pages behind it are let go; 0 frees a sequence.  new_length may be the
+ * cache's length. */
 int qg_kv_truncate(const qg_kv_cache *cache, const int *new_length);
 /* The accepted rows (qg_verify_drafts' path and count) move to the front: the
  * token at length[s] + path[s][i] goes to length[s] + i, in every layer, and

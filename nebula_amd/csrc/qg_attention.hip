@@ -836,7 +836,7 @@ int qg_tree_attention(float *out, const float *q, int q_heads, float scale, cons
     const size_t need = qg_tree_attention_workspace_bytes(cache, batch, q_heads);
     if (!need || qg_kv_check(cache, false, &c) || qg_batch_check(batch, false, &b)) return hipErrorInvalidValue;
     if (!out || !q || !ws || ws_bytes < need || (((uintptr_t)out | (uintptr_t)q | (uintptr_t)ws) & 15)) return hipErrorInvalidValue;
-    if (layer < 0 || layer >= c.layers || !__builtin_isfinite(scale)) return hipErrorInvalidValue;
+    if (layer < 0 || layer >= c.layers || !__builtin_isfinite(scale * 1.44269504088896341f)) return hipErrorInvalidValue;
     const size_t bytes = 4 * (size_t)b.rows * q_heads * c.dim;
     if (qg_overlap(out, bytes, q, bytes) || qg_overlap(ws, need, q, bytes) || qg_overlap(ws, need, out, bytes)) return hipErrorInvalidValue;
     const int group = q_heads / c.heads, rt = row_tiles(c.dim, (long)b.max_rows * group);

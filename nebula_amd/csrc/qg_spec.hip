@@ -727,6 +727,12 @@ int qg_verify_drafts(int *tokens_out, int *path, int *count, const float *p, con
     if (((uintptr_t)tokens_out | (uintptr_t)path | (uintptr_t)count | (uintptr_t)p | (uintptr_t)q | (uintptr_t)token | (uintptr_t)u |
          (uintptr_t)u_last) & 3)
         return hipErrorInvalidValue;
+    const size_t vb = 4 * (size_t)b.rows * cols, ob = 4 * (size_t)sequences * b.max_rows, cb = 4 * (size_t)sequences;
+    // what is written, and p and q, which are read all the while
+    const struct { const void *at; size_t bytes; } own[6] = {{tokens_out, ob}, {path, ob}, {count, cb}, {ws, need}, {p, vb}, {q, vb}};
+    for (int i = 0; i < 4; i++)
+        for (int j = i + 1; j < 6; j++)
+            if (qg_overlap(own[i].at, own[i].bytes, own[j].at, own[j].bytes)) return hipErrorInvalidValue;
     const Pieces pieces = verify_pieces(sequences, cols);
     const int rounds = verify_rounds(b, q != nullptr);
     Walk *walks = (Walk *)ws;

@@ -159,6 +159,22 @@ def test_refused_calls(lib):
     assert lib.qg_kv_truncate(ref(c), A + 2) == INVALID
 
 
+def test_refused_overlaps(lib):
+    """Arrays that a call reads in one workgroup and writes in another, and sizes past an index."""
+    c, b = cache(), batch()
+    W, N = 60 * A, 1 << 30
+    assert lib.qg_kv_truncate(ref(c), c.length + 4) == INVALID and lib.qg_kv_truncate(ref(c), c.length - 8) == INVALID
+    good = [30 * A, 31 * A, 32 * A, 33 * A, 34 * A, 35 * A, 36 * A, 37 * A, 100, 3, ref(b), W, N]
+    for i, bad in ((0, 31 * A), (0, 31 * A + 4), (0, 32 * A), (1, 32 * A - 4), (0, 33 * A), (1, 34 * A + 16), (2, 33 * A + 8), (0, W), (1, W + 64), (2, W + 4),
+                   (3, W), (4, W + 4)):
+        args = list(good)
+        args[i] = bad
+        assert lib.qg_verify_drafts(*args) == INVALID, (i, bad)
+    huge = cache(layers=65537)
+    assert lib.qg_tree_attention_workspace_bytes(ref(huge), ref(b), 4) == 0 and lib.qg_kv_copy_pages(ref(huge), A, A, 1) == INVALID
+    assert lib.qg_tree_attention(20 * A, 21 * A, 4, 3e38, ref(c), 0, ref(b), 22 * A, 1 << 30) == INVALID
+
+
 HARNESS = r"""
 #include "qg_kv_index.h"
 extern "C" int page(const int *table, int pages, int shift, int sequences, int table_pages, const int *length, int s, int t, int *len, long long *at) {
