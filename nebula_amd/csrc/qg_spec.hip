@@ -169,19 +169,17 @@ struct Added {
 };
 struct Lower { __device__ __forceinline__ int operator()(int a, int b) const { return min(a, b); } };
 constexpr int SM_NAN = -1;  // in place of the index of a row's largest value
-
-// The lowest index of value m in x[0..n), SM_NAN if there is a NaN, n without
-// either; in every thread.
-template <int THREADS>
-QG_DEV int lowest_of(const float *x, int n, float m, int *s) {
-    int at = n;
-    for (int i = threadIdx.x; i < n; i += THREADS) {
-        const float v = x[i];
-        if (v != v) at = SM_NAN;
-        else if (v == m) at = min(at, i);
+// Where a thread's values THREADS apart hold the row's largest m first: the number
+// of the value (an index each would cost a register each), -1 without one.
+struct FirstOf {
+    int k = -1;
+    bool nan = false;
+    __device__ __forceinline__ void see(int i, float x, float m) {  // from the last one down
+        if (x == m) k = i;
+        nan |= x != x;
     }
-    return block_all<THREADS>(at, s, Lower());
-}
+    template <int THREADS> __device__ __forceinline__ int index() const { return nan ? SM_NAN : k < 0 ? 0x7fffffff : k * THREADS + (int)threadIdx.x; }
+};
 
 // N values of a thread, THREADS apart, from x[0..n) on: whole groups of G without
 // a bound per value, which would cost an address each.
@@ -219,11 +217,12 @@ QG_DEV void write_spread(float *x, int n, F get) {
 // stay in registers and KEPT in shared memory between the three passes (largest
 // value, sum, output).  96 + 36 values of 1024 threads are a CU's whole store: a row
 // of 135168 is read once and written once (1088 x 131072: 255 us, 4.5 TB/s; read
-// twice, with one value per thread and pass, 631).
-template <int THREADS, int REGS, int KEPT>
+// twice, with one value per thread and pass, 631).  BEST: temperature 0, in a kernel
+// of its own, since the registers hold one of the two (250 us; both in one kernel 350).
+template <int THREADS, int REGS, int KEPT, bool BEST>
 __global__ __launch_bounds__(THREADS) void softmax_row_kernel(float *out, const float *x, int cols, float scale) {
     __shared__ float s_x[KEPT ? KEPT * THREADS : 1], s_f[THREADS / 64];
-    __shared__ int s_i[THREADS / 64];
+    __shared__ int s_i[BEST ? THREADS / 64 : 1];
     const int tid = threadIdx.x;
     const float *row = x + (size_t)blockIdx.x * cols;
     float *to = out + (size_t)blockIdx.x * cols;
@@ -238,13 +237,21 @@ __global__ __launch_bounds__(THREADS) void softmax_row_kernel(float *out, const 
 #pragma unroll
     for (int k = 0; k < REGS; k++) m = fmaxf(m, r[k]);
     m = block_all<THREADS>(m, s_f, Larger());
-    if (scale == 0.0f || m == none) {  // temperature 0, or nothing above -infinity
-        const int at = lowest_of<THREADS>(row, cols, scale == 0.0f ? m : 0.0f, s_i);
-        const bool nan = at == SM_NAN || m == __builtin_inff();
-        __syncthreads();
-        for (int i = tid; i < cols; i += THREADS) to[i] = nan ? __builtin_nanf("") : m != none && i == at ? 1.0f : 0.0f;
+    if constexpr (BEST) {
+        FirstOf first;
+#pragma unroll 4
+        for (int k = KEPT - 1; k >= 0; k--) first.see(REGS + k, s_x[k * THREADS + tid], m);
+#pragma unroll
+        for (int k = REGS - 1; k >= 0; k--) first.see(k, r[k], m);
+        const int at = block_all<THREADS>(first.index<THREADS>(), s_i, Lower());
+        const float rest = at == SM_NAN || m == __builtin_inff() ? __builtin_nanf("") : 0.0f;
+        const int one = rest == 0.0f && m != none && at % THREADS == tid ? at / THREADS : -1;
+        write_spread<THREADS, REGS, 8>(to, cols, [&](int k) { return k == one ? 1.0f : rest; });
+        if constexpr (KEPT > 0)
+            write_spread<THREADS, KEPT, 4>(to + REGS * THREADS, cols - REGS * THREADS, [&](int k) { return REGS + k == one ? 1.0f : rest; });
         return;
     }
+    if (m == none) m = 0.0f;  // nothing but -infinity, or NaN: a sum of 0, or NaN
     float sum = 0.0f;
 #pragma unroll
     for (int k = 0; k < REGS; k++) { r[k] = __builtin_amdgcn_exp2f((r[k] - m) * scale); sum += r[k]; }
@@ -254,7 +261,8 @@ __global__ __launch_bounds__(THREADS) void softmax_row_kernel(float *out, const 
         s_x[k * THREADS + tid] = e;
         sum += e;
     }
-    const float inv = 1.0f / block_all<THREADS>(sum, s_f, Added());
+    sum = block_all<THREADS>(sum, s_f, Added());
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
     write_spread<THREADS, REGS, 8>(to, cols, [&](int k) { return r[k] * inv; });
     if constexpr (KEPT > 0)
         write_spread<THREADS, KEPT, 4>(to + REGS * THREADS, cols - REGS * THREADS, [&](int k) { return s_x[k * THREADS + tid] * inv; });
@@ -281,9 +289,12 @@ __global__ __launch_bounds__(SM_THREADS) void softmax_piece_kernel(float *out, c
 #pragma unroll
         for (int k = 0; k < SM_REGS; k++) m = fmaxf(m, r[k]);
         m = block_all<SM_THREADS>(m, s_f, Larger());
-        int at = n;
+        int at = 0;
         if (scale == 0.0f || m == none) {
-            at = lowest_of<SM_THREADS>(row, n, scale == 0.0f ? m : 0.0f, s_i);
+            FirstOf first;
+#pragma unroll
+            for (int k = SM_REGS - 1; k >= 0; k--) first.see(k, r[k], m);
+            at = block_all<SM_THREADS>(first.index<SM_THREADS>(), s_i, Lower());
         } else {
 #pragma unroll
             for (int k = 0; k < SM_REGS; k++) sum += __builtin_amdgcn_exp2f((r[k] - m) * scale);
@@ -320,6 +331,13 @@ __global__ __launch_bounds__(SM_THREADS) void softmax_piece_kernel(float *out, c
 // rows however few (1 row of 32000: 8.0 / 6.8; 8192: 7.9 / 5.1).
 constexpr int SM_SHORT = 40 * 1024, SM_HELD = (96 + 36) * 1024;
 bool softmax_pieces(int rows, int cols) { return cols > SM_HELD || (cols > SM_SHORT && (long)rows * cols < 13000000); }
+template <bool BEST>
+void softmax_rows(float *out, const float *x, int rows, int cols, float scale, hipStream_t s) {
+    if (cols <= 4096) softmax_row_kernel<256, 16, 0, BEST><<<rows, 256, 0, s>>>(out, x, cols, scale);
+    else if (cols <= 16384) softmax_row_kernel<1024, 16, 0, BEST><<<rows, 1024, 0, s>>>(out, x, cols, scale);
+    else if (cols <= SM_SHORT) softmax_row_kernel<1024, 40, 0, BEST><<<rows, 1024, 0, s>>>(out, x, cols, scale);
+    else softmax_row_kernel<1024, 96, 36, BEST><<<rows, 1024, 0, s>>>(out, x, cols, scale);
+}
 
 // ------------------------------------------------------------------------
 // Verification.  After j rejections at a row the target's distribution without
@@ -700,14 +718,10 @@ int qg_softmax(float *out, const float *x, int rows, int cols, float temperature
         const unsigned grid = (unsigned)((cols + SM_PIECE - 1) / SM_PIECE * rows);
         softmax_piece_kernel<false><<<grid, SM_THREADS, 0, qg_stream()>>>(out, x, cols, scale, (SoftPart *)ws);
         softmax_piece_kernel<true><<<grid, SM_THREADS, 0, qg_stream()>>>(out, x, cols, scale, (SoftPart *)ws);
-    } else if (cols <= 4096) {
-        softmax_row_kernel<256, 16, 0><<<rows, 256, 0, qg_stream()>>>(out, x, cols, scale);
-    } else if (cols <= 16384) {
-        softmax_row_kernel<1024, 16, 0><<<rows, 1024, 0, qg_stream()>>>(out, x, cols, scale);
-    } else if (cols <= SM_SHORT) {
-        softmax_row_kernel<1024, 40, 0><<<rows, 1024, 0, qg_stream()>>>(out, x, cols, scale);
+    } else if (scale > 0.0f) {
+        softmax_rows<false>(out, x, rows, cols, scale, qg_stream());
     } else {
-        softmax_row_kernel<1024, 96, 36><<<rows, 1024, 0, qg_stream()>>>(out, x, cols, scale);
+        softmax_rows<true>(out, x, rows, cols, scale, qg_stream());
     }
     return hipGetLastError();
 }
