@@ -270,3 +270,21 @@ def test_reserve_keeps_forks_apart(qgl):
     same(c)
     np.testing.assert_array_equal(reserve(c, [16, 20, 16]), m.reserve([16, 20, 16]))
     same(c)
+
+
+@pytest.mark.parametrize("n,width", [(1, 4096), (1, 4097), (32, 128), (32, 129), (33, 8), (1000, 9)])
+def test_fork_of_few_and_many_entries(qgl, n, width):
+    """Pairs that chain (a destination is the next pair's source), repeat and are out of range, over tables on both sides
+    of what one workgroup holds."""
+    rng = np.random.default_rng(n + width)
+    B = min(1024, n + 3)
+    lengths = [8 * width - 3, 5] + [0] * (B - 2)
+    c = Cache(rng, lengths, [0] * B, typ=F16, kv_heads=1, page=8, dim=64, spare=5, table_pages=width, fill=False)
+    m = Model(c)
+    for rounds in range(2):
+        dst, src = rng.integers(0, B, n).tolist(), rng.integers(0, min(B, 4), n).tolist()
+        if n > 5:
+            dst[:4], src[:4] = [2, 3, 2, B], [0, 2, 1, 0]
+        fork(c, dst, src)
+        m.fork(dst, src)
+        same(c, pools=False)
