@@ -386,11 +386,12 @@ struct Tile<QT_F32, D> {
     }
 };
 
-// Sums that are no numbers under a weight that is one.  The planes' products make
-// NaN of an infinite value (0 x inf, inf - inf), and a value that is no number
-// reaches the rows of its tile that do not see it (0 x NaN); such rows are taken
-// up again, key by key.
-QG_DEV bool odd_sums(float a, float b, float weight) { return !__builtin_isfinite(a + b) && __builtin_isfinite(weight); }
+// Sums that are no numbers, or a weight that is none.  The planes' products make NaN
+// of an infinite key, query or value (0 x inf, inf - inf) where the score may be minus
+// infinity, and a value that is no number reaches the rows of its tile that do not see
+// it (0 x NaN); such rows are taken up again, key by key.  Weights are at most 2^(M_LAG +
+// P_BASE), so their sum is never infinite.
+QG_DEV bool odd_sums(float a, float b, float weight) { return !__builtin_isfinite(a + b + weight); }
 
 QG_DEV unsigned first_bits(int n, int most) { return (1u << min(max(n, 0), most)) - 1u; }
 

@@ -1,5 +1,7 @@
 """qg_tree_attention against a 64-bit statement of it (spec_oracle.attention)."""
+import copy
 import ctypes as C
+import math
 import sys
 
 import numpy as np
@@ -251,3 +253,44 @@ def test_attention_without_rows(qgl):
     cache = Cache(np.random.default_rng(13), [10, 0], [0, 0], typ=F16, kv_heads=1, page=8, dim=64)
     batch = Batch([0, 0], rows=4, max_rows=2)
     assert np.isnan(attend(cache, batch, np.ones((4, 2, 64), np.float32), 0.125)).all()
+
+
+@pytest.mark.parametrize("typ", [F16, BF16, F32])
+@pytest.mark.parametrize("length,page", [(90, 16), (9000, 64)])
+def test_attention_infinite_keys_and_queries(qgl, typ, length, page):
+    """A key whose score is minus infinity has weight 0, whatever bits the query has: random queries, and queries whose
+    product with the scale is a power of two (every plane but the first is 0)."""
+    rng = np.random.default_rng(length)
+    rows, heads, dim = 3, 8, 64
+    cache = Cache(rng, [length, 40], [rows, 1], typ=typ, kv_heads=1, page=page, dim=dim)
+    batch = Batch([rows, 1])
+    store(cache, batch, rng)
+    low, skip = O.encode([-np.inf], typ)[0], {0: {0, 1, 33, 64, 89} | set(range(100, length, 97)), 1: set(range(41))}
+    for s, positions in skip.items():
+        for t in positions:
+            cache.k[0, cache.page_of(s, t), 0, t % page, 1 + t % 7] = low
+    cache.upload()
+    finite = copy.copy(cache)
+    finite.page_of = lambda s, t: -1 if t in skip[s] else cache.page_of(s, t)
+    for scale, power in ((dim ** -0.5, False), (math.log(2.0), True)):
+        q = rng.standard_normal((rows + 1, heads, dim)).astype(np.float32)
+        if power:
+            q = (np.sign(q) * 2.0 ** np.clip(np.round(np.log2(np.abs(q) + 1e-3)) - 4, -9, -2)).astype(np.float32)
+        q[:, :, 1:8] = np.abs(q[:, :, 1:8]) + (0 if power else 2.0 ** -12)
+        got = attend(cache, batch, q, scale)
+        want, tol, _ = O.attention(finite, batch, q, scale)
+        assert np.all(np.abs(got - want) <= tol), (np.isnan(got).sum(), np.nanmax(np.abs(got - want)))
+        assert (got[rows] == 0).all()
+    # an infinite query whose every score is minus infinity, beside rows with NaN of their own
+    for s in range(2):
+        for t in range(int(cache.length[s]) + (rows if s == 0 else 1)):
+            cache.k[0, cache.page_of(s, t), 0, t % page, 9] = O.encode([-1.0], typ)[0]
+            cache.k[0, cache.page_of(s, t), 0, t % page, 1:8] = 0
+    cache.upload()
+    q[0, 3, 9], q[1, 5, 2] = np.inf, np.nan
+    got = attend(cache, batch, q, 0.25)
+    want, tol, _ = O.attention(cache, batch, np.nan_to_num(q, nan=0, posinf=0), 0.25)
+    assert (got[0, 3] == 0).all() and np.isnan(got[1, 5]).all()
+    keep = np.ones(q.shape[:2], bool)
+    keep[0, 3] = keep[1, 5] = False
+    assert np.all(np.abs(got - want)[keep] <= tol[keep])
