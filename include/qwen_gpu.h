@@ -195,7 +195,7 @@ typedef struct {
     int layers, pages, kv_heads; /* layers 1..65536, kv_heads 1..128 */
     int page_tokens;            /* a power of two, 8..1024 */
     int head_dim;               /* 64, 128 or 256 */
-    int *refs;                  /* [pages] table entries that hold each page, 0 = free; page calls only, else NULL */
+    int *refs;                  /* [pages] table entries that hold each page, 0 = free; NULL without page calls */
     int *table;                 /* [sequences][table_pages] page or -1 */
     int *length;                /* [sequences] tokens held */
     int sequences, table_pages; /* 1..1024 sequences; table_pages * page_tokens <= 2^28 */
@@ -230,8 +230,9 @@ typedef struct {
 /* Per-head RMS norm (as qg_norm) and rotation of q and k, in one pass; q_out
  * [rows][q_heads][head_dim], k_out [rows][kv_heads][head_dim] fp32 (k_out may
  * be NULL).  With a cache, k (normed, rotated) and v are rounded to its type
- * and stored at their positions of `layer`; a row whose position has no page
- * is not stored.  Without a cache, batch is NULL, v is ignored and position is
+ * and stored at their positions of `layer`; a row whose position has no page,
+ * or one that another table entry holds too (where the cache has refs; see
+ * qg_kv_reserve), is not stored.  Without a cache, batch is NULL, v is ignored and position is
  * needed where rope_dims > 0.  Angles are formed in 64 bits.  An output may be its own
  * input where both have the same layout; otherwise they must not overlap.
  * Rows of no sequence are left as they were. */
@@ -291,7 +292,10 @@ size_t qg_kv_workspace_bytes(const qg_kv_cache *cache);
  * (every layer); of several sequences of the batch that share a page no other holds, the
  * first keeps it.  status[s]: 0; 1 there are not enough free pages for the batch
  * (nothing is taken for any of its sequences); 2 the sequence's table is too
- * short (nothing is taken for it, the others are served). */
+ * short (nothing is taken for it, the others are served).  The rest of a captured
+ * step may run on where status[s] is not 0: rows of such a sequence are stored in
+ * pages of its own only, so that no other sequence's tokens change, and what the
+ * step says of them means nothing. */
 int qg_kv_reserve(const qg_kv_cache *cache, const qg_kv_batch *batch, int *status, void *workspace, size_t workspace_bytes);
 /* For each pair i < n: sequence dst[i] lets go of its pages and shares those
  * of src[i]'s tokens; its length is src[i]'s.  Sources are read as before the
@@ -305,7 +309,9 @@ int qg_kv_truncate(const qg_kv_cache *cache, const int *new_length);
 /* The accepted rows (qg_verify_drafts' path and count) move to the front: the
  * token at length[s] + path[s][i] goes to length[s] + i, in every layer, and
  * new_length[s] = length[s] + count[s] (new_length may be the cache's length).
- * A path is followed while it ascends inside its sequence's rows. */
+ * A path is followed while it ascends inside its sequence's rows, and up to the
+ * first row whose page, or the page that it would move to, another table entry
+ * holds too (where the cache has refs). */
 int qg_kv_compact(const qg_kv_cache *cache, const qg_kv_batch *batch, const int *path, const int *count, int *new_length);
 /* Pages dst[i] = copies of pages src[i] in every layer, i < n <= 4096.  A
  * pair whose destination is among the sources or comes again later is left

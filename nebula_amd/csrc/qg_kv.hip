@@ -307,19 +307,25 @@ __global__ __launch_bounds__(256) void kv_copy_pages_kernel(KvView c, const int 
 // Moves are few: 16 sequences x 48 layers take 4.2 us, a launch and three reads.
 // new_length NULL: written by kv_length_kernel, where the workgroups of a
 // sequence read the lengths that it replaces.
-QG_DEV int path_rows(const BatchView &b, const int *path, const int *count, int s, int lane, int &p) {
+// The rows of a sequence's path that are followed; lane i's row p, and the pages that it
+// comes from and goes to.  A path ends where it does not ascend, and at a page that others
+// hold: reserve found no room for a copy, and the row was not stored.
+QG_DEV int path_rows(const KvView &c, const BatchView &b, const int *path, const int *count, int s, int len, int lane, int &p, int &from, int &to) {
     int first, n;
     batch_rows(b, s, first, n);
     const int keep = min(max(count[s], 0), n);
     p = lane < keep ? path[(size_t)s * b.max_rows + lane] : -1;
     const int before = __shfl_up(p, 1);
     const bool ok = lane < keep && p < n && p > (lane ? before : -1);
-    const unsigned long long fault = ~__ballot(ok);
+    from = ok ? kv_page(c, s, len + p) : -1;
+    to = ok ? kv_page(c, s, len + lane) : -1;
+    const bool shared = c.refs && ((from >= 0 && c.refs[from] > 1) || (to >= 0 && c.refs[to] > 1));
+    const unsigned long long fault = ~__ballot(ok && !shared);
     return fault ? __ffsll(fault) - 1 : 64;
 }
 __global__ __launch_bounds__(64) void kv_length_kernel(KvView c, BatchView b, const int *path, const int *count, int *new_length) {
-    int p;
-    const int upto = path_rows(b, path, count, blockIdx.x, threadIdx.x, p), len = kv_length(c, blockIdx.x);
+    int p, from, to;
+    const int len = kv_length(c, blockIdx.x), upto = path_rows(c, b, path, count, blockIdx.x, len, threadIdx.x, p, from, to);
     if (threadIdx.x == 0) new_length[blockIdx.x] = len + upto;
 }
 __global__ __launch_bounds__(256) void kv_compact_kernel(KvView c, BatchView b, const int *path, const int *count, int *new_length) {
@@ -328,12 +334,10 @@ __global__ __launch_bounds__(256) void kv_compact_kernel(KvView c, BatchView b, 
     const int s = blockIdx.y, lane = threadIdx.x & 63, es = c.type == QT_F32 ? 4 : 2;
     if (threadIdx.x < 64) {
         const int len = kv_length(c, s);
-        int p;
-        const int upto = path_rows(b, path, count, s, lane, p);
-        const bool move = lane < upto && p != lane;
-        const int from = move ? kv_page(c, s, len + p) : -1, to = move ? kv_page(c, s, len + lane) : -1;
+        int p, from, to;
+        const int upto = path_rows(c, b, path, count, s, len, lane, p, from, to);
         const int slot = (1 << c.shift) - 1;
-        const bool both = from >= 0 && to >= 0;
+        const bool both = lane < upto && p != lane && from >= 0 && to >= 0;
         const unsigned long long all = __ballot(both);
         if (both) {
             const int at = __popcll(all & ((1ULL << lane) - 1));

@@ -61,7 +61,7 @@ __global__ __launch_bounds__(256) void qk_rope_kernel(RopeArgs A, KvView c, Batc
         if (b.parent) depth = __popcll(__shfl(tree_ancestors(b.parent + first, n, lane), place)) - 1;
         const int len = kv_length(c, s);
         pos = len + depth;
-        page = kv_page(c, s, len + place);
+        page = kv_own_page(c, s, len + place);
         slot = (len + place) & ((1 << c.shift) - 1);
     }
     if (A.position) pos = A.position[row];

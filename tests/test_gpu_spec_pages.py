@@ -1,5 +1,6 @@
 """qg_kv_reserve / fork / truncate / compact / copy_pages against a model of the
 same rules in Python: tables, holders, lengths and every byte of the pages."""
+import ctypes as C
 import sys
 
 import numpy as np
@@ -288,3 +289,50 @@ def test_fork_of_few_and_many_entries(qgl, n, width):
         fork(c, dst, src)
         m.fork(dst, src)
         same(c, pools=False)
+
+
+def store_rows(c, batch, rng):
+    """qg_qk_norm_rope of the batch's rows, neither normalised nor rotated; returns k and v as given."""
+    row = 3 * c.H * c.D
+    x = rng.standard_normal((batch.rows, row)).astype(np.float32)
+    dx, out = Device(x), Device(shape=(batch.rows, c.H, c.D), dtype=np.float32)
+    args = qg.QkRows(q=dx.p, k=dx.p + 4 * c.H * c.D, v=dx.p + 8 * c.H * c.D, q_row=row, q_head=c.D, k_row=row, k_head=c.D, v_row=row, v_head=c.D,
+                     rows=batch.rows, q_heads=c.H, kv_heads=c.H, head_dim=c.D, eps=1e-6)
+    call("qk_norm_rope", out.p, None, C.byref(args), c.ref, 0, batch.ref)
+    return x.reshape(batch.rows, 3, c.H, c.D)[:, 1:].swapaxes(0, 1)
+
+
+@pytest.mark.parametrize("typ", [F16, F32])
+def test_rows_without_room_leave_shared_pages(qgl, typ):
+    """A step that runs on after reserve found no room: neither the store nor the compaction writes into a page that
+    another sequence holds."""
+    rng = np.random.default_rng(21)
+    c = Cache(rng, [14, 0, 0], [0, 0, 0], typ=typ, kv_heads=2, page=16, dim=64, spare=0, table_pages=2)
+    fork(c, [1], [0])
+    truncate(c, [14, 10, 0])
+    m = Model(c)
+    m.fork([1], [0])
+    m.truncate([14, 10, 0])
+    counts = [0, 5, 0]
+    status = m.reserve(counts)
+    assert status[1] == 1
+    np.testing.assert_array_equal(reserve(c, counts), status)
+    batch = Batch(counts)
+    store_rows(c, batch, rng)
+    same(c)
+    for lengths in (c.dlength, Device(np.zeros(3, np.int32))):
+        path, count = np.full((3, 5), -1, np.int32), np.array([0, 3, 0], np.int32)
+        path[1, :3] = (0, 2, 3)
+        dp, dc = Device(path), Device(count)
+        say("compact after no room")
+        call("kv_compact", c.ref, batch.ref, dp.p, dc.p, lengths.p)
+        np.testing.assert_array_equal(lengths.get(), [14, 10, 0])
+        same(c)
+    # a cache without counts of its own: the caller says where rows go
+    desc = qg.KvCache.from_buffer_copy(c.desc)
+    desc.refs, c.ref = None, C.byref(desc)
+    k, v = store_rows(c, batch, rng)
+    for i in range(5):
+        c.put(0, 1, 10 + i, k[i], v[i])
+    np.testing.assert_array_equal(c.dk.get().view(np.uint8), c.k.view(np.uint8))
+    np.testing.assert_array_equal(c.dv.get().view(np.uint8), c.v.view(np.uint8))

@@ -226,3 +226,23 @@ def test_index_arithmetic_stays_inside(index):
         assert 0 <= first.value <= total and 0 <= count.value <= most and first.value + count.value <= total
         i, q = int(rng.integers(0, 64)), int(rng.choice(np.concatenate([wild, rng.integers(-2, 70, 4).astype(np.int32)])))
         assert index.parent(q, i) == (q if 0 <= q < i else -1)
+
+
+OWN = r"""
+#include "qg_kv_index.h"
+extern "C" int own(const int *table, int *refs, int pages, int t) {
+    KvView c{};
+    c.table = (int *)table; c.refs = refs; c.pages = pages; c.shift = 3; c.sequences = 1; c.table_pages = 4;
+    return kv_own_page(c, 0, t);
+}
+"""
+
+
+def test_pages_that_may_be_written(tmp_path):
+    """A page that another table entry holds is not a sequence's own; without counts every held page is."""
+    (tmp_path / "h.cpp").write_text(OWN)
+    subprocess.run(["g++", "-O1", "-shared", "-fPIC", f"-I{ROOT / 'nebula_amd' / 'csrc'}", str(tmp_path / "h.cpp"), "-o", str(tmp_path / "h.so")], check=True)
+    own = C.CDLL(str(tmp_path / "h.so")).own
+    table, refs = (C.c_int * 4)(2, 0, -1, 7), (C.c_int * 3)(2, 0, 1)
+    assert [own(table, refs, 3, t) for t in (0, 7, 8, 16, 24, 32, -1)] == [2, 2, -1, -1, -1, -1, -1]
+    assert [own(table, None, 3, t) for t in (0, 7, 8, 16, 24, 32, -1)] == [2, 2, 0, -1, -1, -1, -1]
