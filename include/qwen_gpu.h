@@ -294,8 +294,9 @@ size_t qg_kv_workspace_bytes(const qg_kv_cache *cache);
  * (nothing is taken for any of its sequences); 2 the sequence's table is too
  * short (nothing is taken for it, the others are served).  The rest of a captured
  * step may run on where status[s] is not 0: rows of such a sequence are stored in
- * pages of its own only, so that no other sequence's tokens change, and what the
- * step says of them means nothing. */
+ * pages of its own only, so that no other sequence's tokens change; its length
+ * grows by the k accepted rows that found one (qg_kv_compact), and of its tokens_out
+ * the first k hold (0: none), since they follow rows that were stored. */
 int qg_kv_reserve(const qg_kv_cache *cache, const qg_kv_batch *batch, int *status, void *workspace, size_t workspace_bytes);
 /* For each pair i < n: sequence dst[i] lets go of its pages and shares those
  * of src[i]'s tokens; its length is src[i]'s.  Sources are read as before the
@@ -308,10 +309,11 @@ int qg_kv_fork(const qg_kv_cache *cache, const int *dst, const int *src, int n, 
 int qg_kv_truncate(const qg_kv_cache *cache, const int *new_length);
 /* The accepted rows (qg_verify_drafts' path and count) move to the front: the
  * token at length[s] + path[s][i] goes to length[s] + i, in every layer, and
- * new_length[s] = length[s] + count[s] (new_length may be the cache's length).
+ * new_length[s] = length[s] + count[s], or the rows followed if fewer (new_length may be the cache's length).
  * A path is followed while it ascends inside its sequence's rows, and up to the
  * first row whose page, or the page that it would move to, another table entry
- * holds too (where the cache has refs). */
+ * holds too (where the cache has refs); rows behind the last one with both pages
+ * are left out, so that a length does not grow over rows that found no room. */
 int qg_kv_compact(const qg_kv_cache *cache, const qg_kv_batch *batch, const int *path, const int *count, int *new_length);
 /* Pages dst[i] = copies of pages src[i] in every layer, i < n <= 4096.  A
  * pair whose destination is among the sources or comes again later is left

@@ -309,7 +309,8 @@ __global__ __launch_bounds__(256) void kv_copy_pages_kernel(KvView c, const int 
 // sequence read the lengths that it replaces.
 // The rows of a sequence's path that are followed; lane i's row p, and the pages that it
 // comes from and goes to.  A path ends where it does not ascend, and at a page that others
-// hold: reserve found no room for a copy, and the row was not stored.
+// hold: reserve found no room for a copy, and the row was not stored.  Nor do rows count
+// behind the last one that has pages: without room there are none from some row on.
 QG_DEV int path_rows(const KvView &c, const BatchView &b, const int *path, const int *count, int s, int len, int lane, int &p, int &from, int &to) {
     int first, n;
     batch_rows(b, s, first, n);
@@ -321,7 +322,8 @@ QG_DEV int path_rows(const KvView &c, const BatchView &b, const int *path, const
     to = ok ? kv_page(c, s, len + lane) : -1;
     const bool shared = c.refs && ((from >= 0 && c.refs[from] > 1) || (to >= 0 && c.refs[to] > 1));
     const unsigned long long fault = ~__ballot(ok && !shared);
-    return fault ? __ffsll(fault) - 1 : 64;
+    const unsigned long long held = __ballot(from >= 0 && to >= 0) & (fault ? (fault & -fault) - 1 : ~0ULL);
+    return held ? 64 - __clzll(held) : 0;
 }
 __global__ __launch_bounds__(64) void kv_length_kernel(KvView c, BatchView b, const int *path, const int *count, int *new_length) {
     int p, from, to;

@@ -336,3 +336,41 @@ def test_rows_without_room_leave_shared_pages(qgl, typ):
         c.put(0, 1, 10 + i, k[i], v[i])
     np.testing.assert_array_equal(c.dk.get().view(np.uint8), c.k.view(np.uint8))
     np.testing.assert_array_equal(c.dv.get().view(np.uint8), c.v.view(np.uint8))
+
+
+@pytest.mark.parametrize("page", [8, 16])
+def test_lengths_stop_where_no_row_was_stored(qgl, page):
+    """After a status of 1 or 2 the rows that found no page do not count, whatever was accepted of them."""
+    rng = np.random.default_rng(22)
+    # a page's rest for some rows (sequences 0, 1), a full page (2), none at all (3), a table too short (4)
+    lengths, counts = [page - 3, 2 * page - 1, page, 0, 3 * page - 2], [9, 4, 3, 2, 9]
+    for full in (False, True):   # the others get pages, or nobody does
+        c = Cache(rng, lengths, [0] * 5, typ=BF16, layers=2, kv_heads=1, page=page, dim=64, spare=0 if full else 9, table_pages=3)
+        m = Model(c)
+        status = m.reserve(counts)
+        np.testing.assert_array_equal(status, [1, 1, 1, 1, 2] if full else [0, 0, 0, 0, 2])
+        np.testing.assert_array_equal(reserve(c, counts), status)
+        batch = Batch(counts)
+        paths = [[0, 1, 2, 3, 8], [0, 1, 3], [0, 2], [0, 1], [0, 1, 2, 5]]
+        room = [3, 1, 0, 0, 2] if full else [5, 3, 2, 2, 2]   # rows of each path up to the last with a page at both ends
+        path, count = np.full((5, 9), -1, np.int32), np.array([len(p) for p in paths], np.int32)
+        for s, p in enumerate(paths):
+            path[s, :len(p)] = p
+        for row, s, place in batch.places():
+            for layer in range(2):
+                c.put(layer, s, int(c.length[s]) + place, *rng.standard_normal((2, 1, 64)))
+        c.upload()
+        want = c_length(c) + np.array(room, np.int32)
+        dp, dc, out = Device(path), Device(count), Device(np.zeros(5, np.int32))
+        m.compact(batch, path, count)
+        say(f"compact page={page} full={full}")
+        call("kv_compact", c.ref, batch.ref, dp.p, dc.p, out.p)
+        np.testing.assert_array_equal(out.get(), want)
+        same(c)
+        # again into the cache's own lengths: the moved rows lie where they are, so only the lengths change
+        identity = np.tile(np.arange(9, dtype=np.int32), (5, 1))
+        dp.set(identity)
+        dc.set(np.array(room, np.int32))
+        call("kv_compact", c.ref, batch.ref, dp.p, dc.p, c.dlength.p)
+        c.length = want
+        same(c)
