@@ -245,7 +245,8 @@ int qg_qk_norm_rope(float *q_out, float *k_out, const qg_qk_rows *in, const qg_k
  * of kv_heads up to 128 times as many, both 16-byte aligned; no overlap.
  * Scores, statistics and sums are held in fp32; the products run on the matrix
  * cores with queries and probabilities in planes of the cache's type that
- * together carry at least 22 bits.  A row that sees no token (or none with a
+ * together carry at least 22 bits (over an F16 cache no less than 2^-38 of a row's
+ * largest probability, or of its largest query value).  A row that sees no token (or none with a
  * score above -infinity) is 0.  Rows of no sequence are left as they were.
  * rows x q_heads at most 2^25.  The workspace of a batch serves every batch of
  * no more rows. */

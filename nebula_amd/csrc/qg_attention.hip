@@ -34,8 +34,13 @@ namespace {
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
-constexpr float P_BASE = 6.0f;  // p is held times 2^6: m may lag by 8 below the fp16 range's end
-constexpr float M_LAG = 8.0f;   // a new maximum counts once it is 2^8 above the old
+// p is held times 2^P_BASE, and a new maximum counts once it is 2^M_LAG above the old.
+// fp16 planes end at 2^-24 and at 2^16: what the base and the lag leave of that below the
+// range's end is what small weights have for their bits.  Base 13 and lag 2 hold a weight
+// within 2^-22 of itself or 2^-38 of the largest (base 6 and lag 8, rounded towards zero:
+// 2^-30, always too little).  bf16 planes and fp32 have the exponent for any weight.
+constexpr float p_base(int type) { return type == QT_F16 ? 13.0f : 6.0f; }
+constexpr float m_lag(int type) { return type == QT_F16 ? 2.0f : 8.0f; }
 
 struct AttnArgs {
     float *out;
@@ -169,7 +174,7 @@ QG_DEV uint32_t pair_lo(uint32_t a, uint32_t b) { return __builtin_amdgcn_perm(b
 QG_DEV uint32_t pair_hi(uint32_t a, uint32_t b) { return __builtin_amdgcn_perm(b, a, 0x07060302u); }
 
 // Eight floats as the planes of an operand: their sum is the value (bf16, exactly) or
-// within 2^-22 of it (fp16).
+// within 2^-23 of it, and 2^-25 where that is more (fp16, both rounded to nearest).
 template <int TYPE> struct Planes;
 template <> struct Planes<QT_F16> {
     static constexpr int N = 2;
@@ -188,7 +193,11 @@ template <> struct Planes<QT_F16> {
         p[0] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
         p[1] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
     }
-    static __device__ __forceinline__ uint32_t cvt2(float a, float b) { return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(a, b)); }
+    static __device__ __forceinline__ uint32_t cvt2(float a, float b) {
+        typedef float f2 __attribute__((ext_vector_type(2)));
+        typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+        return __builtin_bit_cast(uint32_t, __builtin_convertvector((f2{a, b}), h2));
+    }
     static __device__ __forceinline__ qg_f4 mul(uint4 a, uint4 b, qg_f4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(qg_half8, a), __builtin_bit_cast(qg_half8, b), c, 0, 0, 0);
     }
@@ -389,8 +398,8 @@ struct Tile<QT_F32, D> {
 // Sums that are no numbers, or a weight that is none.  The planes' products make NaN
 // of an infinite key, query or value (0 x inf, inf - inf) where the score may be minus
 // infinity, and a value that is no number reaches the rows of its tile that do not see
-// it (0 x NaN); such rows are taken up again, key by key.  Weights are at most 2^(M_LAG +
-// P_BASE), so their sum is never infinite.
+// it (0 x NaN); such rows are taken up again, key by key.  Weights are at most
+// 2^(m_lag + p_base), so their sum is never infinite.
 QG_DEV bool odd_sums(float a, float b, float weight) { return !__builtin_isfinite(a + b + weight); }
 
 QG_DEV unsigned first_bits(int n, int most) { return (1u << min(max(n, 0), most)) - 1u; }
@@ -535,7 +544,7 @@ __global__ __launch_bounds__(64 * NW, (D / 64) * RT <= 6 ? 2 : 1) void attention
 #pragma unroll
             for (int e = 1; e < E; e++) top = fmaxf(top, z[r][e]);
             top *= back[r];
-            if (__any(top > m[r] + M_LAG)) {
+            if (__any(top > m[r] + m_lag(TYPE))) {
                 top = fmaxf(top, __shfl_xor(top, 16));
                 top = fmaxf(top, __shfl_xor(top, 32));
                 const float next = fmaxf(m[r], top);
@@ -545,7 +554,7 @@ __global__ __launch_bounds__(64 * NW, (D / 64) * RT <= 6 ? 2 : 1) void attention
 #pragma unroll
                 for (int t = 0; t < DL; t++) o[r][t] *= a;
             }
-            const float base = m[r] == -__builtin_inff() ? 0.0f : m[r] - P_BASE;
+            const float base = m[r] == -__builtin_inff() ? 0.0f : m[r] - p_base(TYPE);
 #pragma unroll
             for (int e = 0; e < E; e++) {
                 z[r][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(z[r][e], back[r], -base));

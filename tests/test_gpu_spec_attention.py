@@ -10,7 +10,7 @@ import pytest
 import spec_oracle as O
 from nebula_amd import qg
 from nebula_amd.qg import Device, call
-from spec_oracle import BF16, F16, F32, Batch, Cache
+from spec_oracle import BF16, F16, F32, U, Batch, Cache
 
 pytestmark = pytest.mark.gpu
 
@@ -294,3 +294,37 @@ def test_attention_infinite_keys_and_queries(qgl, typ, length, page):
     keep = np.ones(q.shape[:2], bool)
     keep[0, 3] = keep[1, 5] = False
     assert np.all(np.abs(got - want)[keep] <= tol[keep])
+
+
+@pytest.mark.parametrize("typ", [F16, BF16, F32])
+@pytest.mark.parametrize("length", [700, 6000])
+@pytest.mark.parametrize("nats", [8, 12, 16, 20])
+def test_attention_small_weights_beside_a_sink(qgl, typ, length, nats):
+    """Keys far below one in every tile whose value is zero: the output is theirs alone.  A weight is within 2^-22 of
+    itself or 2^-38 of the largest (F16 planes; the others within 2^-22), all of one sign here: the errors add up."""
+    rng = np.random.default_rng(length + nats)
+    dim, page = 64, 32
+    cache = Cache(rng, [length], [1], typ=typ, kv_heads=1, page=page, dim=dim)
+    batch = Batch([1])
+    store(cache, batch, rng)
+    z = np.full(length + 1, 0.0)
+    for t in range(length + 1):
+        sink = t % 32 == 7
+        z[t] = O.decode(O.encode([nats if sink else rng.uniform(-1, 1)], typ), typ)[0]
+        cache.put(0, 0, t, np.eye(1, dim) * z[t], np.zeros((1, dim)) if sink else rng.uniform(0.5, 1.0, (1, dim)))
+    cache.upload()
+    q = np.zeros((1, 2, dim), np.float32)
+    q[0, :, 0] = (1.0, 0.75)
+    got = attend(cache, batch, q, 1.0)
+    V = np.stack([cache.token(cache.v, 0, 0, t)[0] for t in range(length + 1)])
+    for h in range(2):
+        s = z * float(q[0, h, 0])
+        p = np.exp(s - s.max())
+        want = p @ V / p.sum()
+        # a score: log2 e and its product with the query (half a step each), the planes (2^-22), the product's sum (2), the
+        # sum with the maximum (of |s| log2 e + 13, in 64 bits ln 2 of that); the exponential (2); then p's planes, and p
+        # and its sums in fp32 with their roundings as independent
+        ds = (9 * np.abs(s).max() + 11) * U
+        rel = 2 * ds + 2.0 ** -22 + 4 * U * (4 + math.sqrt(length))
+        tol = want * rel + (2.0 ** -38 * V.sum(0) / p.sum() if typ == F16 else 0)
+        assert np.all(np.abs(got[0, h] - want) <= tol), (np.abs(got[0, h] - want).max() / want.max(), (tol / want).max())
