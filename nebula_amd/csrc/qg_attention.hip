@@ -39,7 +39,7 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 // range's end is what small weights have for their bits.  Base 13 and lag 2 hold a weight
 // within 2^-22 of itself or 2^-38 of the largest (base 6 and lag 8, rounded towards zero:
 // 2^-30, always too little).  bf16 planes and fp32 have the exponent for any weight.
-constexpr float p_base(int type) { return type == QT_F16 ? 13.0f : 6.0f; }
+constexpr float p_base(int type) { return type == QT_F16 ? 13.0f : 0.0f; }
 constexpr float m_lag(int type) { return type == QT_F16 ? 2.0f : 8.0f; }
 
 struct AttnArgs {
@@ -398,7 +398,8 @@ struct Tile<QT_F32, D> {
 // Sums that are no numbers, or a weight that is none.  The planes' products make NaN
 // of an infinite key, query or value (0 x inf, inf - inf) where the score may be minus
 // infinity, and a value that is no number reaches the rows of its tile that do not see
-// it (0 x NaN); such rows are taken up again, key by key.  Weights are at most
+// it (0 x NaN); such rows are taken up again, key by key, and so are sums of finite
+// values past the type's range, which their division by the weight may bring back.  Weights are at most
 // 2^(m_lag + p_base), so their sum is never infinite.
 QG_DEV bool odd_sums(float a, float b, float weight) { return !__builtin_isfinite(a + b + weight); }
 
@@ -631,7 +632,8 @@ __global__ __launch_bounds__(64 * NW, (D / 64) * RT <= 6 ? 2 : 1) void attention
 }
 
 // One row and head, key by key: a lane scores one of 64 keys at a time, the
-// output's dimensions lie across the lanes.
+// output's dimensions lie across the lanes.  The weights' sum first, so that the values
+// are taken by weights that sum to 1: nothing overflows that the output holds.
 template <int TYPE, int D>
 QG_DEV void attend_row(const AttnArgs &A, const KvView &c, const BatchView &b, int s, int first, int n, int row, int head, int lane, float *s_q) {
     constexpr int V = D / 64;
@@ -640,26 +642,33 @@ QG_DEV void attend_row(const AttnArgs &A, const KvView &c, const BatchView &b, i
     const float *q = A.q + ((size_t)row * A.q_heads + head) * D;
     for (int d = lane; d < D; d += 64) s_q[d] = q[d] * A.scale;
     __builtin_amdgcn_wave_barrier();  // one wave's own
-    float m = -__builtin_inff(), l = 0.0f, o[V];
-#pragma unroll
-    for (int i = 0; i < V; i++) o[i] = 0.0f;
     const int end = len + (b.parent ? n : place + 1);
-    for (int t0 = 0; t0 < end; t0 += 64) {
-        const int t = t0 + lane, page = t < end ? kv_page(c, s, t) : -1;
+    // key t: whether the row sees it, where it lies, its score
+    auto score = [&](int t, size_t &at, float &z) {
+        const int page = t < end ? kv_page(c, s, t) : -1;
         const bool visible = page >= 0 && (t < len || !b.parent || (seen >> (t - len) & 1));
-        const size_t at = kv_at(c, A.layer, max(page, 0), kv, t & ((1 << c.shift) - 1));
-        float z = -__builtin_inff();
+        at = kv_at(c, A.layer, max(page, 0), kv, t & ((1 << c.shift) - 1));
+        z = -__builtin_inff();
         if (visible) {
             z = 0.0f;
             for (int d = 0; d < D; d++) z = __builtin_fmaf(s_q[d], kv_load<TYPE>(c.k, at + d), z);
         }
-        const float top = fmaxf(m, qg_wave_max(z));
-        const float a = top == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f(m - top);
-        const float p = visible ? __builtin_amdgcn_exp2f(z - (top == -__builtin_inff() ? 0.0f : top)) : 0.0f;
+        return visible;
+    };
+    size_t at;
+    float m = -__builtin_inff(), l = 0.0f, z, o[V];
+    for (int t0 = 0; t0 < end; t0 += 64) {
+        const bool visible = score(t0 + lane, at, z);
+        const float top = fmaxf(m, qg_wave_max(z)), base = top == -__builtin_inff() ? 0.0f : top;
+        l = l * __builtin_amdgcn_exp2f(m - base) + qg_sum_lanes<64>(visible ? __builtin_amdgcn_exp2f(z - base) : 0.0f);
         m = top;
-        l = l * a + qg_sum_lanes<64>(p);
+    }
 #pragma unroll
-        for (int i = 0; i < V; i++) o[i] *= a;
+    for (int i = 0; i < V; i++) o[i] = 0.0f;
+    const float base = m == -__builtin_inff() ? 0.0f : m;
+    for (int t0 = 0; t0 < end && l != 0.0f; t0 += 64) {
+        const bool visible = score(t0 + lane, at, z);
+        const float p = visible ? __builtin_amdgcn_exp2f(z - base) / l : 0.0f;
         for (unsigned long long left = __ballot(visible); left; left &= left - 1) {
             const int k = __builtin_ctzll(left);
             const float w = __shfl(p, k);
@@ -669,7 +678,7 @@ QG_DEV void attend_row(const AttnArgs &A, const KvView &c, const BatchView &b, i
         }
     }
 #pragma unroll
-    for (int i = 0; i < V; i++) A.out[((size_t)row * A.q_heads + head) * D + lane * V + i] = l == 0.0f ? 0.0f : o[i] / l;
+    for (int i = 0; i < V; i++) A.out[((size_t)row * A.q_heads + head) * D + lane * V + i] = o[i];
 }
 
 // Joins the parts of sequences that were cut, and takes up odd rows again.  Few

@@ -328,3 +328,17 @@ def test_attention_small_weights_beside_a_sink(qgl, typ, length, nats):
         rel = 2 * ds + 2.0 ** -22 + 4 * U * (4 + math.sqrt(length))
         tol = want * rel + (2.0 ** -38 * V.sum(0) / p.sum() if typ == F16 else 0)
         assert np.all(np.abs(got[0, h] - want) <= tol), (np.abs(got[0, h] - want).max() / want.max(), (tol / want).max())
+
+
+@pytest.mark.parametrize("typ", [F16, BF16, F32])
+@pytest.mark.parametrize("length,page", [(70, 16), (9000, 64)])
+def test_attention_values_near_the_types_end(qgl, typ, length, page):
+    """The output is a mean of the values: it is finite where they are, however large."""
+    rng = np.random.default_rng(length + 1)
+    big = {F16: 6.5e4, BF16: 3.3e38, F32: 3.3e38}[typ]
+    cache = Cache(rng, [length], [3], typ=typ, kv_heads=1, page=page, dim=64)
+    batch = Batch([3])
+    for t in range(length + 3):
+        cache.put(0, 0, t, rng.standard_normal((1, 64)), big * np.concatenate([np.ones((1, 32)), rng.uniform(-1, 1, (1, 32))], 1))
+    cache.upload()
+    check(cache, batch, rng.standard_normal((3, 4, 64)).astype(np.float32), 0.125)
