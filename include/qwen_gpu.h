@@ -255,7 +255,7 @@ int qg_tree_attention(float *out, const float *q, int q_heads, float scale, cons
                       const qg_kv_batch *batch, void *workspace, size_t workspace_bytes);
 
 /* out = softmax(x / temperature) of each row of [rows][cols]; out may be x.
- * temperature 0: 1 at the lowest index of the largest value.  -infinity gives
+ * temperature 0: 1 at the lowest index of the largest value; others from 2^-126 on.  -infinity gives
  * 0; a row of nothing but -infinity is 0; a row with NaN or +infinity is NaN.
  * rows 1..65536, cols 1..2^24, at most 2^35 values; 4-byte aligned. */
 size_t qg_softmax_workspace_bytes(int rows, int cols);

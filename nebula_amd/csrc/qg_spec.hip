@@ -149,6 +149,14 @@ void launch_rope(const RopeArgs &A, const KvView &c, const BatchView &b, int lay
 // one float per lane, so that a row may start anywhere.
 // ------------------------------------------------------------------------
 
+// 1 / T as the kernels use it: exponents are (x a - m a) b, in one fused step and a
+// product.  a is 1, or 2^-64 for temperatures from 2^64 on, where x - m may be past the
+// range although its share of T is not.  b 0 stands for temperature 0.
+struct SoftScale {
+    float a, b;
+    __device__ __forceinline__ float power(float x, float ma) const { return __builtin_amdgcn_exp2f(__builtin_fmaf(x, a, -ma) * b); }
+};
+
 // A workgroup's value by `op`, in every thread; s holds one per wave.
 template <int THREADS, typename T, typename F>
 QG_DEV T block_all(T v, T *s, F op) {
@@ -220,7 +228,7 @@ QG_DEV void write_spread(float *x, int n, F get) {
 // twice, with one value per thread and pass, 631).  BEST: temperature 0, in a kernel
 // of its own, since the registers hold one of the two (250 us; both in one kernel 350).
 template <int THREADS, int REGS, int KEPT, bool BEST>
-__global__ __launch_bounds__(THREADS) void softmax_row_kernel(float *out, const float *x, int cols, float scale) {
+__global__ __launch_bounds__(THREADS) void softmax_row_kernel(float *out, const float *x, int cols, SoftScale scale) {
     __shared__ float s_x[KEPT ? KEPT * THREADS : 1], s_f[THREADS / 64];
     __shared__ int s_i[BEST ? THREADS / 64 : 1];
     const int tid = threadIdx.x;
@@ -252,12 +260,13 @@ __global__ __launch_bounds__(THREADS) void softmax_row_kernel(float *out, const 
         return;
     }
     if (m == none) m = 0.0f;  // nothing but -infinity, or NaN: a sum of 0, or NaN
+    const float ma = m * scale.a;
     float sum = 0.0f;
 #pragma unroll
-    for (int k = 0; k < REGS; k++) { r[k] = __builtin_amdgcn_exp2f((r[k] - m) * scale); sum += r[k]; }
+    for (int k = 0; k < REGS; k++) { r[k] = scale.power(r[k], ma); sum += r[k]; }
 #pragma unroll 8
     for (int k = 0; k < KEPT; k++) {
-        const float e = __builtin_amdgcn_exp2f((s_x[k * THREADS + tid] - m) * scale);
+        const float e = scale.power(s_x[k * THREADS + tid], ma);
         s_x[k * THREADS + tid] = e;
         sum += e;
     }
@@ -276,7 +285,7 @@ constexpr int SM_THREADS = 256, SM_REGS = 16, SM_PIECE = SM_THREADS * SM_REGS;
 struct SoftPart { float m, sum; int at, pad; };
 
 template <bool LAST>
-__global__ __launch_bounds__(SM_THREADS) void softmax_piece_kernel(float *out, const float *x, int cols, float scale, SoftPart *parts) {
+__global__ __launch_bounds__(SM_THREADS) void softmax_piece_kernel(float *out, const float *x, int cols, SoftScale scale, SoftPart *parts) {
     __shared__ float s_f[4];
     __shared__ int s_i[4];
     const int pieces = (cols + SM_PIECE - 1) / SM_PIECE, which = blockIdx.x / pieces, piece = blockIdx.x % pieces;
@@ -290,14 +299,14 @@ __global__ __launch_bounds__(SM_THREADS) void softmax_piece_kernel(float *out, c
         for (int k = 0; k < SM_REGS; k++) m = fmaxf(m, r[k]);
         m = block_all<SM_THREADS>(m, s_f, Larger());
         int at = 0;
-        if (scale == 0.0f || m == none) {
+        if (scale.b == 0.0f || m == none) {
             FirstOf first;
 #pragma unroll
             for (int k = SM_REGS - 1; k >= 0; k--) first.see(k, r[k], m);
             at = block_all<SM_THREADS>(first.index<SM_THREADS>(), s_i, Lower());
         } else {
 #pragma unroll
-            for (int k = 0; k < SM_REGS; k++) sum += __builtin_amdgcn_exp2f((r[k] - m) * scale);
+            for (int k = 0; k < SM_REGS; k++) sum += scale.power(r[k], m * scale.a);
             sum = block_all<SM_THREADS>(sum, s_f, Added());
         }
         if (tid == 0) parts[piece] = SoftPart{m, sum, at == SM_NAN ? SM_NAN : c0 + at, 0};
@@ -306,20 +315,21 @@ __global__ __launch_bounds__(SM_THREADS) void softmax_piece_kernel(float *out, c
     float *to = out + (size_t)which * cols + c0;
     for (int i = tid; i < pieces; i += SM_THREADS) m = fmaxf(m, parts[i].m);
     m = block_all<SM_THREADS>(m, s_f, Larger());
+    const float ma = m * scale.a;
     int at = 0x7fffffff;
     for (int i = tid; i < pieces; i += SM_THREADS) {
         const SoftPart p = parts[i];
         if (p.at == SM_NAN) at = SM_NAN;
         else if (p.m == m) at = min(at, p.at);
-        if (p.m != none) sum += p.sum * __builtin_amdgcn_exp2f((p.m - m) * scale);
+        if (p.m != none) sum += p.sum * scale.power(p.m, ma);
     }
     sum = block_all<SM_THREADS>(sum, s_f, Added());
     at = block_all<SM_THREADS>(at, s_i, Lower());
     const bool nan = at == SM_NAN || m == __builtin_inff();
     const float inv = 1.0f / sum;
-    const bool one = scale == 0.0f || m == none;
+    const bool one = scale.b == 0.0f || m == none;
     write_spread<SM_THREADS, SM_REGS, SM_REGS>(to, n, [&](int k) {
-        float y = __builtin_amdgcn_exp2f((r[k] - m) * scale) * inv;
+        float y = scale.power(r[k], ma) * inv;
         if (one) y = m != none && c0 + k * SM_THREADS + tid == at ? 1.0f : 0.0f;
         return nan ? __builtin_nanf("") : y;
     });
@@ -332,7 +342,7 @@ __global__ __launch_bounds__(SM_THREADS) void softmax_piece_kernel(float *out, c
 constexpr int SM_SHORT = 40 * 1024, SM_HELD = (96 + 36) * 1024;
 bool softmax_pieces(int rows, int cols) { return cols > SM_HELD || (cols > SM_SHORT && (long)rows * cols < 13000000); }
 template <bool BEST>
-void softmax_rows(float *out, const float *x, int rows, int cols, float scale, hipStream_t s) {
+void softmax_rows(float *out, const float *x, int rows, int cols, SoftScale scale, hipStream_t s) {
     if (cols <= 4096) softmax_row_kernel<256, 16, 0, BEST><<<rows, 256, 0, s>>>(out, x, cols, scale);
     else if (cols <= 16384) softmax_row_kernel<1024, 16, 0, BEST><<<rows, 1024, 0, s>>>(out, x, cols, scale);
     else if (cols <= SM_SHORT) softmax_row_kernel<1024, 40, 0, BEST><<<rows, 1024, 0, s>>>(out, x, cols, scale);
@@ -709,16 +719,16 @@ size_t qg_softmax_workspace_bytes(int rows, int cols) {
 int qg_softmax(float *out, const float *x, int rows, int cols, float temperature, void *ws, size_t ws_bytes) {
     const size_t need = qg_softmax_workspace_bytes(rows, cols);
     if (!need || !out || !x || !ws || ws_bytes < need || (((uintptr_t)out | (uintptr_t)x) & 3) || ((uintptr_t)ws & 15)) return hipErrorInvalidValue;
-    if (!(temperature >= 0.0f) || !__builtin_isfinite(temperature)) return hipErrorInvalidValue;
+    if (!(temperature == 0.0f || temperature >= 0x1p-126f) || !__builtin_isfinite(temperature)) return hipErrorInvalidValue;
     const size_t bytes = 4 * (size_t)rows * cols;
     if ((out != x && qg_overlap(out, bytes, x, bytes)) || qg_overlap(ws, need, x, bytes) || qg_overlap(ws, need, out, bytes)) return hipErrorInvalidValue;
-    // log2 e / T, finite and not 0, which stands for temperature 0
-    const float scale = temperature > 0.0f ? fminf(fmaxf(1.44269504088896341f / temperature, 1e-37f), 3e38f) : 0.0f;
+    const float a = temperature >= 0x1p64f ? 0x1p-64f : 1.0f;
+    const SoftScale scale{a, temperature > 0.0f ? 1.44269504088896341f / (temperature * a) : 0.0f};
     if (softmax_pieces(rows, cols)) {
         const unsigned grid = (unsigned)((cols + SM_PIECE - 1) / SM_PIECE * rows);
         softmax_piece_kernel<false><<<grid, SM_THREADS, 0, qg_stream()>>>(out, x, cols, scale, (SoftPart *)ws);
         softmax_piece_kernel<true><<<grid, SM_THREADS, 0, qg_stream()>>>(out, x, cols, scale, (SoftPart *)ws);
-    } else if (scale > 0.0f) {
+    } else if (scale.b > 0.0f) {
         softmax_rows<false>(out, x, rows, cols, scale, qg_stream());
     } else {
         softmax_rows<true>(out, x, rows, cols, scale, qg_stream());

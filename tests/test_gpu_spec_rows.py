@@ -197,6 +197,20 @@ def test_softmax_greedy(qgl, rows, cols):
     np.testing.assert_array_equal(got, want)
 
 
+@pytest.mark.parametrize("rows,cols", [(3, 300), (3, 5000), (3, 30000), (3, 100003), (140, 100003)])
+@pytest.mark.parametrize("T,size", [(3e38, 3.4e38), (1e38, 1e38), (2.0 ** 64, 1e22), (1e19, 1e22), (2.0 ** -126, 2.0 ** -124), (1e-30, 1e-29)])
+def test_softmax_temperatures_near_the_types_ends(qgl, rows, cols, T, size):
+    """Values on the temperature's own scale, whose differences may pass the type's range or be below its normal numbers."""
+    rng = np.random.default_rng(cols)
+    x = (rng.uniform(-1, 1, (rows, cols)) * size).astype(np.float32)
+    x[1] = np.where(rng.random(cols) < 0.5, -np.inf, x[1])
+    x[2, :2] = np.float32(size), np.float32(-size)
+    T = float(np.float32(T))
+    want, tol = softmax_oracle(x, T)
+    got = softmax(x, T)
+    assert np.all(np.abs(got - want) <= tol * want + 2.0 ** -126), np.max(np.abs(got - want) / (tol * want + 2.0 ** -126))
+
+
 # ---------------- verification ----------------
 
 def verify(p, q, token, u, u_last, batch):

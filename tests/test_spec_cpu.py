@@ -246,3 +246,8 @@ def test_pages_that_may_be_written(tmp_path):
     table, refs = (C.c_int * 4)(2, 0, -1, 7), (C.c_int * 3)(2, 0, 1)
     assert [own(table, refs, 3, t) for t in (0, 7, 8, 16, 24, 32, -1)] == [2, 2, -1, -1, -1, -1, -1]
     assert [own(table, None, 3, t) for t in (0, 7, 8, 16, 24, 32, -1)] == [2, 2, 0, -1, -1, -1, -1]
+
+
+def test_refused_temperatures(lib):
+    for t in (1e-40, 2.0 ** -127, -0.5, float("-inf")):
+        assert lib.qg_softmax(A, 2 * A, 3, 100, t, 22 * A, 1 << 30) == INVALID, t
