@@ -277,14 +277,16 @@ int qg_softmax(float *out, const float *x, int rows, int cols, float temperature
  * u, u_last in [0, 1).  Outputs: count[s] = accepted rows with row 0 (0 for a
  * sequence without rows); path[s][0..count-1] their places; tokens_out[s]
  * [0..count-1] the accepted tokens and the last one; -1 behind them
- * ([sequences][max_rows] both; outputs, workspace, p and q do not overlap).  A token outside [0, cols) is never accepted. */
+ * ([sequences][max_rows] both).  The outputs overlap neither each other nor p, q,
+ * u_last and start, the workspace nothing.  A token outside [0, cols) is never accepted. */
 size_t qg_verify_workspace_bytes(int sequences, int cols);
 int qg_verify_drafts(int *tokens_out, int *path, int *count, const float *p, const float *q, const int *token,
                      const float *u, const float *u_last, int cols, int sequences, const qg_kv_batch *batch,
                      void *workspace, size_t workspace_bytes);
 
 /* Pages.  Calls that change tables take one stream at a time; each result is
- * the same on every run.  qg_kv_workspace_bytes serves fork (of up to
+ * the same on every run.  The arrays given overlap neither each other nor the
+ * cache's where one of them is written, but for lengths as said.  qg_kv_workspace_bytes serves fork (of up to
  * `sequences` pairs) and reserve. */
 size_t qg_kv_workspace_bytes(const qg_kv_cache *cache);
 /* Room for the batch's rows behind each sequence's tokens: pages are taken in
@@ -311,6 +313,8 @@ int qg_kv_truncate(const qg_kv_cache *cache, const int *new_length);
 /* The accepted rows (qg_verify_drafts' path and count) move to the front: the
  * token at length[s] + path[s][i] goes to length[s] + i, in every layer, and
  * new_length[s] = length[s] + count[s], or the rows followed if fewer (new_length may be the cache's length).
+ * max_rows is at most 64, for chains too: a longer prompt chunk, all of whose
+ * rows stay where they are, is taken by adding its rows to `length`.
  * A path is followed while it ascends inside its sequence's rows, and up to the
  * first row whose page, or the page that it would move to, another table entry
  * holds too (where the cache has refs); rows behind the last one with both pages

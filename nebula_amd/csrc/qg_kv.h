@@ -13,6 +13,17 @@ int qg_batch_check(const qg_kv_batch *b, bool tree, BatchView *v);
 static inline bool qg_overlap(const void *a, size_t n, const void *b, size_t m) {
     return a && b && (uintptr_t)a < (uintptr_t)b + m && (uintptr_t)b < (uintptr_t)a + n;
 }
+struct QgSpan { const void *at; size_t bytes; };
+// Whether a span of the first list shares an address with one of the second.
+template <int N, int M>
+static inline bool qg_any_overlap(const QgSpan (&a)[N], const QgSpan (&b)[M]) {
+    for (const QgSpan &x : a)
+        for (const QgSpan &y : b)
+            if (qg_overlap(x.at, x.bytes, y.at, y.bytes)) return true;
+    return false;
+}
+static inline size_t qg_ints(size_t n) { return 4 * n; }
+static inline size_t qg_table_bytes(const KvView &c) { return qg_ints((size_t)c.sequences * c.table_pages); }
 
 // The sequence of a row (a wave's lanes together), or -1: the last one whose
 // first row is not behind it, if its rows reach that far.

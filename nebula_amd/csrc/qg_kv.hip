@@ -392,6 +392,12 @@ int qg_kv_reserve(const qg_kv_cache *cache, const qg_kv_batch *batch, int *statu
     BatchView b;
     if (qg_kv_check(cache, true, &c) || qg_batch_check(batch, false, &b)) return hipErrorInvalidValue;
     if (!status || !ws || (((uintptr_t)status | (uintptr_t)ws) & 3) || ws_bytes < qg_kv_workspace_bytes(cache)) return hipErrorInvalidValue;
+    const size_t S = c.sequences;
+    const QgSpan cached[3] = {{c.table, qg_table_bytes(c)}, {c.length, qg_ints(S)}, {c.refs, qg_ints(c.pages)}}, starts[1] = {{b.start, qg_ints(S + 1)}},
+                 said[1] = {{status, qg_ints(S)}}, space[1] = {{ws, qg_kv_workspace_bytes(cache)}};
+    if (qg_any_overlap(said, cached) || qg_any_overlap(said, starts) || qg_any_overlap(said, space) || qg_any_overlap(space, cached) ||
+        qg_any_overlap(space, starts) || qg_any_overlap(starts, cached))
+        return hipErrorInvalidValue;
     kv_reserve_kernel<<<1, 1024, 0, qg_stream()>>>(c, b, status, (int *)ws);
     const long work = 2L * c.layers * page_parts(c) * c.sequences;
     kv_cow_kernel<<<(unsigned)(work < 8192 ? work : 8192), 256, 0, qg_stream()>>>(c, (const int *)ws, (int)page_parts(c));
@@ -404,6 +410,9 @@ int qg_kv_fork(const qg_kv_cache *cache, const int *dst, const int *src, int n, 
     if (!dst || !src || n < 1 || n > c.sequences || !ws || ws_bytes < qg_kv_workspace_bytes(cache) ||
         (((uintptr_t)dst | (uintptr_t)src | (uintptr_t)ws) & 3))
         return hipErrorInvalidValue;
+    const QgSpan pairs[2] = {{dst, qg_ints(n)}, {src, qg_ints(n)}}, space[1] = {{ws, qg_kv_workspace_bytes(cache)}},
+                 cached[3] = {{c.table, qg_table_bytes(c)}, {c.length, qg_ints(c.sequences)}, {c.refs, qg_ints(c.pages)}};
+    if (qg_any_overlap(pairs, cached) || qg_any_overlap(pairs, space) || qg_any_overlap(space, cached)) return hipErrorInvalidValue;
     if (n <= FORK_PAIRS && (long)n * c.table_pages <= FORK_HELD * 1024) {
         kv_fork_small_kernel<<<1, 1024, 0, qg_stream()>>>(c, dst, src, n);
         return hipGetLastError();
@@ -416,7 +425,9 @@ int qg_kv_fork(const qg_kv_cache *cache, const int *dst, const int *src, int n, 
 int qg_kv_truncate(const qg_kv_cache *cache, const int *new_length) {
     KvView c;
     if (qg_kv_check(cache, true, &c) || ((uintptr_t)new_length & 3)) return hipErrorInvalidValue;
-    if (new_length != c.length && qg_overlap(new_length, 4 * (size_t)c.sequences, c.length, 4 * (size_t)c.sequences)) return hipErrorInvalidValue;
+    const QgSpan given[1] = {{new_length, qg_ints(c.sequences)}}, lengths[1] = {{c.length, qg_ints(c.sequences)}},
+                 others[2] = {{c.table, qg_table_bytes(c)}, {c.refs, qg_ints(c.pages)}};
+    if ((new_length != c.length && qg_any_overlap(given, lengths)) || qg_any_overlap(given, others)) return hipErrorInvalidValue;
     kv_truncate_kernel<<<c.sequences, 256, 0, qg_stream()>>>(c, new_length);
     return hipGetLastError();
 }
@@ -427,7 +438,11 @@ int qg_kv_compact(const qg_kv_cache *cache, const qg_kv_batch *batch, const int 
     if (qg_kv_check(cache, false, &c) || qg_batch_check(batch, true, &b)) return hipErrorInvalidValue;
     if (!path || !count || !new_length || (((uintptr_t)path | (uintptr_t)count | (uintptr_t)new_length) & 3)) return hipErrorInvalidValue;
     const bool own = new_length == cache->length;
-    if (!own && qg_overlap(new_length, 4 * (size_t)c.sequences, cache->length, 4 * (size_t)c.sequences)) return hipErrorInvalidValue;
+    // a sequence's first workgroup writes its new length while the others read what the path is made of
+    const size_t S = c.sequences;
+    const QgSpan written[1] = {{new_length, qg_ints(S)}}, lengths[1] = {{c.length, qg_ints(S)}},
+                 read[5] = {{path, qg_ints(S * b.max_rows)}, {count, qg_ints(S)}, {b.start, qg_ints(S + 1)}, {c.table, qg_table_bytes(c)}, {c.refs, qg_ints(c.pages)}};
+    if ((!own && qg_any_overlap(written, lengths)) || qg_any_overlap(written, read)) return hipErrorInvalidValue;
     const long all = 2L * c.layers * c.heads * (c.dim * (c.type == QT_F32 ? 4 : 2) / 16), blocks = (all + 255) / 256;
     kv_compact_kernel<<<dim3((unsigned)(blocks < 1024 ? blocks : 1024), c.sequences), 256, 0, qg_stream()>>>(c, b, path, count,
                                                                                                           own ? nullptr : new_length);

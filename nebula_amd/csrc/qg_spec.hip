@@ -752,11 +752,13 @@ int qg_verify_drafts(int *tokens_out, int *path, int *count, const float *p, con
          (uintptr_t)u_last) & 3)
         return hipErrorInvalidValue;
     const size_t vb = 4 * (size_t)b.rows * cols, ob = 4 * (size_t)sequences * b.max_rows, cb = 4 * (size_t)sequences;
-    // what is written, and p and q, which are read all the while
-    const struct { const void *at; size_t bytes; } own[6] = {{tokens_out, ob}, {path, ob}, {count, cb}, {ws, need}, {p, vb}, {q, vb}};
-    for (int i = 0; i < 4; i++)
-        for (int j = i + 1; j < 6; j++)
-            if (qg_overlap(own[i].at, own[i].bytes, own[j].at, own[j].bytes)) return hipErrorInvalidValue;
+    // the last kernel writes the outputs where its other workgroups read; the first ones read every input and write the workspace
+    const QgSpan out[3] = {{tokens_out, ob}, {path, ob}, {count, cb}}, space[1] = {{ws, need}},
+                 all_along[4] = {{p, vb}, {q, vb}, {u_last, cb}, {b.start, qg_ints((size_t)sequences + 1)}},
+                 first[3] = {{token, qg_ints(b.rows)}, {u, qg_ints(b.rows)}, {b.parent, qg_ints(b.rows)}};
+    if (qg_any_overlap(out, space) || qg_any_overlap(out, all_along) || qg_any_overlap(space, all_along) || qg_any_overlap(space, first) ||
+        qg_overlap(tokens_out, ob, path, ob) || qg_overlap(tokens_out, ob, count, cb) || qg_overlap(path, ob, count, cb))
+        return hipErrorInvalidValue;
     const Pieces pieces = verify_pieces(sequences, cols);
     const int rounds = verify_rounds(b, q != nullptr);
     Walk *walks = (Walk *)ws;

@@ -251,3 +251,39 @@ def test_pages_that_may_be_written(tmp_path):
 def test_refused_temperatures(lib):
     for t in (1e-40, 2.0 ** -127, -0.5, float("-inf")):
         assert lib.qg_softmax(A, 2 * A, 3, 100, t, 22 * A, 1 << 30) == INVALID, t
+
+
+def test_refused_overlaps_of_page_calls(lib):
+    """What a page call writes and what its other workgroups read, cache arrays among it; sizes of the caches above:
+    3 sequences, tables of 4 entries, 10 pages."""
+    c, b = cache(), batch()
+    W, N = 60 * A, lib.qg_kv_workspace_bytes(ref(c))
+    path, count, out = 30 * A, 31 * A, 32 * A
+    for new in (path, path + 4 * 14, count, count + 8, count - 8, b.start, b.start + 12, c.table + 44, c.table - 8, c.refs + 36, c.length + 8, c.length - 8):
+        assert lib.qg_kv_compact(ref(c), ref(b), path, count, new) == INVALID, hex(new)
+    for own in (dict(count=c.length), dict(path=c.length - 4), dict(start=c.length + 4)):   # the cache's lengths as the new ones
+        p, n, starts = own.get("path", path), own.get("count", count), own.get("start", b.start)
+        assert lib.qg_kv_compact(ref(c), ref(batch(start=starts)), p, n, c.length) == INVALID, own
+    for new in (c.table + 44, c.table - 8, c.refs, c.refs + 36):
+        assert lib.qg_kv_truncate(ref(c), new) == INVALID, hex(new)
+    for status, ws in ((W, W), (W + N - 4, W), (c.length, W), (c.table + 44, W), (c.refs + 36, W), (b.start + 12, W), (out, c.length - N + 4), (out, c.table),
+                       (out, c.refs + 36), (out, b.start + 12)):
+        assert lib.qg_kv_reserve(ref(c), ref(b), status, ws, N) == INVALID, (hex(status), hex(ws))
+    for dst, src, n, ws in ((c.length, path, 1, W), (path, c.length + 8, 1, W), (c.table + 40, path, 2, W), (path, c.refs + 32, 3, W), (W + 4, path, 1, W),
+                            (path, W + N - 4, 1, W), (path, count, 1, c.length - 4), (path, count, 1, c.table + 44), (path, count, 1, c.refs)):
+        assert lib.qg_kv_fork(ref(c), dst, src, n, ws, N) == INVALID, (hex(dst), hex(src))
+
+
+def test_refused_overlaps_of_verification(lib):
+    """Outputs over what the last kernel reads, the workspace over any input."""
+    b, W = batch(), 60 * A
+    N = lib.qg_verify_workspace_bytes(3, 100)
+    good = [30 * A, 31 * A, 32 * A, 33 * A, 34 * A, 35 * A, 36 * A, 37 * A, 100, 3, ref(b), W, N]
+    for i, bad in ((0, 37 * A), (1, 37 * A + 8), (2, 37 * A - 8), (0, b.start), (1, b.start + 12), (2, b.start - 8), (5, W), (6, W + N - 4), (7, W + 16)):
+        args = list(good)
+        args[i] = bad
+        assert lib.qg_verify_drafts(*args) == INVALID, (i, hex(bad))
+    for kw in (dict(start=W), dict(parent=W + N - 4)):
+        args = list(good)
+        args[10] = ref(batch(**kw))
+        assert lib.qg_verify_drafts(*args) == INVALID, kw
