@@ -257,7 +257,8 @@ int qg_tree_attention(float *out, const float *q, int q_heads, float scale, cons
 /* out = softmax(x / temperature) of each row of [rows][cols]; out may be x.
  * temperature 0: 1 at the lowest index of the largest value; others from 2^-126 on.  -infinity gives
  * 0; a row of nothing but -infinity is 0; a row with NaN or +infinity is NaN.
- * rows 1..65536, cols 1..2^24, at most 2^35 values; 4-byte aligned. */
+ * rows 1..65536, cols 1..2^24, at most 2^35 values; 4-byte aligned.  The
+ * workspace of a number of rows serves fewer of them too. */
 size_t qg_softmax_workspace_bytes(int rows, int cols);
 int qg_softmax(float *out, const float *x, int rows, int cols, float temperature, void *workspace, size_t workspace_bytes);
 
@@ -278,7 +279,8 @@ int qg_softmax(float *out, const float *x, int rows, int cols, float temperature
  * sequence without rows); path[s][0..count-1] their places; tokens_out[s]
  * [0..count-1] the accepted tokens and the last one; -1 behind them
  * ([sequences][max_rows] both).  The outputs overlap neither each other nor p, q,
- * u_last and start, the workspace nothing.  A token outside [0, cols) is never accepted. */
+ * u_last and start, the workspace nothing.  A token outside [0, cols) is never
+ * accepted.  The workspace of a number of sequences serves fewer of them too. */
 size_t qg_verify_workspace_bytes(int sequences, int cols);
 int qg_verify_drafts(int *tokens_out, int *path, int *count, const float *p, const float *q, const int *token,
                      const float *u, const float *u_last, int cols, int sequences, const qg_kv_batch *batch,

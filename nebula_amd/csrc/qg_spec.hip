@@ -340,7 +340,9 @@ __global__ __launch_bounds__(SM_THREADS) void softmax_piece_kernel(float *out, c
 // 29.1; 70000: 64 11.3 / 20.3, 256 35.6 / 32.7).  Rows of up to 40960 are faster by
 // rows however few (1 row of 32000: 8.0 / 6.8; 8192: 7.9 / 5.1).
 constexpr int SM_SHORT = 40 * 1024, SM_HELD = (96 + 36) * 1024;
-bool softmax_pieces(int rows, int cols) { return cols > SM_HELD || (cols > SM_SHORT && (long)rows * cols < 13000000); }
+// The rows up to which rows of `cols` values go in pieces.
+int softmax_piece_rows(int cols) { return cols > SM_HELD ? 0x7fffffff : cols > SM_SHORT ? 12999999 / cols : 0; }
+bool softmax_pieces(int rows, int cols) { return rows <= softmax_piece_rows(cols); }
 template <bool BEST>
 void softmax_rows(float *out, const float *x, int rows, int cols, SoftScale scale, hipStream_t s) {
     if (cols <= 4096) softmax_row_kernel<256, 16, 0, BEST><<<rows, 256, 0, s>>>(out, x, cols, scale);
@@ -657,6 +659,12 @@ Pieces verify_pieces(int sequences, int cols) {
     const size_t blocks = ((size_t)cols + VF_BLOCK - 1) / VF_BLOCK, per = (blocks * sequences + 2047) / 2048;
     return Pieces{per * VF_BLOCK, (blocks + per - 1) / per};
 }
+// No number of sequences up to this one has more pieces together: each has at most
+// blocks / per + 1, and blocks * sequences / per is at most 2048.
+size_t verify_sums(int sequences, int cols) {
+    const size_t each = (((size_t)cols + VF_BLOCK - 1) / VF_BLOCK) * sequences, all = 2048 + (size_t)sequences;
+    return each < all ? each : all;
+}
 // Sums by launches over the whole card; a tree's later ones (each takes another
 // rejection with drafts left to try) are few and fall to the drawing workgroup.
 // With 2 / 4 / 7: 64 trees of 17 rows x 131072 tokens 75 / 38 / 46 us, 16 of 33 x
@@ -713,7 +721,9 @@ int qg_qk_norm_rope(float *q_out, float *k_out, const qg_qk_rows *in, const qg_k
 
 size_t qg_softmax_workspace_bytes(int rows, int cols) {
     if (rows < 1 || rows > QG_MAX_ROWS || cols < 1 || cols > 1 << 24 || (long)rows * cols > 1L << 35) return 0;
-    return softmax_pieces(rows, cols) ? (size_t)rows * ((cols + SM_PIECE - 1) / SM_PIECE) * sizeof(SoftPart) : sizeof(SoftPart);
+    // of every number of rows up to this one, the largest that goes in pieces
+    const int most = rows < softmax_piece_rows(cols) ? rows : softmax_piece_rows(cols);
+    return most ? (size_t)most * ((cols + SM_PIECE - 1) / SM_PIECE) * sizeof(SoftPart) : sizeof(SoftPart);
 }
 
 int qg_softmax(float *out, const float *x, int rows, int cols, float temperature, void *ws, size_t ws_bytes) {
@@ -738,8 +748,7 @@ int qg_softmax(float *out, const float *x, int rows, int cols, float temperature
 
 size_t qg_verify_workspace_bytes(int sequences, int cols) {
     if (sequences < 1 || sequences > QG_MAX_SEQUENCES || cols < 1 || cols > 1 << 24) return 0;
-    return 2 * (size_t)sequences * (verify_pieces(sequences, cols).y * sizeof(double) + sizeof(Walk)) +
-           (size_t)sequences * QG_MAX_TREE * sizeof(Draft);
+    return 2 * (verify_sums(sequences, cols) * sizeof(double) + (size_t)sequences * sizeof(Walk)) + (size_t)sequences * QG_MAX_TREE * sizeof(Draft);
 }
 
 int qg_verify_drafts(int *tokens_out, int *path, int *count, const float *p, const float *q, const int *token, const float *u,

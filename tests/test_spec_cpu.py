@@ -287,3 +287,20 @@ def test_refused_overlaps_of_verification(lib):
         args = list(good)
         args[10] = ref(batch(**kw))
         assert lib.qg_verify_drafts(*args) == INVALID, kw
+
+
+@pytest.mark.parametrize("cols", [1, 4096, 4097, 40960, 40961, 50000, 131072, 135168, 135169, 151936, 300001, 1 << 24])
+def test_workspaces_serve_smaller_batches(lib, cols):
+    """A workspace for the largest batch is enough for every smaller one, and none is smaller than what a call of that
+    size lays out in it."""
+    rows = [lib.qg_softmax_workspace_bytes(r, cols) for r in range(1, 1200)]
+    assert rows == sorted(rows) and rows[0] > 0
+    seqs = [lib.qg_verify_workspace_bytes(s, cols) for s in range(1, 1025)]
+    assert seqs == sorted(seqs)
+    blocks = -(-cols // 4096)
+    for s, n in enumerate(seqs, 1):
+        pieces = -(-blocks // -(-blocks * s // 2048))
+        assert n >= 2 * s * (8 * pieces + 48) + s * 64 * 20, (s, n)
+    for r, n in enumerate(rows, 1):
+        if cols > 135168 or (cols > 40960 and r * cols < 13000000):
+            assert n >= 16 * r * -(-cols // 4096), (r, n)
