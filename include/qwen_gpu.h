@@ -192,7 +192,7 @@ int qg_moe_forward_residual(float *h, int *ids, float *weights, unsigned char *f
 typedef struct {
     void *k, *v;                /* [layers][pages][kv_heads][page_tokens][head_dim], 16-byte aligned */
     int type;                   /* 0 F32, 1 F16, 30 BF16 */
-    int layers, pages, kv_heads; /* layers 1..65536, kv_heads 1..128 */
+    int layers, pages, kv_heads; /* layers 1..65536, pages 1..2^30, kv_heads 1..128 */
     int page_tokens;            /* a power of two, 8..1024 */
     int head_dim;               /* 64, 128 or 256 */
     int *refs;                  /* [pages] table entries that hold each page, 0 = free; NULL without page calls */

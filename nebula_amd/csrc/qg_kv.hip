@@ -11,7 +11,7 @@ int qg_kv_check(const qg_kv_cache *c, bool pages, KvView *v) {
     if ((((uintptr_t)c->k | (uintptr_t)c->v) & 15) || (((uintptr_t)c->table | (uintptr_t)c->length | (uintptr_t)c->refs) & 3))
         return hipErrorInvalidValue;
     if (c->type != QT_F32 && c->type != QT_F16 && c->type != QT_BF16) return hipErrorInvalidValue;
-    if (c->layers < 1 || c->layers > 65536 || c->pages < 1 || c->kv_heads < 1 || c->kv_heads > 128) return hipErrorInvalidValue;
+    if (c->layers < 1 || c->layers > 65536 || c->pages < 1 || c->pages > 1 << 30 || c->kv_heads < 1 || c->kv_heads > 128) return hipErrorInvalidValue;
     if (c->head_dim != 64 && c->head_dim != 128 && c->head_dim != 256) return hipErrorInvalidValue;
     if (c->page_tokens < 8 || c->page_tokens > 1024 || (c->page_tokens & (c->page_tokens - 1))) return hipErrorInvalidValue;
     if (c->sequences < 1 || c->sequences > QG_MAX_SEQUENCES || c->table_pages < 1) return hipErrorInvalidValue;

@@ -304,3 +304,13 @@ def test_workspaces_serve_smaller_batches(lib, cols):
     for r, n in enumerate(rows, 1):
         if cols > 135168 or (cols > 40960 and r * cols < 13000000):
             assert n >= 16 * r * -(-cols // 4096), (r, n)
+
+
+def test_refused_page_counts(lib):
+    """Page numbers are marked as -2 - page and counted 16384 at a time: both stay inside an int up to 2^30 pages."""
+    small = dict(layers=1, kv_heads=1, page_tokens=8)
+    assert lib.qg_kv_workspace_bytes(ref(cache(pages=1 << 30, **small))) == 4 * (2 + 2 * 3 + (1 << 30))
+    for pages in ((1 << 30) + 1, 2 ** 31 - 1):
+        c = cache(pages=pages, **small)
+        assert lib.qg_kv_workspace_bytes(ref(c)) == 0
+        assert lib.qg_kv_reserve(ref(c), ref(batch()), 30 * A, 60 * A, 1 << 40) == INVALID
