@@ -31,7 +31,7 @@ void nm_stack_destroy(nm_stack *s);
 float *nm_stack_hidden(nm_stack *s);
 /* Runs all layers on the first `tokens` rows of the hidden state, on the
  * calling thread's stream.  use_graph: capture on first use per token count,
- * then replay. */
+ * then replay; inside a capture of the caller's the calls join that graph. */
 int nm_stack_forward(nm_stack *s, int tokens, int use_graph);
 /* With record != 0: device arrays of layer l: normalised input [tokens][D],
  * ids [tokens][10], weights [tokens][10], MoE output [tokens][D]. */
@@ -62,7 +62,10 @@ int nm_stack_attend(nm_stack *s, const nm_attention_layer *layers, const nm_atte
  * weight); rows of no sequence take the MoE alone.  Keys and values of the rows are stored behind the cached tokens;
  * lengths do not change (qg_kv_compact does that once drafts are accepted).
  * use_graph: captured on first use per number of rows and replayed while the
- * batch's arrays stay where they are; what they hold may change. */
+ * batch's arrays stay where they are; what they hold may change.  Inside a capture
+ * of the caller's (qg_graph_begin) the calls join that graph, whatever use_graph
+ * says.  A stack has one hidden state and one workspace: one call, or one graph that
+ * holds it, runs at a time. */
 int nm_stack_verify(nm_stack *s, const qg_kv_batch *batch, int use_graph);
 
 /* CPU handoff of one layer's flag-2 tokens (the hybrid path of

@@ -36,6 +36,7 @@ int qg_graph_begin(void **graph);                               /* gpu.h:18 */
 int qg_graph_end(void *graph);                                  /* gpu.h:19 */
 int qg_graph_launch(void *graph);                               /* gpu.h:20 */
 void qg_graph_destroy(void *graph);                             /* gpu.h:21 */
+int qg_graph_recording(void);   /* 1 between the calling thread's qg_graph_begin and qg_graph_end (an addition) */
 int qg_memory(size_t *free_bytes, size_t *total_bytes);         /* gpu.h:24 */
 const char *qg_error(int error);                                /* gpu.h:30 */
 int qg_tensor_bytes(int type, const uint64_t dims[4], uint64_t *bytes); /* gpu.h:31 */

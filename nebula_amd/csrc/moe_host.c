@@ -117,7 +117,7 @@ static int run_layers(nm_stack *s, int nt) {
 
 int nm_stack_forward(nm_stack *s, int nt, int use_graph) {
     if (!s || nt < 1 || nt > s->max_tokens) return fail("invalid token count");
-    if (!use_graph) return run_layers(s, nt);
+    if (!use_graph || qg_graph_recording()) return run_layers(s, nt);
     void **g = &s->graphs[nt];
     if (!*g) {
         GPU(qg_graph_begin(g));
@@ -204,7 +204,7 @@ int nm_stack_verify(nm_stack *s, const qg_kv_batch *batch, int use_graph) {
     if (!s || !s->attn_layers || !batch) return fail("invalid verify arguments");
     if (batch->rows < 1 || batch->rows > s->max_tokens) return fail("%d rows for a stack of %d tokens", batch->rows, s->max_tokens);
     if (!batch->start || batch->max_rows < 1 || batch->max_rows > batch->rows) return fail("invalid batch");
-    if (!use_graph) return run_verify(s, batch);
+    if (!use_graph || qg_graph_recording()) return run_verify(s, batch);
     void **g = &s->verify_graphs[batch->rows];
     qg_kv_batch *b = &s->verify_batches[batch->rows];
     if (*g && (b->max_rows != batch->max_rows || b->start != batch->start || b->parent != batch->parent)) {

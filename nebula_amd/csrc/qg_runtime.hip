@@ -175,6 +175,8 @@ int qg_graph_end(void *ptr) {
     return rc;
 }
 
+int qg_graph_recording(void) { return tl_stream != nullptr; }
+
 int qg_graph_launch(void *ptr) {
     qg_graph *g = (qg_graph *)ptr;
     return g && g->exec ? hipGraphLaunch(g->exec, tl_stream) : hipErrorInvalidValue;

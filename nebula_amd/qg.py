@@ -21,7 +21,7 @@ SIGNATURES = {
     "alloc": ([Z], P), "free": ([P], None), "write": ([P, P, Z], I), "read": ([P, P, Z], I),
     "copy": ([P, P, Z], I), "zero": ([P, Z], I), "sync": ([], I), "error": ([I], C.c_char_p),
     "memory": ([P, P], I), "tensor_bytes": ([I, P, P], I),
-    "graph_begin": ([P], I), "graph_end": ([P], I), "graph_launch": ([P], I), "graph_destroy": ([P], None),
+    "graph_begin": ([P], I), "graph_end": ([P], I), "graph_launch": ([P], I), "graph_destroy": ([P], None), "graph_recording": ([], I),
     "upload_create": ([Z], P), "upload_destroy": ([P], None), "upload_expert": ([P, P, P, Z, P, Z, P, Z], I),
     "upload_seconds": ([P], D64),
     # operators (gpu.h:37-43,62-78)

@@ -344,6 +344,76 @@ def test_stack_verify_rows_of_no_sequence(stack_parts):
         host.nm_stack_destroy(stack)
 
 
+@pytest.mark.parametrize("use_graph", [0, 1])
+@pytest.mark.parametrize("used", [False, True])
+def test_stack_inside_a_callers_capture(stack_parts, use_graph, used):
+    """Room for the rows, the stack and the new lengths in one graph of the caller's, replayed on new rows, trees and
+    lengths: bit for bit the same calls on a cache of its own.  used: the stack has graphs of its own, for other arrays."""
+    host, lib = qg.host(), qg.lib()
+    counts = [5, 4]
+    make = lambda: Cache(np.random.default_rng(31), [40, 7], [0, 0], typ=F16, layers=LAYERS, kv_heads=HK, page=16, dim=HD, spare=24, table_pages=12)
+    caches = [make(), make()]
+    stacks = [make_stack(stack_parts, c, 17) for c in caches]
+    batches = [Batch(counts, [O.random_tree(np.random.default_rng(32), n) for n in counts]) for _ in caches]
+    n = lib.qg_kv_workspace_bytes(caches[0].ref)
+    ws, status, path, count = ([f() for _ in caches] for f in (lambda: Device(nbytes=n), lambda: Device(shape=(2,), dtype=np.int32),
+                                                              lambda: Device(shape=(2, 5), dtype=np.int32), lambda: Device(shape=(2,), dtype=np.int32)))
+
+    def step(i, graphed):
+        c, b = caches[i], batches[i]
+        call("kv_reserve", c.ref, b.ref, status[i].p, ws[i].p, n)
+        assert host.nm_stack_verify(stacks[i], b.ref, graphed) == 0, host.nm_last_error()
+        call("kv_compact", c.ref, b.ref, path[i].p, count[i].p, c.dlength.p)
+        assert host.nm_stack_forward(stacks[i], sum(counts), graphed) == 0, host.nm_last_error()
+
+    rng = np.random.default_rng(33)
+    graph = C.c_void_p()
+    try:
+        if used:  # on rows of their own, whose pages are let go again
+            other = Batch(counts)
+            lengths = Device(np.array([40, 7], np.int32))
+            for i in range(2):
+                call("kv_reserve", caches[i].ref, other.ref, status[i].p, ws[i].p, n)
+                assert host.nm_stack_verify(stacks[i], other.ref, 1) == 0 and host.nm_stack_forward(stacks[i], 3, 1) == 0, host.nm_last_error()
+                call("kv_truncate", caches[i].ref, lengths.p)
+            call("sync")
+        assert lib.qg_graph_recording() == 0
+        say(f"capture a stack, use_graph={use_graph} used={used}")
+        call("graph_begin", C.byref(graph))
+        assert lib.qg_graph_recording() == 1
+        step(0, use_graph)
+        call("graph_end", graph)
+        assert lib.qg_graph_recording() == 0
+        for replay in range(4):
+            h0 = rng.standard_normal((sum(counts), WIDTH)).astype(np.float32)
+            tree = np.concatenate([O.random_tree(rng, k) for k in counts]).astype(np.int32)
+            ways = [[0] + sorted(rng.choice(np.arange(1, k), 2, replace=False)) for k in counts]
+            for i in range(2):
+                call("write", host.nm_stack_hidden(stacks[i]), h0.ctypes.data, h0.nbytes)
+                batches[i].dparent.set(tree)
+                path[i].set(np.array([w + [-1, -1] for w in ways], np.int32))
+                count[i].set(np.array([3, 1 + replay % 3], np.int32))
+            say(f"replay {replay}")
+            call("graph_launch", graph)
+            call("sync")
+            step(1, 0)
+            call("sync")
+            got = [np.empty_like(h0) for _ in range(2)]
+            for i in range(2):
+                call("read", got[i].ctypes.data, host.nm_stack_hidden(stacks[i]), h0.nbytes)
+            np.testing.assert_array_equal(got[0].view(np.uint32), got[1].view(np.uint32))
+            for name in ("dk", "dv", "dtable", "drefs", "dlength"):
+                np.testing.assert_array_equal(*(getattr(c, name).get().view(np.uint8) for c in caches))
+            np.testing.assert_array_equal(caches[0].dlength.get(), [40 + 3 * (replay + 1), 7 + sum(1 + k % 3 for k in range(replay + 1))])
+            assert (status[0].get() == 0).all() and np.isfinite(got[0]).all()
+    finally:
+        if not lib.qg_graph_recording():
+            call("sync")
+        lib.qg_graph_destroy(graph)
+        for stack in stacks:
+            host.nm_stack_destroy(stack)
+
+
 def test_stack_attend_refusals(stack_parts):
     layers, qkv, out, norms, freq = stack_parts
     host = qg.host()
