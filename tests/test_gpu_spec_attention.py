@@ -342,3 +342,20 @@ def test_attention_values_near_the_types_end(qgl, typ, length, page):
         cache.put(0, 0, t, rng.standard_normal((1, 64)), big * np.concatenate([np.ones((1, 32)), rng.uniform(-1, 1, (1, 32))], 1))
     cache.upload()
     check(cache, batch, rng.standard_normal((3, 4, 64)).astype(np.float32), 0.125)
+
+
+@pytest.mark.parametrize("typ", [F16, BF16, F32])
+@pytest.mark.parametrize("tree", [False, True])
+def test_attention_starts_beyond_the_rows(qgl, typ, tree):
+    """Row starts below the first row, of more rows than max_rows and behind the last row are cut to what there is."""
+    rng = np.random.default_rng(14)
+    counts, lengths = [2, 0, 5, 5], [60, 8, 40, 0]
+    cache = Cache(rng, lengths, counts, typ=typ, kv_heads=2, page=16, dim=64)
+    batch = Batch(counts, [O.random_tree(rng, n) if n else [] for n in counts] if tree else None, rows=14, max_rows=5)
+    if tree:
+        batch.parent = np.concatenate([batch.parent[:7], [-1, -1], batch.parent[7:12]]).astype(np.int32)
+        batch.dparent.set(batch.parent)
+    batch.dstart.set(np.array([-7, 2, 2, 9, 1 << 30], np.int32))
+    batch.places = lambda: [(0, 0, 0), (1, 0, 1)] + [(2 + i, 2, i) for i in range(5)] + [(9 + i, 3, i) for i in range(5)]
+    store(cache, batch, rng)
+    check(cache, batch, rng.standard_normal((14, 6, 64)).astype(np.float32), 0.125)

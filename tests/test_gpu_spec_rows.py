@@ -125,6 +125,67 @@ def test_rope_many_sequences(qgl):
     np.testing.assert_array_equal(cache.dv.get().view(np.uint32), cache.v.view(np.uint32))
 
 
+def norm_rope_rows(x, w, eps, pos, freq, rope, interleaved):
+    """spec_oracle.norm_rope of every row and head at once."""
+    x = x.astype(np.float64)
+    if w is not None:
+        x = x / np.sqrt((x * x).mean(-1, keepdims=True) + eps) * w.astype(np.float64)
+    y, size, half = x.copy(), np.abs(x), rope // 2
+    i = np.arange(half)
+    a, b = (2 * i, 2 * i + 1) if interleaved else (i, i + half)
+    angle = pos.astype(np.float64)[:, None, None] * freq[:half]
+    c, s = np.cos(angle), np.sin(angle)
+    y[..., a], y[..., b] = x[..., a] * c - x[..., b] * s, x[..., b] * c + x[..., a] * s
+    size[..., a] = size[..., b] = np.abs(x[..., a]) + np.abs(x[..., b])
+    return y, size
+
+
+@pytest.mark.parametrize("D,Hq,Hkv,rope,interleaved,typ", [(64, 19, 2, 64, 0, F16), (64, 19, 2, 32, 1, F32), (128, 9, 2, 32, 0, BF16), (128, 9, 2, 128, 1, F16),
+                                                           (256, 5, 1, 256, 0, BF16), (256, 5, 1, 64, 1, F32)])
+@pytest.mark.parametrize("shape", ["chunk", "trees", "positions"])
+def test_rope_of_many_rows(qgl, D, Hq, Hkv, rope, interleaved, typ, shape):
+    """Batches whose waves take five groups of heads each, the last group in part: a prompt chunk beside short chains, many
+    trees, and rows without a cache."""
+    rng = np.random.default_rng(D + rope + typ)
+    counts = [3, 1700, 1, 0, 40] if shape != "trees" else [33, 0] + [int(x) for x in rng.integers(25, 41, 52)]
+    groups = -(-(Hq + Hkv * (1 if shape == "positions" else 2)) // (256 // D))
+    assert sum(counts) * groups > 8192 and groups % 5
+    lengths = [int(x) for x in rng.integers(0, 70, len(counts))]
+    cache = Cache(rng, lengths, counts, typ=typ, layers=1, kv_heads=Hkv, page=32, dim=D, fill=False)
+    batch = Batch(counts, [O.random_tree(rng, n) if n else [] for n in counts] if shape == "trees" else None, rows=sum(counts) + 3)
+    N = batch.rows
+    args, keep, q, k, v = rope_rows(rng, N, Hq, Hkv, D, False, 4)
+    freq = 10000.0 ** (-2 * np.arange(rope // 2) / rope)
+    wq, wk = (1 + 0.1 * rng.standard_normal(D)).astype(np.float32), (1 + 0.1 * rng.standard_normal(D)).astype(np.float32)
+    dwq, dwk, dfreq = Device(wq), Device(wk), Device(freq)
+    args.q_norm, args.k_norm, args.rope_dims, args.interleaved, args.freq = dwq.p, dwk.p, rope, interleaved, dfreq.p
+    qo, ko = Device(np.full((N, Hq, D), np.nan, np.float32)), Device(np.full((N, Hkv, D), np.nan, np.float32))
+    say(f"rope D={D} rows={N} {shape}")
+    pos, seen = np.zeros(N, np.int32), np.zeros(N, bool)
+    if shape == "positions":
+        pos, seen = rng.integers(0, 200000, N).astype(np.int32), ~seen
+        dpos = Device(pos)
+        args.position = dpos.p
+        call("qk_norm_rope", qo.p, ko.p, C.byref(args), None, 0, None)
+    else:
+        call("qk_norm_rope", qo.p, ko.p, C.byref(args), cache.ref, 0, batch.ref)
+        for row, s, place in batch.places():
+            seen[row] = True
+            pos[row] = lengths[s] + len(batch.line(row, place)) - 1 if shape == "trees" else lengths[s] + place
+    for got, x, w in ((qo.get(), q, wq), (ko.get(), k, wk)):
+        y, size = norm_rope_rows(x, w, 1e-6, pos, freq, rope, interleaved)
+        assert np.all((np.abs(got - y) <= ROPE_TOL * size)[seen]), np.argwhere((np.abs(got - y) > ROPE_TOL * size) & seen[:, None, None])[:5]
+        assert np.isnan(got[~seen]).all()
+    if shape == "positions":
+        return
+    # the cache: the keys that were given out, rounded, the values as they came, nothing else
+    stored = ko.get()
+    for row, s, place in batch.places():
+        cache.put(0, s, lengths[s] + place, stored[row], v[row])
+    for got, want in ((cache.dk.get(), cache.k), (cache.dv.get(), cache.v)):
+        np.testing.assert_array_equal(got.view(np.uint8), want.view(np.uint8))
+
+
 # ---------------- softmax ----------------
 
 def softmax(x, T, out=None):
@@ -197,6 +258,31 @@ def test_softmax_greedy(qgl, rows, cols):
     np.testing.assert_array_equal(got, want)
 
 
+@pytest.mark.parametrize("rows,cols", [(130, 131071), (140, 98305), (140, 98304), (128, 135168), (700, 20001), (300, 4097)])
+def test_softmax_greedy_where_the_row_is_kept(qgl, rows, cols):
+    """Temperature 0 of rows held in registers and shared memory (from value 98304 on): the largest, ties of it and NaN on
+    either side of every border."""
+    rng = np.random.default_rng(cols)
+    x = rng.standard_normal((rows, cols)).astype(np.float32)
+    borders = [b for b in (1024, 2048, 16384, 40960, 98304, 99328, 131072) if b < cols] + [cols]
+    for r in range(rows):
+        at = sorted({int(rng.choice(borders)) + int(d) for d in rng.integers(-2, 2, int(rng.integers(1, 4)))} | {int(rng.integers(0, cols))})
+        x[r, [a for a in at if r % 3 and 0 <= a < cols] or [at[-1] % cols]] = 9.0
+    x[1], x[2, cols - 1] = -np.inf, np.inf
+    x[3] = -np.inf
+    x[3, cols - 1] = -3e38
+    x[4, cols - 1] = x[5, min(98304, cols - 1)] = np.nan
+    x[6, :] = 0.0
+    x[7, :] = -1.0
+    x[7, cols - 2:] = 0.0
+    for out in (None, Device(np.full((rows, cols), np.nan, np.float32))):
+        got = softmax(x, 0.0, out)
+        want = (np.arange(cols) == x.argmax(-1)[:, None]).astype(np.float32)
+        want[1] = 0
+        want[[2, 4, 5]] = np.nan
+        np.testing.assert_array_equal(got, want)
+
+
 @pytest.mark.parametrize("rows,cols", [(3, 300), (3, 5000), (3, 30000), (3, 100003), (140, 100003)])
 @pytest.mark.parametrize("T,size", [(3e38, 3.4e38), (1e38, 1e38), (2.0 ** 64, 1e22), (1e19, 1e22), (2.0 ** -126, 2.0 ** -124), (1e-30, 1e-29)])
 def test_softmax_temperatures_near_the_types_ends(qgl, rows, cols, T, size):
@@ -249,6 +335,37 @@ def test_verify(qgl, counts, cols, tree, greedy):
         case = draft_case(rng, counts, cols, tree, greedy)
         for got, want in zip(verify(*case[1:], case[0]), O.verify(*case[1:], case[0])):
             np.testing.assert_array_equal(got, want)
+
+
+@pytest.mark.parametrize("tree", [False, True])
+@pytest.mark.parametrize("greedy", [False, True])
+def test_verify_pieces_of_several_blocks(qgl, tree, greedy):
+    """More blocks of the vocabulary in all than there are workgroups for: a piece is two of them."""
+    rng = np.random.default_rng(71 + tree)
+    case = draft_case(rng, [3] * 65, 131072, tree, greedy)
+    case[5][:3] = 0.0, np.float32(1 - 2 ** -24), 0.5
+    for got, want in zip(verify(*case[1:], case[0]), O.verify(*case[1:], case[0])):
+        np.testing.assert_array_equal(got, want)
+
+
+@pytest.mark.parametrize("tree", [False, True])
+@pytest.mark.parametrize("greedy", [False, True])
+@pytest.mark.parametrize("cols", [262144, 262145, 300001, 600000])
+def test_verify_more_pieces_than_lanes(qgl, cols, tree, greedy):
+    """Sums over more than 64 pieces, some of them with nothing in them, and tokens drawn from either end."""
+    rng = np.random.default_rng(cols)
+    for sparse in (False, True):
+        batch, p, q, token, u, last = draft_case(rng, [5, 0, 4, 3], cols, tree, greedy)
+        if sparse:  # mass in a few blocks alone, before and behind the 64th
+            keep = np.zeros(cols, bool)
+            for at in (4096 * 3, 4096 * 63 + 4000, cols - 5):
+                keep[at:at + 100] = True
+            p = np.where(keep, p, 0).astype(np.float32)
+            p /= p.sum(-1, keepdims=True)
+            token[rng.random(len(token)) < 0.5] = cols - 3
+        for lasts in (last, np.zeros(4, np.float32), np.full(4, 1 - 2 ** -24, np.float32)):
+            for got, want in zip(verify(p, q, token, u, lasts, batch), O.verify(p, q, token, u, lasts, batch)):
+                np.testing.assert_array_equal(got, want)
 
 
 def test_verify_special_rows(qgl):
