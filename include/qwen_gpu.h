@@ -248,7 +248,9 @@ int qg_qk_norm_rope(float *q_out, float *k_out, const qg_qk_rows *in, const qg_k
  * cores with queries and probabilities in planes of the cache's type that
  * together carry at least 22 bits (over an F16 cache no less than 2^-38 of a row's
  * largest probability, or of its largest query value).  A row that sees no token (or none with a
- * score above -infinity) is 0.  Rows of no sequence are left as they were.
+ * score above -infinity) is 0, one with a NaN or a score of +infinity is NaN.
+ * Rows that see infinities, or values whose sum passes fp32's range, are computed
+ * key by key, which is slow (18 ms over 98304 tokens).  Rows of no sequence are left as they were.
  * rows x q_heads at most 2^25.  The workspace of a batch serves every batch of
  * no more rows. */
 size_t qg_tree_attention_workspace_bytes(const qg_kv_cache *cache, const qg_kv_batch *batch, int q_heads);

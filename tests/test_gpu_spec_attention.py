@@ -359,3 +359,32 @@ def test_attention_starts_beyond_the_rows(qgl, typ, tree):
     batch.places = lambda: [(0, 0, 0), (1, 0, 1)] + [(2 + i, 2, i) for i in range(5)] + [(9 + i, 3, i) for i in range(5)]
     store(cache, batch, rng)
     check(cache, batch, rng.standard_normal((14, 6, 64)).astype(np.float32), 0.125)
+
+
+@pytest.mark.parametrize("typ", [F16, BF16, F32])
+@pytest.mark.parametrize("dim,length", [(64, 50), (128, 3000), (256, 700)])
+def test_attention_nan_rows_beside_others(qgl, typ, dim, length):
+    """NaN in a query, in a key and in a value that some rows see and others do not, rows that are taken up again for an
+    infinite value, all in one batch over holes: each row's own answer."""
+    rng = np.random.default_rng(dim)
+    rows, heads, page = 8, 4, 32
+    cache = Cache(rng, [length], [rows], typ=typ, kv_heads=2, page=page, dim=dim)
+    parents = [-1, 0, 0, 1, 2, 2, 4, 3]      # rows below 1: 1, 3, 7; below 2: 2, 4, 5, 6
+    batch = Batch([rows], [parents])
+    store(cache, batch, rng)
+    at = lambda place: (0, cache.page_of(0, length + place), slice(None), (length + place) % page)
+    cache.k[at(1)][:, 3] = O.encode([np.nan], typ)[0]
+    cache.v[at(5)][:, 2] = O.encode([np.nan], typ)[0]
+    cache.v[at(4)][:, 7] = O.encode([np.inf], typ)[0]
+    if length > 100:
+        cache.table[0, 1] = -1
+    cache.upload()
+    q = rng.standard_normal((rows, heads, dim)).astype(np.float32)
+    q[2, 1, 5] = np.nan
+    got = attend(cache, batch, q, dim ** -0.5)
+    want, tol, _ = O.attention(cache, batch, np.nan_to_num(q, nan=0.0), dim ** -0.5)
+    assert np.isnan(got[[1, 3, 7]]).all() and np.isnan(got[2, 1]).all() and np.isnan(got[5, :, 2]).all()
+    assert (got[[4, 6], :, 7] == np.inf).all()
+    keep = np.ones(q.shape, bool)
+    keep[[1, 3, 7]], keep[2, 1], keep[5, :, 2], keep[4, :, 7], keep[6, :, 7] = False, False, False, False, False
+    assert np.all(np.abs(got[keep] - want[keep]) <= tol[keep])
