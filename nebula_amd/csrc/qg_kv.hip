@@ -320,7 +320,7 @@ QG_DEV int path_rows(const KvView &c, const BatchView &b, const int *path, const
     const bool ok = lane < keep && p < n && p > (lane ? before : -1);
     from = ok ? kv_page(c, s, len + p) : -1;
     to = ok ? kv_page(c, s, len + lane) : -1;
-    const bool shared = c.refs && ((from >= 0 && c.refs[from] > 1) || (to >= 0 && c.refs[to] > 1));
+    const bool shared = kv_shared(c, from) || kv_shared(c, to);
     const unsigned long long fault = ~__ballot(ok && !shared);
     const unsigned long long held = __ballot(from >= 0 && to >= 0) & (fault ? (fault & -fault) - 1 : ~0ULL);
     return held ? 64 - __clzll(held) : 0;

@@ -36,12 +36,9 @@ KV_FN int kv_page(const KvView &c, int s, int t) {
     const int p = c.table[(size_t)s * c.table_pages + (t >> c.shift)];
     return (unsigned)p < (unsigned)c.pages ? p : -1;
 }
-// The page of position t if its tokens may be written: one that no other table entry
-// holds, as far as the cache says (refs may be NULL).
-KV_FN int kv_own_page(const KvView &c, int s, int t) {
-    const int p = kv_page(c, s, t);
-    return p >= 0 && c.refs && c.refs[p] > 1 ? -1 : p;
-}
+// Whether tokens of a page (or -1) belong to more than one table entry, as far as the
+// cache says (refs may be NULL): then they may not be written.
+KV_FN bool kv_shared(const KvView &c, int page) { return page >= 0 && c.refs && c.refs[page] > 1; }
 // Element offset of token `slot` (0..page_tokens-1) of a page.
 KV_FN size_t kv_at(const KvView &c, int layer, int page, int head, int slot) {
     return ((((size_t)layer * c.pages + page) * c.heads + head) << c.shift | (unsigned)slot) * c.dim;

@@ -61,7 +61,7 @@ __global__ __launch_bounds__(256) void qk_rope_kernel(RopeArgs A, KvView c, Batc
         if (b.parent) depth = __popcll(__shfl(tree_ancestors(b.parent + first, n, lane), place)) - 1;
         const int len = kv_length(c, s);
         pos = len + depth;
-        page = kv_own_page(c, s, len + place);
+        page = kv_page(c, s, len + place);
         slot = (len + place) & ((1 << c.shift) - 1);
     }
     if (A.position) pos = A.position[row];
@@ -77,6 +77,7 @@ __global__ __launch_bounds__(256) void qk_rope_kernel(RopeArgs A, KvView c, Batc
             turn_of((double)pos * A.freq[f + i], sn[i], cs[i]);
         }
     }
+    if (A.cached && kv_shared(c, page)) page = -1;  // behind the angles, which do not wait for it
     const int other = (lane + (low ? half / 4 : -(half / 4))) & 63;
 #pragma unroll
     for (int u = 0; u < U; u++) {

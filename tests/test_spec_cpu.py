@@ -230,22 +230,22 @@ def test_index_arithmetic_stays_inside(index):
 
 OWN = r"""
 #include "qg_kv_index.h"
-extern "C" int own(const int *table, int *refs, int pages, int t) {
+extern "C" int shared(const int *table, int *refs, int pages, int t) {
     KvView c{};
     c.table = (int *)table; c.refs = refs; c.pages = pages; c.shift = 3; c.sequences = 1; c.table_pages = 4;
-    return kv_own_page(c, 0, t);
+    return kv_shared(c, kv_page(c, 0, t));
 }
 """
 
 
 def test_pages_that_may_be_written(tmp_path):
-    """A page that another table entry holds is not a sequence's own; without counts every held page is."""
+    """A page that another table entry holds too is shared; without counts none is, and no page is none."""
     (tmp_path / "h.cpp").write_text(OWN)
     subprocess.run(["g++", "-O1", "-shared", "-fPIC", f"-I{ROOT / 'nebula_amd' / 'csrc'}", str(tmp_path / "h.cpp"), "-o", str(tmp_path / "h.so")], check=True)
-    own = C.CDLL(str(tmp_path / "h.so")).own
+    shared = C.CDLL(str(tmp_path / "h.so")).shared
     table, refs = (C.c_int * 4)(2, 0, -1, 7), (C.c_int * 3)(2, 0, 1)
-    assert [own(table, refs, 3, t) for t in (0, 7, 8, 16, 24, 32, -1)] == [2, 2, -1, -1, -1, -1, -1]
-    assert [own(table, None, 3, t) for t in (0, 7, 8, 16, 24, 32, -1)] == [2, 2, 0, -1, -1, -1, -1]
+    assert [shared(table, refs, 3, t) for t in (0, 7, 8, 16, 24, 32, -1)] == [0, 0, 1, 0, 0, 0, 0]
+    assert [shared(table, None, 3, t) for t in (0, 7, 8, 16, 24, 32, -1)] == [0] * 7
 
 
 def test_refused_temperatures(lib):
