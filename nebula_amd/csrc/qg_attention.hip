@@ -18,12 +18,12 @@
 // between lanes.
 //
 // What bounds it (MI355X, fp16 cache, 16 heads over 2, 128 dimensions).  Up to 48 rows
-// of a head (one row group): memory, 16 sequences x 98304 keys 289 us with 2 rows
-// and 303 with 6, 5.3 to 5.6 TB/s.  More row groups share the reads in the L2 but each
-// adds its products and softmax: 451 us with 12 rows, 617 with 17 (the matrix cores
-// busy for a third of the time, the rest a wave's latencies with two waves per SIMD).
-// One sequence of 24576 keys, 17 rows: 31 us, of which 13 before the first product
-// and after the last.
+// of a head (one row group): memory, 16 sequences x 98304 keys 282 us with 1 row of each,
+// 286 with 2 and 291 with 6, 5.6 to 5.7 TB/s (a large read reaches 6.1).  More row groups
+// share the reads in the L2 but each adds its products and softmax: 431 us with 12 rows,
+// 621 with 17 (the matrix cores busy for a third of the time, the rest a wave's latencies
+// with two waves per SIMD).  One sequence of 24576 keys, 17 rows (bf16): 34 us and 5 for the
+// join, of which 13 before the first product and after the last.
 //
 // Precision: q and p enter as planes that the 16-bit cores multiply exactly with
 // the cache's values: two fp16 planes (22 bits; q scaled by a power of two per
@@ -847,7 +847,7 @@ void launch_dim(int rt, const AttnArgs &A, const KvView &c, const BatchView &b, 
 }
 
 // Workgroups that run at once: a wave per SIMD each, so what the registers allow
-// (in 64-dimension row tiles: 1 takes 104 registers, 2 up to 154, 6 up to 256).
+// (in 64-dimension row tiles: 1 takes up to 110 registers, 2 up to 160, 6 up to 256).
 int resident(int dim, int rt) {
     const int w = dim / 64 * rt;
     return qg_cu_count() * (w == 1 ? 4 : w == 2 ? 3 : w <= 6 ? 2 : 1);

@@ -282,7 +282,7 @@ QG_DEV void copy_page(const KvView &c, int dst, int src, int layer, bool v, int 
     uint4 *to = (uint4 *)(base + dst * bytes);
     for (size_t i = (size_t)part * 256 + threadIdx.x; i < bytes / 16; i += (size_t)parts * 256) to[i] = from[i];
 }
-// The copies that reserve listed: 56 pages of 1 MB over 8 layers in 11 us (117 MB read
+// The copies that reserve listed: 56 pages of 1 MB over 8 layers in 11 to 13 us (117 MB read
 // and written; forks of one page read it from the caches).
 __global__ __launch_bounds__(256) void kv_cow_kernel(KvView c, const int *ws, int parts) {
     const int per = 2 * c.layers * parts;  // of one page: layers, k and v, parts
@@ -304,7 +304,7 @@ __global__ __launch_bounds__(256) void kv_copy_pages_kernel(KvView c, const int 
 // owns one 16-byte column of one head, layer and side and carries it through
 // all moves, so no two threads meet; a path ascends, so row i never lands
 // where a later one starts, and eight rows may be read before the first is written.
-// Moves are few: 16 sequences x 48 layers take 4.2 us, a launch and three reads.
+// Moves are few: 16 sequences x 48 layers take 4.8 us, a launch and four reads.
 // new_length NULL: written by kv_length_kernel, where the workgroups of a
 // sequence read the lengths that it replaces.
 // The rows of a sequence's path that are followed; lane i's row p, and the pages that it

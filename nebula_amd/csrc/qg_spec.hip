@@ -31,8 +31,8 @@ QG_DEV void turn_of(double angle, float &s, float &c) {
 
 // A wave takes U heads-per-wave of one row: the row's place, its angles' sines and
 // the loads of all its heads once.  Bound by memory where rows are many (8192 rows
-// of 16 + 2 + 2 heads of 128: 35 us, 4.6 TB/s; with one head per wave 59), by the
-// launch and two dependent reads where they are few (one row 3.6 us).
+// of 16 + 2 + 2 heads of 128: 35 us, 4.5 TB/s; with one head per wave 59), by the
+// launch and three dependent reads where they are few (one row 3.7 us).
 template <int D, int U>
 __global__ __launch_bounds__(256) void qk_rope_kernel(RopeArgs A, KvView c, BatchView b, int layer, int parts) {
     constexpr int LPH = D / 4, HPW = 64 / LPH;  // lanes per head, heads per wave
@@ -280,7 +280,7 @@ __global__ __launch_bounds__(THREADS) void softmax_row_kernel(float *out, const 
 
 // Few rows: pieces of SM_PIECE values, a workgroup each; first every piece's
 // largest value, its index and the sum, then every piece's outputs from the row's
-// (the second read is served by the caches).  17 x 151936: 3.6 + 5.0 us for 4.3 us of
+// (the second read is served by the caches).  17 x 151936: 3.7 + 6.1 us for 4.3 us of
 // memory traffic, each kernel a launch and two or three dependent reads.
 constexpr int SM_THREADS = 256, SM_REGS = 16, SM_PIECE = SM_THREADS * SM_REGS;
 struct SoftPart { float m, sum; int at, pad; };
