@@ -233,8 +233,8 @@ typedef struct {
  * be NULL).  With a cache, k (normed, rotated) and v are rounded to its type
  * and stored at their positions of `layer`; a row whose position has no page,
  * or one that another table entry holds too (where the cache has refs; see
- * qg_kv_reserve), is not stored.  Without a cache, batch is NULL, v is ignored and position is
- * needed where rope_dims > 0.  Angles are formed in 64 bits.  An output may be its own
+ * qg_kv_reserve), is not stored.  Without a cache, batch is NULL, v is ignored and
+ * position is needed where rope_dims > 0.  Angles are formed in 64 bits.  An output may be its own
  * input where both have the same layout; otherwise they must not overlap.
  * Rows of no sequence are left as they were. */
 int qg_qk_norm_rope(float *q_out, float *k_out, const qg_qk_rows *in, const qg_kv_cache *cache, int layer,
@@ -246,11 +246,12 @@ int qg_qk_norm_rope(float *q_out, float *k_out, const qg_qk_rows *in, const qg_k
  * of kv_heads up to 128 times as many, both 16-byte aligned; no overlap.
  * Scores, statistics and sums are held in fp32; the products run on the matrix
  * cores with queries and probabilities in planes of the cache's type that
- * together carry at least 22 bits (over an F16 cache no less than 2^-38 of a row's
- * largest probability, or of its largest query value).  A row that sees no token (or none with a
+ * together carry at least 22 bits, over an F16 cache down to 2^-38 of a row's
+ * largest probability or query value.  A row that sees no token (or none with a
  * score above -infinity) is 0, one with a NaN or a score of +infinity is NaN.
  * Rows that see infinities, or values whose sum passes fp32's range, are computed
- * key by key, which is slow (18 ms over 98304 tokens).  Rows of no sequence are left as they were.
+ * key by key, which is slow (18 ms over 98304 tokens).  Rows of no sequence are
+ * left as they were.
  * rows x q_heads at most 2^25.  The workspace of a batch serves every batch of
  * no more rows. */
 size_t qg_tree_attention_workspace_bytes(const qg_kv_cache *cache, const qg_kv_batch *batch, int q_heads);
@@ -258,8 +259,9 @@ int qg_tree_attention(float *out, const float *q, int q_heads, float scale, cons
                       const qg_kv_batch *batch, void *workspace, size_t workspace_bytes);
 
 /* out = softmax(x / temperature) of each row of [rows][cols]; out may be x.
- * temperature 0: 1 at the lowest index of the largest value; others from 2^-126 on.  -infinity gives
- * 0; a row of nothing but -infinity is 0; a row with NaN or +infinity is NaN.
+ * temperature 0: 1 at the lowest index of the largest value; others from 2^-126
+ * on.  -infinity gives 0; a row of nothing but -infinity is 0; a row with NaN or
+ * +infinity is NaN.
  * rows 1..65536, cols 1..2^24, at most 2^35 values; 4-byte aligned.  The
  * workspace of a number of rows serves fewer of them too. */
 size_t qg_softmax_workspace_bytes(int rows, int cols);
@@ -291,8 +293,8 @@ int qg_verify_drafts(int *tokens_out, int *path, int *count, const float *p, con
 
 /* Pages.  Calls that change tables take one stream at a time; each result is
  * the same on every run.  The arrays given overlap neither each other nor the
- * cache's where one of them is written, but for lengths as said.  qg_kv_workspace_bytes serves fork (of up to
- * `sequences` pairs) and reserve. */
+ * cache's where one of them is written, but for lengths as said.
+ * qg_kv_workspace_bytes serves fork (of up to `sequences` pairs) and reserve. */
 size_t qg_kv_workspace_bytes(const qg_kv_cache *cache);
 /* Room for the batch's rows behind each sequence's tokens: pages are taken in
  * ascending order, for the sequences in order.  A held page that would be
@@ -317,7 +319,8 @@ int qg_kv_fork(const qg_kv_cache *cache, const int *dst, const int *src, int n, 
 int qg_kv_truncate(const qg_kv_cache *cache, const int *new_length);
 /* The accepted rows (qg_verify_drafts' path and count) move to the front: the
  * token at length[s] + path[s][i] goes to length[s] + i, in every layer, and
- * new_length[s] = length[s] + count[s], or the rows followed if fewer (new_length may be the cache's length).
+ * new_length[s] = length[s] + count[s], or the rows followed if fewer (new_length
+ * may be the cache's length).
  * max_rows is at most 64, for chains too: a longer prompt chunk, all of whose
  * rows stay where they are, is taken by adding its rows to `length`.
  * A path is followed while it ascends inside its sequence's rows, and up to the

@@ -634,7 +634,7 @@ __global__ __launch_bounds__(64 * NW, (D / 64) * RT <= 6 ? 2 : 1) void attention
 // One row and head, key by key: a lane scores one of 64 keys at a time, the
 // output's dimensions lie across the lanes.  The weights' sum first, so that the values
 // are taken by weights that sum to 1: nothing overflows that the output holds.  A NaN in
-// the query or in that sum is the row's.  A wave's latencies bound it: 128 rows and heads
+// the query or in that sum is the row's.  A wave's latencies bound it: a sequence's rows
 // over 98304 keys 18 ms with 16 bytes of a key and eight values on their way at once, 42
 // with one; NaN queries cost nothing.
 template <int TYPE, int D>
