@@ -374,3 +374,74 @@ def test_lengths_stop_where_no_row_was_stored(qgl, page):
         call("kv_compact", c.ref, batch.ref, dp.p, dc.p, c.dlength.p)
         c.length = want
         same(c)
+
+
+class Careful(Model):
+    """The rules for steps that run on whatever reserve said."""
+
+    def shared(self, p):
+        return p >= 0 and self.c.refs[p] > 1
+
+    def store(self, batch, k, v):
+        c = self.c
+        for row, s, place in batch.places():
+            t = int(c.length[s]) + place
+            if not self.shared(c.page_of(s, t)):
+                c.put(0, s, t, k[row], v[row])
+
+    def compact(self, batch, path, count):
+        c, new = self.c, c_length(self.c)
+        for s in range(c.B):
+            n, L = int(batch.start[s + 1] - batch.start[s]), int(c.length[s])
+            before, rows = -1, []
+            for i in range(min(max(int(count[s]), 0), n)):
+                p = int(path[s, i])
+                a, b = c.page_of(s, L + p), c.page_of(s, L + i)
+                if not before < p < n or self.shared(a) or self.shared(b):
+                    break
+                before = p
+                rows.append((p, a, b))
+            while rows and (rows[-1][1] < 0 or rows[-1][2] < 0):
+                rows.pop()
+            for i, (p, a, b) in enumerate(rows):
+                if p != i and a >= 0 and b >= 0:
+                    for pool in (c.k, c.v):
+                        pool[:, b, :, (L + i) % c.P] = pool[:, a, :, (L + p) % c.P]
+            new[s] += len(rows)
+        return new
+
+
+@pytest.mark.parametrize("typ,page,heads,seed", [(F16, 8, 1, 1), (BF16, 16, 2, 2), (F32, 8, 2, 3), (F16, 32, 1, 4)])
+def test_steps_that_run_on_without_room(qgl, typ, page, heads, seed):
+    """Steps of forked sequences over few pages, every call of each step made whatever reserve's status: tables, holders,
+    lengths and every byte of the pages."""
+    rng = np.random.default_rng(seed)
+    B = 5
+    c = Cache(rng, [3 * page // 2, 0, 0, page - 1, 2 * page], [0] * B, typ=typ, layers=2, kv_heads=heads, page=page, dim=64, spare=2, table_pages=4)
+    m, seen = Careful(c), np.zeros(3, int)
+    for step in range(30):
+        if rng.random() < 0.5:
+            dst, src = rng.integers(0, B, 2).tolist(), rng.integers(0, B, 2).tolist()
+            fork(c, dst, src)
+            m.fork(dst, src)
+        if rng.random() < 0.4:
+            new = rng.integers(0, 3 * page, B).tolist()
+            truncate(c, new)
+            m.truncate(new)
+        counts = rng.integers(0, 9, B).tolist()
+        counts[int(rng.integers(0, B))] += 1
+        status = m.reserve(counts)
+        np.testing.assert_array_equal(reserve(c, counts), status)
+        seen += np.bincount(status, minlength=3)
+        batch = Batch(counts)
+        m.store(batch, *store_rows(c, batch, rng))
+        path, count = np.full((B, batch.max_rows), -1, np.int32), np.zeros(B, np.int32)
+        for s, n in enumerate(counts):
+            count[s] = rng.integers(0, n + 1)
+            path[s, :count[s]] = np.sort(rng.choice(n, count[s], replace=False)) if n else []
+        dp, dc = Device(path), Device(count)
+        say("compact", count.tolist(), "status", status.tolist())
+        call("kv_compact", c.ref, batch.ref, dp.p, dc.p, c.dlength.p)
+        c.length = m.compact(batch, path, count)
+        same(c)
+    assert (seen[:2] > 3).all(), seen
