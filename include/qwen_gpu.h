@@ -291,6 +291,39 @@ int qg_verify_drafts(int *tokens_out, int *path, int *count, const float *p, con
                      const float *u, const float *u_last, int cols, int sequences, const qg_kv_batch *batch,
                      void *workspace, size_t workspace_bytes);
 
+/* Truncated distributions.  What each row's request asks for: device arrays
+ * [rows], or NULL for all rows without.  Of the weights w_i = exp((x_i - max) /
+ * temperature) stay: with top_k > 0 the top_k largest values; of these, with
+ * top_p < 1, in falling order those before which less than top_p of their sum
+ * lies; of these, with min_p > 0, those of at least min_p times the largest.  Of
+ * equal values the lower index counts as larger (0 and -0 are equal); the
+ * largest always stays.  temperature 0, and one that is not at least 2^-126,
+ * is the first largest token alone; top_k <= 0 or >= cols, a top_p that is not
+ * below 1 and a min_p that is not above 0 keep all. */
+typedef struct {
+    const float *temperature;   /* NULL: 1 */
+    const int *top_k;
+    const float *top_p, *min_p;
+} qg_sampling;
+
+/* token[rows][draws]: the first i with sum_{j<=i} w_j > u[r][d] sum_j w_j over
+ * what stays of row r of x [rows][cols], u [rows][draws] in [0, 1);
+ * logprob[rows][draws] (or NULL): log(w_i / sum_j w_j).  Weights and sums in 64
+ * bits.  -infinity is never drawn; a row of nothing else, or with NaN or
+ * +infinity, gives -1 and NaN.  draws 1..64 of each row, independent of each
+ * other (drafted siblings, several answers' first tokens).
+ * qg_sampling_softmax: out = w_i / sum_j w_j, 0 where a token does not stay,
+ * what the draws of qg_sample are distributed as: p and q of qg_verify_drafts.
+ * out may be x; a row of nothing but -infinity is 0, one with NaN or +infinity
+ * NaN.  Both: rows 1..65536, cols 1..2^24, at most 2^35 values, 4-byte aligned;
+ * no output or workspace overlaps what else is given.  The workspace of a number
+ * of rows serves fewer of them too. */
+size_t qg_sample_workspace_bytes(int rows, int cols);
+int qg_sample(int *token, float *logprob, const float *x, int rows, int cols, int draws, const qg_sampling *sampling,
+              const float *u, void *workspace, size_t workspace_bytes);
+int qg_sampling_softmax(float *out, const float *x, int rows, int cols, const qg_sampling *sampling, void *workspace,
+                        size_t workspace_bytes);
+
 /* Pages.  Calls that change tables take one stream at a time; each result is
  * the same on every run.  The arrays given overlap neither each other nor the
  * cache's where one of them is written, but for lengths as said.

@@ -47,6 +47,7 @@ SIGNATURES = {
     "verify_drafts": ([P, P, P, P, P, P, P, P, I, I, P, P, Z], I), "kv_workspace_bytes": ([P], Z),
     "kv_reserve": ([P, P, P, P, Z], I), "kv_fork": ([P, P, P, I, P, Z], I), "kv_truncate": ([P, P], I),
     "kv_compact": ([P, P, P, P, P], I), "kv_copy_pages": ([P, P, P, I], I),
+    "sample_workspace_bytes": ([I, I], Z), "sample": ([P, P, P, I, I, I, P, P, P, Z], I), "sampling_softmax": ([P, P, I, I, P, P, Z], I),
 }
 
 # nm_cpu_moe_fn of include/nebula_moe.h: (ctx, out, x, ids, weights, tokens) -> 0 on success
@@ -135,6 +136,11 @@ class QkRows(C.Structure):
     _fields_ = [("q", P), ("k", P), ("v", P)] + [(n, C.c_int64) for n in ("q_row", "q_head", "k_row", "k_head", "v_row", "v_head")] + [
         ("rows", I), ("q_heads", I), ("kv_heads", I), ("head_dim", I), ("q_norm", P), ("k_norm", P), ("eps", F),
         ("rope_dims", I), ("interleaved", I), ("freq", P), ("position", P)]
+
+
+class Sampling(C.Structure):
+    """qg_sampling of include/qwen_gpu.h."""
+    _fields_ = [("temperature", P), ("top_k", P), ("top_p", P), ("min_p", P)]
 
 
 _LIB = None
