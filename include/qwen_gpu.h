@@ -258,6 +258,30 @@ size_t qg_tree_attention_workspace_bytes(const qg_kv_cache *cache, const qg_kv_b
 int qg_tree_attention(float *out, const float *q, int q_heads, float scale, const qg_kv_cache *cache, int layer,
                       const qg_kv_batch *batch, void *workspace, size_t workspace_bytes);
 
+/* Sequences that begin with the same pages (qg_kv_fork), as the attention below
+ * takes them: shared[s] = the most leading tokens, in whole pages, that a
+ * sequence s with rows in the batch has in common with an earlier one that has
+ * rows, link[s] the first such (-1 and 0: none, or s has no rows).  A page
+ * counts where both tables hold the same one and both sequences' cached tokens
+ * fill it.  link, shared [sequences], or NULL.  `prefixes` (16-byte aligned) is
+ * filled for the attention of every layer, up to the next change of the cache's
+ * tables or lengths or of the batch's rows; after one it must not be used (nothing
+ * outside the buffers is then touched, but outputs may be anything).  Outputs
+ * overlap neither each other nor table, length and start. */
+size_t qg_kv_prefixes_bytes(const qg_kv_cache *cache, const qg_kv_batch *batch);
+int qg_kv_prefixes(int *link, int *shared, const qg_kv_cache *cache, const qg_kv_batch *batch, void *prefixes, size_t prefixes_bytes);
+
+/* qg_tree_attention of a batch in which sequences share pages: the same outputs
+ * (within the same error), but a page that several sequences hold is read once
+ * for all of them.  `prefixes` as qg_kv_prefixes filled it for this cache and batch;
+ * other arguments, refusals and special values as there.  The workspace serves
+ * every batch of no more rows over a cache of no more sequences and the same heads
+ * and head_dim. */
+size_t qg_prefix_attention_workspace_bytes(const qg_kv_cache *cache, const qg_kv_batch *batch, int q_heads);
+int qg_prefix_attention(float *out, const float *q, int q_heads, float scale, const qg_kv_cache *cache, int layer,
+                        const qg_kv_batch *batch, const void *prefixes, size_t prefixes_bytes, void *workspace,
+                        size_t workspace_bytes);
+
 /* out = softmax(x / temperature) of each row of [rows][cols]; out may be x.
  * temperature 0: 1 at the lowest index of the largest value; others from 2^-126
  * on.  -infinity gives 0; a row of nothing but -infinity is 0; a row with NaN or

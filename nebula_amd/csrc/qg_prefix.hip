@@ -1,0 +1,757 @@
+// Attention of a batch whose sequences begin with the same pages
+// (qg_kv_prefixes, qg_prefix_attention of include/qwen_gpu.h).
+//
+// Forked sequences hold one page of a common prompt in several tables.  Each
+// sequence hangs on the earlier one that it has the most leading pages in common
+// with, which makes a tree of sequences, and the places where sequences leave one
+// another cut their tokens into segments: a run of keys that the same sequences
+// see.  A segment's rows, of all its sequences, share one read of its keys; what
+// a row sees is the segments on its way to the root, whose partial results are
+// joined as the parts of one sequence are (o = sum p v, l = sum p, m = max per part).
+// In the order in which the tree is walked, longest common part first, a segment's
+// sequences lie next to each other, so that its rows are a range.
+#include "qg_attention.h"
+#include "qg_prefix_index.h"
+
+namespace {
+
+// ------------------------------------------------------------------------
+// Which sequences begin with the same pages: a wave per sequence.
+// ------------------------------------------------------------------------
+QG_DEV int whole_pages(const KvView &c, int s) { return kv_length(c, s) >> c.shift; }
+QG_DEV int table_page(const KvView &c, int s, int j) {
+    const int p = c.table[(size_t)s * c.table_pages + j];
+    return (unsigned)p < (unsigned)c.pages ? p : -1;
+}
+// Leading pages that sequences s and t have in common, of `most`.
+QG_DEV int common_pages(const KvView &c, int s, int t, int most, int lane) {
+    for (int j0 = 0; j0 < most; j0 += 256) {
+        bool same[4];
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const int j = j0 + 64 * k + lane;
+            const int a = j < most ? table_page(c, s, j) : -1, b = j < most ? table_page(c, t, j) : -1;
+            same[k] = a >= 0 && a == b;
+        }
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const unsigned long long not_same = __ballot(!same[k]);
+            if (not_same) return j0 + 64 * k + __builtin_ctzll(not_same);
+        }
+    }
+    return most;
+}
+__global__ __launch_bounds__(256) void prefix_link_kernel(KvView c, BatchView b, PrefixView v, int *link, int *shared) {
+    const int lane = threadIdx.x & 63, s = blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (s >= c.sequences) return;
+    int first, n, best = 0, with = -1;
+    batch_rows(b, s, first, n);
+    const int whole = whole_pages(c, s);
+    // an earlier sequence has more in common than the best so far only if its page there is the same
+    for (int t0 = 0; n > 0 && t0 < s && best < whole;) {
+        const int t = t0 + lane;
+        bool may = false;
+        if (t < s) {
+            int f, m;
+            batch_rows(b, t, f, m);
+            const int p = table_page(c, s, best);
+            may = m > 0 && whole_pages(c, t) > best && p >= 0 && table_page(c, t, best) == p;
+        }
+        const unsigned long long all = __ballot(may);
+        if (!all) { t0 += 64; continue; }
+        const int u = t0 + __builtin_ctzll(all), x = common_pages(c, s, u, min(whole, whole_pages(c, u)), lane);
+        if (x > best) { best = x; with = u; }
+        t0 = u + 1;
+    }
+    if (lane == 0) {
+        const int tokens = best << c.shift;
+        v.link[s] = with;
+        v.shared[s] = tokens;
+        if (link) link[s] = with;
+        if (shared) shared[s] = tokens;
+    }
+}
+
+// ------------------------------------------------------------------------
+// Segments, by one workgroup, a thread per sequence.
+// ------------------------------------------------------------------------
+// Common parts count in steps of a quantum: shorter segments would cost more than
+// they save.  It is doubled until the rows of all shared segments together are few
+// enough for the partial results that a workspace holds.
+constexpr int QUANTUM = 256;
+__host__ __device__ inline long shared_rows_most(long rows) {
+    const long most = 16 * rows < 16384 ? 16 * rows : 16384;
+    return most > 3 * rows ? most : 3 * rows;
+}
+constexpr int PLAN_THREADS = QG_MAX_SEQUENCES;
+__global__ __launch_bounds__(PLAN_THREADS) void prefix_plan_kernel(KvView c, BatchView b, PrefixView v) {
+    __shared__ int s_link[PLAN_THREADS], s_cut[PLAN_THREADS], s_n[PLAN_THREADS], s_size[PLAN_THREADS], s_off[PLAN_THREADS], s_top[PLAN_THREADS],
+        s_id[PLAN_THREADS], s_same[PLAN_THREADS], s_wave[PLAN_THREADS / 64 + 1];
+    __shared__ unsigned long long s_sum;
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6, S = c.sequences;
+    int first = 0, n = 0, len = 0, link0 = -1, shared0 = 0;
+    if (t < S) {
+        batch_rows(b, t, first, n);
+        len = kv_length(c, t);
+        if (n > 0) { link0 = v.link[t]; shared0 = v.shared[t]; }
+    }
+    s_n[t] = n;
+    int link = -1, cut = 0, off = 0, rep = t, below = -1, below_rep = -1, sees = 0;
+    for (int quantum = QUANTUM > 1 << c.shift ? QUANTUM : 1 << c.shift;; quantum *= 2) {
+        // the nearest on the way up that has less in common with the one above it
+        cut = shared0 / quantum * quantum;
+        s_link[t] = link0;
+        s_cut[t] = cut;
+        s_size[t] = 0;
+        s_top[t] = 0;
+        if (t == 0) s_sum = 0;
+        __syncthreads();
+        link = cut ? link0 : -1;
+        while (link >= 0 && s_cut[link] >= cut) link = s_link[link];
+        if (link < 0) cut = 0;
+        __syncthreads();
+        s_link[t] = link;
+        s_cut[t] = cut;
+        __syncthreads();
+        // rows of a sequence and those that hang on it
+        if (n > 0) {
+            int total = 0;
+            for (int u = t; u >= 0 && total < S; u = s_link[u], total++) atomicAdd(&s_size[u], n);
+        }
+        __syncthreads();
+        // among those on the same sequence: rows that come before, the first with the same cut, the next lower cut, rows of at least this cut
+        off = sees = 0;
+        rep = t;
+        below = -1;
+        below_rep = -1;
+        if (n > 0)
+            for (int u = 0; u < S; u++) {
+                if (s_link[u] != link || !s_n[u]) continue;
+                const int x = s_cut[u];
+                if (x > cut || (x == cut && u < t)) off += s_size[u];
+                if (x >= cut) sees += s_size[u];
+                if (x == cut && u < rep) rep = u;
+                if (x < cut && x > below) { below = x; below_rep = u; }
+            }
+        const bool is = n > 0 && link >= 0 && rep == t;
+        if (is) {
+            sees += s_n[link];
+            atomicAdd(&s_sum, (unsigned long long)sees);
+        }
+        if (n > 0 && link >= 0) atomicMax(&s_top[link], cut);
+        __syncthreads();
+        if ((long)s_sum <= shared_rows_most(b.rows)) break;
+        __syncthreads();
+    }
+    // first rows in walking order
+    s_off[t] = off;
+    s_same[t] = rep;
+    __syncthreads();
+    int pos = off;
+    for (int u = link, steps = 0; u >= 0 && steps < S; u = s_link[u], steps++) pos += s_n[u] + s_off[u];
+    // the segments' numbers: shared ones and tails in one order
+    const bool shares = n > 0 && link >= 0 && rep == t;
+    const unsigned long long tails = __ballot(n > 0), heads = __ballot(shares);
+    if (lane == 0) s_wave[wave] = __popcll(tails) + __popcll(heads);
+    __syncthreads();
+    if (t == 0) {
+        int sum = 0;
+        for (int w = 0; w <= PLAN_THREADS / 64; w++) {
+            const int x = w < PLAN_THREADS / 64 ? s_wave[w] : 0;
+            s_wave[w] = sum;
+            sum += x;
+        }
+    }
+    __syncthreads();
+    const unsigned long long before = (1ULL << lane) - 1;
+    const int tail_id = s_wave[wave] + __popcll(tails & before) + __popcll(heads & before), head_id = tail_id + 1;
+    s_id[t] = shares ? head_id : -1;
+    s_size[t] = pos;
+    __syncthreads();
+    if (t == 0) v.head[0] = s_wave[PLAN_THREADS / 64];
+    if (t < S) {
+        v.leaf[t] = n > 0 ? tail_id : -1;
+        v.pos[t] = pos;
+    }
+    auto put = [&](int id, const Segment &x) {
+        int4 *to = (int4 *)(v.segments + (size_t)id * SEG_INTS);
+        to[0] = make_int4(x.owner, x.begin, x.end, x.row0);
+        to[1] = make_int4(x.rows, x.up, x.tail, 0);
+    };
+    // the segment of sequence u's keys that ends where it leaves the one that it hangs on
+    auto above = [&](int u) { return s_link[u] >= 0 ? s_id[s_same[u]] : -1; };
+    if (n > 0) {
+        const int begin = max(s_top[t], cut);
+        int up = above(t);
+        if (s_top[t] > cut) {  // of those that hang here with the largest cut, the first
+            up = -1;
+            for (int u = 0; u < S; u++)
+                if (s_link[u] == t && s_n[u] && s_cut[u] == s_top[t]) { up = s_id[u]; break; }
+        }
+        put(tail_id, Segment{t, begin, len + n, pos, n, up, 1, 0});
+        for (int i = 0; i < n; i++)
+            if (pos + i < b.rows) v.row_of[pos + i] = first + i;
+    }
+    if (shares) {
+        const int base = s_cut[link];
+        const int up = below > base ? s_id[s_same[below_rep]] : above(link);
+        put(head_id, Segment{link, max(below, base), cut, s_size[link], sees, up, 0, 0});
+    }
+}
+
+// ------------------------------------------------------------------------
+// Attention.
+// ------------------------------------------------------------------------
+struct PrefixArgs : AttnRows {
+    float *part_o;    // [tiles][16][D]
+    float2 *part_ml;  // [tiles][16]
+    int4 *joins;      // [2 sequences] SegmentParts
+    int *odd;         // [rows][q_heads]: results that are no numbers, where they are written at once
+    int resident, tiles;
+};
+
+QG_DEV Segment read_segment(const KvView &c, const BatchView &b, const PrefixView &v, int i) {
+    const int4 *p = (const int4 *)(v.segments + (size_t)i * SEG_INTS);
+    const int4 x = p[0], y = p[1];
+    return segment_inside(c, b, Segment{x.x, x.y, x.z, x.w, y.x, y.y, y.z, 0});
+}
+
+// A unit of work: a part of a segment's keys, a head, a group of its rows.
+struct Unit {
+    Segment s;
+    int id, groups, chunk, parts, part, z, h, tile;  // tile: the first of the segment's
+};
+constexpr int CHUNK = 128;  // keys per unit, at least and in steps of
+
+struct UnitLane { int keys, groups, tiles; };
+template <int RS, int RT>
+QG_DEV bool find_unit(const KvView &c, const BatchView &b, const PrefixArgs &A, const PrefixView &v, int lane, int block, Unit &p) {
+    const int count = segment_count(c, v);
+    auto lane_of = [&](int i) {
+        UnitLane x{0, 0, 0};
+        if (i < count) {
+            const Segment s = read_segment(c, b, v, i);
+            const int tiles = s.tail ? RT : RS;
+            if (s.rows && s.end > s.begin) x = UnitLane{s.end - s.begin, (s.rows * A.group + 16 * tiles - 1) / (16 * tiles), tiles};
+        }
+        return x;
+    };
+    const UnitLane mine = lane_of(lane);
+    auto over = [&](auto f) {
+        float r = f(mine);
+        for (int i = lane + 64; i < count; i += 64) r += f(lane_of(i));
+        r = qg_row_sum(r);
+        float x = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 64; i += 16) x += __int_as_float(__builtin_amdgcn_readlane(__float_as_int(r), i));
+        return x * (float)c.heads;
+    };
+    // one round of resident workgroups, two where the row groups alone come to half a round
+    const float least = over([](const UnitLane &x) { return (float)x.groups; });
+    const float room = (2.0f * least <= (float)A.resident ? 1.0f : 2.0f) * (float)A.resident;
+    // 1.0001: above the sum whatever its roundings, so that the tiles suffice
+    const float even = 1.0001f * over([](const UnitLane &x) { return (float)x.groups * (float)x.keys; }) / room;
+    int chunk = ((int)fminf(even, (float)(1 << 28)) / CHUNK + 1) * CHUNK;
+    for (int i = 0; i < 4 && least <= room; i++) {  // the parts round up: longer ones until they fit
+        const float units = over([&](const UnitLane &x) { return x.groups ? (float)(((x.keys - 1) / chunk + 1) * x.groups) : 0.0f; });
+        if (units <= room) break;
+        chunk = max((int)fminf((float)chunk * units / room, (float)(1 << 28)) / CHUNK, chunk / CHUNK) * CHUNK + CHUNK;
+    }
+    auto scan = [&](int i0, UnitLane &x, int &parts, int &upto, int &upto_tiles) {
+        x = i0 ? lane_of(i0 + lane) : mine;
+        parts = x.groups ? (x.keys - 1) / chunk + 1 : 0;
+        upto = parts * x.groups * c.heads;
+        upto_tiles = upto * x.tiles;
+#pragma unroll
+        for (int d = 1; d < 64; d *= 2) {
+            const int u = __shfl_up(upto, d), e = __shfl_up(upto_tiles, d);
+            if (lane >= d) { upto += u; upto_tiles += e; }
+        }
+    };
+    UnitLane x;
+    int parts, upto, upto_tiles, units = 0;
+    for (int i0 = 0; i0 < count; i0 += 64) {
+        scan(i0, x, parts, upto, upto_tiles);
+        units += __builtin_amdgcn_readlane(upto, 63);
+    }
+    if (units <= 0) return false;
+    // an eighth of the units to each XCD: row groups with the same keys meet in its L2
+    const int run = (units + 7) / 8, unit = (block & 7) * run + (block >> 3);
+    if (unit >= units || (block >> 3) >= run) return false;
+    int before = 0, tiles = 0;
+    for (int i0 = 0; i0 < count; i0 += 64) {
+        if (count > 64) scan(i0, x, parts, upto, upto_tiles);
+        const int own = parts * x.groups * c.heads;
+        const unsigned long long here = __ballot(unit < before + upto && unit >= before + upto - own);
+        if (here) {
+            const int l = __builtin_ctzll(here);
+            p.id = i0 + l;
+            p.s = read_segment(c, b, v, p.id);
+            p.groups = __builtin_amdgcn_readlane(x.groups, l);
+            p.parts = __builtin_amdgcn_readlane(parts, l);
+            p.tile = tiles + __builtin_amdgcn_readlane(upto_tiles - own * x.tiles, l);
+            const int rest = unit - (before + __builtin_amdgcn_readlane(upto - own, l));
+            if (rest < 0 || rest >= __builtin_amdgcn_readlane(own, l)) return false;  // row starts that overlap, past 2^31 units
+            p.part = rest / (p.groups * c.heads);
+            p.h = rest / p.groups % c.heads;
+            p.z = rest % p.groups;
+            p.chunk = chunk;
+            return true;
+        }
+        before += __builtin_amdgcn_readlane(upto, 63);
+        tiles += __builtin_amdgcn_readlane(upto_tiles, 63);
+    }
+    return false;
+}
+
+template <int TYPE, int D, int RS, int NW>
+struct PrefixShared {
+    typedef Tile<TYPE, D> T;
+    static constexpr int JOIN = NW * 16 * (D + 4) * 4, Q = RS * T::Q_BYTES;
+    __attribute__((aligned(16))) uint8_t mem[Q > JOIN ? Q : JOIN];
+    float m[NW][16 * RS], l[NW][16 * RS], back[16 * RS];
+    unsigned long long seen[QG_MAX_TREE];
+};
+
+// One unit, as qg_tree_attention takes a part of a sequence: each wave walks tiles of
+// keys of its own, for RT row tiles, and the waves' sums are joined in shared memory.
+template <int TYPE, int D, int RT, bool TAIL, int NW, typename SHARED>
+QG_DEV void unit_attention(const PrefixArgs &A, const KvView &c, const BatchView &b, const PrefixView &v, const Unit &p, SHARED &s) {
+    typedef Tile<TYPE, D> T;
+    constexpr int RG = 16 * RT, E = T::E, DL = T::DL, KEYS = T::KEYS;
+    constexpr bool FIRST = D > 64;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = lane & 15, g = lane >> 4;
+    const int row0 = p.z * RG, rows = p.s.rows * A.group, owner = p.s.owner;
+    int first = 0, count = 0, len = p.s.end;
+    if (TAIL) {
+        batch_rows(b, owner, first, count);
+        len = kv_length(c, owner);
+    }
+    // the unit's keys, and the first one that some row may not see
+    const int begin = p.s.begin + p.part * p.chunk;
+    int keys = p.s.end, open = p.s.end;
+    if (TAIL) {
+        if (!b.parent) keys = min(keys, len + by_group(A, min(row0 + RG, rows) - 1) + 1);
+        open = len + (b.parent ? 0 : by_group(A, row0) + 1);
+    }
+    const int end = min(begin + p.chunk, keys);
+    const bool direct = TAIL && p.parts == 1 && p.s.begin == 0;
+    const int tile0 = p.tile + ((p.part * c.heads + p.h) * p.groups + p.z) * RT;
+    const bool fits = tile0 >= 0 && tile0 + RT <= A.tiles;
+    if (tid == 0 && p.part == 0 && p.h == 0 && p.z == 0) A.joins[p.id] = make_int4(p.tile, p.parts, p.groups, RT);
+    if (begin >= end) {  // rows that come before the sequence's last keys
+        if (fits && tid < RG) A.part_ml[(size_t)tile0 * 16 + tid] = make_float2(-__builtin_inff(), 0.0f);
+        return;
+    }
+    float x[RG / (4 * NW)][DL];
+    size_t at_q[RG / (4 * NW)];  // the row and head, or -1
+#pragma unroll
+    for (int i = 0; i < RG / (4 * NW); i++) {
+        const int at = row0 + (i * NW + wave) * 4 + g, t = by_group(A, at);
+        int row = -1;
+        if (at < rows) row = TAIL ? (t < count ? first + t : -1) : kv_clamp(v.row_of[p.s.row0 + t], 0, b.rows - 1);
+        at_q[i] = row >= 0 ? (size_t)row * A.q_heads + p.h * A.group + (at - t * A.group) : (size_t)-1;
+#pragma unroll
+        for (int d = 0; d < DL; d += 4) {
+            const float4 y = row >= 0 ? *(const float4 *)(A.q + at_q[i] * D + n * DL + d) : make_float4(0, 0, 0, 0);
+            x[i][d] = y.x; x[i][d + 1] = y.y; x[i][d + 2] = y.z; x[i][d + 3] = y.w;
+        }
+    }
+    const size_t page_bytes = ((size_t)c.heads << c.shift) * D * T::ES;
+    const uint8_t *kbase = c.k + (((size_t)A.layer * c.pages * c.heads + p.h) << c.shift) * D * T::ES;
+    const uint8_t *vbase = c.v + (((size_t)A.layer * c.pages * c.heads + p.h) << c.shift) * D * T::ES;
+    const int slot_mask = (1 << c.shift) - 1;
+    // a run of E keys from position pos, aligned to E: inside one page
+    auto run = [&](const uint8_t *base, int page, int pos) { return base + (size_t)max(page, 0) * page_bytes + (size_t)((pos & slot_mask) * (D * T::ES)); };
+    T tile;
+    int t0 = begin + wave * KEYS, kpos = t0 + E * (n >> 2), vpos = t0 + E * g;
+    int kpage = kv_page(c, owner, kpos), vpage = kv_page(c, owner, vpos);
+    int kpage1 = kv_page(c, owner, kpos + NW * KEYS), vpage1 = kv_page(c, owner, vpos + NW * KEYS);
+    if (t0 < end) {
+        tile.load_k(run(kbase, kpage, kpos), n, g);
+        tile.load_v(run(vbase, vpage, vpos), n);
+    }
+#pragma unroll
+    for (int i = 0; i < RG / (4 * NW); i++) {
+        const int r = (i * NW + wave) * 4 + g;
+#pragma unroll
+        for (int d = 0; d < DL; d++) x[i][d] *= A.scale;
+        float back = 1.0f;
+        if constexpr (TYPE == QT_F16) {
+            float top = 0.0f;
+#pragma unroll
+            for (int d = 0; d < DL; d++) top = fmaxf(top, fabsf(x[i][d]));
+            top = qg_row_max(top);
+            // 2^e with top 2^e in [2^13, 2^14): fp16's whole precision for what matters of the row
+            const int e = min(max(127 + 13 - (int)(__float_as_uint(top) >> 23), -126), 126);
+            if (top > 0.0f && top < __builtin_inff()) {
+                const float f = __uint_as_float((uint32_t)(e + 127) << 23);
+                back = __uint_as_float((uint32_t)(127 - e) << 23);
+#pragma unroll
+                for (int d = 0; d < DL; d++) x[i][d] *= f;
+            }
+        }
+        if (n == 0) s.back[r] = back;
+        if (n == 0 && TAIL && p.part == 0 && at_q[i] != (size_t)-1) A.odd[at_q[i]] = 0;
+        uint8_t *frag = s.mem + (r >> 4) * T::Q_BYTES;
+#pragma unroll
+        for (int d = 0; d < DL; d += 8) {
+            float y[8];
+#pragma unroll
+            for (int j = 0; j < 8; j++) y[j] = d + j < DL ? x[i][(d + j) % DL] : 0.0f;
+            T::put_q(frag, r & 15, n * DL + d, y, DL - d);
+        }
+    }
+    if (TAIL && b.parent && wave == 0) s.seen[lane] = tree_ancestors(b.parent + first, count, lane);
+    __syncthreads();
+
+    qg_f4 o[RT][DL];
+    float m[RT], l[RT], back[RT];
+#pragma unroll
+    for (int r = 0; r < RT; r++) {
+        back[r] = TYPE == QT_F16 ? s.back[16 * r + n] : 1.0f;
+        m[r] = -__builtin_inff();
+        l[r] = 0.0f;
+#pragma unroll
+        for (int t = 0; t < DL; t++) o[r][t] = qg_f4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+    for (; t0 < end; t0 += NW * KEYS) {
+        float z[RT][E];
+        if (FIRST) __builtin_amdgcn_s_setprio(1);
+        tile.template scores<RT>(s.mem, lane, z);
+        if (FIRST) __builtin_amdgcn_s_setprio(0);
+        // the next tile's keys, whose pages are known, and the pages of the one after it
+        const int here = vpage, here_pos = vpos;
+        const bool more = t0 + NW * KEYS < end;
+        kpos += NW * KEYS;
+        vpos += NW * KEYS;
+        vpage = vpage1;
+        if (more) {
+            tile.load_k(run(kbase, kpage1, kpos), n, g);
+            kpage1 = kv_page(c, owner, kpos + NW * KEYS);
+            vpage1 = kv_page(c, owner, vpos + NW * KEYS);
+        }
+        if (t0 + KEYS > open || !__all(here >= 0)) {
+#pragma unroll
+            for (int e = 0; e < E; e++)
+                if (here < 0 || here_pos + e >= end) tile.drop_v(e);
+#pragma unroll
+            for (int r = 0; r < RT; r++) {
+                // bit e: key here_pos + e, below the row's prefix or among the rows that it descends from
+                unsigned seen = first_bits(end - here_pos, E);
+                if (TAIL) {
+                    const int t = by_group(A, row0 + 16 * r + n), prefix = b.parent ? len : len + t + 1, k = here_pos - len;
+                    unsigned mine = first_bits(prefix - here_pos, E);
+                    if (b.parent && t < count && k < 64 && k > -E) mine |= (unsigned)(k < 0 ? s.seen[t] << -k : s.seen[t] >> k);
+                    seen &= mine;
+                }
+                if (here < 0) seen = 0;
+#pragma unroll
+                for (int e = 0; e < E; e++) z[r][e] = seen >> e & 1 ? z[r][e] : -__builtin_inff();
+            }
+        }
+        // scores to weights: the maximum is renewed only where it moves by more than the lag
+#pragma unroll
+        for (int r = 0; r < RT; r++) {
+            float top = z[r][0];
+#pragma unroll
+            for (int e = 1; e < E; e++) top = fmaxf(top, z[r][e]);
+            top *= back[r];
+            if (__any(top > m[r] + m_lag(TYPE))) {
+                top = fmaxf(top, __shfl_xor(top, 16));
+                top = fmaxf(top, __shfl_xor(top, 32));
+                const float next = fmaxf(m[r], top);
+                const float a = next == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f(m[r] - next);
+                m[r] = next;
+                l[r] *= a;
+#pragma unroll
+                for (int t = 0; t < DL; t++) o[r][t] *= a;
+            }
+            const float base = m[r] == -__builtin_inff() ? 0.0f : m[r] - p_base(TYPE);
+#pragma unroll
+            for (int e = 0; e < E; e++) {
+                z[r][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(z[r][e], back[r], -base));
+                l[r] += z[r][e];
+            }
+        }
+        if (FIRST) __builtin_amdgcn_s_setprio(1);
+        tile.template outputs<RT>(z, o);
+        if (FIRST) __builtin_amdgcn_s_setprio(0);
+        if (more) tile.load_v(run(vbase, vpage, vpos), n);
+    }
+
+    // the waves' sums are joined row tile by row tile: their weights first
+#pragma unroll
+    for (int r = 0; r < RT; r++) {
+        l[r] += __shfl_xor(l[r], 16);
+        l[r] += __shfl_xor(l[r], 32);
+        if (g == 0) { s.m[wave][16 * r + n] = m[r]; s.l[wave][16 * r + n] = l[r]; }
+    }
+    __syncthreads();  // the queries' fragments are done with, too
+    if (tid < RG) {
+        float top = -__builtin_inff(), sum = 0.0f;
+#pragma unroll
+        for (int w = 0; w < NW; w++) top = fmaxf(top, s.m[w][tid]);
+#pragma unroll
+        for (int w = 0; w < NW; w++) {
+            const float lw = s.l[w][tid], f = part_weight(s.m[w][tid], lw, top);
+            if (f >= 0.0f) sum = __builtin_fmaf(f, lw, sum);
+            s.m[w][tid] = f;
+        }
+        s.l[0][tid] = sum;
+        if (!direct && fits) A.part_ml[(size_t)tile0 * 16 + tid] = make_float2(top, sum);
+    }
+    float *join = (float *)s.mem;
+#pragma unroll
+    for (int r = 0; r < RT; r++) {
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+#pragma unroll
+            for (int t = 0; t < DL; t += 4)
+                *(float4 *)(join + (wave * 16 + n) * (D + 4) + DL * (4 * g + i) + t) =
+                    make_float4(o[r][t][i], o[r][t + 1][i], o[r][t + 2][i], o[r][t + 3][i]);
+        __syncthreads();
+#pragma unroll
+        for (int x0 = 0; x0 < 16 * D / 4; x0 += 64 * NW) {
+            const int at4 = x0 + tid, row = at4 / (D / 4), d = at4 % (D / 4) * 4, at = row0 + 16 * r + row;
+            float4 y = make_float4(0, 0, 0, 0);
+#pragma unroll
+            for (int w = 0; w < NW; w++) {
+                const float f = s.m[w][16 * r + row];
+                const float4 u = *(const float4 *)(join + (w * 16 + row) * (D + 4) + d);
+                y.x = f < 0.0f ? y.x : __builtin_fmaf(f, u.x, y.x);
+                y.y = f < 0.0f ? y.y : __builtin_fmaf(f, u.y, y.y);
+                y.z = f < 0.0f ? y.z : __builtin_fmaf(f, u.z, y.z);
+                y.w = f < 0.0f ? y.w : __builtin_fmaf(f, u.w, y.w);
+            }
+            if (at >= rows) continue;
+            if (direct) {
+                const float sum = s.l[0][16 * r + row], inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+                const int t = by_group(A, at);
+                if (t >= count) continue;
+                const size_t to = (size_t)(first + t) * A.q_heads + p.h * A.group + (at - t * A.group);
+                *(float4 *)(A.out + to * D + d) = make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv);
+                if (odd_sums(y.x, y.y, sum) || odd_sums(y.z, y.w, sum)) A.odd[to] = 1;
+            } else if (fits) {
+                *(float4 *)(A.part_o + ((size_t)(tile0 + r) * 16 + row) * D + d) = y;
+            }
+        }
+        __syncthreads();
+    }
+}
+
+// RS row tiles of shared segments, RT of the sequences' own.
+template <int TYPE, int D, int RS, int RT, int NW>
+__global__ __launch_bounds__(64 * NW, (D / 64) * RS <= 6 ? 2 : 1) void prefix_attention_kernel(PrefixArgs A, KvView c, BatchView b, PrefixView v) {
+    __shared__ PrefixShared<TYPE, D, RS, NW> s;
+    Unit p;
+    if (!find_unit<RS, RT>(c, b, A, v, threadIdx.x & 63, blockIdx.x, p)) return;
+    if (p.s.tail) unit_attention<TYPE, D, RT, true, NW>(A, c, b, v, p, s);
+    else unit_attention<TYPE, D, RS, false, NW>(A, c, b, v, p, s);
+}
+
+// Joins a row's segments.  Few rows and heads: a workgroup each, whose four waves
+// share the parts; many: a wave each.
+constexpr int JOIN_WAVES = 4;
+constexpr size_t JOIN_FEW = 1024;
+
+// Parts i0, i0 + by, .. of a row, `step` rows of partial results apart from `slot` on:
+// added to the sums y under the largest m so far.  A lane holds the weight of one part.
+template <int D>
+QG_DEV void join_parts(const PrefixArgs &A, long slot, long step, int parts, int i0, int by, int lane, float &top, float &sum, float (&y)[D / 64]) {
+    constexpr int V = D / 64;
+    const float2 *ml = A.part_ml + slot;
+    const float *po = A.part_o + slot * D + lane * V;
+    for (; i0 < parts; i0 += 64 * by) {
+        const int mine = i0 + lane * by, count = min((parts - i0 + by - 1) / by, 64);
+        const float2 x = mine < parts ? ml[mine * step] : make_float2(-__builtin_inff(), 0.0f);
+        const float next = fmaxf(top, qg_wave_max(x.x));
+        const float old = next == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f(top - next);
+        const float f = part_weight(x.x, x.y, next);
+        top = next;
+        sum = sum * old + qg_sum_lanes<64>(f < 0.0f ? 0.0f : f * x.y);
+#pragma unroll
+        for (int w = 0; w < V; w++) y[w] *= old;
+        for (int i = 0; i < count; i += 8) {
+            float u[8][V];
+#pragma unroll
+            for (int k = 0; k < 8; k++) {
+                const float *from = po + (i0 + min(i + k, count - 1) * by) * step * D;
+#pragma unroll
+                for (int w = 0; w < V; w++) u[k][w] = from[w];
+            }
+#pragma unroll
+            for (int k = 0; k < 8; k++) {
+                const float q = i + k < count ? __int_as_float(__builtin_amdgcn_readlane(__float_as_int(f), (i + k) & 63)) : -1.0f;
+#pragma unroll
+                for (int w = 0; w < V; w++) y[w] = q < 0.0f ? y[w] : __builtin_fmaf(q, u[k][w], y[w]);
+            }
+        }
+    }
+}
+template <int TYPE, int D, int EACH>
+__global__ __launch_bounds__(64 * JOIN_WAVES) void prefix_join_kernel(PrefixArgs A, KvView c, BatchView b, PrefixView v) {
+    constexpr int V = D / 64;
+    __shared__ float s_y[JOIN_WAVES][D];
+    __shared__ float2 s_w[JOIN_WAVES];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const size_t at = EACH == 1 ? blockIdx.x : (size_t)blockIdx.x * EACH + wave;
+    if (at >= (size_t)b.rows * A.q_heads) return;
+    const int row = (int)(at / A.q_heads), head = (int)(at % A.q_heads), h = by_group(A, head);
+    int first, n;
+    const int s = batch_sequence(b, c.sequences, row, lane, first, n);
+    if (s < 0) return;  // nothing was written for it
+    const int count = segment_count(c, v), pos = v.pos[s] + (row - first);
+    int id = v.leaf[s];
+    if (id < 0 || id >= count) return;
+    bool odd = false;
+    Segment g = read_segment(c, b, v, id);
+    int4 j = A.joins[id];
+    if (g.begin == 0 && j.y == 1) {
+        odd = A.odd[at] == 1;
+    } else {
+        float top = -__builtin_inff(), sum = 0.0f, y[V];
+#pragma unroll
+        for (int w = 0; w < V; w++) y[w] = 0.0f;
+        for (int k = 0; k < count; k++) {
+            const int x = (pos - g.row0) * A.group + (head - h * A.group);
+            long slot, step;
+            if (pos >= g.row0 && pos < g.row0 + g.rows && segment_place(SegmentParts{j.x, j.y, j.z, j.w}, c.heads, h, x, A.tiles, slot, step)) {
+                if (EACH > 1) join_parts<D>(A, slot, step, j.y, 0, 1, lane, top, sum, y);
+                else join_parts<D>(A, slot, step, j.y, (wave + k) & (JOIN_WAVES - 1), JOIN_WAVES, lane, top, sum, y);
+            }
+            id = g.up;
+            if (id < 0 || id >= count) break;
+            g = read_segment(c, b, v, id);
+            j = A.joins[id];
+        }
+        if (EACH == 1) {
+#pragma unroll
+            for (int w = 0; w < V; w++) s_y[wave][lane * V + w] = y[w];
+            if (lane == 0) s_w[wave] = make_float2(top, sum);
+            __syncthreads();
+            if (wave) return;
+            const float most = fmaxf(fmaxf(s_w[0].x, s_w[1].x), fmaxf(s_w[2].x, s_w[3].x));
+            sum = 0.0f;
+#pragma unroll
+            for (int w = 0; w < V; w++) y[w] = 0.0f;
+#pragma unroll
+            for (int w = 0; w < JOIN_WAVES; w++) {
+                const float2 u = s_w[w];
+                const float f = part_weight(u.x, u.y, most);
+                if (f < 0.0f) continue;
+                sum = __builtin_fmaf(f, u.y, sum);
+#pragma unroll
+                for (int i = 0; i < V; i++) y[i] = __builtin_fmaf(f, s_y[w][lane * V + i], y[i]);
+            }
+        }
+        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+#pragma unroll
+        for (int w = 0; w < V; w++) {
+            odd |= odd_sums(y[w], 0.0f, sum);
+            A.out[at * D + lane * V + w] = y[w] * inv;
+        }
+        odd = __any(odd);
+    }
+    if (odd && (EACH > 1 || wave == 0)) attend_row<TYPE, D>(A, c, b, s, first, n, row, head, lane, s_y[wave]);
+}
+
+// Row groups of all segments, at most (each rounds up), for the segments' own tiles.
+long groups_most(const BatchView &b, int S, int group, int rs, int rt) {
+    return shared_rows_most(b.rows) * group / (16 * rs) + (long)b.rows * group / (16 * rt) + 2L * S;
+}
+// Tiles of partial results that the units can ask for: parts of a segment are at most its keys / chunk + 1.
+long tiles_most(const BatchView &b, int S, int heads, int group, int dim) {
+    const int rs = most_tiles(dim);
+    return 2L * resident(dim, rs) * rs + heads * (shared_rows_most(b.rows) * group / 16 + (long)b.rows * group / 16 + 2L * S * rs);
+}
+template <int TYPE, int D, int RT>
+void launch(const PrefixArgs &A, const KvView &c, const BatchView &b, const PrefixView &v, hipStream_t s) {
+    constexpr int RS = most_tiles(D);
+    const long units = 2 * A.resident + groups_most(b, c.sequences, A.group, RS, RT) * c.heads;
+    prefix_attention_kernel<TYPE, D, RS, RT, WAVES><<<(unsigned)((units + 7) / 8 * 8), 64 * WAVES, 0, s>>>(A, c, b, v);
+    const size_t jobs = (size_t)b.rows * A.q_heads;
+    if (jobs > JOIN_FEW) prefix_join_kernel<TYPE, D, 4><<<(unsigned)((jobs + 3) / 4), 256, 0, s>>>(A, c, b, v);
+    else prefix_join_kernel<TYPE, D, 1><<<(unsigned)jobs, 256, 0, s>>>(A, c, b, v);
+}
+template <int TYPE, int D>
+void launch_rt(int rt, const PrefixArgs &A, const KvView &c, const BatchView &b, const PrefixView &v, hipStream_t s) {
+    if (rt == 1) launch<TYPE, D, 1>(A, c, b, v, s);
+    else if (rt == 2) launch<TYPE, D, 2>(A, c, b, v, s);
+    else if constexpr (D != 256) {
+        if (rt == 3) launch<TYPE, D, 3>(A, c, b, v, s);
+        else if constexpr (D == 64) launch<TYPE, D, 4>(A, c, b, v, s);
+    }
+}
+template <int TYPE>
+void launch_dim(int rt, const PrefixArgs &A, const KvView &c, const BatchView &b, const PrefixView &v, hipStream_t s) {
+    if (c.dim == 64) launch_rt<TYPE, 64>(rt, A, c, b, v, s);
+    else if (c.dim == 128) launch_rt<TYPE, 128>(rt, A, c, b, v, s);
+    else launch_rt<TYPE, 256>(rt, A, c, b, v, s);
+}
+constexpr long JOBS = 1L << 25;  // rows x heads: of the join kernel, a wave each, within 2^32 threads
+constexpr long TILES = 1L << 27; // of partial results, within an int of rows
+}  // namespace
+
+extern "C" {
+
+size_t qg_kv_prefixes_bytes(const qg_kv_cache *cache, const qg_kv_batch *batch) {
+    if (qg_kv_check(cache, false, nullptr) || qg_batch_check(batch, false, nullptr)) return 0;
+    return prefix_bytes(cache->sequences, batch->rows);
+}
+
+int qg_kv_prefixes(int *link, int *shared, const qg_kv_cache *cache, const qg_kv_batch *batch, void *prefixes, size_t prefixes_bytes) {
+    KvView c;
+    BatchView b;
+    const size_t need = qg_kv_prefixes_bytes(cache, batch);
+    if (!need || qg_kv_check(cache, false, &c) || qg_batch_check(batch, false, &b)) return hipErrorInvalidValue;
+    if (!prefixes || prefixes_bytes < need || ((uintptr_t)prefixes & 15) || (((uintptr_t)link | (uintptr_t)shared) & 3)) return hipErrorInvalidValue;
+    const size_t each = qg_ints(c.sequences);
+    const QgSpan out[3] = {{link, each}, {shared, each}, {prefixes, need}},
+                 in[3] = {{c.table, qg_table_bytes(c)}, {c.length, each}, {b.start, each + 4}};
+    if (qg_any_overlap(out, in) || qg_overlap(link, each, shared, each) || qg_overlap(prefixes, need, link, each) || qg_overlap(prefixes, need, shared, each))
+        return hipErrorInvalidValue;
+    const PrefixView v = prefix_view(prefixes, c.sequences);
+    prefix_link_kernel<<<(c.sequences + 3) / 4, 256, 0, qg_stream()>>>(c, b, v, link, shared);
+    prefix_plan_kernel<<<1, PLAN_THREADS, 0, qg_stream()>>>(c, b, v);
+    return hipGetLastError();
+}
+
+size_t qg_prefix_attention_workspace_bytes(const qg_kv_cache *cache, const qg_kv_batch *batch, int q_heads) {
+    BatchView b;
+    if (qg_kv_check(cache, false, nullptr) || qg_batch_check(batch, false, &b)) return 0;
+    if (q_heads < 1 || q_heads % cache->kv_heads || q_heads / cache->kv_heads > 128) return 0;
+    if ((long)batch->rows * q_heads > JOBS) return 0;
+    const long tiles = tiles_most(b, cache->sequences, cache->kv_heads, q_heads / cache->kv_heads, cache->head_dim);
+    if (tiles > TILES) return 0;
+    return (size_t)tiles * 16 * (4 * (size_t)cache->head_dim + sizeof(float2)) + sizeof(int4) * 2 * (size_t)cache->sequences +
+           4 * (size_t)batch->rows * q_heads;
+}
+
+int qg_prefix_attention(float *out, const float *q, int q_heads, float scale, const qg_kv_cache *cache, int layer, const qg_kv_batch *batch,
+                        const void *prefixes, size_t prefixes_bytes, void *ws, size_t ws_bytes) {
+    KvView c;
+    BatchView b;
+    const size_t need = qg_prefix_attention_workspace_bytes(cache, batch, q_heads), plan = qg_kv_prefixes_bytes(cache, batch);
+    if (!need || !plan || qg_kv_check(cache, false, &c) || qg_batch_check(batch, false, &b)) return hipErrorInvalidValue;
+    if (!out || !q || !ws || ws_bytes < need || (((uintptr_t)out | (uintptr_t)q | (uintptr_t)ws) & 15)) return hipErrorInvalidValue;
+    if (!prefixes || prefixes_bytes < plan || ((uintptr_t)prefixes & 15)) return hipErrorInvalidValue;
+    if (layer < 0 || layer >= c.layers || !__builtin_isfinite(scale * 1.44269504088896341f)) return hipErrorInvalidValue;
+    const size_t bytes = 4 * (size_t)b.rows * q_heads * c.dim;
+    const QgSpan written[2] = {{out, bytes}, {ws, need}}, read[2] = {{q, bytes}, {prefixes, plan}};
+    if (qg_any_overlap(written, read) || qg_overlap(out, bytes, ws, need)) return hipErrorInvalidValue;
+    const int group = q_heads / c.heads, rt = row_tiles(c.dim, (long)b.max_rows * group), rs = most_tiles(c.dim);
+    const long tiles = tiles_most(b, c.sequences, c.heads, group, c.dim);
+    float *part_o = (float *)ws;
+    float2 *part_ml = (float2 *)(part_o + (size_t)tiles * 16 * c.dim);
+    int4 *joins = (int4 *)(part_ml + (size_t)tiles * 16);
+    const PrefixArgs A{attn_rows(out, q, q_heads, group, layer, scale), part_o, part_ml, joins, (int *)(joins + 2 * (size_t)c.sequences),
+                       resident(c.dim, rs), (int)tiles};
+    const PrefixView v = prefix_view(const_cast<void *>(prefixes), c.sequences);
+    if (c.type == QT_F32) launch_dim<QT_F32>(rt, A, c, b, v, qg_stream());
+    else if (c.type == QT_F16) launch_dim<QT_F16>(rt, A, c, b, v, qg_stream());
+    else launch_dim<QT_BF16>(rt, A, c, b, v, qg_stream());
+    return hipGetLastError();
+}
+
+}  // extern "C"
