@@ -16,12 +16,23 @@ namespace {
 constexpr int SA_THREADS = 1024, SA_WAVES = SA_THREADS / 64, SA_DIGIT = 11, SA_BINS = 1 << SA_DIGIT, SA_PIECE = 4096;
 constexpr int SA_MAX_COLS = 1 << 24, SA_MAX_DRAWS = 64;
 
+// What the pass over a piece of a row leaves: its largest value (NaN if there is one), that
+// value's place on the grid, whether weights lie below the bins, and the sum of the weights in no
+// bin, in units of 2^(place / 4).
+struct PieceStat { float top; int at, below, pad; double rest; };
+// What a row came to: its cut, and what its probabilities are formed from.
+struct RowResult { uint32_t t; int last; float top; int state; double a, total; };
+enum { ROW_NAN = 0, ROW_NONE = 1, ROW_CUT = 2 };
+
 struct SampleArgs {
     const float *x, *temperature, *top_p, *min_p, *u;
     const int *top_k;
     float *out, *logprob;
     int *token;
     int cols, draws, fixed;  // fixed: weights are added up as whole numbers of 2^-fixed where their order is not given
+    unsigned long long *bins;  // [rows][pieces][SA_GRID]
+    PieceStat *stats;          // [rows][pieces]
+    RowResult *results;        // [rows]
 };
 
 // Unsigned keys in the values' order; the zeros of both signs are one value.
@@ -49,6 +60,7 @@ QG_DEV double exp2_d(double d) {
 struct Request {
     double a, top_p, min_p;
     int top_k;
+    __device__ __forceinline__ bool filters() const { return top_k || top_p < 1.0 || min_p > 0.0; }
 };
 QG_DEV Request read_request(const SampleArgs &A, int row) {
     const float T = A.temperature ? A.temperature[row] : 1.0f, p = A.top_p ? A.top_p[row] : 1.0f, least = A.min_p ? A.min_p[row] : 0.0f;
@@ -98,10 +110,8 @@ QG_DEV void each_value(const float *x, int i0, int end, F f) {
 }
 
 struct RowShared {
-    union {
-        struct { unsigned long long mass[SA_BINS]; unsigned count[SA_BINS]; };
-        double piece[SA_MAX_COLS / SA_PIECE];
-    };
+    unsigned long long mass[SA_BINS];
+    unsigned count[SA_BINS];
     unsigned long long wave_mass[SA_WAVES], found_mass, found_own;
     unsigned wave_count[SA_WAVES], found_count, found_ties;
     int found_bin, bad;
@@ -246,47 +256,404 @@ struct Row {
     }
 };
 
+// ------------------------------------------------------------------------
+// One pass over the values, in pieces.  The weights' exponents x a lie on a grid of quarter
+// bits; each piece counts and weighs the values of the SA_GRID bins from its
+// largest down, so that all pieces together cover the 16 bits of weight below the row's
+// largest, where filters usually cut.  A weight is 1..2^(1/4) times its bin's lower end: what it
+// has above that, to 2^-39, is added up as a whole number under the count, in one 64-bit atomic
+// whose order does not matter.
+// ------------------------------------------------------------------------
+constexpr int SA_GRID = 64, PIECE_THREADS = 256, PIECE_VALUES = SA_PIECE / PIECE_THREADS, GRID_COUNT = 49, GRID_BITS = 39;
+constexpr double GRID_ZERO = 4400.0;        // quarter bits below which a weight is 0 in 64 bits
+constexpr double GRID_FAR = (double)(1 << 21);  // places further out are left to the search over the row
+constexpr int GRID_LOW = -0x7fffffff;       // in place of one: all of the piece's weights are 0 beside a row's largest within half of that
+
+// 2^(f / 4), 0 <= f < 1, at least 1: the Taylor series about f = 1/2, whose next term is below 1e-17.
+QG_DEV double quarter_power(double f) {
+    constexpr double h = 0.173286795139986327354, at_half = 1.09050773266525765921;  // ln 2 / 4, 2^(1/8)
+    constexpr double c1 = at_half * h, c2 = c1 * h / 2, c3 = c2 * h / 3, c4 = c3 * h / 4, c5 = c4 * h / 5, c6 = c5 * h / 6, c7 = c6 * h / 7, c8 = c7 * h / 8,
+                     c9 = c8 * h / 9;
+    const double c[9] = {at_half, c1, c2, c3, c4, c5, c6, c7, c8}, y = f - 0.5;
+    double p = c9;
+#pragma unroll
+    for (int i = 8; i >= 0; i--) p = __builtin_fma(p, y, c[i]);
+    return __builtin_fmax(p, 1.0);
+}
+QG_DEV double grid_scale(int quarters) {  // 2^(quarters / 4)
+    const int j = quarters & 3;
+    const double c = j == 0 ? 1.0 : j == 1 ? 1.18920711500272106672 : j == 2 ? 1.41421356237309504880 : 1.68179283050742908606;
+    return __builtin_amdgcn_ldexp(c, quarters >> 2);
+}
+QG_DEV double grid_place(float x, double a4) { return __builtin_floor((double)x * a4); }
+QG_DEV float larger_or_nan(float a, float b) { return a != a || b != b ? __builtin_nanf("") : fmaxf(a, b); }
+
+__global__ __launch_bounds__(PIECE_THREADS) void sample_piece_kernel(SampleArgs A, int pieces) {
+    constexpr int W = PIECE_THREADS / 64;
+    __shared__ unsigned long long s_bin[SA_GRID];
+    __shared__ float s_top[W];
+    __shared__ double s_rest[W];
+    __shared__ int s_below[W];
+    const int row = blockIdx.x / pieces, piece = blockIdx.x % pieces, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const Request q = read_request(A, row);
+    const int n = min(SA_PIECE, A.cols - piece * SA_PIECE);
+    const float *x = A.x + (size_t)row * A.cols + (size_t)piece * SA_PIECE + tid;
+    float v[PIECE_VALUES], top = -__builtin_inff();
+    if (n == SA_PIECE) {
+#pragma unroll
+        for (int k = 0; k < PIECE_VALUES; k++) v[k] = x[k * PIECE_THREADS];
+    } else {
+#pragma unroll
+        for (int k = 0; k < PIECE_VALUES; k++) v[k] = k * PIECE_THREADS + tid < n ? x[k * PIECE_THREADS] : -__builtin_inff();
+    }
+    if (tid < SA_GRID) s_bin[tid] = 0;
+    bool nan = false;
+#pragma unroll
+    for (int k = 0; k < PIECE_VALUES; k++) { top = fmaxf(top, v[k]); nan |= v[k] != v[k]; }
+    top = qg_wave_max(top);
+    if (__any(nan)) top = __builtin_nanf("");
+    if (lane == 0) s_top[wave] = top;
+    __syncthreads();
+    top = s_top[0];
+#pragma unroll
+    for (int w = 1; w < W; w++) top = larger_or_nan(top, s_top[w]);
+    const double a4 = q.a * 4.0, place = grid_place(top, a4);
+    const size_t at = (size_t)row * pieces + piece;
+    if (!(__builtin_fabs(place) < GRID_FAR)) {  // NaN and infinities too
+        if (tid == 0) A.stats[at] = PieceStat{top, GRID_LOW, 0, 0, 0.0};
+        return;
+    }
+    const bool filter = q.filters(), rest_counts = !q.top_k;
+    double rest = 0.0;
+    bool below = false;
+#pragma unroll
+    for (int k = 0; k < PIECE_VALUES; k++) {
+        const double e = (double)v[k] * a4, b = __builtin_floor(e), d = place - b;
+        if (!(d < GRID_ZERO)) continue;
+        if (filter && d < SA_GRID) {
+            const unsigned long long m = (unsigned long long)__double_as_longlong(quarter_power(e - b)) & ((1ULL << 52) - 1);
+            atomicAdd(&s_bin[(int)d], ((m + (1ULL << (51 - GRID_BITS))) >> (52 - GRID_BITS)) + (1ULL << GRID_COUNT));
+        } else {
+            below = true;
+            if (rest_counts) rest += quarter_power(e - b) * grid_scale(-(int)d);
+        }
+    }
+    rest = wave_all_add(rest);
+    below = __any(below);
+    if (lane == 0) { s_rest[wave] = rest; s_below[wave] = below; }
+    __syncthreads();
+    if (filter && tid < SA_GRID) A.bins[at * SA_GRID + tid] = s_bin[tid];
+    if (tid == 0) {
+        PieceStat p{top, (int)place, 0, 0, 0.0};
+#pragma unroll
+        for (int w = 0; w < W; w++) { p.rest += s_rest[w]; p.below |= s_below[w]; }
+        A.stats[at] = p;
+    }
+}
+
+// ------------------------------------------------------------------------
+// A row's cut, and its draws, by one workgroup.  The bins of all pieces together say in which one
+// a filter cuts; where in it say its values, read again from the pieces that have some
+// and ranked.  What the bins do not reach is left to the search over the whole row.
+// ------------------------------------------------------------------------
+constexpr int SA_LIST = 1024;
+struct GridShared {
+    unsigned count[SA_WAVES][SA_GRID];
+    unsigned long long mant[SA_WAVES][SA_GRID];
+    uint32_t key[SA_LIST], sorted_key[SA_LIST];
+    int index[SA_LIST], sorted_index[SA_LIST];
+    double upto[SA_LIST], wave_sum[SA_WAVES];
+    int listed;
+};
+struct SelectShared {
+    union { RowShared row; GridShared grid; };
+    double piece[SA_MAX_COLS / SA_PIECE];  // what stays of each piece
+    float top[SA_WAVES];
+    int flag[SA_WAVES];
+};
+
+struct Grid {
+    const SampleArgs &A;
+    GridShared &s;
+    const Row &r;
+    const unsigned long long *bins;
+    const PieceStat *stats;
+    const int pieces, tid, lane, wave, place;  // place: of the row's largest value
+    const double a4, unit;                     // unit: of a weight of place's lower end, the largest value's being 1
+    // lane D of each wave: values in bin D from the top, their weight, and both with the bins above
+    unsigned count, count_upto;
+    double mass, mass_upto;
+    int bin, kept;                             // the listed bin (-1: none), and how many of its values stay
+
+    // A piece's bin of a lane, moved to the row's grid; 0 where it has none.
+    __device__ __forceinline__ unsigned long long bin_of(int p, int &delta) const {
+        const int at = stats[p].at;
+        delta = at == GRID_LOW ? SA_GRID : min(place - at, SA_GRID);
+        const unsigned long long own = delta < SA_GRID ? bins[(size_t)p * SA_GRID + lane] : 0;
+        return own;
+    }
+    __device__ __forceinline__ unsigned long long moved(unsigned long long own, int delta) const {
+        const unsigned long long b = __shfl(own, (lane - delta) & 63);
+        return lane >= delta ? b : 0;
+    }
+    static __device__ __forceinline__ double mass_of(unsigned n, unsigned long long mant, int bin) {
+        return ((double)n + (double)mant * __builtin_amdgcn_ldexp(1.0, -GRID_BITS)) * grid_scale(-bin);
+    }
+    // All pieces' bins; whether the row has weights below them.
+    __device__ bool add_up(int *flag) {
+        unsigned n = 0;
+        unsigned long long m = 0;
+        bool below = false;
+        for (int p = wave; p < pieces; p += SA_WAVES) {
+            int delta;
+            const unsigned long long own = bin_of(p, delta), b = moved(own, delta);
+            below |= own && lane + delta >= SA_GRID;
+            if (stats[p].at != GRID_LOW && place - stats[p].at < (int)GRID_ZERO) below |= stats[p].below || delta >= SA_GRID;
+            n += (unsigned)(b >> GRID_COUNT);
+            m += b & ((1ULL << GRID_COUNT) - 1);
+        }
+        below = __any(below);
+        s.count[wave][lane] = n;
+        s.mant[wave][lane] = m;
+        if (lane == 0) flag[wave] = below;
+        __syncthreads();
+        count = 0;
+        m = 0;
+        below = false;
+#pragma unroll
+        for (int w = 0; w < SA_WAVES; w++) {
+            count += s.count[w][lane];
+            m += s.mant[w][lane];
+            below |= flag[w] != 0;
+        }
+        mass = mass_of(count, m, lane) * unit;
+        count_upto = wave_upto(count, lane);
+        mass_upto = wave_upto(mass, lane);
+        return below;
+    }
+    __device__ __forceinline__ double above(int D) const { return D ? __shfl(mass_upto, D - 1) : 0.0; }
+    // The values of bin D in falling order with the sums of their weights; false if they are too many.
+    __device__ bool list(int D) {
+        const unsigned n = __shfl(count, D);
+        if (n > SA_LIST) return false;
+        __syncthreads();
+        if (tid == 0) s.listed = 0;
+        __syncthreads();
+        const double b = (double)(place - D);
+        for (int p = wave; p < pieces; p += SA_WAVES) {
+            int delta;
+            const unsigned long long own = bin_of(p, delta);
+            if (D < delta || !(__shfl(own, (D - delta) & 63) >> GRID_COUNT)) continue;
+            each_value<64>(r.x, p * SA_PIECE + lane, min((p + 1) * SA_PIECE, A.cols), [&](int i, float v) {
+                if (grid_place(v, a4) != b) return;
+                const int k = atomicAdd(&s.listed, 1);
+                if (k < SA_LIST) { s.key[k] = order_key(v); s.index[k] = i; }
+            });
+        }
+        __syncthreads();
+        double w = 0.0;
+        if (tid < (int)n) {
+            const uint32_t key = s.key[tid];
+            const int i = s.index[tid];
+            int rank = 0;
+            for (int k = 0; k < (int)n; k++) rank += s.key[k] > key || (s.key[k] == key && s.index[k] < i);
+            s.sorted_key[rank] = key;
+            s.sorted_index[rank] = i;
+        }
+        __syncthreads();
+        if (tid < (int)n) w = r.weight(key_value(s.sorted_key[tid]));
+        w = wave_upto(w, lane);
+        if (lane == 63) s.wave_sum[wave] = w;
+        __syncthreads();
+        for (int k = 0; k < wave; k++) w += s.wave_sum[k];
+        s.upto[tid] = w;
+        __syncthreads();
+        bin = D;
+        kept = (int)n;
+        return true;
+    }
+    // The least key of place b, which is the place of some value of a piece or more: a search in 64 ways.
+    __device__ uint32_t first_key(double b) const {
+        uint32_t lo = 0x007fffffu, hi = order_key(r.m);
+        while (hi - lo > 1) {
+            const uint32_t step = (hi - lo - 1) / 64 + 1, k = lo + min((uint32_t)(lane + 1) * step, hi - lo);
+            const int first = __builtin_ctzll(__ballot(grid_place(key_value(k), a4) >= b));
+            const uint32_t up = lo + min((uint32_t)(first + 1) * step, hi - lo);
+            lo += min((uint32_t)first * step, hi - lo);
+            hi = up;
+        }
+        return hi;
+    }
+    // The row's cut and the weight that stays; false where the bins do not reach.
+    __device__ bool select(const Request &q, Cut &cut, double &total, int &last_bin, int *flag) {
+        const bool below = add_up(flag);
+        bin = -1;
+        kept = 0;
+        last_bin = SA_GRID;  // bins above it stay whole
+        if (q.top_k) {
+            const unsigned long long enough = __ballot(count_upto >= (unsigned)q.top_k);
+            if (!enough && below) return false;
+            if (enough) {
+                const int D = __builtin_ctzll(enough);
+                const int left = q.top_k - (int)(__shfl(count_upto, D) - __shfl(count, D));
+                if (left == (int)__shfl(count, D)) {  // all of the bin
+                    cut = Cut{first_key((double)(place - D)), 0x7fffffff};
+                    last_bin = D + 1;
+                    total = __shfl(mass_upto, D);
+                } else {
+                    if (!list(D)) return false;
+                    kept = left;
+                    last_bin = D;
+                    cut = Cut{s.sorted_key[left - 1], s.sorted_index[left - 1]};
+                    total = above(D) + s.upto[left - 1];
+                }
+            } else {
+                total = __shfl(mass_upto, SA_GRID - 1);
+            }
+        }
+        if (q.top_p < 1.0) {
+            if (!q.top_k) {
+                total = 0.0;  // of all pieces, whatever lies in bins
+                for (int p = wave; p < pieces; p += SA_WAVES) {
+                    int delta;
+                    const unsigned long long own = bin_of(p, delta);
+                    const double in = wave_all_add(mass_of((unsigned)(own >> GRID_COUNT), own & ((1ULL << GRID_COUNT) - 1), lane));
+                    if (stats[p].at != GRID_LOW) total += (in + stats[p].rest) * grid_scale(stats[p].at - place) * unit;
+                }
+                __syncthreads();
+                if (lane == 0) s.wave_sum[wave] = total;
+                __syncthreads();
+                total = 0.0;
+#pragma unroll
+                for (int w = 0; w < SA_WAVES; w++) total += s.wave_sum[w];
+            }
+            const double goal = q.top_p * total;
+            const unsigned long long enough = __ballot(count_upto > 0 && mass_upto >= goal);
+            if (!enough && below) return false;
+            const int D = enough ? __builtin_ctzll(enough) : SA_GRID - 1;
+            if (D < last_bin || D == bin) {
+                if (D != bin && !list(D)) return false;
+                const double before = above(D);
+                // the first of the bin's values that reaches the goal
+                __syncthreads();
+                if (tid == 0) s.listed = kept - 1;
+                __syncthreads();
+                if (tid < kept && before + s.upto[tid] >= goal) atomicMin(&s.listed, tid);
+                __syncthreads();
+                if (kept > 0) {
+                    kept = s.listed + 1;
+                    last_bin = D;
+                    cut = Cut{s.sorted_key[kept - 1], s.sorted_index[kept - 1]};
+                    total = before + s.upto[kept - 1];
+                }
+            }
+        }
+        if (q.min_p > 0.0) {
+            const uint32_t t = r.least_key(q.min_p);
+            if (t > cut.t) {
+                const double d = (double)place - grid_place(key_value(t), a4);
+                if (!(d < SA_GRID)) {
+                    if (below) return false;
+                } else {
+                    const int D = (int)d;
+                    if (D != bin && !list(D)) return false;
+                    const int n = __syncthreads_count(tid < kept && s.sorted_key[tid] >= t);
+                    kept = n;
+                    last_bin = D;
+                    cut = Cut{t, 0x7fffffff};
+                    total = above(D) + (n ? s.upto[n - 1] : 0.0);
+                }
+            }
+        }
+        if (!q.top_k && !(q.top_p < 1.0) && last_bin == SA_GRID) total = __shfl(mass_upto, SA_GRID - 1);  // min-p that drops nothing
+        return true;
+    }
+    // What stays of each piece: its bins above the last one, and the listed values that are its.
+    __device__ void weigh_pieces(int last_bin, double *piece) const {
+        for (int p = wave; p < pieces; p += SA_WAVES) {
+            int delta;
+            const unsigned long long b = moved(bin_of(p, delta), delta);
+            double sum = lane < last_bin ? mass_of((unsigned)(b >> GRID_COUNT), b & ((1ULL << GRID_COUNT) - 1), lane) * unit : 0.0;
+            if (last_bin == bin)
+                for (int k = lane; k < kept; k += 64)
+                    if (s.sorted_index[k] / SA_PIECE == p) sum += r.weight(key_value(s.sorted_key[k]));
+            sum = wave_all_add(sum);
+            if (lane == 0) piece[p] = sum;
+        }
+    }
+};
+
 template <bool DRAW>
-__global__ __launch_bounds__(SA_THREADS) void sample_row_kernel(SampleArgs A) {
-    __shared__ RowShared s;
+__global__ __launch_bounds__(SA_THREADS) void sample_select_kernel(SampleArgs A, int pieces) {
+    __shared__ SelectShared s;
     const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const Request q = read_request(A, row);
-    Row r{A, s, A.x + (size_t)row * A.cols, tid, lane, wave, q.a, 0.0f};
-    const bool some = r.largest();
-    float *out = DRAW ? nullptr : A.out + (size_t)row * A.cols;
-    if (!some) {
+    const PieceStat *stats = A.stats + (size_t)row * pieces;
+    float top = -__builtin_inff();
+    for (int p = tid; p < pieces; p += SA_THREADS) top = larger_or_nan(top, stats[p].top);
+    const bool nan = __any(top != top);
+    top = nan ? __builtin_nanf("") : qg_wave_max(top);
+    if (lane == 0) s.top[wave] = top;
+    __syncthreads();
+    top = s.top[0];
+#pragma unroll
+    for (int w = 1; w < SA_WAVES; w++) top = larger_or_nan(top, s.top[w]);
+    if (!__builtin_isfinite(top)) {
         if (DRAW) {
             if (tid < A.draws) {
                 A.token[(size_t)row * A.draws + tid] = -1;
                 if (A.logprob) A.logprob[(size_t)row * A.draws + tid] = __builtin_nanf("");
             }
-        } else {
-            const float none = r.m == -__builtin_inff() ? 0.0f : __builtin_nanf("");
-            for (int i = tid; i < A.cols; i += SA_THREADS) out[i] = none;
+        } else if (tid == 0) {
+            A.results[row] = RowResult{0, 0, top, top == -__builtin_inff() ? ROW_NONE : ROW_NAN, 0.0, 0.0};
         }
         return;
     }
+    Row r{A, s.row, A.x + (size_t)row * A.cols, tid, lane, wave, q.a, top};
     Cut cut;
-    if (q.top_k) r.shorten(cut, false, q.top_k);
-    if (q.top_p < 1.0) r.shorten(cut, true, q.top_p);
-    if (q.min_p > 0.0) {
-        const uint32_t k = r.least_key(q.min_p);
-        if (k > cut.t) cut = Cut{k, 0x7fffffff};
-    }
-    // sums of pieces, each by one wave
-    const int pieces = (A.cols + SA_PIECE - 1) / SA_PIECE;
-    __syncthreads();
-    for (int p = wave; p < pieces; p += SA_WAVES) {
-        double sum = 0.0;
-        each_value<64>(r.x, p * SA_PIECE + lane, min((p + 1) * SA_PIECE, A.cols), [&](int i, float v) { sum += cut.keeps(order_key(v), i) ? r.weight(v) : 0.0; });
-        sum = wave_all_add(sum);
-        if (lane == 0) s.piece[p] = sum;
-    }
-    __syncthreads();
     double total = 0.0;
-    for (int p0 = 0; p0 < pieces; p0 += 64) total += wave_all_add(p0 + lane < pieces ? s.piece[p0 + lane] : 0.0);
+    const double a4 = q.a * 4.0, place = grid_place(top, a4);
+    bool found = false, weighed = false;
+    if (__builtin_fabs(place) < 0.5 * GRID_FAR) {
+        const double unit = 1.0 / quarter_power((double)top * a4 - place);
+        if (!q.filters()) {
+            for (int p = tid; p < pieces; p += SA_THREADS) s.piece[p] = stats[p].at == GRID_LOW ? 0.0 : stats[p].rest * grid_scale(stats[p].at - (int)place) * unit;
+            found = weighed = true;
+        } else {
+            Grid g{A, s.grid, r, A.bins + (size_t)row * pieces * SA_GRID, stats, pieces, tid, lane, wave, (int)place, a4, unit};
+            int last_bin;
+            found = g.select(q, cut, total, last_bin, s.flag);
+            if (found && DRAW) {
+                g.weigh_pieces(last_bin, s.piece);
+                weighed = true;
+            }
+        }
+    }
+    if (!found) {
+        __syncthreads();
+        cut = Cut{};
+        if (q.top_k) r.shorten(cut, false, q.top_k);
+        if (q.top_p < 1.0) r.shorten(cut, true, q.top_p);
+        if (q.min_p > 0.0) {
+            const uint32_t k = r.least_key(q.min_p);
+            if (k > cut.t) cut = Cut{k, 0x7fffffff};
+        }
+        __syncthreads();
+        for (int p = wave; p < pieces; p += SA_WAVES) {
+            double sum = 0.0;
+            each_value<64>(r.x, p * SA_PIECE + lane, min((p + 1) * SA_PIECE, A.cols), [&](int i, float v) { sum += cut.keeps(order_key(v), i) ? r.weight(v) : 0.0; });
+            sum = wave_all_add(sum);
+            if (lane == 0) s.piece[p] = sum;
+        }
+        weighed = true;
+    }
+    if (weighed) {
+        __syncthreads();
+        total = 0.0;
+        for (int p0 = 0; p0 < pieces; p0 += 64) total += wave_all_add(p0 + lane < pieces ? s.piece[p0 + lane] : 0.0);
+    }
     if (!DRAW) {
-        each_value<SA_THREADS>(r.x, tid, A.cols, [&](int i, float v) { out[i] = cut.keeps(order_key(v), i) ? (float)(r.weight(v) / total) : 0.0f; });
+        if (tid == 0) A.results[row] = RowResult{cut.t, cut.last, top, ROW_CUT, q.a, total};
         return;
     }
     for (int d = wave; d < A.draws; d += SA_WAVES) {
@@ -329,11 +696,44 @@ __global__ __launch_bounds__(SA_THREADS) void sample_row_kernel(SampleArgs A) {
     }
 }
 
+// Probabilities of a piece; one that lies below the cut is not read.
+__global__ __launch_bounds__(PIECE_THREADS) void sample_probs_kernel(SampleArgs A, int pieces) {
+    const int row = blockIdx.x / pieces, piece = blockIdx.x % pieces, tid = threadIdx.x;
+    const RowResult q = A.results[row];
+    const float top = A.stats[(size_t)row * pieces + piece].top;
+    const int c0 = piece * SA_PIECE, n = min(SA_PIECE, A.cols - c0);
+    const size_t at = (size_t)row * A.cols + c0 + tid;
+    float *to = A.out + at;
+    const Cut cut{q.t, q.last};
+    if (q.state != ROW_CUT || order_key(top) < q.t) {
+        const float y = q.state == ROW_NAN ? __builtin_nanf("") : 0.0f;
+        if (n == SA_PIECE) {
+#pragma unroll
+            for (int k = 0; k < PIECE_VALUES; k++) to[k * PIECE_THREADS] = y;
+        } else {
+            for (int k = tid; k < n; k += PIECE_THREADS) to[k - tid] = y;
+        }
+        return;
+    }
+    const float *x = A.x + at;
+    float v[PIECE_VALUES];
+#pragma unroll
+    for (int k = 0; k < PIECE_VALUES; k++) v[k] = n == SA_PIECE || k * PIECE_THREADS + tid < n ? x[k * PIECE_THREADS] : -__builtin_inff();
+    const double share = 1.0 / q.total;
+#pragma unroll
+    for (int k = 0; k < PIECE_VALUES; k++) {
+        float y = 0.0f;
+        if (cut.keeps(order_key(v[k]), c0 + k * PIECE_THREADS + tid)) y = (float)(exp2_d(((double)v[k] - (double)q.top) * q.a) * share);
+        if (n == SA_PIECE || k * PIECE_THREADS + tid < n) to[k * PIECE_THREADS] = y;
+    }
+}
+
 // Host checks that both calls share.
 bool sampling_ok(const qg_sampling *p) {
     return p && !(((uintptr_t)p->temperature | (uintptr_t)p->top_k | (uintptr_t)p->top_p | (uintptr_t)p->min_p) & 3);
 }
-SampleArgs sample_args(const float *x, int rows, int cols, const qg_sampling *p) {
+int sample_pieces(int cols) { return (cols + SA_PIECE - 1) / SA_PIECE; }
+SampleArgs sample_args(const float *x, int rows, int cols, const qg_sampling *p, void *ws) {
     SampleArgs A{};
     A.x = x;
     A.temperature = p->temperature;
@@ -344,6 +744,10 @@ SampleArgs sample_args(const float *x, int rows, int cols, const qg_sampling *p)
     int bits = 0;
     while (1 << bits < cols) bits++;
     A.fixed = 62 - bits;
+    const size_t all = (size_t)rows * sample_pieces(cols);
+    A.results = (RowResult *)ws;
+    A.stats = (PieceStat *)(A.results + rows);
+    A.bins = (unsigned long long *)(A.stats + all);
     return A;
 }
 }  // namespace
@@ -352,7 +756,7 @@ extern "C" {
 
 size_t qg_sample_workspace_bytes(int rows, int cols) {
     if (rows < 1 || rows > QG_MAX_ROWS || cols < 1 || cols > SA_MAX_COLS || (long)rows * cols > 1L << 35) return 0;
-    return 16;
+    return (size_t)rows * (sizeof(RowResult) + sample_pieces(cols) * (sizeof(PieceStat) + SA_GRID * sizeof(unsigned long long)));
 }
 
 int qg_sample(int *token, float *logprob, const float *x, int rows, int cols, int draws, const qg_sampling *sampling, const float *u,
@@ -365,12 +769,14 @@ int qg_sample(int *token, float *logprob, const float *x, int rows, int cols, in
                  in[6] = {{x, xb}, {u, db}, {sampling->temperature, rb}, {sampling->top_k, rb}, {sampling->top_p, rb}, {sampling->min_p, rb}};
     if (qg_any_overlap(out, in) || qg_overlap(token, db, logprob, db) || qg_overlap(ws, need, token, db) || qg_overlap(ws, need, logprob, db))
         return hipErrorInvalidValue;
-    SampleArgs A = sample_args(x, rows, cols, sampling);
+    SampleArgs A = sample_args(x, rows, cols, sampling, ws);
     A.u = u;
     A.token = token;
     A.logprob = logprob;
     A.draws = draws;
-    sample_row_kernel<true><<<rows, SA_THREADS, 0, qg_stream()>>>(A);
+    const int pieces = sample_pieces(cols);
+    sample_piece_kernel<<<(unsigned)((size_t)rows * pieces), PIECE_THREADS, 0, qg_stream()>>>(A, pieces);
+    sample_select_kernel<true><<<rows, SA_THREADS, 0, qg_stream()>>>(A, pieces);
     return hipGetLastError();
 }
 
@@ -383,9 +789,12 @@ int qg_sampling_softmax(float *out, const float *x, int rows, int cols, const qg
                  in[4] = {{sampling->temperature, rb}, {sampling->top_k, rb}, {sampling->top_p, rb}, {sampling->min_p, rb}};
     if (qg_any_overlap(written, in) || (out != x && qg_overlap(out, xb, x, xb)) || qg_overlap(ws, need, x, xb) || qg_overlap(ws, need, out, xb))
         return hipErrorInvalidValue;
-    SampleArgs A = sample_args(x, rows, cols, sampling);
+    SampleArgs A = sample_args(x, rows, cols, sampling, ws);
     A.out = out;
-    sample_row_kernel<false><<<rows, SA_THREADS, 0, qg_stream()>>>(A);
+    const int pieces = sample_pieces(cols);
+    sample_piece_kernel<<<(unsigned)((size_t)rows * pieces), PIECE_THREADS, 0, qg_stream()>>>(A, pieces);
+    sample_select_kernel<false><<<rows, SA_THREADS, 0, qg_stream()>>>(A, pieces);
+    sample_probs_kernel<<<(unsigned)((size_t)rows * pieces), PIECE_THREADS, 0, qg_stream()>>>(A, pieces);
     return hipGetLastError();
 }
 
