@@ -13,13 +13,15 @@
 
 namespace {
 
-constexpr int SA_THREADS = 1024, SA_WAVES = SA_THREADS / 64, SA_DIGIT = 11, SA_BINS = 1 << SA_DIGIT, SA_PIECE = 4096;
+constexpr int SA_DIGIT = 11, SA_BINS = 1 << SA_DIGIT, SA_PIECE = 4096;
 constexpr int SA_MAX_COLS = 1 << 24, SA_MAX_DRAWS = 64;
+constexpr int SA_GRID = 64, SA_LISTED = 128;
 
-// What the pass over a piece of a row leaves: its largest value (NaN if there is one), that
-// value's place on the grid, whether weights lie below the bins, and the sum of the weights in no
-// bin, in units of 2^(place / 4).
-struct PieceStat { float top; int at, below, pad; double rest; };
+// What the pass over a piece of a row leaves: its largest value (NaN if there is one) and that
+// value's bin, whether weights lie below the bins it keeps, the last of these, the last whose values
+// are listed, how many are in bins and in the list, and the sums of the weights in no bin and of
+// all, in units of 2^at.
+struct PieceStat { float top; int at, below, known, cover, counted, listed, pad; double rest, all; };
 // What a row came to: its cut, and what its probabilities are formed from.
 struct RowResult { uint32_t t; int last; float top; int state; double a, total; };
 enum { ROW_NAN = 0, ROW_NONE = 1, ROW_CUT = 2 };
@@ -31,6 +33,8 @@ struct SampleArgs {
     int *token;
     int cols, draws, fixed;  // fixed: weights are added up as whole numbers of 2^-fixed where their order is not given
     unsigned long long *bins;  // [rows][pieces][SA_GRID]
+    uint2 *listed;             // [rows][pieces][SA_LISTED] key and index
+    double *kept;              // [rows][pieces] the weight that stays of a piece
     PieceStat *stats;          // [rows][pieces]
     RowResult *results;        // [rows]
 };
@@ -61,6 +65,8 @@ struct Request {
     double a, top_p, min_p;
     int top_k;
     __device__ __forceinline__ bool filters() const { return top_k || top_p < 1.0 || min_p > 0.0; }
+    // whether the sum of all weights matters
+    __device__ __forceinline__ bool weighs_all() const { return !top_k && (top_p < 1.0 || !(min_p > 0.0)); }
 };
 QG_DEV Request read_request(const SampleArgs &A, int row) {
     const float T = A.temperature ? A.temperature[row] : 1.0f, p = A.top_p ? A.top_p[row] : 1.0f, least = A.min_p ? A.min_p[row] : 0.0f;
@@ -109,19 +115,35 @@ QG_DEV void each_value(const float *x, int i0, int end, F f) {
     }
 }
 
+// The least key up to hi for which f holds, which grows with the keys, holds at hi and not at
+// -infinity: a search in 64 ways, by every wave.
+template <typename F>
+QG_DEV uint32_t first_key(uint32_t hi, int lane, F f) {
+    for (uint32_t lo = 0x007fffffu; hi - lo > 1;) {
+        const uint32_t step = (hi - lo - 1) / 64 + 1;
+        const int first = __builtin_ctzll(__ballot(f(key_value(lo + min((uint32_t)(lane + 1) * step, hi - lo)))));
+        const uint32_t up = lo + min((uint32_t)(first + 1) * step, hi - lo);
+        lo += min((uint32_t)first * step, hi - lo);
+        hi = up;
+    }
+    return hi;
+}
+
+template <int WAVES>
 struct RowShared {
     unsigned long long mass[SA_BINS];
     unsigned count[SA_BINS];
-    unsigned long long wave_mass[SA_WAVES], found_mass, found_own;
-    unsigned wave_count[SA_WAVES], found_count, found_ties;
-    int found_bin, bad;
-    float wave_max[SA_WAVES];
+    unsigned long long wave_mass[WAVES], found_mass, found_own;
+    unsigned wave_count[WAVES], found_count, found_ties;
+    int found_bin;
 };
 
 // A row of any shape by one workgroup, which reads it again for every step.
+template <int WAVES>
 struct Row {
+    static constexpr int THREADS = 64 * WAVES, OWN = SA_BINS / THREADS;  // bins of a thread
     const SampleArgs &A;
-    RowShared &s;
+    RowShared<WAVES> &s;
     const float *x;
     const int tid, lane, wave;
     double a;
@@ -130,27 +152,9 @@ struct Row {
     __device__ __forceinline__ double weight(float v) const { return exp2_d(((double)v - (double)m) * a); }
     __device__ __forceinline__ unsigned long long fixed(float v) const { return (unsigned long long)__builtin_rint(__builtin_amdgcn_ldexp(weight(v), A.fixed)); }
 
-    // The largest value; false where nothing can be drawn from the row.
-    __device__ bool largest() {
-        float top = -__builtin_inff();
-        bool nan = false;
-        each_value<SA_THREADS>(x, tid, A.cols, [&](int, float v) { top = fmaxf(top, v); nan |= v != v; });
-        top = qg_wave_max(top);
-        if (__any(nan)) top = __builtin_nanf("");
-        if (lane == 0) s.wave_max[wave] = top;
-        __syncthreads();
-        m = s.wave_max[0];
-        for (int w = 1; w < SA_WAVES; w++) {
-            const float o = s.wave_max[w];
-            m = m != m || o != o ? __builtin_nanf("") : fmaxf(m, o);
-        }
-        __syncthreads();
-        return __builtin_isfinite(m);
-    }
-
     // From the cut's tokens in falling order the first ones that reach `goal` tokens
     // (by_mass false), or the share goal of their weight: never none.
-    __device__ void shorten(Cut &cut, bool by_mass, double goal) {
+    __device__ __forceinline__ void shorten(Cut &cut, bool by_mass, double goal) {
         uint32_t prefix = 0;
         unsigned long long above = 0;
         unsigned over = 0;
@@ -158,39 +162,47 @@ struct Row {
         for (int left = 32; left > 0;) {
             const int bits = left < SA_DIGIT ? left : SA_DIGIT;
             const int shift = left - bits;
-            for (int b = tid; b < SA_BINS; b += SA_THREADS) { s.mass[b] = 0; s.count[b] = 0; }
+            for (int b = tid; b < SA_BINS; b += THREADS) { s.mass[b] = 0; s.count[b] = 0; }
             __syncthreads();
-            each_value<SA_THREADS>(x, tid, A.cols, [&](int i, float v) {
+            each_value<THREADS>(x, tid, A.cols, [&](int i, float v) {
                 const uint32_t key = order_key(v);
                 if ((left < 32 && (key >> left) != prefix) || !cut.keeps(key, i)) return;
-                const int bin = (key >> shift) & (SA_BINS - 1) & ((1 << bits) - 1);
+                const int bin = (key >> shift) & ((1 << bits) - 1);
                 atomicAdd(&s.count[bin], 1u);
                 if (by_mass) atomicAdd(&s.mass[bin], fixed(v));
             });
             __syncthreads();
-            // sums from the largest bin down, two bins a thread
-            const int b1 = SA_BINS - 1 - 2 * tid, b0 = b1 - 1;
-            const unsigned c1 = s.count[b1], c0 = s.count[b0];
-            const unsigned long long m1 = s.mass[b1], m0 = s.mass[b0];
-            unsigned c = wave_upto(c1 + c0, lane);
-            unsigned long long w = wave_upto(m1 + m0, lane);
+            // sums from the largest bin down, OWN neighbours a thread
+            const int b0 = SA_BINS - 1 - OWN * tid;
+            unsigned c = 0;
+            unsigned long long w = 0;
+#pragma unroll
+            for (int k = 0; k < OWN; k++) { c += s.count[b0 - k]; w += s.mass[b0 - k]; }
+            const unsigned own_c = c;
+            const unsigned long long own_w = w;
+            c = wave_upto(c, lane);
+            w = wave_upto(w, lane);
             if (lane == 63) { s.wave_count[wave] = c; s.wave_mass[wave] = w; }
             if (tid == 0) s.found_bin = -1;
             __syncthreads();
             unsigned long long all = 0;
-            for (int k = 0; k < SA_WAVES; k++) {
+            for (int k = 0; k < WAVES; k++) {
                 if (k < wave) { c += s.wave_count[k]; w += s.wave_mass[k]; }
                 all += s.wave_mass[k];
             }
             if (left == 32 && by_mass) need = goal * (double)all;
-            c += over;
-            w += above;
+            c += over - own_c;
+            w += above - own_w;
             // the first bin with which there is enough
             auto enough = [&](unsigned cc, unsigned long long ww) { return cc > 0 && (by_mass ? (double)ww >= need : cc >= (unsigned)need); };
-            const bool e1 = c1 && enough(c - c0, w - m0), e0 = c0 && enough(c, w);
-            const bool was1 = enough(c - c0 - c1, w - m0 - m1), was0 = enough(c - c0, w - m0);
-            if (e1 && !was1) { s.found_bin = b1; s.found_count = c - c0 - c1; s.found_mass = w - m0 - m1; s.found_ties = c1; s.found_own = m1; }
-            if (e0 && !was0) { s.found_bin = b0; s.found_count = c - c0; s.found_mass = w - m0; s.found_ties = c0; s.found_own = m0; }
+#pragma unroll
+            for (int k = 0; k < OWN; k++) {
+                const unsigned n = s.count[b0 - k];
+                const unsigned long long m = s.mass[b0 - k];
+                if (n && enough(c + n, w + m) && !enough(c, w)) { s.found_bin = b0 - k; s.found_count = c; s.found_mass = w; s.found_ties = n; s.found_own = m; }
+                c += n;
+                w += m;
+            }
             __syncthreads();
             if (s.found_bin < 0) return;  // more is asked for than there is
             prefix = prefix << bits | (uint32_t)s.found_bin;
@@ -215,8 +227,8 @@ struct Row {
         __syncthreads();
     }
     // The index of the r-th of the cut's tokens with key t (r from 1), which there are.
-    __device__ int nth(uint32_t t, const Cut &cut, unsigned r) {
-        const int per = ((A.cols + SA_WAVES - 1) / SA_WAVES + 63) / 64 * 64, i0 = wave * per, end = min(i0 + per, A.cols);
+    __device__ __forceinline__ int nth(uint32_t t, const Cut &cut, unsigned r) {
+        const int per = ((A.cols + WAVES - 1) / WAVES + 63) / 64 * 64, i0 = wave * per, end = min(i0 + per, A.cols);
         unsigned n = 0;
         each_value<64>(x, i0 + lane, end, [&](int i, float v) { n += order_key(v) == t && cut.keeps(t, i); });
         n = wave_all_add(n);
@@ -241,64 +253,69 @@ struct Row {
         __syncthreads();
         return s.found_bin;
     }
-    // The least key whose weight is at least `least` (0 < least <= 1): a search in 64 ways, by every wave.
-    __device__ uint32_t least_key(double least) const {
-        uint32_t lo = 0x007fffffu, hi = order_key(m);  // lo's weight is less, hi's is not
-        while (hi - lo > 1) {
-            const uint32_t step = (hi - lo - 1) / 64 + 1, k = lo + min((uint32_t)(lane + 1) * step, hi - lo);
-            const unsigned long long ok = __ballot(weight(key_value(k)) >= least);
-            const int first = __builtin_ctzll(ok);  // the last lane's is hi's
-            const uint32_t up = lo + min((uint32_t)(first + 1) * step, hi - lo);
-            lo += min((uint32_t)first * step, hi - lo);
-            hi = up;
-        }
-        return hi;
+    // The least key whose weight is at least `least` (0 < least <= 1).
+    __device__ __forceinline__ uint32_t least_key(double least) const {
+        return first_key(order_key(m), lane, [&](float v) { return weight(v) >= least; });
     }
 };
 
 // ------------------------------------------------------------------------
-// One pass over the values, in pieces.  The weights' exponents x a lie on a grid of quarter
-// bits; each piece counts and weighs the values of the SA_GRID bins from its
-// largest down, so that all pieces together cover the 16 bits of weight below the row's
-// largest, where filters usually cut.  A weight is 1..2^(1/4) times its bin's lower end: what it
-// has above that, to 2^-39, is added up as a whole number under the count, in one 64-bit atomic
-// whose order does not matter.
+// One pass over the values, in pieces.  The bins are whole bits of the weights' exponents x a,
+// the same for all pieces of a row, so that those of all pieces can be added; a piece keeps the
+// SA_GRID bins from its largest value down, of these only as many as the row's filters
+// may cut in.  A weight is 1..2 times its bin's lower end: what it has above that, to 2^-36, is
+// added up as a whole number under the count, in one 64-bit atomic whose order does not
+// matter.  The values of the first bins, up to SA_LISTED of them, are listed: few tokens
+// stay of most rows, and then nothing is read again.
 // ------------------------------------------------------------------------
-constexpr int SA_GRID = 64, PIECE_THREADS = 256, PIECE_VALUES = SA_PIECE / PIECE_THREADS, GRID_COUNT = 49, GRID_BITS = 39;
-constexpr double GRID_ZERO = 4400.0;        // quarter bits below which a weight is 0 in 64 bits
-constexpr double GRID_FAR = (double)(1 << 21);  // places further out are left to the search over the row
-constexpr int GRID_LOW = -0x7fffffff;       // in place of one: all of the piece's weights are 0 beside a row's largest within half of that
+constexpr int PIECE_THREADS = 256, PIECE_WAVES = PIECE_THREADS / 64, PIECE_VALUES = SA_PIECE / PIECE_THREADS, BIN_COUNT = 49, BIN_BITS = 36;
+constexpr double GRID_ZERO = 1100.0;            // bits below which a weight is 0
+constexpr double GRID_FAR = (double)(1 << 19);  // places further out are left to the search over the row
+constexpr int GRID_LOW = -(1 << 30);           // in place of one: the piece's weights are 0 beside a row's largest within half of that
 
-// 2^(f / 4), 0 <= f < 1, at least 1: the Taylor series about f = 1/2, whose next term is below 1e-17.
-QG_DEV double quarter_power(double f) {
-    constexpr double h = 0.173286795139986327354, at_half = 1.09050773266525765921;  // ln 2 / 4, 2^(1/8)
-    constexpr double c1 = at_half * h, c2 = c1 * h / 2, c3 = c2 * h / 3, c4 = c3 * h / 4, c5 = c4 * h / 5, c6 = c5 * h / 6, c7 = c6 * h / 7, c8 = c7 * h / 8,
-                     c9 = c8 * h / 9;
-    const double c[9] = {at_half, c1, c2, c3, c4, c5, c6, c7, c8}, y = f - 0.5;
-    double p = c9;
+QG_DEV double grid_place(float x, double a) { return __builtin_floor((double)x * a); }
+// 2^f, 0 <= f < 1, at least 1: the Taylor series about f = 1/2, whose next term is below 1e-16.
+QG_DEV double power_of(double f) {
+    constexpr double h = 0.693147180559945309417, c0 = 1.41421356237309504880;
+    constexpr double c1 = c0 * h, c2 = c1 * h / 2, c3 = c2 * h / 3, c4 = c3 * h / 4, c5 = c4 * h / 5, c6 = c5 * h / 6, c7 = c6 * h / 7, c8 = c7 * h / 8,
+                     c9 = c8 * h / 9, c10 = c9 * h / 10, c11 = c10 * h / 11, c12 = c11 * h / 12;
+    const double c[12] = {c0, c1, c2, c3, c4, c5, c6, c7, c8, c9, c10, c11}, y = f - 0.5;
+    double p = c12;
 #pragma unroll
-    for (int i = 8; i >= 0; i--) p = __builtin_fma(p, y, c[i]);
+    for (int i = 11; i >= 0; i--) p = __builtin_fma(p, y, c[i]);
     return __builtin_fmax(p, 1.0);
 }
-QG_DEV double grid_scale(int quarters) {  // 2^(quarters / 4)
-    const int j = quarters & 3;
-    const double c = j == 0 ? 1.0 : j == 1 ? 1.18920711500272106672 : j == 2 ? 1.41421356237309504880 : 1.68179283050742908606;
-    return __builtin_amdgcn_ldexp(c, quarters >> 2);
+// What a weight 2^f adds to its bin; a bin's weights in units of the lower end of bin 0.
+QG_DEV unsigned long long bin_entry(double f) {
+    // f may have been rounded to 1, and its power to 2
+    const unsigned long long m = (unsigned long long)__double_as_longlong(__builtin_fmin(power_of(f), 0x1.fffffffffffffp0)) & ((1ULL << 52) - 1);
+    return ((m + (1ULL << (51 - BIN_BITS))) >> (52 - BIN_BITS)) + (1ULL << BIN_COUNT);
 }
-QG_DEV double grid_place(float x, double a4) { return __builtin_floor((double)x * a4); }
+QG_DEV unsigned bin_count(unsigned long long b) { return (unsigned)(b >> BIN_COUNT); }
+QG_DEV unsigned long long bin_excess(unsigned long long b) { return b & ((1ULL << BIN_COUNT) - 1); }
+QG_DEV double bin_mass(unsigned n, unsigned long long excess, int bin) {
+    return __builtin_amdgcn_ldexp((double)n + __builtin_amdgcn_ldexp((double)excess, -BIN_BITS), -bin);
+}
 QG_DEV float larger_or_nan(float a, float b) { return a != a || b != b ? __builtin_nanf("") : fmaxf(a, b); }
+// The last bin that a row's filters may cut in, from what they ask for: less than 2^bits values of a weight
+// below 2^-d of the largest are less than 2^(bits - d) of the sum.
+QG_DEV int deepest_bin(const Request &q, int bits) {
+    if (q.top_k) return SA_GRID - 1;
+    const double least = q.top_p < 1.0 ? (1.0 - q.top_p) * __builtin_amdgcn_ldexp(1.0, -bits) : q.min_p;
+    return min(2 - __builtin_amdgcn_frexp_exp(least), SA_GRID - 1);
+}
 
 __global__ __launch_bounds__(PIECE_THREADS) void sample_piece_kernel(SampleArgs A, int pieces) {
-    constexpr int W = PIECE_THREADS / 64;
     __shared__ unsigned long long s_bin[SA_GRID];
-    __shared__ float s_top[W];
-    __shared__ double s_rest[W];
-    __shared__ int s_below[W];
+    __shared__ unsigned s_most[SA_GRID];
+    __shared__ float s_top[PIECE_WAVES], s_value[SA_PIECE];
+    __shared__ uint16_t s_index[SA_PIECE];
+    __shared__ double s_rest[PIECE_WAVES];
+    __shared__ int s_below[PIECE_WAVES], s_cover, s_listed;
     const int row = blockIdx.x / pieces, piece = blockIdx.x % pieces, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const Request q = read_request(A, row);
-    const int n = min(SA_PIECE, A.cols - piece * SA_PIECE);
-    const float *x = A.x + (size_t)row * A.cols + (size_t)piece * SA_PIECE + tid;
-    float v[PIECE_VALUES], top = -__builtin_inff();
+    const int c0 = piece * SA_PIECE, n = min(SA_PIECE, A.cols - c0);
+    const float *x = A.x + (size_t)row * A.cols + c0 + tid;
+    float v[PIECE_VALUES], own = -__builtin_inff();
     if (n == SA_PIECE) {
 #pragma unroll
         for (int k = 0; k < PIECE_VALUES; k++) v[k] = x[k * PIECE_THREADS];
@@ -306,369 +323,539 @@ __global__ __launch_bounds__(PIECE_THREADS) void sample_piece_kernel(SampleArgs 
 #pragma unroll
         for (int k = 0; k < PIECE_VALUES; k++) v[k] = k * PIECE_THREADS + tid < n ? x[k * PIECE_THREADS] : -__builtin_inff();
     }
-    if (tid < SA_GRID) s_bin[tid] = 0;
+    const Request q = read_request(A, row);
+    if (tid < SA_GRID) { s_bin[tid] = 0; s_most[tid] = 0; }
+    if (tid == 0) s_listed = 0;
     bool nan = false;
 #pragma unroll
-    for (int k = 0; k < PIECE_VALUES; k++) { top = fmaxf(top, v[k]); nan |= v[k] != v[k]; }
-    top = qg_wave_max(top);
+    for (int k = 0; k < PIECE_VALUES; k++) { own = fmaxf(own, v[k]); nan |= v[k] != v[k]; }
+    float top = qg_wave_max(own);
     if (__any(nan)) top = __builtin_nanf("");
     if (lane == 0) s_top[wave] = top;
     __syncthreads();
     top = s_top[0];
 #pragma unroll
-    for (int w = 1; w < W; w++) top = larger_or_nan(top, s_top[w]);
-    const double a4 = q.a * 4.0, place = grid_place(top, a4);
+    for (int w = 1; w < PIECE_WAVES; w++) top = larger_or_nan(top, s_top[w]);
+    const double place = grid_place(top, q.a);
     const size_t at = (size_t)row * pieces + piece;
     if (!(__builtin_fabs(place) < GRID_FAR)) {  // NaN and infinities too
-        if (tid == 0) A.stats[at] = PieceStat{top, GRID_LOW, 0, 0, 0.0};
+        if (tid == 0) A.stats[at] = PieceStat{top, GRID_LOW, 0, SA_GRID - 1, SA_GRID - 1, 0, 0, 0, 0.0, 0.0};
         return;
     }
-    const bool filter = q.filters(), rest_counts = !q.top_k;
-    double rest = 0.0;
+    const bool filter = q.filters(), weigh = q.weighs_all();
+    int known = filter ? deepest_bin(q, 62 - A.fixed) : -1;
+    if (q.top_k && q.top_k <= PIECE_THREADS / 2) {
+        // the row's top_k values are not below the piece's, and these not below the top_k-th of its threads' largest
+        const double d = place - grid_place(own, q.a);
+        if (d < SA_GRID) atomicAdd(&s_most[(int)d], 1u);
+        __syncthreads();
+        const unsigned long long enough = __ballot(wave_upto(s_most[lane], lane) >= (unsigned)q.top_k);
+        if (enough) known = __builtin_ctzll(enough);
+    }
+    // the wave's values that may be in a bin go together, so that few of its steps form a weight
+    float *mine = s_value + wave * (64 * PIECE_VALUES);
+    uint16_t *mine_at = s_index + wave * (64 * PIECE_VALUES);
+    const float near = filter ? (float)((double)top - (known + 2) / q.a - 1e-6 * __builtin_fabs((double)top)) : __builtin_inff();
+    const float zero = (float)((double)top - GRID_ZERO / q.a);
+    int held = 0;
     bool below = false;
 #pragma unroll
     for (int k = 0; k < PIECE_VALUES; k++) {
-        const double e = (double)v[k] * a4, b = __builtin_floor(e), d = place - b;
-        if (!(d < GRID_ZERO)) continue;
-        if (filter && d < SA_GRID) {
-            const unsigned long long m = (unsigned long long)__double_as_longlong(quarter_power(e - b)) & ((1ULL << 52) - 1);
-            atomicAdd(&s_bin[(int)d], ((m + (1ULL << (51 - GRID_BITS))) >> (52 - GRID_BITS)) + (1ULL << GRID_COUNT));
-        } else {
+        const bool is = v[k] >= near;
+        const unsigned long long all = __ballot(is);
+        if (is) {
+            const int to = held + __popcll(all & ((1ULL << lane) - 1));
+            mine[to] = v[k];
+            mine_at[to] = (uint16_t)(k * PIECE_THREADS + tid);
+        }
+        held += __popcll(all);
+        below |= !is && v[k] >= zero;
+    }
+    double rest = 0.0;
+    if (weigh) {
+#pragma unroll
+        for (int k = 0; k < PIECE_VALUES; k++) {
+            const double e = (double)v[k] * q.a, b = __builtin_floor(e), d = place - b;
+            if (!(v[k] >= near) && d < GRID_ZERO) rest += __builtin_amdgcn_ldexp(power_of(e - b), -(int)d);
+        }
+    }
+    __builtin_amdgcn_wave_barrier();  // a wave's own values
+    for (int i = lane; i < held; i += 64) {
+        const double e = (double)mine[i] * q.a, b = __builtin_floor(e), d = place - b;
+        if (d <= (double)known) {
+            atomicAdd(&s_bin[(int)d], bin_entry(e - b));
+        } else if (d < GRID_ZERO) {
             below = true;
-            if (rest_counts) rest += quarter_power(e - b) * grid_scale(-(int)d);
+            rest += __builtin_amdgcn_ldexp(power_of(e - b), -(int)d);
         }
     }
     rest = wave_all_add(rest);
     below = __any(below);
     if (lane == 0) { s_rest[wave] = rest; s_below[wave] = below; }
     __syncthreads();
-    if (filter && tid < SA_GRID) A.bins[at * SA_GRID + tid] = s_bin[tid];
-    if (tid == 0) {
-        PieceStat p{top, (int)place, 0, 0, 0.0};
+    if (wave == 0) {
+        const int most = q.top_k ? min(max(2 * q.top_k, 32), SA_LISTED) : SA_LISTED;  // a piece may hold all top_k, of a bin's about half
+        const unsigned long long b = s_bin[lane];
+        const unsigned upto = wave_upto(bin_count(b), lane);
+        const int cover = min((int)__popcll(__ballot(upto <= (unsigned)most)) - 1, known), listed = cover < 0 ? 0 : (int)__shfl(upto, cover);
+        const int counted = (int)__shfl(upto, SA_GRID - 1);
+        const double in = wave_all_add(bin_mass(bin_count(b), bin_excess(b), lane));
+        if (filter) A.bins[at * SA_GRID + lane] = b;
+        if (lane == 0) {
+            s_cover = cover;
+            PieceStat p{top, (int)place, 0, known, cover, counted, listed, 0, 0.0, 0.0};
 #pragma unroll
-        for (int w = 0; w < W; w++) { p.rest += s_rest[w]; p.below |= s_below[w]; }
-        A.stats[at] = p;
+            for (int w = 0; w < PIECE_WAVES; w++) { p.rest += s_rest[w]; p.below |= s_below[w]; }
+            p.all = in + p.rest;
+            A.stats[at] = p;
+        }
+    }
+    if (!filter) return;
+    __syncthreads();
+    const int cover = s_cover;
+    uint2 *listed = A.listed + at * SA_LISTED;
+    for (int i = lane; i < held; i += 64) {
+        const float y = mine[i];
+        if (!(place - grid_place(y, q.a) <= (double)cover)) continue;
+        const int to = atomicAdd(&s_listed, 1);
+        if (to < SA_LISTED) listed[to] = make_uint2(order_key(y), c0 + mine_at[i]);
     }
 }
 
 // ------------------------------------------------------------------------
-// A row's cut, and its draws, by one workgroup.  The bins of all pieces together say in which one
-// a filter cuts; where in it say its values, read again from the pieces that have some
-// and ranked.  What the bins do not reach is left to the search over the whole row.
+// A row's cut, and its draws, by one workgroup.  The bins of all pieces say in which one a filter cuts; its
+// values, from the lists where these reach and else read again from the pieces that have some, are
+// ranked (of a bin with too many, those of the 64th part in which the cut is).  What the bins do not
+// hold is left to the search over the whole row.
 // ------------------------------------------------------------------------
-constexpr int SA_LIST = 1024;
+constexpr int SA_LIST = 1024;  // values that are ranked
+template <int WAVES>
 struct GridShared {
-    unsigned count[SA_WAVES][SA_GRID];
-    unsigned long long mant[SA_WAVES][SA_GRID];
+    unsigned count[WAVES][SA_GRID];
+    unsigned long long excess[WAVES][SA_GRID];
     uint32_t key[SA_LIST], sorted_key[SA_LIST];
     int index[SA_LIST], sorted_index[SA_LIST];
-    double upto[SA_LIST], wave_sum[SA_WAVES];
-    int listed;
+    double upto[SA_LIST], wave_sum[WAVES];
+    int n, hits;
 };
+template <int WAVES>
 struct SelectShared {
-    union { RowShared row; GridShared grid; };
-    double piece[SA_MAX_COLS / SA_PIECE];  // what stays of each piece
-    float top[SA_WAVES];
-    int flag[SA_WAVES];
+    union { RowShared<WAVES> row; GridShared<WAVES> grid; };
+    float top[WAVES];
+    int flag[WAVES], reach[WAVES], known[WAVES];
 };
 
+template <int WAVES>
 struct Grid {
-    const SampleArgs &A;
-    GridShared &s;
-    const Row &r;
+    static constexpr int THREADS = 64 * WAVES;
+    GridShared<WAVES> &s;
+    const float *x;
     const unsigned long long *bins;
     const PieceStat *stats;
-    const int pieces, tid, lane, wave, place;  // place: of the row's largest value
-    const double a4, unit;                     // unit: of a weight of place's lower end, the largest value's being 1
-    // lane D of each wave: values in bin D from the top, their weight, and both with the bins above
+    const uint2 *lists;
+    const int cols, pieces, tid, lane, wave, place;  // place: of the row's largest value
+    const float m;
+    const double a, unit;                            // unit: of a weight at place's lower end, the largest value's being 1
+    int reach, known;                                // bins 0..reach are in the lists, 0..known in the bins
+    bool below;                                      // whether the row has weights below the known bins
+    // lane D of each wave: values in bin D from the top and with the bins above, and their weight
     unsigned count, count_upto;
     double mass, mass_upto;
-    int bin, kept;                             // the listed bin (-1: none), and how many of its values stay
+    int deepest;                                     // the bin of the cut
+    int bin, kept;                                   // the ranked bin (-1: none, or a part of one), and how many of the ranked values stay
+    bool part;                                       // the cut is in a part of its bin
 
-    // A piece's bin of a lane, moved to the row's grid; 0 where it has none.
-    __device__ __forceinline__ unsigned long long bin_of(int p, int &delta) const {
+    __device__ __forceinline__ double weight(uint32_t key) const { return exp2_d(((double)key_value(key) - (double)m) * a); }
+    __device__ __forceinline__ double place_of(uint32_t key) const { return grid_place(key_value(key), a); }
+    // the 64th of its bin that a value is in, from the top
+    static __device__ __forceinline__ int part_of(double e) { return 63 - min((int)((e - __builtin_floor(e)) * 64.0), 63); }
+    // A piece's bin of a lane, moved to the row's.
+    __device__ __forceinline__ int moved_by(int p) const {
         const int at = stats[p].at;
-        delta = at == GRID_LOW ? SA_GRID : min(place - at, SA_GRID);
-        const unsigned long long own = delta < SA_GRID ? bins[(size_t)p * SA_GRID + lane] : 0;
-        return own;
+        return at == GRID_LOW ? SA_GRID : min(place - at, SA_GRID);
     }
-    __device__ __forceinline__ unsigned long long moved(unsigned long long own, int delta) const {
-        const unsigned long long b = __shfl(own, (lane - delta) & 63);
-        return lane >= delta ? b : 0;
+    __device__ __forceinline__ unsigned long long row_bin(int p) const {
+        const int delta = moved_by(p);
+        return lane >= delta ? bins[(size_t)p * SA_GRID + lane - delta] : 0;
     }
-    static __device__ __forceinline__ double mass_of(unsigned n, unsigned long long mant, int bin) {
-        return ((double)n + (double)mant * __builtin_amdgcn_ldexp(1.0, -GRID_BITS)) * grid_scale(-bin);
-    }
-    // All pieces' bins; whether the row has weights below them.
-    __device__ bool add_up(int *flag) {
-        unsigned n = 0;
-        unsigned long long m = 0;
-        bool below = false;
-        for (int p = wave; p < pieces; p += SA_WAVES) {
-            int delta;
-            const unsigned long long own = bin_of(p, delta), b = moved(own, delta);
-            below |= own && lane + delta >= SA_GRID;
-            if (stats[p].at != GRID_LOW && place - stats[p].at < (int)GRID_ZERO) below |= stats[p].below || delta >= SA_GRID;
-            n += (unsigned)(b >> GRID_COUNT);
-            m += b & ((1ULL << GRID_COUNT) - 1);
-        }
-        below = __any(below);
-        s.count[wave][lane] = n;
-        s.mant[wave][lane] = m;
-        if (lane == 0) flag[wave] = below;
+    __device__ __forceinline__ void all_waves(unsigned n, unsigned long long excess, unsigned &c, unsigned long long &e) {
         __syncthreads();
-        count = 0;
-        m = 0;
-        below = false;
+        s.count[wave][lane] = n;
+        s.excess[wave][lane] = excess;
+        __syncthreads();
+        c = 0;
+        e = 0;
 #pragma unroll
-        for (int w = 0; w < SA_WAVES; w++) {
-            count += s.count[w][lane];
-            m += s.mant[w][lane];
-            below |= flag[w] != 0;
+        for (int w = 0; w < WAVES; w++) { c += s.count[w][lane]; e += s.excess[w][lane]; }
+    }
+    __device__ __forceinline__ void add_up() {
+        unsigned n = 0;
+        unsigned long long e = 0;
+        for (int p0 = wave; p0 < pieces; p0 += 4 * WAVES) {
+            unsigned long long b[4];
+#pragma unroll
+            for (int k = 0; k < 4; k++) b[k] = p0 + k * WAVES < pieces ? row_bin(p0 + k * WAVES) : 0;
+#pragma unroll
+            for (int k = 0; k < 4; k++) { n += bin_count(b[k]); e += bin_excess(b[k]); }
         }
-        mass = mass_of(count, m, lane) * unit;
+        all_waves(n, e, count, e);
+        mass = bin_mass(count, e, lane) * unit;
         count_upto = wave_upto(count, lane);
         mass_upto = wave_upto(mass, lane);
-        return below;
-    }
-    __device__ __forceinline__ double above(int D) const { return D ? __shfl(mass_upto, D - 1) : 0.0; }
-    // The values of bin D in falling order with the sums of their weights; false if they are too many.
-    __device__ bool list(int D) {
-        const unsigned n = __shfl(count, D);
-        if (n > SA_LIST) return false;
-        __syncthreads();
-        if (tid == 0) s.listed = 0;
-        __syncthreads();
-        const double b = (double)(place - D);
-        for (int p = wave; p < pieces; p += SA_WAVES) {
-            int delta;
-            const unsigned long long own = bin_of(p, delta);
-            if (D < delta || !(__shfl(own, (D - delta) & 63) >> GRID_COUNT)) continue;
-            each_value<64>(r.x, p * SA_PIECE + lane, min((p + 1) * SA_PIECE, A.cols), [&](int i, float v) {
-                if (grid_place(v, a4) != b) return;
-                const int k = atomicAdd(&s.listed, 1);
-                if (k < SA_LIST) { s.key[k] = order_key(v); s.index[k] = i; }
-            });
-        }
-        __syncthreads();
-        double w = 0.0;
-        if (tid < (int)n) {
-            const uint32_t key = s.key[tid];
-            const int i = s.index[tid];
-            int rank = 0;
-            for (int k = 0; k < (int)n; k++) rank += s.key[k] > key || (s.key[k] == key && s.index[k] < i);
-            s.sorted_key[rank] = key;
-            s.sorted_index[rank] = i;
-        }
-        __syncthreads();
-        if (tid < (int)n) w = r.weight(key_value(s.sorted_key[tid]));
-        w = wave_upto(w, lane);
-        if (lane == 63) s.wave_sum[wave] = w;
-        __syncthreads();
-        for (int k = 0; k < wave; k++) w += s.wave_sum[k];
-        s.upto[tid] = w;
-        __syncthreads();
-        bin = D;
-        kept = (int)n;
-        return true;
-    }
-    // The least key of place b, which is the place of some value of a piece or more: a search in 64 ways.
-    __device__ uint32_t first_key(double b) const {
-        uint32_t lo = 0x007fffffu, hi = order_key(r.m);
-        while (hi - lo > 1) {
-            const uint32_t step = (hi - lo - 1) / 64 + 1, k = lo + min((uint32_t)(lane + 1) * step, hi - lo);
-            const int first = __builtin_ctzll(__ballot(grid_place(key_value(k), a4) >= b));
-            const uint32_t up = lo + min((uint32_t)(first + 1) * step, hi - lo);
-            lo += min((uint32_t)first * step, hi - lo);
-            hi = up;
-        }
-        return hi;
-    }
-    // The row's cut and the weight that stays; false where the bins do not reach.
-    __device__ bool select(const Request &q, Cut &cut, double &total, int &last_bin, int *flag) {
-        const bool below = add_up(flag);
+        deepest = SA_GRID - 1;
         bin = -1;
         kept = 0;
-        last_bin = SA_GRID;  // bins above it stay whole
-        if (q.top_k) {
-            const unsigned long long enough = __ballot(count_upto >= (unsigned)q.top_k);
-            if (!enough && below) return false;
-            if (enough) {
-                const int D = __builtin_ctzll(enough);
-                const int left = q.top_k - (int)(__shfl(count_upto, D) - __shfl(count, D));
-                if (left == (int)__shfl(count, D)) {  // all of the bin
-                    cut = Cut{first_key((double)(place - D)), 0x7fffffff};
-                    last_bin = D + 1;
-                    total = __shfl(mass_upto, D);
-                } else {
-                    if (!list(D)) return false;
-                    kept = left;
-                    last_bin = D;
-                    cut = Cut{s.sorted_key[left - 1], s.sorted_index[left - 1]};
-                    total = above(D) + s.upto[left - 1];
-                }
-            } else {
-                total = __shfl(mass_upto, SA_GRID - 1);
-            }
-        }
-        if (q.top_p < 1.0) {
-            if (!q.top_k) {
-                total = 0.0;  // of all pieces, whatever lies in bins
-                for (int p = wave; p < pieces; p += SA_WAVES) {
-                    int delta;
-                    const unsigned long long own = bin_of(p, delta);
-                    const double in = wave_all_add(mass_of((unsigned)(own >> GRID_COUNT), own & ((1ULL << GRID_COUNT) - 1), lane));
-                    if (stats[p].at != GRID_LOW) total += (in + stats[p].rest) * grid_scale(stats[p].at - place) * unit;
-                }
-                __syncthreads();
-                if (lane == 0) s.wave_sum[wave] = total;
-                __syncthreads();
-                total = 0.0;
+        part = false;
+    }
+    __device__ __forceinline__ void put(uint32_t key, int i) {
+        const int k = atomicAdd(&s.n, 1);
+        if (k < SA_LIST) { s.key[k] = key; s.index[k] = i; }
+    }
+    // f(key, index) of the values in bin D (every lane of some waves each), and of more
+    template <typename F>
+    __device__ __forceinline__ void each_of_bin(int D, F f) {
+        if (D <= reach) {
+            for (int e0 = wave; e0 < pieces * (SA_LISTED / 64); e0 += 4 * WAVES) {
+                uint2 y[4];
 #pragma unroll
-                for (int w = 0; w < SA_WAVES; w++) total += s.wave_sum[w];
-            }
-            const double goal = q.top_p * total;
-            const unsigned long long enough = __ballot(count_upto > 0 && mass_upto >= goal);
-            if (!enough && below) return false;
-            const int D = enough ? __builtin_ctzll(enough) : SA_GRID - 1;
-            if (D < last_bin || D == bin) {
-                if (D != bin && !list(D)) return false;
-                const double before = above(D);
-                // the first of the bin's values that reaches the goal
-                __syncthreads();
-                if (tid == 0) s.listed = kept - 1;
-                __syncthreads();
-                if (tid < kept && before + s.upto[tid] >= goal) atomicMin(&s.listed, tid);
-                __syncthreads();
-                if (kept > 0) {
-                    kept = s.listed + 1;
-                    last_bin = D;
-                    cut = Cut{s.sorted_key[kept - 1], s.sorted_index[kept - 1]};
-                    total = before + s.upto[kept - 1];
+                for (int k = 0; k < 4; k++) {
+                    const int e = e0 + k * WAVES, p = e / (SA_LISTED / 64), i = e % (SA_LISTED / 64) * 64 + lane;
+                    y[k] = e < pieces * (SA_LISTED / 64) && stats[p].at != GRID_LOW && i < min(stats[p].listed, SA_LISTED) ? lists[(size_t)p * SA_LISTED + i] : make_uint2(0, 0);
                 }
+#pragma unroll
+                for (int k = 0; k < 4; k++)
+                    if (y[k].x) f(y[k].x, (int)y[k].y);
+            }
+            return;
+        }
+        // the pieces that have some, then their quarters
+        int *hits = s.sorted_index;
+        __syncthreads();
+        if (tid == 0) s.hits = 0;
+        __syncthreads();
+        for (int p = tid; p < pieces; p += THREADS) {
+            const int delta = moved_by(p);
+            if (D >= delta && bins[(size_t)p * SA_GRID + D - delta]) {
+                const int k = atomicAdd(&s.hits, 1);
+                if (k < SA_LIST) hits[k] = p;
             }
         }
-        if (q.min_p > 0.0) {
-            const uint32_t t = r.least_key(q.min_p);
-            if (t > cut.t) {
-                const double d = (double)place - grid_place(key_value(t), a4);
-                if (!(d < SA_GRID)) {
-                    if (below) return false;
+        __syncthreads();
+        const bool fit = s.hits <= SA_LIST;
+        const int items = (fit ? s.hits : pieces) * 4;
+        for (int it = wave; it < items; it += WAVES) {
+            const int i0 = (fit ? hits[it >> 2] : it >> 2) * SA_PIECE + (it & 3) * (SA_PIECE / 4) + lane;
+            float v[16];
+#pragma unroll
+            for (int k = 0; k < 16; k++) v[k] = i0 + k * 64 < cols ? x[i0 + k * 64] : -__builtin_inff();
+#pragma unroll
+            for (int k = 0; k < 16; k++)
+                if (v[k] > -__builtin_inff()) f(order_key(v[k]), i0 + k * 64);
+        }
+    }
+    // Ranks s.key, s.index [s.n]: by falling value, or by index.
+    template <bool BY_INDEX>
+    __device__ __forceinline__ void rank(int n) {
+        __syncthreads();
+        for (int i = tid; i < n; i += THREADS) {
+            const uint32_t key = s.key[i];
+            const int at = s.index[i];
+            int rank = 0;
+            for (int k = 0; k < n; k++) rank += BY_INDEX ? s.index[k] < at : s.key[k] > key || (s.key[k] == key && s.index[k] < at);
+            s.sorted_key[rank] = key;
+            s.sorted_index[rank] = at;
+        }
+        __syncthreads();
+        // the sums of their weights
+        double before = 0.0;
+        for (int i0 = 0; i0 < n; i0 += THREADS) {
+            const int i = i0 + tid;
+            double w = wave_upto(i < n ? weight(s.sorted_key[i]) : 0.0, lane);
+            __syncthreads();
+            if (lane == 63) s.wave_sum[wave] = w;
+            __syncthreads();
+            double all = 0.0;
+#pragma unroll
+            for (int k = 0; k < WAVES; k++) {
+                if (k < wave) w += s.wave_sum[k];
+                all += s.wave_sum[k];
+            }
+            if (i < n) s.upto[i] = before + w;
+            before += all;
+        }
+        __syncthreads();
+    }
+    // Shortens the cut: to the first `target` tokens, to the first that weigh `target`, or to keys from t on; total: what
+    // stays weighs.  False where the known bins do not reach.
+    enum { BY_COUNT, BY_MASS, BY_KEY };
+    template <int BY>
+    __device__ __forceinline__ bool shorten(double target, uint32_t t, Cut &cut, double &total) {
+        int D;
+        if (BY == BY_KEY) {
+            const double d = (double)place - place_of(t);
+            if (!(d <= (double)known)) return !below;  // nothing that weighs lies below
+            D = (int)d;
+        } else {
+            const unsigned long long enough = __ballot(lane <= known && count_upto > 0 && (BY == BY_MASS ? mass_upto >= target : (double)count_upto >= target));
+            if (!enough) return !below;
+            D = __builtin_ctzll(enough);
+            if (D > deepest) return true;  // sums that differ in their last bits
+        }
+        const int n = (int)__shfl(count, D);
+        int first = (int)__shfl(count_upto, D) - n;
+        double before = D ? __shfl(mass_upto, D - 1) : 0.0;
+        if (BY == BY_COUNT && first + n == (int)target) {  // all of the bin
+            cut = Cut{first_key(order_key(m), lane, [&](float v) { return grid_place(v, a) >= (double)(place - D); }), 0x7fffffff};
+            deepest = D;
+            total = __shfl(mass_upto, D);
+            return true;
+        }
+        if (D != bin) {
+            const double b = (double)(place - D);
+            int sub = -1;
+            if (n > SA_LIST) {
+                __syncthreads();
+                if (wave == 0) { s.count[0][lane] = 0; s.excess[0][lane] = 0; }
+                __syncthreads();
+                each_of_bin(D, [&](uint32_t key, int i) {
+                    const double e = (double)key_value(key) * a;
+                    if (__builtin_floor(e) != b || !cut.keeps(key, i)) return;
+                    atomicAdd(&s.count[0][part_of(e)], 1u);
+                    // up to 2^24 values of less than 2^37 above their count
+                    atomicAdd(&s.excess[0][part_of(e)], bin_excess(bin_entry(e - b)));
+                });
+                __syncthreads();
+                const unsigned c = s.count[0][lane], c_upto = wave_upto(c, lane);
+                const double w = bin_mass(c, s.excess[0][lane], D) * unit, w_upto = wave_upto(w, lane);
+                if (BY == BY_KEY) {
+                    sub = part_of((double)key_value(t) * a);
                 } else {
-                    const int D = (int)d;
-                    if (D != bin && !list(D)) return false;
-                    const int n = __syncthreads_count(tid < kept && s.sorted_key[tid] >= t);
-                    kept = n;
-                    last_bin = D;
-                    cut = Cut{t, 0x7fffffff};
-                    total = above(D) + (n ? s.upto[n - 1] : 0.0);
+                    const unsigned long long enough = __ballot(c > 0 && (BY == BY_MASS ? before + w_upto >= target : (double)first + c_upto >= target));
+                    const unsigned long long some = __ballot(c > 0);
+                    if (!some) return true;
+                    sub = enough ? __builtin_ctzll(enough) : 63 - __builtin_clzll(some);
                 }
+                if (__shfl(c, sub) > SA_LIST) return false;
+                first += (int)__shfl(c_upto - c, sub);
+                before += __shfl(w_upto - w, sub);
             }
+            __syncthreads();
+            if (tid == 0) s.n = 0;
+            __syncthreads();
+            each_of_bin(D, [&](uint32_t key, int i) {
+                const double e = (double)key_value(key) * a;
+                if (__builtin_floor(e) == b && cut.keeps(key, i) && (sub < 0 || part_of(e) == sub)) put(key, i);
+            });
+            __syncthreads();
+            kept = min(s.n, SA_LIST);
+            rank<false>(kept);
+            part = sub >= 0;
+            bin = part ? -1 : D;
         }
-        if (!q.top_k && !(q.top_p < 1.0) && last_bin == SA_GRID) total = __shfl(mass_upto, SA_GRID - 1);  // min-p that drops nothing
+        int stay;
+        if (BY == BY_COUNT) {
+            stay = min((int)target - first, kept);
+        } else {
+            __syncthreads();
+            if (tid == 0) s.n = kept;
+            __syncthreads();
+            for (int i = tid; i < kept; i += THREADS)
+                if (BY == BY_MASS ? before + s.upto[i] >= target : s.sorted_key[i] < t) atomicMin(&s.n, i);
+            __syncthreads();
+            stay = BY == BY_MASS ? min(s.n + 1, kept) : s.n;
+        }
+        if (BY != BY_KEY && stay <= 0) return true;
+        kept = stay;
+        deepest = D;
+        cut = BY == BY_KEY ? Cut{t, 0x7fffffff} : Cut{s.sorted_key[kept - 1], s.sorted_index[kept - 1]};
+        total = before + (kept ? s.upto[kept - 1] : 0.0);
         return true;
     }
-    // What stays of each piece: its bins above the last one, and the listed values that are its.
-    __device__ void weigh_pieces(int last_bin, double *piece) const {
-        for (int p = wave; p < pieces; p += SA_WAVES) {
-            int delta;
-            const unsigned long long b = moved(bin_of(p, delta), delta);
-            double sum = lane < last_bin ? mass_of((unsigned)(b >> GRID_COUNT), b & ((1ULL << GRID_COUNT) - 1), lane) * unit : 0.0;
-            if (last_bin == bin)
+    // What stays of each piece: its bins above the last one, and the ranked values that are its.  False where the bins do not say.
+    __device__ __forceinline__ bool weigh_pieces(const Cut &cut, double *piece) const {
+        if (part) return false;
+        const int whole = cut.t == 0 || deepest != bin ? deepest + 1 : deepest;
+        for (int p = wave; p < pieces; p += WAVES) {
+            const unsigned long long b = row_bin(p);
+            double sum = lane < whole ? bin_mass(bin_count(b), bin_excess(b), lane) * unit : 0.0;
+            if (whole == deepest)
                 for (int k = lane; k < kept; k += 64)
-                    if (s.sorted_index[k] / SA_PIECE == p) sum += r.weight(key_value(s.sorted_key[k]));
+                    if (s.sorted_index[k] / SA_PIECE == p) sum += weight(s.sorted_key[k]);
             sum = wave_all_add(sum);
             if (lane == 0) piece[p] = sum;
         }
+        return true;
+    }
+    // All that stays, from the lists, in the tokens' order: s.sorted_key, s.sorted_index and s.upto; their number, 0 where the lists do
+    // not hold it or it is too many.
+    __device__ __forceinline__ int order(const Cut &cut) {
+        if (deepest > reach || __shfl(count_upto, deepest) > 4 * SA_LIST) return 0;
+        __syncthreads();
+        if (tid == 0) s.n = 0;
+        __syncthreads();
+        each_of_bin(0, [&](uint32_t key, int i) {
+            if ((double)place - place_of(key) <= (double)deepest && cut.keeps(key, i)) put(key, i);
+        });
+        __syncthreads();
+        const int n = s.n;
+        if (n > SA_LIST) return 0;
+        rank<true>(n);
+        return n;
     }
 };
 
+// A row from which nothing can be drawn.
 template <bool DRAW>
-__global__ __launch_bounds__(SA_THREADS) void sample_select_kernel(SampleArgs A, int pieces) {
-    __shared__ SelectShared s;
+QG_DEV void no_draw(const SampleArgs &A, int row, int tid, float top) {
+    if (DRAW) {
+        if (tid < A.draws) {
+            A.token[(size_t)row * A.draws + tid] = -1;
+            if (A.logprob) A.logprob[(size_t)row * A.draws + tid] = __builtin_nanf("");
+        }
+    } else if (tid == 0) {
+        A.results[row] = RowResult{0, 0, top, top == -__builtin_inff() ? ROW_NONE : ROW_NAN, 0.0, 0.0};
+    }
+}
+
+template <bool DRAW, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void sample_select_kernel(SampleArgs A, int pieces) {
+    constexpr int THREADS = 64 * WAVES;
+    __shared__ SelectShared<WAVES> s;
     const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const Request q = read_request(A, row);
     const PieceStat *stats = A.stats + (size_t)row * pieces;
+    const Request q = read_request(A, row);
     float top = -__builtin_inff();
-    for (int p = tid; p < pieces; p += SA_THREADS) top = larger_or_nan(top, stats[p].top);
+    for (int p = tid; p < pieces; p += THREADS) top = larger_or_nan(top, stats[p].top);
     const bool nan = __any(top != top);
     top = nan ? __builtin_nanf("") : qg_wave_max(top);
     if (lane == 0) s.top[wave] = top;
     __syncthreads();
     top = s.top[0];
 #pragma unroll
-    for (int w = 1; w < SA_WAVES; w++) top = larger_or_nan(top, s.top[w]);
-    if (!__builtin_isfinite(top)) {
-        if (DRAW) {
-            if (tid < A.draws) {
-                A.token[(size_t)row * A.draws + tid] = -1;
-                if (A.logprob) A.logprob[(size_t)row * A.draws + tid] = __builtin_nanf("");
-            }
-        } else if (tid == 0) {
-            A.results[row] = RowResult{0, 0, top, top == -__builtin_inff() ? ROW_NONE : ROW_NAN, 0.0, 0.0};
-        }
-        return;
-    }
-    Row r{A, s.row, A.x + (size_t)row * A.cols, tid, lane, wave, q.a, top};
+    for (int w = 1; w < WAVES; w++) top = larger_or_nan(top, s.top[w]);
+    if (!__builtin_isfinite(top)) return no_draw<DRAW>(A, row, tid, top);
+    Row<WAVES> r{A, s.row, A.x + (size_t)row * A.cols, tid, lane, wave, q.a, top};
+    double *piece = A.kept + (size_t)row * pieces;
     Cut cut;
     double total = 0.0;
-    const double a4 = q.a * 4.0, place = grid_place(top, a4);
+    const double place = grid_place(top, q.a);
     bool found = false, weighed = false;
     if (__builtin_fabs(place) < 0.5 * GRID_FAR) {
-        const double unit = 1.0 / quarter_power((double)top * a4 - place);
+        const double unit = 1.0 / power_of((double)top * q.a - place);
+        // the bins that every piece's list and bins cover, and the weight of all
+        int reach = SA_GRID - 1, known = SA_GRID - 1, counted = 0;
+        bool below = false;
+        double all = 0.0;
+        for (int p = tid; p < pieces; p += THREADS) {
+            const PieceStat y = stats[p];
+            const int delta = (int)place - y.at;
+            const bool counts = y.at != GRID_LOW && delta < (int)GRID_ZERO;
+            const double w = counts ? __builtin_amdgcn_ldexp(y.all, -delta) * unit : 0.0;
+            if (!q.filters()) piece[p] = w;
+            all += w;
+            if (!counts) continue;
+            reach = min(reach, delta + y.cover);
+            known = min(known, delta + y.known);
+            counted += y.counted;
+            below |= y.below != 0;
+        }
         if (!q.filters()) {
-            for (int p = tid; p < pieces; p += SA_THREADS) s.piece[p] = stats[p].at == GRID_LOW ? 0.0 : stats[p].rest * grid_scale(stats[p].at - (int)place) * unit;
             found = weighed = true;
         } else {
-            Grid g{A, s.grid, r, A.bins + (size_t)row * pieces * SA_GRID, stats, pieces, tid, lane, wave, (int)place, a4, unit};
-            int last_bin;
-            found = g.select(q, cut, total, last_bin, s.flag);
+            all = wave_all_add(all);
+#pragma unroll
+            for (int d = 32; d >= 1; d /= 2) {
+                reach = min(reach, __shfl_xor(reach, d));
+                known = min(known, __shfl_xor(known, d));
+            }
+            counted = wave_all_add(counted) + (__any(below) ? 1 << 30 : 0);  // as many as there are, or more
+            if (lane == 0) { s.reach[wave] = reach; s.known[wave] = known; s.flag[wave] = counted; s.grid.wave_sum[wave] = all; }
+            __syncthreads();
+            long in_all = 0;
+            all = 0.0;
+#pragma unroll
+            for (int w = 0; w < WAVES; w++) {
+                reach = min(reach, s.reach[w]);
+                known = min(known, s.known[w]);
+                in_all += s.flag[w];
+                all += s.grid.wave_sum[w];
+            }
+            Grid<WAVES> g{s.grid, r.x, A.bins + (size_t)row * pieces * SA_GRID, stats, A.listed + (size_t)row * pieces * SA_LISTED, A.cols, pieces,
+                          tid, lane, wave, (int)place, top, q.a, unit, reach, known, false};
+            g.add_up();
+            g.below = in_all > (long)__shfl(g.count_upto, known);
+            total = q.top_k ? __shfl(g.mass_upto, SA_GRID - 1) : all;
+            found = true;
+            if (q.top_k) found = g.template shorten<Grid<WAVES>::BY_COUNT>(q.top_k, 0, cut, total);
+            if (found && q.top_p < 1.0) found = g.template shorten<Grid<WAVES>::BY_MASS>(q.top_p * total, 0, cut, total);
+            if (found && q.min_p > 0.0) {
+                const uint32_t t = r.least_key(q.min_p);
+                if (t > cut.t) found = g.template shorten<Grid<WAVES>::BY_KEY>(0.0, t, cut, total);
+            }
             if (found && DRAW) {
-                g.weigh_pieces(last_bin, s.piece);
-                weighed = true;
+                const int n = g.order(cut);
+                if (n) {
+                    for (int d = wave; d < A.draws; d += WAVES) {
+                        const size_t at = (size_t)row * A.draws + d;
+                        const double goal = (double)A.u[at] * s.grid.upto[n - 1];
+                        int pick = -1;
+                        for (int i0 = 0; i0 < n && pick < 0; i0 += 64) {
+                            const unsigned long long hit = __ballot(i0 + lane < n && s.grid.upto[i0 + lane] > goal);
+                            if (hit) pick = i0 + __builtin_ctzll(hit);
+                        }
+                        if (pick < 0) pick = n - 1;
+                        if (lane == 0) {
+                            A.token[at] = s.grid.sorted_index[pick];
+                            if (A.logprob) A.logprob[at] = (float)log(g.weight(s.grid.sorted_key[pick]) / s.grid.upto[n - 1]);
+                        }
+                    }
+                    return;
+                }
+                weighed = g.weigh_pieces(cut, piece);
             }
         }
     }
     if (!found) {
         __syncthreads();
         cut = Cut{};
-        if (q.top_k) r.shorten(cut, false, q.top_k);
-        if (q.top_p < 1.0) r.shorten(cut, true, q.top_p);
+        for (int by = 0; by < 2; by++)
+            if (by ? q.top_p < 1.0 : q.top_k > 0) r.shorten(cut, by != 0, by ? q.top_p : q.top_k);
         if (q.min_p > 0.0) {
             const uint32_t k = r.least_key(q.min_p);
             if (k > cut.t) cut = Cut{k, 0x7fffffff};
         }
-        __syncthreads();
-        for (int p = wave; p < pieces; p += SA_WAVES) {
+    }
+    if (!weighed && (DRAW || !found)) {
+        for (int p = wave; p < pieces; p += WAVES) {
             double sum = 0.0;
             each_value<64>(r.x, p * SA_PIECE + lane, min((p + 1) * SA_PIECE, A.cols), [&](int i, float v) { sum += cut.keeps(order_key(v), i) ? r.weight(v) : 0.0; });
             sum = wave_all_add(sum);
-            if (lane == 0) s.piece[p] = sum;
+            if (lane == 0) piece[p] = sum;
         }
         weighed = true;
     }
     if (weighed) {
         __syncthreads();
         total = 0.0;
-        for (int p0 = 0; p0 < pieces; p0 += 64) total += wave_all_add(p0 + lane < pieces ? s.piece[p0 + lane] : 0.0);
+        for (int p0 = 0; p0 < pieces; p0 += 64) total += wave_all_add(p0 + lane < pieces ? piece[p0 + lane] : 0.0);
     }
     if (!DRAW) {
         if (tid == 0) A.results[row] = RowResult{cut.t, cut.last, top, ROW_CUT, q.a, total};
         return;
     }
-    for (int d = wave; d < A.draws; d += SA_WAVES) {
+    for (int d = wave; d < A.draws; d += WAVES) {
         const size_t at = (size_t)row * A.draws + d;
         const double goal = (double)A.u[at] * total;
         // the piece that passes the goal, or the last one that holds something
         double before = 0.0;
-        int piece = -1;
+        int p = -1;
         bool past = false;
         for (int p0 = 0; p0 < pieces && !past; p0 += 64) {
-            const double v = p0 + lane < pieces ? s.piece[p0 + lane] : 0.0, upto = wave_upto(v, lane) + before;
+            const double v = p0 + lane < pieces ? piece[p0 + lane] : 0.0, upto = wave_upto(v, lane) + before;
             const unsigned long long hit = __ballot(v > 0.0 && upto > goal), any = __ballot(v > 0.0);
             if (!any) continue;
             const int l = hit ? __builtin_ctzll(hit) : 63 - __builtin_clzll(any);
-            piece = p0 + l;
+            p = p0 + l;
             past = hit != 0;
             before = past ? __shfl(upto - v, l) : __shfl(upto, 63);
         }
@@ -676,24 +863,43 @@ __global__ __launch_bounds__(SA_THREADS) void sample_select_kernel(SampleArgs A,
         int pick = -1;
         double won = 0.0;
         past = false;
-        for (int i0 = piece * SA_PIECE; i0 < min((piece + 1) * SA_PIECE, A.cols) && !past; i0 += 64) {
-            const int i = i0 + lane;
-            const float v = i < A.cols ? r.x[i] : -__builtin_inff();
-            const double w = i < A.cols && cut.keeps(order_key(v), i) ? r.weight(v) : 0.0;
-            const double upto = wave_upto(w, lane) + before;
-            const unsigned long long hit = __ballot(!last && w > 0.0 && upto > goal), any = __ballot(w > 0.0);
-            if (!any) continue;
-            const int l = hit ? __builtin_ctzll(hit) : 63 - __builtin_clzll(any);
-            pick = i0 + l;
-            won = __shfl(w, l);
-            past = hit != 0;
-            before = __shfl(upto, 63);
+        for (int i0 = p * SA_PIECE; i0 < min((p + 1) * SA_PIECE, A.cols) && !past; i0 += 16 * 64) {
+            float v[16];
+            double sum = 0.0;
+#pragma unroll
+            for (int k = 0; k < 16; k++) v[k] = i0 + k * 64 + lane < A.cols ? r.x[i0 + k * 64 + lane] : -__builtin_inff();
+            unsigned stays = 0;
+#pragma unroll
+            for (int k = 0; k < 16; k++) {
+                if (v[k] > -__builtin_inff() && cut.keeps(order_key(v[k]), i0 + k * 64 + lane)) { stays |= 1u << k; sum += r.weight(v[k]); }
+            }
+            sum = wave_all_add(sum);
+            if (sum == 0.0) continue;
+            if (!last && !(before + sum * (1.0 + 1e-12) > goal)) { before += sum; continue; }
+#pragma unroll
+            for (int k = 0; k < 16; k++) {
+                if (past || !__any(stays >> k & 1)) continue;
+                const double w = stays >> k & 1 ? r.weight(v[k]) : 0.0, upto = wave_upto(w, lane) + before;
+                const unsigned long long hit = __ballot(!last && w > 0.0 && upto > goal), any = __ballot(w > 0.0);
+                if (!any) continue;
+                const int l = hit ? __builtin_ctzll(hit) : 63 - __builtin_clzll(any);
+                pick = i0 + k * 64 + l;
+                won = __shfl(w, l);
+                past = hit != 0;
+                before = __shfl(upto, 63);
+            }
         }
         if (lane == 0) {
             A.token[at] = pick;
             if (A.logprob) A.logprob[at] = (float)log(won / total);
         }
     }
+}
+// Workgroups of sixteen waves, or of four where the rows are many.
+template <bool DRAW>
+void select_rows(const SampleArgs &A, int rows, int pieces, hipStream_t s) {
+    if (rows > 256) sample_select_kernel<DRAW, 4><<<rows, 256, 0, s>>>(A, pieces);
+    else sample_select_kernel<DRAW, 16><<<rows, 1024, 0, s>>>(A, pieces);
 }
 
 // Probabilities of a piece; one that lies below the cut is not read.
@@ -748,6 +954,8 @@ SampleArgs sample_args(const float *x, int rows, int cols, const qg_sampling *p,
     A.results = (RowResult *)ws;
     A.stats = (PieceStat *)(A.results + rows);
     A.bins = (unsigned long long *)(A.stats + all);
+    A.listed = (uint2 *)(A.bins + all * SA_GRID);
+    A.kept = (double *)(A.listed + all * SA_LISTED);
     return A;
 }
 }  // namespace
@@ -756,7 +964,7 @@ extern "C" {
 
 size_t qg_sample_workspace_bytes(int rows, int cols) {
     if (rows < 1 || rows > QG_MAX_ROWS || cols < 1 || cols > SA_MAX_COLS || (long)rows * cols > 1L << 35) return 0;
-    return (size_t)rows * (sizeof(RowResult) + sample_pieces(cols) * (sizeof(PieceStat) + SA_GRID * sizeof(unsigned long long)));
+    return (size_t)rows * (sizeof(RowResult) + sample_pieces(cols) * (sizeof(PieceStat) + SA_GRID * sizeof(unsigned long long) + SA_LISTED * sizeof(uint2) + sizeof(double)));
 }
 
 int qg_sample(int *token, float *logprob, const float *x, int rows, int cols, int draws, const qg_sampling *sampling, const float *u,
@@ -776,7 +984,7 @@ int qg_sample(int *token, float *logprob, const float *x, int rows, int cols, in
     A.draws = draws;
     const int pieces = sample_pieces(cols);
     sample_piece_kernel<<<(unsigned)((size_t)rows * pieces), PIECE_THREADS, 0, qg_stream()>>>(A, pieces);
-    sample_select_kernel<true><<<rows, SA_THREADS, 0, qg_stream()>>>(A, pieces);
+    select_rows<true>(A, rows, pieces, qg_stream());
     return hipGetLastError();
 }
 
@@ -793,7 +1001,7 @@ int qg_sampling_softmax(float *out, const float *x, int rows, int cols, const qg
     A.out = out;
     const int pieces = sample_pieces(cols);
     sample_piece_kernel<<<(unsigned)((size_t)rows * pieces), PIECE_THREADS, 0, qg_stream()>>>(A, pieces);
-    sample_select_kernel<false><<<rows, SA_THREADS, 0, qg_stream()>>>(A, pieces);
+    select_rows<false>(A, rows, pieces, qg_stream());
     sample_probs_kernel<<<(unsigned)((size_t)rows * pieces), PIECE_THREADS, 0, qg_stream()>>>(A, pieces);
     return hipGetLastError();
 }
