@@ -323,7 +323,8 @@ int qg_verify_drafts(int *tokens_out, int *path, int *count, const float *p, con
  * equal values the lower index counts as larger (0 and -0 are equal); the
  * largest always stays.  temperature 0, and one that is not at least 2^-126,
  * is the first largest token alone; top_k <= 0 or >= cols, a top_p that is not
- * below 1 and a min_p that is not above 0 keep all. */
+ * below 1 and a min_p that is not above 0 keep all.  Weights below 2^-1000
+ * count as 0. */
 typedef struct {
     const float *temperature;   /* NULL: 1 */
     const int *top_k;

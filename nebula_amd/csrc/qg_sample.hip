@@ -46,17 +46,28 @@ QG_DEV uint32_t order_key(float x) {
 }
 QG_DEV float key_value(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k); }
 
-// 2^d for d <= 0, within 2^-52: the Taylor series of e^r, |r| <= ln 2 / 2, whose
-// next term is below 1e-17.
-QG_DEV double exp2_d(double d) {
-    if (!(d > -1100.0)) return 0.0;
-    const double n = __builtin_rint(d), r = (d - n) * 0.693147180559945309417;
-    double p = 1.0 / 6227020800.0;
-    const double c[13] = {1.0, 1.0, 1.0 / 2, 1.0 / 6, 1.0 / 24, 1.0 / 120, 1.0 / 720, 1.0 / 5040, 1.0 / 40320, 1.0 / 362880, 1.0 / 3628800,
-                          1.0 / 39916800, 1.0 / 479001600};
+// A weight's exponent e = n + y, n whole and |y| <= 1/2, and p = 2^y (HALF: 2^(y + 1/2), in [1, 2]) by the Taylor series,
+// whose next term is below 2e-16 of it.  The whole part falls out of the sum with 1.5 2^52, in the low bits; |e| < 2^31.
+struct Power { double p; int n; };
+template <bool HALF>
+QG_DEV Power power_of(double e) {
+    constexpr double h = 0.693147180559945309417, c0 = HALF ? 1.41421356237309504880 : 1.0, whole = 6755399441055744.0;
+    constexpr double c1 = c0 * h, c2 = c1 * h / 2, c3 = c2 * h / 3, c4 = c3 * h / 4, c5 = c4 * h / 5, c6 = c5 * h / 6, c7 = c6 * h / 7, c8 = c7 * h / 8,
+                     c9 = c8 * h / 9, c10 = c9 * h / 10, c11 = c10 * h / 11, c12 = c11 * h / 12;
+    const double c[12] = {c0, c1, c2, c3, c4, c5, c6, c7, c8, c9, c10, c11}, t = e + whole, y = e - (t - whole);
+    double p = c12;
 #pragma unroll
-    for (int i = 12; i >= 0; i--) p = __builtin_fma(p, r, c[i]);
-    return __builtin_amdgcn_ldexp(p, (int)n);
+    for (int i = 11; i >= 0; i--) p = __builtin_fma(p, y, c[i]);
+    return Power{p, (int)(uint32_t)__double_as_longlong(t)};
+}
+// p 2^n for results that are normal numbers
+QG_DEV double scaled(double p, int n) { return __longlong_as_double(__double_as_longlong(p) + ((long long)n << 52)); }
+constexpr int SA_ZERO = 1000;  // weights below 2^-1000 of the largest count as 0
+// 2^d, d <= 0
+QG_DEV double exp2_d(double d) {
+    if (!(d > -SA_ZERO)) return 0.0;
+    const Power x = power_of<false>(d);
+    return scaled(x.p, x.n);
 }
 
 // What a row asks for.  Temperature 0 (or none that counts) is the first largest
@@ -121,7 +132,8 @@ template <typename F>
 QG_DEV uint32_t first_key(uint32_t hi, int lane, F f) {
     for (uint32_t lo = 0x007fffffu; hi - lo > 1;) {
         const uint32_t step = (hi - lo - 1) / 64 + 1;
-        const int first = __builtin_ctzll(__ballot(f(key_value(lo + min((uint32_t)(lane + 1) * step, hi - lo)))));
+        // the last lane's is hi
+        const int first = __builtin_ctzll(__ballot(f(key_value(lo + min((uint32_t)(lane + 1) * step, hi - lo)))) | 1ULL << 63);
         const uint32_t up = lo + min((uint32_t)(first + 1) * step, hi - lo);
         lo += min((uint32_t)first * step, hi - lo);
         hi = up;
@@ -260,8 +272,8 @@ struct Row {
 };
 
 // ------------------------------------------------------------------------
-// One pass over the values, in pieces.  The bins are whole bits of the weights' exponents x a,
-// the same for all pieces of a row, so that those of all pieces can be added; a piece keeps the
+// One pass over the values, in pieces.  A bin holds the weights whose exponents x a round to one whole
+// number, the same for all pieces of a row, so that those of all pieces can be added; a piece keeps the
 // SA_GRID bins from its largest value down, of these only as many as the row's filters
 // may cut in.  A weight is 1..2 times its bin's lower end: what it has above that, to 2^-36, is
 // added up as a whole number under the count, in one 64-bit atomic whose order does not
@@ -269,26 +281,14 @@ struct Row {
 // stay of most rows, and then nothing is read again.
 // ------------------------------------------------------------------------
 constexpr int PIECE_THREADS = 256, PIECE_WAVES = PIECE_THREADS / 64, PIECE_VALUES = SA_PIECE / PIECE_THREADS, BIN_COUNT = 49, BIN_BITS = 36;
-constexpr double GRID_ZERO = 1100.0;            // bits below which a weight is 0
 constexpr double GRID_FAR = (double)(1 << 19);  // places further out are left to the search over the row
-constexpr int GRID_LOW = -(1 << 30);           // in place of one: the piece's weights are 0 beside a row's largest within half of that
+constexpr int GRID_LOW = -(1 << 30);            // in place of one: the piece's weights are 0 beside a row's largest within half of that
 
-QG_DEV double grid_place(float x, double a) { return __builtin_floor((double)x * a); }
-// 2^f, 0 <= f < 1, at least 1: the Taylor series about f = 1/2, whose next term is below 1e-16.
-QG_DEV double power_of(double f) {
-    constexpr double h = 0.693147180559945309417, c0 = 1.41421356237309504880;
-    constexpr double c1 = c0 * h, c2 = c1 * h / 2, c3 = c2 * h / 3, c4 = c3 * h / 4, c5 = c4 * h / 5, c6 = c5 * h / 6, c7 = c6 * h / 7, c8 = c7 * h / 8,
-                     c9 = c8 * h / 9, c10 = c9 * h / 10, c11 = c10 * h / 11, c12 = c11 * h / 12;
-    const double c[12] = {c0, c1, c2, c3, c4, c5, c6, c7, c8, c9, c10, c11}, y = f - 0.5;
-    double p = c12;
-#pragma unroll
-    for (int i = 11; i >= 0; i--) p = __builtin_fma(p, y, c[i]);
-    return __builtin_fmax(p, 1.0);
-}
-// What a weight 2^f adds to its bin; a bin's weights in units of the lower end of bin 0.
-QG_DEV unsigned long long bin_entry(double f) {
-    // f may have been rounded to 1, and its power to 2
-    const unsigned long long m = (unsigned long long)__double_as_longlong(__builtin_fmin(power_of(f), 0x1.fffffffffffffp0)) & ((1ULL << 52) - 1);
+QG_DEV double grid_place(float x, double a) { return __builtin_rint((double)x * a); }
+// What a weight of p times its bin's lower end adds to the bin; a bin's weights in units of the lower end of bin 0.
+QG_DEV unsigned long long bin_entry(double p) {
+    // p may have been rounded below 1 or up to 2
+    const unsigned long long m = (unsigned long long)__double_as_longlong(__builtin_fmin(__builtin_fmax(p, 1.0), 0x1.fffffffffffffp0)) & ((1ULL << 52) - 1);
     return ((m + (1ULL << (51 - BIN_BITS))) >> (52 - BIN_BITS)) + (1ULL << BIN_COUNT);
 }
 QG_DEV unsigned bin_count(unsigned long long b) { return (unsigned)(b >> BIN_COUNT); }
@@ -309,9 +309,8 @@ __global__ __launch_bounds__(PIECE_THREADS) void sample_piece_kernel(SampleArgs 
     __shared__ unsigned long long s_bin[SA_GRID];
     __shared__ unsigned s_most[SA_GRID];
     __shared__ float s_top[PIECE_WAVES], s_value[SA_PIECE];
-    __shared__ uint16_t s_index[SA_PIECE];
     __shared__ double s_rest[PIECE_WAVES];
-    __shared__ int s_below[PIECE_WAVES], s_cover, s_listed;
+    __shared__ int s_below[PIECE_WAVES], s_cover, s_listed[SA_GRID];
     const int row = blockIdx.x / pieces, piece = blockIdx.x % pieces, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int c0 = piece * SA_PIECE, n = min(SA_PIECE, A.cols - c0);
     const float *x = A.x + (size_t)row * A.cols + c0 + tid;
@@ -325,7 +324,6 @@ __global__ __launch_bounds__(PIECE_THREADS) void sample_piece_kernel(SampleArgs 
     }
     const Request q = read_request(A, row);
     if (tid < SA_GRID) { s_bin[tid] = 0; s_most[tid] = 0; }
-    if (tid == 0) s_listed = 0;
     bool nan = false;
 #pragma unroll
     for (int k = 0; k < PIECE_VALUES; k++) { own = fmaxf(own, v[k]); nan |= v[k] != v[k]; }
@@ -336,58 +334,55 @@ __global__ __launch_bounds__(PIECE_THREADS) void sample_piece_kernel(SampleArgs 
     top = s_top[0];
 #pragma unroll
     for (int w = 1; w < PIECE_WAVES; w++) top = larger_or_nan(top, s_top[w]);
-    const double place = grid_place(top, q.a);
+    const double far = grid_place(top, q.a);
     const size_t at = (size_t)row * pieces + piece;
-    if (!(__builtin_fabs(place) < GRID_FAR)) {  // NaN and infinities too
+    if (!(__builtin_fabs(far) < GRID_FAR)) {  // NaN and infinities too
         if (tid == 0) A.stats[at] = PieceStat{top, GRID_LOW, 0, SA_GRID - 1, SA_GRID - 1, 0, 0, 0, 0.0, 0.0};
         return;
     }
+    const int place = (int)far;
     const bool filter = q.filters(), weigh = q.weighs_all();
     int known = filter ? deepest_bin(q, 62 - A.fixed) : -1;
-    if (q.top_k && q.top_k <= PIECE_THREADS / 2) {
+    if (q.top_k && q.top_k <= PIECE_THREADS - 16) {
         // the row's top_k values are not below the piece's, and these not below the top_k-th of its threads' largest
-        const double d = place - grid_place(own, q.a);
+        const double d = far - grid_place(own, q.a);
         if (d < SA_GRID) atomicAdd(&s_most[(int)d], 1u);
         __syncthreads();
         const unsigned long long enough = __ballot(wave_upto(s_most[lane], lane) >= (unsigned)q.top_k);
         if (enough) known = __builtin_ctzll(enough);
     }
-    // the wave's values that may be in a bin go together, so that few of its steps form a weight
-    float *mine = s_value + wave * (64 * PIECE_VALUES);
-    uint16_t *mine_at = s_index + wave * (64 * PIECE_VALUES);
-    const float near = filter ? (float)((double)top - (known + 2) / q.a - 1e-6 * __builtin_fabs((double)top)) : __builtin_inff();
-    const float zero = (float)((double)top - GRID_ZERO / q.a);
-    int held = 0;
-    bool below = false;
-#pragma unroll
-    for (int k = 0; k < PIECE_VALUES; k++) {
-        const bool is = v[k] >= near;
-        const unsigned long long all = __ballot(is);
-        if (is) {
-            const int to = held + __popcll(all & ((1ULL << lane) - 1));
-            mine[to] = v[k];
-            mine_at[to] = (uint16_t)(k * PIECE_THREADS + tid);
-        }
-        held += __popcll(all);
-        below |= !is && v[k] >= zero;
-    }
+    const float zero = (float)(((double)place - SA_ZERO) / q.a);
     double rest = 0.0;
+    bool below = false;
+    auto weigh_one = [&](float y) {  // not below zero
+        const Power w = power_of<true>((double)y * q.a);
+        const int d = place - w.n;
+        if (d <= known) {
+            atomicAdd(&s_bin[d], bin_entry(w.p));
+        } else {
+            below = true;
+            rest += scaled(w.p, -d);
+        }
+    };
     if (weigh) {
 #pragma unroll
+        for (int k = 0; k < PIECE_VALUES; k++)
+            if (v[k] > zero) weigh_one(v[k]);
+    } else {
+        // the wave's values that may be in a bin go together, so that few of its steps form a weight
+        float *mine = s_value + wave * (64 * PIECE_VALUES);
+        const float near = fmaxf((float)((double)(place - known - 1) / q.a), zero);
+        int held = 0;
+#pragma unroll
         for (int k = 0; k < PIECE_VALUES; k++) {
-            const double e = (double)v[k] * q.a, b = __builtin_floor(e), d = place - b;
-            if (!(v[k] >= near) && d < GRID_ZERO) rest += __builtin_amdgcn_ldexp(power_of(e - b), -(int)d);
+            const bool is = v[k] > near;
+            const unsigned long long all = __ballot(is);
+            if (is) mine[held + __popcll(all & ((1ULL << lane) - 1))] = v[k];
+            held += __popcll(all);
+            below |= !is && v[k] > zero;
         }
-    }
-    __builtin_amdgcn_wave_barrier();  // a wave's own values
-    for (int i = lane; i < held; i += 64) {
-        const double e = (double)mine[i] * q.a, b = __builtin_floor(e), d = place - b;
-        if (d <= (double)known) {
-            atomicAdd(&s_bin[(int)d], bin_entry(e - b));
-        } else if (d < GRID_ZERO) {
-            below = true;
-            rest += __builtin_amdgcn_ldexp(power_of(e - b), -(int)d);
-        }
+        __builtin_amdgcn_wave_barrier();  // a wave's own values
+        for (int i = lane; i < held; i += 64) weigh_one(mine[i]);
     }
     rest = wave_all_add(rest);
     below = __any(below);
@@ -403,7 +398,7 @@ __global__ __launch_bounds__(PIECE_THREADS) void sample_piece_kernel(SampleArgs 
         if (filter) A.bins[at * SA_GRID + lane] = b;
         if (lane == 0) {
             s_cover = cover;
-            PieceStat p{top, (int)place, 0, known, cover, counted, listed, 0, 0.0, 0.0};
+            PieceStat p{top, place, 0, known, cover, counted, listed, 0, 0.0, 0.0};
 #pragma unroll
             for (int w = 0; w < PIECE_WAVES; w++) { p.rest += s_rest[w]; p.below |= s_below[w]; }
             p.all = in + p.rest;
@@ -412,13 +407,31 @@ __global__ __launch_bounds__(PIECE_THREADS) void sample_piece_kernel(SampleArgs 
     }
     if (!filter) return;
     __syncthreads();
+    // the values down to bin `cover`, in order
     const int cover = s_cover;
+    if (cover < 0) return;
+    const float near = (float)((double)(place - cover - 1) / q.a);
+    unsigned mine = 0;
+    int counts = 0;  // lane k: the wave's of value k
+#pragma unroll
+    for (int k = 0; k < PIECE_VALUES; k++) {
+        bool is = v[k] > near;
+        if (!__any(is)) continue;
+        is = is && far - grid_place(v[k], q.a) <= (double)cover;
+        const int n = __popcll(__ballot(is));
+        if (lane == k) counts = n;
+        mine |= (unsigned)is << k;
+    }
+    if (lane < PIECE_VALUES) s_listed[lane * PIECE_WAVES + wave] = counts;
+    __syncthreads();
+    const int before = wave_upto(s_listed[lane], lane) - s_listed[lane];  // of value lane / 4 and wave lane % 4
     uint2 *listed = A.listed + at * SA_LISTED;
-    for (int i = lane; i < held; i += 64) {
-        const float y = mine[i];
-        if (!(place - grid_place(y, q.a) <= (double)cover)) continue;
-        const int to = atomicAdd(&s_listed, 1);
-        if (to < SA_LISTED) listed[to] = make_uint2(order_key(y), c0 + mine_at[i]);
+#pragma unroll
+    for (int k = 0; k < PIECE_VALUES; k++) {
+        const unsigned long long all = __ballot(mine >> k & 1);
+        if (!all) continue;
+        const int to = __builtin_amdgcn_readlane(before, k * PIECE_WAVES + wave) + __popcll(all & ((1ULL << lane) - 1));
+        if ((mine >> k & 1) && to < SA_LISTED) listed[to] = make_uint2(order_key(v[k]), c0 + k * PIECE_THREADS + tid);
     }
 }
 
@@ -433,8 +446,9 @@ template <int WAVES>
 struct GridShared {
     unsigned count[WAVES][SA_GRID];
     unsigned long long excess[WAVES][SA_GRID];
-    uint32_t key[SA_LIST], sorted_key[SA_LIST];
-    int index[SA_LIST], sorted_index[SA_LIST];
+    unsigned long long put[SA_LIST];  // key, then the complement of the index: of equal keys the lower index is the larger
+    uint32_t sorted_key[SA_LIST];
+    int sorted_index[SA_LIST];
     double upto[SA_LIST], wave_sum[WAVES];
     int n, hits;
 };
@@ -468,7 +482,7 @@ struct Grid {
     __device__ __forceinline__ double weight(uint32_t key) const { return exp2_d(((double)key_value(key) - (double)m) * a); }
     __device__ __forceinline__ double place_of(uint32_t key) const { return grid_place(key_value(key), a); }
     // the 64th of its bin that a value is in, from the top
-    static __device__ __forceinline__ int part_of(double e) { return 63 - min((int)((e - __builtin_floor(e)) * 64.0), 63); }
+    static __device__ __forceinline__ int part_of(double e) { return 63 - min(max((int)((e - __builtin_rint(e) + 0.5) * 64.0), 0), 63); }
     // A piece's bin of a lane, moved to the row's.
     __device__ __forceinline__ int moved_by(int p) const {
         const int at = stats[p].at;
@@ -509,7 +523,7 @@ struct Grid {
     }
     __device__ __forceinline__ void put(uint32_t key, int i) {
         const int k = atomicAdd(&s.n, 1);
-        if (k < SA_LIST) { s.key[k] = key; s.index[k] = i; }
+        if (k < SA_LIST) s.put[k] = (unsigned long long)key << 32 | ~(uint32_t)i;
     }
     // f(key, index) of the values in bin D (every lane of some waves each), and of more
     template <typename F>
@@ -543,6 +557,7 @@ struct Grid {
         __syncthreads();
         const bool fit = s.hits <= SA_LIST;
         const int items = (fit ? s.hits : pieces) * 4;
+        const float low = (float)((double)(place - D - 1) / a), high = (float)((double)(place - D + 1) / a);
         for (int it = wave; it < items; it += WAVES) {
             const int i0 = (fit ? hits[it >> 2] : it >> 2) * SA_PIECE + (it & 3) * (SA_PIECE / 4) + lane;
             float v[16];
@@ -550,23 +565,21 @@ struct Grid {
             for (int k = 0; k < 16; k++) v[k] = i0 + k * 64 < cols ? x[i0 + k * 64] : -__builtin_inff();
 #pragma unroll
             for (int k = 0; k < 16; k++)
-                if (v[k] > -__builtin_inff()) f(order_key(v[k]), i0 + k * 64);
+                if (v[k] > low && v[k] < high) f(order_key(v[k]), i0 + k * 64);
         }
     }
-    // Ranks s.key, s.index [s.n]: by falling value, or by index.
-    template <bool BY_INDEX>
+    // Ranks what was put by falling value, with the sums of the weights.
     __device__ __forceinline__ void rank(int n) {
         __syncthreads();
         for (int i = tid; i < n; i += THREADS) {
-            const uint32_t key = s.key[i];
-            const int at = s.index[i];
+            const unsigned long long own = s.put[i];
             int rank = 0;
-            for (int k = 0; k < n; k++) rank += BY_INDEX ? s.index[k] < at : s.key[k] > key || (s.key[k] == key && s.index[k] < at);
-            s.sorted_key[rank] = key;
-            s.sorted_index[rank] = at;
+#pragma unroll 8
+            for (int k = 0; k < n; k++) rank += s.put[k] > own;
+            s.sorted_key[rank] = (uint32_t)(own >> 32);
+            s.sorted_index[rank] = (int)~(uint32_t)own;
         }
         __syncthreads();
-        // the sums of their weights
         double before = 0.0;
         for (int i0 = 0; i0 < n; i0 += THREADS) {
             const int i = i0 + tid;
@@ -619,10 +632,10 @@ struct Grid {
                 __syncthreads();
                 each_of_bin(D, [&](uint32_t key, int i) {
                     const double e = (double)key_value(key) * a;
-                    if (__builtin_floor(e) != b || !cut.keeps(key, i)) return;
+                    if (__builtin_rint(e) != b || !cut.keeps(key, i)) return;
                     atomicAdd(&s.count[0][part_of(e)], 1u);
                     // up to 2^24 values of less than 2^37 above their count
-                    atomicAdd(&s.excess[0][part_of(e)], bin_excess(bin_entry(e - b)));
+                    atomicAdd(&s.excess[0][part_of(e)], bin_excess(bin_entry(power_of<true>(e).p)));
                 });
                 __syncthreads();
                 const unsigned c = s.count[0][lane], c_upto = wave_upto(c, lane);
@@ -644,11 +657,11 @@ struct Grid {
             __syncthreads();
             each_of_bin(D, [&](uint32_t key, int i) {
                 const double e = (double)key_value(key) * a;
-                if (__builtin_floor(e) == b && cut.keeps(key, i) && (sub < 0 || part_of(e) == sub)) put(key, i);
+                if (__builtin_rint(e) == b && cut.keeps(key, i) && (sub < 0 || part_of(e) == sub)) put(key, i);
             });
             __syncthreads();
             kept = min(s.n, SA_LIST);
-            rank<false>(kept);
+            rank(kept);
             part = sub >= 0;
             bin = part ? -1 : D;
         }
@@ -671,36 +684,31 @@ struct Grid {
         total = before + (kept ? s.upto[kept - 1] : 0.0);
         return true;
     }
-    // What stays of each piece: its bins above the last one, and the ranked values that are its.  False where the bins do not say.
+    // What stays of each piece: from its list where this holds it, or its bins above the last one and the ranked values
+    // that are its.  False where neither says.
+    __device__ __forceinline__ bool in_lists() const { return deepest <= reach; }
     __device__ __forceinline__ bool weigh_pieces(const Cut &cut, double *piece) const {
-        if (part) return false;
-        const int whole = cut.t == 0 || deepest != bin ? deepest + 1 : deepest;
+        if (!in_lists() && part) return false;
+        const int whole = deepest != bin ? deepest + 1 : deepest;
         for (int p = wave; p < pieces; p += WAVES) {
-            const unsigned long long b = row_bin(p);
-            double sum = lane < whole ? bin_mass(bin_count(b), bin_excess(b), lane) * unit : 0.0;
-            if (whole == deepest)
-                for (int k = lane; k < kept; k += 64)
-                    if (s.sorted_index[k] / SA_PIECE == p) sum += weight(s.sorted_key[k]);
+            double sum = 0.0;
+            if (in_lists()) {
+                const int n = stats[p].at == GRID_LOW ? 0 : min(stats[p].listed, SA_LISTED);
+                for (int i = lane; i < n; i += 64) {
+                    const uint2 y = lists[(size_t)p * SA_LISTED + i];
+                    if (cut.keeps(y.x, (int)y.y)) sum += weight(y.x);
+                }
+            } else {
+                const unsigned long long b = row_bin(p);
+                if (lane < whole) sum = bin_mass(bin_count(b), bin_excess(b), lane) * unit;
+                if (whole == deepest)
+                    for (int k = lane; k < kept; k += 64)
+                        if (s.sorted_index[k] / SA_PIECE == p) sum += weight(s.sorted_key[k]);
+            }
             sum = wave_all_add(sum);
             if (lane == 0) piece[p] = sum;
         }
         return true;
-    }
-    // All that stays, from the lists, in the tokens' order: s.sorted_key, s.sorted_index and s.upto; their number, 0 where the lists do
-    // not hold it or it is too many.
-    __device__ __forceinline__ int order(const Cut &cut) {
-        if (deepest > reach || __shfl(count_upto, deepest) > 4 * SA_LIST) return 0;
-        __syncthreads();
-        if (tid == 0) s.n = 0;
-        __syncthreads();
-        each_of_bin(0, [&](uint32_t key, int i) {
-            if ((double)place - place_of(key) <= (double)deepest && cut.keeps(key, i)) put(key, i);
-        });
-        __syncthreads();
-        const int n = s.n;
-        if (n > SA_LIST) return 0;
-        rank<true>(n);
-        return n;
     }
 };
 
@@ -739,9 +747,9 @@ __global__ __launch_bounds__(64 * WAVES) void sample_select_kernel(SampleArgs A,
     Cut cut;
     double total = 0.0;
     const double place = grid_place(top, q.a);
-    bool found = false, weighed = false;
+    bool found = false, weighed = false, listed = false;  // listed: the pieces' lists hold what stays
     if (__builtin_fabs(place) < 0.5 * GRID_FAR) {
-        const double unit = 1.0 / power_of((double)top * q.a - place);
+        const double unit = 1.0 / power_of<true>((double)top * q.a).p;
         // the bins that every piece's list and bins cover, and the weight of all
         int reach = SA_GRID - 1, known = SA_GRID - 1, counted = 0;
         bool below = false;
@@ -749,7 +757,7 @@ __global__ __launch_bounds__(64 * WAVES) void sample_select_kernel(SampleArgs A,
         for (int p = tid; p < pieces; p += THREADS) {
             const PieceStat y = stats[p];
             const int delta = (int)place - y.at;
-            const bool counts = y.at != GRID_LOW && delta < (int)GRID_ZERO;
+            const bool counts = y.at != GRID_LOW && delta < SA_ZERO;
             const double w = counts ? __builtin_amdgcn_ldexp(y.all, -delta) * unit : 0.0;
             if (!q.filters()) piece[p] = w;
             all += w;
@@ -793,25 +801,8 @@ __global__ __launch_bounds__(64 * WAVES) void sample_select_kernel(SampleArgs A,
                 if (t > cut.t) found = g.template shorten<Grid<WAVES>::BY_KEY>(0.0, t, cut, total);
             }
             if (found && DRAW) {
-                const int n = g.order(cut);
-                if (n) {
-                    for (int d = wave; d < A.draws; d += WAVES) {
-                        const size_t at = (size_t)row * A.draws + d;
-                        const double goal = (double)A.u[at] * s.grid.upto[n - 1];
-                        int pick = -1;
-                        for (int i0 = 0; i0 < n && pick < 0; i0 += 64) {
-                            const unsigned long long hit = __ballot(i0 + lane < n && s.grid.upto[i0 + lane] > goal);
-                            if (hit) pick = i0 + __builtin_ctzll(hit);
-                        }
-                        if (pick < 0) pick = n - 1;
-                        if (lane == 0) {
-                            A.token[at] = s.grid.sorted_index[pick];
-                            if (A.logprob) A.logprob[at] = (float)log(g.weight(s.grid.sorted_key[pick]) / s.grid.upto[n - 1]);
-                        }
-                    }
-                    return;
-                }
                 weighed = g.weigh_pieces(cut, piece);
+                listed = g.in_lists();
             }
         }
     }
@@ -863,7 +854,22 @@ __global__ __launch_bounds__(64 * WAVES) void sample_select_kernel(SampleArgs A,
         int pick = -1;
         double won = 0.0;
         past = false;
-        for (int i0 = p * SA_PIECE; i0 < min((p + 1) * SA_PIECE, A.cols) && !past; i0 += 16 * 64) {
+        if (listed) {
+            const uint2 *list = A.listed + ((size_t)row * pieces + p) * SA_LISTED;
+            const int n = min(stats[p].listed, SA_LISTED);
+            for (int i0 = 0; i0 < n && !past; i0 += 64) {
+                const uint2 y = i0 + lane < n ? list[i0 + lane] : make_uint2(0, 0);
+                const double w = i0 + lane < n && cut.keeps(y.x, (int)y.y) ? r.weight(key_value(y.x)) : 0.0, upto = wave_upto(w, lane) + before;
+                const unsigned long long hit = __ballot(!last && w > 0.0 && upto > goal), any = __ballot(w > 0.0);
+                if (!any) continue;
+                const int l = hit ? __builtin_ctzll(hit) : 63 - __builtin_clzll(any);
+                pick = (int)__shfl(y.y, l);
+                won = __shfl(w, l);
+                past = hit != 0;
+                before = __shfl(upto, 63);
+            }
+        }
+        for (int i0 = p * SA_PIECE; !listed && i0 < min((p + 1) * SA_PIECE, A.cols) && !past; i0 += 16 * 64) {
             float v[16];
             double sum = 0.0;
 #pragma unroll
