@@ -98,21 +98,42 @@ struct Cut {
     __device__ __forceinline__ bool keeps(uint32_t key, int i) const { return key > t || (key == t && i <= last); }
 };
 
-template <typename T>
-QG_DEV T wave_all_add(T v) {
-#pragma unroll
-    for (int d = 32; d >= 1; d /= 2) v += __shfl_xor(v, d);
-    return v;
-}
-template <typename T>
-QG_DEV T wave_upto(T v, int lane) {
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-        const T o = __shfl_up(v, d);
-        if (lane >= d) v += o;
+// A value of another lane by a VALU move, 0 where there is none or the row is not in ROWS; in 32-bit words.
+template <int CTRL, int ROWS, typename T>
+QG_DEV T moved_lane(T v) {
+    if constexpr (sizeof(T) == 8) {
+        const unsigned long long b = __builtin_bit_cast(unsigned long long, v);
+        const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)b, CTRL, ROWS, 0xf, false);
+        const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(b >> 32), CTRL, ROWS, 0xf, false);
+        return __builtin_bit_cast(T, (unsigned long long)hi << 32 | lo);
+    } else {
+        return __builtin_bit_cast(T, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, ROWS, 0xf, false));
     }
+}
+// Sums over the lanes up to each: within rows of 16, then the rows' last lanes to those behind.
+template <typename T>
+QG_DEV T wave_upto(T v) {
+    v += moved_lane<0x111, 0xf>(v);  // row_shr 1, 2, 4, 8
+    v += moved_lane<0x112, 0xf>(v);
+    v += moved_lane<0x114, 0xf>(v);
+    v += moved_lane<0x118, 0xf>(v);
+    v += moved_lane<0x142, 0xa>(v);  // row_bcast 15, 31
+    v += moved_lane<0x143, 0xc>(v);
     return v;
 }
+// The value of a lane that all lanes name.
+template <typename T>
+QG_DEV T of_lane(T v, int l) {
+    if constexpr (sizeof(T) == 8) {
+        const unsigned long long b = __builtin_bit_cast(unsigned long long, v);
+        const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)b, l), hi = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(b >> 32), l);
+        return __builtin_bit_cast(T, (unsigned long long)hi << 32 | lo);
+    } else {
+        return __builtin_bit_cast(T, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), l));
+    }
+}
+template <typename T>
+QG_DEV T wave_all_add(T v) { return of_lane(wave_upto(v), 63); }
 // f(i, x_i) for the values of a row that are a thread's, eight on their way at once
 template <int STEP, typename F>
 QG_DEV void each_value(const float *x, int i0, int end, F f) {
@@ -192,8 +213,8 @@ struct Row {
             for (int k = 0; k < OWN; k++) { c += s.count[b0 - k]; w += s.mass[b0 - k]; }
             const unsigned own_c = c;
             const unsigned long long own_w = w;
-            c = wave_upto(c, lane);
-            w = wave_upto(w, lane);
+            c = wave_upto(c);
+            w = wave_upto(w);
             if (lane == 63) { s.wave_count[wave] = c; s.wave_mass[wave] = w; }
             if (tid == 0) s.found_bin = -1;
             __syncthreads();
@@ -348,7 +369,7 @@ __global__ __launch_bounds__(PIECE_THREADS) void sample_piece_kernel(SampleArgs 
         const double d = far - grid_place(own, q.a);
         if (d < SA_GRID) atomicAdd(&s_most[(int)d], 1u);
         __syncthreads();
-        const unsigned long long enough = __ballot(wave_upto(s_most[lane], lane) >= (unsigned)q.top_k);
+        const unsigned long long enough = __ballot(wave_upto(s_most[lane]) >= (unsigned)q.top_k);
         if (enough) known = __builtin_ctzll(enough);
     }
     const float zero = (float)(((double)place - SA_ZERO) / q.a);
@@ -384,17 +405,17 @@ __global__ __launch_bounds__(PIECE_THREADS) void sample_piece_kernel(SampleArgs 
         __builtin_amdgcn_wave_barrier();  // a wave's own values
         for (int i = lane; i < held; i += 64) weigh_one(mine[i]);
     }
-    rest = wave_all_add(rest);
+    if (weigh) rest = wave_all_add(rest);
     below = __any(below);
     if (lane == 0) { s_rest[wave] = rest; s_below[wave] = below; }
     __syncthreads();
     if (wave == 0) {
         const int most = q.top_k ? min(max(2 * q.top_k, 32), SA_LISTED) : SA_LISTED;  // a piece may hold all top_k, of a bin's about half
         const unsigned long long b = s_bin[lane];
-        const unsigned upto = wave_upto(bin_count(b), lane);
-        const int cover = min((int)__popcll(__ballot(upto <= (unsigned)most)) - 1, known), listed = cover < 0 ? 0 : (int)__shfl(upto, cover);
-        const int counted = (int)__shfl(upto, SA_GRID - 1);
-        const double in = wave_all_add(bin_mass(bin_count(b), bin_excess(b), lane));
+        const unsigned upto = wave_upto(bin_count(b));
+        const int cover = min((int)__popcll(__ballot(upto <= (unsigned)most)) - 1, known), listed = cover < 0 ? 0 : (int)of_lane(upto, cover);
+        const int counted = (int)of_lane(upto, SA_GRID - 1);
+        const double in = weigh && filter ? wave_all_add(bin_mass(bin_count(b), bin_excess(b), lane)) : 0.0;
         if (filter) A.bins[at * SA_GRID + lane] = b;
         if (lane == 0) {
             s_cover = cover;
@@ -424,7 +445,7 @@ __global__ __launch_bounds__(PIECE_THREADS) void sample_piece_kernel(SampleArgs 
     }
     if (lane < PIECE_VALUES) s_listed[lane * PIECE_WAVES + wave] = counts;
     __syncthreads();
-    const int before = wave_upto(s_listed[lane], lane) - s_listed[lane];  // of value lane / 4 and wave lane % 4
+    const int before = wave_upto(s_listed[lane]) - s_listed[lane];  // of value lane / 4 and wave lane % 4
     uint2 *listed = A.listed + at * SA_LISTED;
 #pragma unroll
     for (int k = 0; k < PIECE_VALUES; k++) {
@@ -514,8 +535,8 @@ struct Grid {
         }
         all_waves(n, e, count, e);
         mass = bin_mass(count, e, lane) * unit;
-        count_upto = wave_upto(count, lane);
-        mass_upto = wave_upto(mass, lane);
+        count_upto = wave_upto(count);
+        mass_upto = wave_upto(mass);
         deepest = SA_GRID - 1;
         bin = -1;
         kept = 0;
@@ -583,7 +604,7 @@ struct Grid {
         double before = 0.0;
         for (int i0 = 0; i0 < n; i0 += THREADS) {
             const int i = i0 + tid;
-            double w = wave_upto(i < n ? weight(s.sorted_key[i]) : 0.0, lane);
+            double w = wave_upto(i < n ? weight(s.sorted_key[i]) : 0.0);
             __syncthreads();
             if (lane == 63) s.wave_sum[wave] = w;
             __syncthreads();
@@ -614,13 +635,13 @@ struct Grid {
             D = __builtin_ctzll(enough);
             if (D > deepest) return true;  // sums that differ in their last bits
         }
-        const int n = (int)__shfl(count, D);
-        int first = (int)__shfl(count_upto, D) - n;
-        double before = D ? __shfl(mass_upto, D - 1) : 0.0;
+        const int n = (int)of_lane(count, D);
+        int first = (int)of_lane(count_upto, D) - n;
+        double before = D ? of_lane(mass_upto, D - 1) : 0.0;
         if (BY == BY_COUNT && first + n == (int)target) {  // all of the bin
             cut = Cut{first_key(order_key(m), lane, [&](float v) { return grid_place(v, a) >= (double)(place - D); }), 0x7fffffff};
             deepest = D;
-            total = __shfl(mass_upto, D);
+            total = of_lane(mass_upto, D);
             return true;
         }
         if (D != bin) {
@@ -638,8 +659,8 @@ struct Grid {
                     atomicAdd(&s.excess[0][part_of(e)], bin_excess(bin_entry(power_of<true>(e).p)));
                 });
                 __syncthreads();
-                const unsigned c = s.count[0][lane], c_upto = wave_upto(c, lane);
-                const double w = bin_mass(c, s.excess[0][lane], D) * unit, w_upto = wave_upto(w, lane);
+                const unsigned c = s.count[0][lane], c_upto = wave_upto(c);
+                const double w = bin_mass(c, s.excess[0][lane], D) * unit, w_upto = wave_upto(w);
                 if (BY == BY_KEY) {
                     sub = part_of((double)key_value(t) * a);
                 } else {
@@ -648,9 +669,9 @@ struct Grid {
                     if (!some) return true;
                     sub = enough ? __builtin_ctzll(enough) : 63 - __builtin_clzll(some);
                 }
-                if (__shfl(c, sub) > SA_LIST) return false;
-                first += (int)__shfl(c_upto - c, sub);
-                before += __shfl(w_upto - w, sub);
+                if (of_lane(c, sub) > SA_LIST) return false;
+                first += (int)of_lane(c_upto - c, sub);
+                before += of_lane(w_upto - w, sub);
             }
             __syncthreads();
             if (tid == 0) s.n = 0;
@@ -771,11 +792,8 @@ __global__ __launch_bounds__(64 * WAVES) void sample_select_kernel(SampleArgs A,
             found = weighed = true;
         } else {
             all = wave_all_add(all);
-#pragma unroll
-            for (int d = 32; d >= 1; d /= 2) {
-                reach = min(reach, __shfl_xor(reach, d));
-                known = min(known, __shfl_xor(known, d));
-            }
+            reach = -(int)qg_wave_max(-(float)reach);
+            known = -(int)qg_wave_max(-(float)known);
             counted = wave_all_add(counted) + (__any(below) ? 1 << 30 : 0);  // as many as there are, or more
             if (lane == 0) { s.reach[wave] = reach; s.known[wave] = known; s.flag[wave] = counted; s.grid.wave_sum[wave] = all; }
             __syncthreads();
@@ -791,8 +809,8 @@ __global__ __launch_bounds__(64 * WAVES) void sample_select_kernel(SampleArgs A,
             Grid<WAVES> g{s.grid, r.x, A.bins + (size_t)row * pieces * SA_GRID, stats, A.listed + (size_t)row * pieces * SA_LISTED, A.cols, pieces,
                           tid, lane, wave, (int)place, top, q.a, unit, reach, known, false};
             g.add_up();
-            g.below = in_all > (long)__shfl(g.count_upto, known);
-            total = q.top_k ? __shfl(g.mass_upto, SA_GRID - 1) : all;
+            g.below = in_all > (long)of_lane(g.count_upto, known);
+            total = q.weighs_all() ? all : of_lane(g.mass_upto, SA_GRID - 1);
             found = true;
             if (q.top_k) found = g.template shorten<Grid<WAVES>::BY_COUNT>(q.top_k, 0, cut, total);
             if (found && q.top_p < 1.0) found = g.template shorten<Grid<WAVES>::BY_MASS>(q.top_p * total, 0, cut, total);
@@ -842,13 +860,13 @@ __global__ __launch_bounds__(64 * WAVES) void sample_select_kernel(SampleArgs A,
         int p = -1;
         bool past = false;
         for (int p0 = 0; p0 < pieces && !past; p0 += 64) {
-            const double v = p0 + lane < pieces ? piece[p0 + lane] : 0.0, upto = wave_upto(v, lane) + before;
+            const double v = p0 + lane < pieces ? piece[p0 + lane] : 0.0, upto = wave_upto(v) + before;
             const unsigned long long hit = __ballot(v > 0.0 && upto > goal), any = __ballot(v > 0.0);
             if (!any) continue;
             const int l = hit ? __builtin_ctzll(hit) : 63 - __builtin_clzll(any);
             p = p0 + l;
             past = hit != 0;
-            before = past ? __shfl(upto - v, l) : __shfl(upto, 63);
+            before = past ? of_lane(upto - v, l) : of_lane(upto, 63);
         }
         const bool last = !past;  // no token passes: the last one
         int pick = -1;
@@ -859,14 +877,14 @@ __global__ __launch_bounds__(64 * WAVES) void sample_select_kernel(SampleArgs A,
             const int n = min(stats[p].listed, SA_LISTED);
             for (int i0 = 0; i0 < n && !past; i0 += 64) {
                 const uint2 y = i0 + lane < n ? list[i0 + lane] : make_uint2(0, 0);
-                const double w = i0 + lane < n && cut.keeps(y.x, (int)y.y) ? r.weight(key_value(y.x)) : 0.0, upto = wave_upto(w, lane) + before;
+                const double w = i0 + lane < n && cut.keeps(y.x, (int)y.y) ? r.weight(key_value(y.x)) : 0.0, upto = wave_upto(w) + before;
                 const unsigned long long hit = __ballot(!last && w > 0.0 && upto > goal), any = __ballot(w > 0.0);
                 if (!any) continue;
                 const int l = hit ? __builtin_ctzll(hit) : 63 - __builtin_clzll(any);
-                pick = (int)__shfl(y.y, l);
-                won = __shfl(w, l);
+                pick = (int)of_lane(y.y, l);
+                won = of_lane(w, l);
                 past = hit != 0;
-                before = __shfl(upto, 63);
+                before = of_lane(upto, 63);
             }
         }
         for (int i0 = p * SA_PIECE; !listed && i0 < min((p + 1) * SA_PIECE, A.cols) && !past; i0 += 16 * 64) {
@@ -885,14 +903,14 @@ __global__ __launch_bounds__(64 * WAVES) void sample_select_kernel(SampleArgs A,
 #pragma unroll
             for (int k = 0; k < 16; k++) {
                 if (past || !__any(stays >> k & 1)) continue;
-                const double w = stays >> k & 1 ? r.weight(v[k]) : 0.0, upto = wave_upto(w, lane) + before;
+                const double w = stays >> k & 1 ? r.weight(v[k]) : 0.0, upto = wave_upto(w) + before;
                 const unsigned long long hit = __ballot(!last && w > 0.0 && upto > goal), any = __ballot(w > 0.0);
                 if (!any) continue;
                 const int l = hit ? __builtin_ctzll(hit) : 63 - __builtin_clzll(any);
                 pick = i0 + k * 64 + l;
-                won = __shfl(w, l);
+                won = of_lane(w, l);
                 past = hit != 0;
-                before = __shfl(upto, 63);
+                before = of_lane(upto, 63);
             }
         }
         if (lane == 0) {
