@@ -11,6 +11,7 @@
 // In the order in which the tree is walked, longest common part first, a segment's
 // sequences lie next to each other, so that its rows are a range.
 #include "qg_attention.h"
+#include "qg_lanes.h"
 #include "qg_prefix_index.h"
 
 namespace {
@@ -25,41 +26,38 @@ QG_DEV int table_page(const KvView &c, int s, int j) {
 }
 // Leading pages that sequences s and t have in common, of `most`.
 QG_DEV int common_pages(const KvView &c, int s, int t, int most, int lane) {
-    for (int j0 = 0; j0 < most; j0 += 256) {
-        bool same[4];
+    constexpr int EACH = 8;  // of a lane at once
+    for (int j0 = 0; j0 < most; j0 += 64 * EACH) {
+        int x[EACH], y[EACH];
 #pragma unroll
-        for (int k = 0; k < 4; k++) {
-            const int j = j0 + 64 * k + lane;
-            const int a = j < most ? table_page(c, s, j) : -1, b = j < most ? table_page(c, t, j) : -1;
-            same[k] = a >= 0 && a == b;
+        for (int k = 0; k < EACH; k++) {
+            const int j = min(j0 + 64 * k + lane, most - 1);
+            x[k] = c.table[(size_t)s * c.table_pages + j];
+            y[k] = c.table[(size_t)t * c.table_pages + j];
         }
 #pragma unroll
-        for (int k = 0; k < 4; k++) {
-            const unsigned long long not_same = __ballot(!same[k]);
-            if (not_same) return j0 + 64 * k + __builtin_ctzll(not_same);
+        for (int k = 0; k < EACH; k++) {
+            const int j = j0 + 64 * k + lane;
+            const unsigned long long not_same = __ballot(j >= most || x[k] != y[k] || (unsigned)x[k] >= (unsigned)c.pages);
+            if (not_same) return min(j0 + 64 * k + (int)__builtin_ctzll(not_same), most);
         }
     }
     return most;
 }
-__global__ __launch_bounds__(256) void prefix_link_kernel(KvView c, BatchView b, PrefixView v, int *link, int *shared) {
-    const int lane = threadIdx.x & 63, s = blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (s >= c.sequences) return;
+// Sequence s by a wave.
+QG_DEV void link_sequence(const KvView &c, const BatchView &b, const PrefixView &v, int *link, int *shared, int s, int lane) {
     int first, n, best = 0, with = -1;
     batch_rows(b, s, first, n);
     const int whole = whole_pages(c, s);
     // an earlier sequence has more in common than the best so far only if its page there is the same
     for (int t0 = 0; n > 0 && t0 < s && best < whole;) {
-        const int t = t0 + lane;
-        bool may = false;
-        if (t < s) {
-            int f, m;
-            batch_rows(b, t, f, m);
-            const int p = table_page(c, s, best);
-            may = m > 0 && whole_pages(c, t) > best && p >= 0 && table_page(c, t, best) == p;
-        }
-        const unsigned long long all = __ballot(may);
+        const int t = min(t0 + lane, s - 1);
+        int f, m;
+        batch_rows(b, t, f, m);
+        const int p = table_page(c, s, best), length = whole_pages(c, t), q = table_page(c, t, best);
+        const unsigned long long all = __ballot(t0 + lane < s && m > 0 && length > best && p >= 0 && q == p);
         if (!all) { t0 += 64; continue; }
-        const int u = t0 + __builtin_ctzll(all), x = common_pages(c, s, u, min(whole, whole_pages(c, u)), lane);
+        const int l = __builtin_ctzll(all), u = t0 + l, x = common_pages(c, s, u, min(whole, __builtin_amdgcn_readlane(length, l)), lane);
         if (x > best) { best = x; with = u; }
         t0 = u + 1;
     }
@@ -71,9 +69,15 @@ __global__ __launch_bounds__(256) void prefix_link_kernel(KvView c, BatchView b,
         if (shared) shared[s] = tokens;
     }
 }
+__global__ __launch_bounds__(256) void prefix_link_kernel(KvView c, BatchView b, PrefixView v, int *link, int *shared) {
+    const int s = blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (s < c.sequences) link_sequence(c, b, v, link, shared, s, threadIdx.x & 63);
+}
 
 // ------------------------------------------------------------------------
-// Segments, by one workgroup, a thread per sequence.
+// Segments, by one workgroup or wave, a thread per sequence.  Sorted by the sequence that they hang on, and by
+// falling common part there, the ones that leave it behind some token are a run, and what a segment needs of
+// its siblings are sums over runs.
 // ------------------------------------------------------------------------
 // Common parts count in steps of a quantum: shorter segments would cost more than
 // they save.  It is doubled until the rows of all shared segments together are few
@@ -83,120 +87,174 @@ __host__ __device__ inline long shared_rows_most(long rows) {
     const long most = 16 * rows < 16384 ? 16 * rows : 16384;
     return most > 3 * rows ? most : 3 * rows;
 }
-constexpr int PLAN_THREADS = QG_MAX_SEQUENCES;
-__global__ __launch_bounds__(PLAN_THREADS) void prefix_plan_kernel(KvView c, BatchView b, PrefixView v) {
-    __shared__ int s_link[PLAN_THREADS], s_cut[PLAN_THREADS], s_n[PLAN_THREADS], s_size[PLAN_THREADS], s_off[PLAN_THREADS], s_top[PLAN_THREADS],
-        s_id[PLAN_THREADS], s_same[PLAN_THREADS], s_wave[PLAN_THREADS / 64 + 1];
-    __shared__ unsigned long long s_sum;
-    const int t = threadIdx.x, lane = t & 63, wave = t >> 6, S = c.sequences;
+template <int THREADS>
+struct PlanShared {
+    unsigned long long key[THREADS];
+    int link[THREADS], cut[THREADS], n[THREADS], size[THREADS], off[THREADS], rep[THREADS], next[THREADS], sees[THREADS], top[THREADS], upto[THREADS + 1],
+        run[THREADS + 1], first[THREADS + 1], wave[THREADS / 64 + 1];
+    unsigned long long sum;
+};
+template <int THREADS>
+QG_DEV void plan_sync() {
+    if (THREADS > 64) __syncthreads();
+    else { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); __builtin_amdgcn_wave_barrier(); }
+}
+// Sum over the threads before this one; all: over all.
+template <int THREADS>
+QG_DEV int plan_before(PlanShared<THREADS> &s, int x, int t, int &all) {
+    const int upto = wave_upto(x);
+    if (THREADS == 64) { all = of_lane(upto, 63); return upto - x; }
+    plan_sync<THREADS>();
+    if ((t & 63) == 63) s.wave[t >> 6] = upto;
+    plan_sync<THREADS>();
+    int before = 0;
+    all = 0;
+#pragma unroll
+    for (int w = 0; w < THREADS / 64; w++) {
+        const int y = s.wave[w];
+        if (w < t >> 6) before += y;
+        all += y;
+    }
+    return before + upto - x;
+}
+// Sorts a key of each thread: exchanges at a distance of 64 and more through shared memory.
+template <int THREADS>
+QG_DEV unsigned long long plan_sort(PlanShared<THREADS> &s, unsigned long long key, int t) {
+#pragma unroll 1
+    for (int k = 2; k <= THREADS; k *= 2)
+#pragma unroll 1
+        for (int j = k / 2; j >= 1; j /= 2) {
+            unsigned long long other;
+            if (j >= 64) {
+                plan_sync<THREADS>();
+                s.key[t] = key;
+                plan_sync<THREADS>();
+                other = s.key[t ^ j];
+            } else {
+                other = __shfl_xor(key, j);
+            }
+            const bool low = (t & j) == 0, up = (t & k) == 0;
+            key = (key < other) == (low == up) ? key : other;
+        }
+    plan_sync<THREADS>();
+    s.key[t] = key;
+    plan_sync<THREADS>();
+    return key;
+}
+template <int THREADS>
+QG_DEV void plan_segments(const KvView &c, const BatchView &b, const PrefixView &v, PlanShared<THREADS> &s, int t) {
+    const int S = c.sequences;
     int first = 0, n = 0, len = 0, link0 = -1, shared0 = 0;
     if (t < S) {
         batch_rows(b, t, first, n);
         len = kv_length(c, t);
         if (n > 0) { link0 = v.link[t]; shared0 = v.shared[t]; }
     }
-    s_n[t] = n;
-    int link = -1, cut = 0, off = 0, rep = t, below = -1, below_rep = -1, sees = 0;
+    s.n[t] = n;
+    int link = -1, cut = 0;
     for (int quantum = QUANTUM > 1 << c.shift ? QUANTUM : 1 << c.shift;; quantum *= 2) {
         // the nearest on the way up that has less in common with the one above it
         cut = shared0 / quantum * quantum;
-        s_link[t] = link0;
-        s_cut[t] = cut;
-        s_size[t] = 0;
-        s_top[t] = 0;
-        if (t == 0) s_sum = 0;
-        __syncthreads();
+        plan_sync<THREADS>();
+        s.link[t] = link0;
+        s.cut[t] = cut;
+        s.size[t] = 0;
+        s.top[t] = -1;
+        if (t == 0) s.sum = 0;
+        plan_sync<THREADS>();
         link = cut ? link0 : -1;
-        while (link >= 0 && s_cut[link] >= cut) link = s_link[link];
+        while (link >= 0 && s.cut[link] >= cut) link = s.link[link];
         if (link < 0) cut = 0;
-        __syncthreads();
-        s_link[t] = link;
-        s_cut[t] = cut;
-        __syncthreads();
+        plan_sync<THREADS>();
+        s.link[t] = link;
+        s.cut[t] = cut;
+        plan_sync<THREADS>();
         // rows of a sequence and those that hang on it
-        if (n > 0) {
-            int total = 0;
-            for (int u = t; u >= 0 && total < S; u = s_link[u], total++) atomicAdd(&s_size[u], n);
-        }
-        __syncthreads();
-        // among those on the same sequence: rows that come before, the first with the same cut, the next lower cut, rows of at least this cut
-        off = sees = 0;
-        rep = t;
-        below = -1;
-        below_rep = -1;
         if (n > 0)
-            for (int u = 0; u < S; u++) {
-                if (s_link[u] != link || !s_n[u]) continue;
-                const int x = s_cut[u];
-                if (x > cut || (x == cut && u < t)) off += s_size[u];
-                if (x >= cut) sees += s_size[u];
-                if (x == cut && u < rep) rep = u;
-                if (x < cut && x > below) { below = x; below_rep = u; }
-            }
-        const bool is = n > 0 && link >= 0 && rep == t;
-        if (is) {
-            sees += s_n[link];
-            atomicAdd(&s_sum, (unsigned long long)sees);
+            for (int u = t; u >= 0; u = s.link[u]) atomicAdd(&s.size[u], n);
+        const unsigned long long own = n > 0 ? (unsigned long long)(link + 1) << 40 | (unsigned long long)((1 << 29) - cut) << 10 | (unsigned)t : ~0ULL;
+        const unsigned long long key = plan_sort(s, own, t);
+        // thread t now stands for the t-th in order, sequence u
+        const bool is = key != ~0ULL;
+        const int u = (int)(key & 1023);
+        const unsigned long long before = t ? s.key[t - 1] : ~0ULL;
+        const bool group = is && (t == 0 || before >> 40 != key >> 40), run = is && (t == 0 || before >> 10 != key >> 10);
+        int rows, runs;
+        const int upto = plan_before(s, is ? s.size[u] : 0, t, rows), mine = plan_before(s, (int)run, t, runs) + run - 1;
+        s.upto[t] = upto;
+        if (run) s.run[mine] = t;
+        if (t == 0) {
+            s.upto[THREADS] = rows;
+            s.run[runs] = THREADS;
         }
-        if (n > 0 && link >= 0) atomicMax(&s_top[link], cut);
-        __syncthreads();
-        if ((long)s_sum <= shared_rows_most(b.rows)) break;
-        __syncthreads();
+        const int on = (int)(key >> 40) - 1;  // what u hangs on
+        if (group) {
+            s.first[on + 1] = upto;
+            if (on >= 0) s.top[on] = u;
+        }
+        plan_sync<THREADS>();
+        if (is) {
+            const int start = s.run[mine], behind = s.run[mine + 1];
+            s.off[u] = upto - s.first[on + 1];
+            s.rep[u] = (int)(s.key[start] & 1023);
+            s.next[u] = behind < THREADS && s.key[behind] >> 40 == key >> 40 ? (int)(s.key[behind] & 1023) : -1;
+            s.sees[u] = s.upto[behind] - s.first[on + 1];
+            if (run && on >= 0) atomicAdd(&s.sum, (unsigned long long)(s.sees[u] + s.n[on]));
+        }
+        plan_sync<THREADS>();
+        if ((long)s.sum <= shared_rows_most(b.rows)) break;
     }
     // first rows in walking order
-    s_off[t] = off;
-    s_same[t] = rep;
-    __syncthreads();
-    int pos = off;
-    for (int u = link, steps = 0; u >= 0 && steps < S; u = s_link[u], steps++) pos += s_n[u] + s_off[u];
-    // the segments' numbers: shared ones and tails in one order
-    const bool shares = n > 0 && link >= 0 && rep == t;
-    const unsigned long long tails = __ballot(n > 0), heads = __ballot(shares);
-    if (lane == 0) s_wave[wave] = __popcll(tails) + __popcll(heads);
-    __syncthreads();
-    if (t == 0) {
-        int sum = 0;
-        for (int w = 0; w <= PLAN_THREADS / 64; w++) {
-            const int x = w < PLAN_THREADS / 64 ? s_wave[w] : 0;
-            s_wave[w] = sum;
-            sum += x;
-        }
+    int pos = 0;
+    if (n > 0) {
+        pos = s.off[t];
+        for (int u = link; u >= 0; u = s.link[u]) pos += s.n[u] + s.off[u];
     }
-    __syncthreads();
-    const unsigned long long before = (1ULL << lane) - 1;
-    const int tail_id = s_wave[wave] + __popcll(tails & before) + __popcll(heads & before), head_id = tail_id + 1;
-    s_id[t] = shares ? head_id : -1;
-    s_size[t] = pos;
-    __syncthreads();
-    if (t == 0) v.head[0] = s_wave[PLAN_THREADS / 64];
+    // the segments' numbers: shared ones and tails in one order
+    const bool shares = n > 0 && link >= 0 && s.rep[t] == t;
+    int all;
+    const int tail_id = plan_before(s, (n > 0) + shares, t, all), head_id = tail_id + 1;
+    plan_sync<THREADS>();
+    int *id = s.run, *at = s.first;  // done with
+    id[t] = shares ? head_id : -1;
+    at[t] = pos;
+    plan_sync<THREADS>();
+    if (t == 0) v.head[0] = all;
     if (t < S) {
         v.leaf[t] = n > 0 ? tail_id : -1;
         v.pos[t] = pos;
     }
-    auto put = [&](int id, const Segment &x) {
-        int4 *to = (int4 *)(v.segments + (size_t)id * SEG_INTS);
+    auto put = [&](int i, const Segment &x) {
+        int4 *to = (int4 *)(v.segments + (size_t)i * SEG_INTS);
         to[0] = make_int4(x.owner, x.begin, x.end, x.row0);
         to[1] = make_int4(x.rows, x.up, x.tail, 0);
     };
-    // the segment of sequence u's keys that ends where it leaves the one that it hangs on
-    auto above = [&](int u) { return s_link[u] >= 0 ? s_id[s_same[u]] : -1; };
+    // the segment that ends where sequence u leaves the one that it hangs on
+    auto above = [&](int u) { return s.link[u] >= 0 ? id[s.rep[u]] : -1; };
     if (n > 0) {
-        const int begin = max(s_top[t], cut);
-        int up = above(t);
-        if (s_top[t] > cut) {  // of those that hang here with the largest cut, the first
-            up = -1;
-            for (int u = 0; u < S; u++)
-                if (s_link[u] == t && s_n[u] && s_cut[u] == s_top[t]) { up = s_id[u]; break; }
-        }
-        put(tail_id, Segment{t, begin, len + n, pos, n, up, 1, 0});
+        const int top = s.top[t];  // the first of those that leave it last
+        put(tail_id, Segment{t, top >= 0 ? s.cut[top] : cut, len + n, pos, n, top >= 0 ? id[top] : above(t), 1, 0});
         for (int i = 0; i < n; i++)
             if (pos + i < b.rows) v.row_of[pos + i] = first + i;
     }
     if (shares) {
-        const int base = s_cut[link];
-        const int up = below > base ? s_id[s_same[below_rep]] : above(link);
-        put(head_id, Segment{link, max(below, base), cut, s_size[link], sees, up, 0, 0});
+        const int next = s.next[t], up = next >= 0 ? id[s.rep[next]] : above(link);
+        put(head_id, Segment{link, next >= 0 ? s.cut[next] : s.cut[link], cut, at[link], s.sees[t] + s.n[link], up, 0, 0});
     }
+}
+template <int THREADS>
+__global__ __launch_bounds__(THREADS) void prefix_plan_kernel(KvView c, BatchView b, PrefixView v) {
+    __shared__ PlanShared<THREADS> s;
+    plan_segments<THREADS>(c, b, v, s, threadIdx.x);
+}
+// Both for few sequences, a wave each.
+constexpr int SMALL = 16;
+__global__ __launch_bounds__(64 * SMALL) void prefix_small_kernel(KvView c, BatchView b, PrefixView v, int *link, int *shared) {
+    __shared__ PlanShared<64> s;
+    const int wave = threadIdx.x >> 6;
+    if (wave < c.sequences) link_sequence(c, b, v, link, shared, wave, threadIdx.x & 63);
+    __syncthreads();
+    if (wave == 0) plan_segments<64>(c, b, v, s, threadIdx.x);
 }
 
 // ------------------------------------------------------------------------
@@ -712,8 +770,13 @@ int qg_kv_prefixes(int *link, int *shared, const qg_kv_cache *cache, const qg_kv
     if (qg_any_overlap(out, in) || qg_overlap(link, each, shared, each) || qg_overlap(prefixes, need, link, each) || qg_overlap(prefixes, need, shared, each))
         return hipErrorInvalidValue;
     const PrefixView v = prefix_view(prefixes, c.sequences);
+    if (c.sequences <= SMALL) {
+        prefix_small_kernel<<<1, 64 * SMALL, 0, qg_stream()>>>(c, b, v, link, shared);
+        return hipGetLastError();
+    }
     prefix_link_kernel<<<(c.sequences + 3) / 4, 256, 0, qg_stream()>>>(c, b, v, link, shared);
-    prefix_plan_kernel<<<1, PLAN_THREADS, 0, qg_stream()>>>(c, b, v);
+    if (c.sequences <= 64) prefix_plan_kernel<64><<<1, 64, 0, qg_stream()>>>(c, b, v);
+    else prefix_plan_kernel<QG_MAX_SEQUENCES><<<1, QG_MAX_SEQUENCES, 0, qg_stream()>>>(c, b, v);
     return hipGetLastError();
 }
 
