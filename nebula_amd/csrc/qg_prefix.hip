@@ -210,16 +210,16 @@ QG_DEV void plan_segments(const KvView &c, const BatchView &b, const PrefixView 
         pos = s.off[t];
         for (int u = link; u >= 0; u = s.link[u]) pos += s.n[u] + s.off[u];
     }
-    // the segments' numbers: shared ones and tails in one order
+    // the segments' numbers: the shared ones first
     const bool shares = n > 0 && link >= 0 && s.rep[t] == t;
-    int all;
-    const int tail_id = plan_before(s, (n > 0) + shares, t, all), head_id = tail_id + 1;
+    int heads, tails;
+    const int head_id = plan_before(s, (int)shares, t, heads), tail_id = heads + plan_before(s, (int)(n > 0), t, tails);
     plan_sync<THREADS>();
     int *id = s.run, *at = s.first;  // done with
     id[t] = shares ? head_id : -1;
     at[t] = pos;
     plan_sync<THREADS>();
-    if (t == 0) v.head[0] = all;
+    if (t == 0) { v.head[0] = heads + tails; v.head[1] = heads; }
     if (t < S) {
         v.leaf[t] = n > 0 ? tail_id : -1;
         v.pos[t] = pos;
@@ -277,98 +277,137 @@ QG_DEV Segment read_segment(const KvView &c, const BatchView &b, const PrefixVie
 // A unit of work: a part of a segment's keys, a head, a group of its rows.
 struct Unit {
     Segment s;
-    int id, groups, chunk, parts, part, z, h, tile;  // tile: the first of the segment's
+    int id, groups, tiles, chunk, parts, part, z, h, tile;  // tiles: of a group; tile: the first of the segment's
 };
 constexpr int CHUNK = 128;  // keys per unit, at least and in steps of
+// What a unit costs, in key x weight: a key weighs 1 more than its row tiles (its reads, and the products and
+// weights of each tile), and to begin and to end takes as long as 1000 do.
+constexpr float UNIT_COST = 1000.0f;
+__host__ __device__ constexpr int key_weight(int tiles) { return 1 + tiles; }
 
+// A segment's row groups of equal size and as few as the registers allow.
 struct UnitLane { int keys, groups, tiles; };
-template <int RS, int RT>
-QG_DEV bool find_unit(const KvView &c, const BatchView &b, const PrefixArgs &A, const PrefixView &v, int lane, int block, Unit &p) {
-    const int count = segment_count(c, v);
-    auto lane_of = [&](int i) {
-        UnitLane x{0, 0, 0};
-        if (i < count) {
-            const Segment s = read_segment(c, b, v, i);
-            const int tiles = s.tail ? RT : RS;
-            if (s.rows && s.end > s.begin) x = UnitLane{s.end - s.begin, (s.rows * A.group + 16 * tiles - 1) / (16 * tiles), tiles};
-        }
-        return x;
-    };
-    const UnitLane mine = lane_of(lane);
-    auto over = [&](auto f) {
-        float r = f(mine);
-        for (int i = lane + 64; i < count; i += 64) r += f(lane_of(i));
-        r = qg_row_sum(r);
-        float x = 0.0f;
+template <int MOST>
+QG_DEV UnitLane unit_lane(const PrefixArgs &A, const Segment &s) {
+    const int rows = s.rows * A.group, keys = s.end - s.begin;
+    if (rows <= 0 || keys <= 0) return UnitLane{0, 0, 1};
+    const int groups = (rows + 16 * MOST - 1) / (16 * MOST);
+    int tiles = 1;
 #pragma unroll
-        for (int i = 0; i < 64; i += 16) x += __int_as_float(__builtin_amdgcn_readlane(__float_as_int(r), i));
-        return x * (float)c.heads;
+    for (int k = 1; k < MOST; k++) tiles += rows > 16 * k * groups;
+    return UnitLane{keys, groups, tiles};
+}
+// The keys of a segment's part where a unit's keys cost `even`, and the parts.
+QG_DEV int part_keys(float even, int tiles) {
+    return ((int)fminf(even * __builtin_amdgcn_rcpf((float)key_weight(tiles)), (float)(1 << 28)) / CHUNK + 1) * CHUNK;
+}
+QG_DEV int part_count(float even, const UnitLane &x) {
+    const int chunk = part_keys(even, x.tiles), n = (int)(((float)x.keys - 0.5f) * __builtin_amdgcn_rcpf((float)chunk)) + 1;
+    return x.groups ? n + (n * chunk < x.keys) : 0;  // the product may be off in its last bits: never a key too few
+}
+// Every workgroup finds its unit by itself: in one round of resident workgroups (two, where the row groups alone come to
+// half of one) units that cost about the same, of the shared segments first, and of both an eighth to each XCD, in whose
+// L2 the row groups with the same keys meet.  False if there is none.  A thread per segment and nothing unrolled:
+// what runs once is bound by the fetch of its instructions (four segments a lane in every wave: 5 to 13 us, now 2 to 4).
+template <int NW>
+struct FindShared { float f[2][2][NW]; int i[2][2][NW], found[8]; };
+template <int MOST, int NW>
+QG_DEV bool find_unit(const KvView &c, const BatchView &b, const PrefixArgs &A, const PrefixView &v, int block, FindShared<NW> &s, Unit &p) {
+    constexpr int THREADS = 64 * NW;
+    const int tid = threadIdx.x, wave = tid >> 6, most = 2 * c.sequences;
+    const Segment own = read_segment(c, b, v, min(tid, most - 1));
+    const int count = segment_count(c, v), shared = kv_clamp(v.head[1], 0, count);
+    if (tid == 0) s.found[0] = -1;
+    auto lane_of = [&](const Segment &x, int i) { return i < count ? unit_lane<MOST>(A, x) : UnitLane{0, 0, 1}; };
+    const UnitLane mine = lane_of(own, tid);
+    // f(a thread's segment, its number) for all
+    auto each = [&](auto f) {
+#pragma unroll 1
+        for (int i = tid; i - tid < count; i += THREADS) f(i < THREADS ? mine : lane_of(read_segment(c, b, v, min(i, most - 1)), i), i);
     };
-    // one round of resident workgroups, two where the row groups alone come to half a round
-    const float least = over([](const UnitLane &x) { return (float)x.groups; });
-    const float room = (2.0f * least <= (float)A.resident ? 1.0f : 2.0f) * (float)A.resident;
-    // 1.0001: above the sum whatever its roundings, so that the tiles suffice
-    const float even = 1.0001f * over([](const UnitLane &x) { return (float)x.groups * (float)x.keys; }) / room;
-    int chunk = ((int)fminf(even, (float)(1 << 28)) / CHUNK + 1) * CHUNK;
-    for (int i = 0; i < 4 && least <= room; i++) {  // the parts round up: longer ones until they fit
-        const float units = over([&](const UnitLane &x) { return x.groups ? (float)(((x.keys - 1) / chunk + 1) * x.groups) : 0.0f; });
-        if (units <= room) break;
-        chunk = max((int)fminf((float)chunk * units / room, (float)(1 << 28)) / CHUNK, chunk / CHUNK) * CHUNK + CHUNK;
-    }
-    auto scan = [&](int i0, UnitLane &x, int &parts, int &upto, int &upto_tiles) {
-        x = i0 ? lane_of(i0 + lane) : mine;
-        parts = x.groups ? (x.keys - 1) / chunk + 1 : 0;
-        upto = parts * x.groups * c.heads;
-        upto_tiles = upto * x.tiles;
+    // sums of two values over the workgroup; the places alternate, so that one barrier does
+    int turn = 0;
+    auto sum2 = [&](auto (&at)[2][2][NW], auto &x, auto &y) {
+        turn ^= 1;
+        x = wave_all_add(x);
+        y = wave_all_add(y);
+        if ((tid & 63) == 0) { at[turn][0][wave] = x; at[turn][1][wave] = y; }
+        __syncthreads();
+        x = at[turn][0][0];
+        y = at[turn][1][0];
 #pragma unroll
-        for (int d = 1; d < 64; d *= 2) {
-            const int u = __shfl_up(upto, d), e = __shfl_up(upto_tiles, d);
-            if (lane >= d) { upto += u; upto_tiles += e; }
-        }
+        for (int w = 1; w < NW; w++) { x += at[turn][0][w]; y += at[turn][1][w]; }
     };
-    UnitLane x;
-    int parts, upto, upto_tiles, units = 0;
-    for (int i0 = 0; i0 < count; i0 += 64) {
-        scan(i0, x, parts, upto, upto_tiles);
-        units += __builtin_amdgcn_readlane(upto, 63);
-    }
-    if (units <= 0) return false;
-    // an eighth of the units to each XCD: row groups with the same keys meet in its L2
-    const int run = (units + 7) / 8, unit = (block & 7) * run + (block >> 3);
-    if (unit >= units || (block >> 3) >= run) return false;
+    float groups = 0.0f, cost = 0.0f;
+    each([&](const UnitLane &x, int) {
+        groups += (float)x.groups;
+        cost += (float)x.groups * ((float)x.keys * (float)key_weight(x.tiles) + UNIT_COST);
+    });
+    sum2(s.f, groups, cost);
+    groups *= (float)c.heads;
+    cost *= (float)c.heads;
+    const float room = (2.0f * groups <= (float)A.resident ? 1.0f : 2.0f) * (float)A.resident;
+    // 1.0001: above the sum whatever its roundings, so that the tiles suffice.  Groups that are cut round up by a part at
+    // most: with that much less room what the units cost together fits.
+    float even = 1.0001f * cost / room, cut = 0.0f, none = 0.0f;
+    each([&](const UnitLane &x, int) { cut += (float)(x.keys * key_weight(x.tiles)) > even ? (float)x.groups : 0.0f; });
+    sum2(s.f, cut, none);
+    cut *= (float)c.heads;
+    if (groups <= room) even = 1.0001f * cost / (room - fminf(cut, 0.5f * room));
+    int of_shared = 0, units = 0;
+    each([&](const UnitLane &x, int i) {
+        const int n = part_count(even, x) * x.groups * c.heads;
+        units += n;
+        of_shared += i < shared ? n : 0;
+    });
+    sum2(s.i, units, of_shared);
+    // blocks go round the XCDs
+    const int run = (of_shared + 7) / 8, tail_run = (units - of_shared + 7) / 8, x = block & 7, k = block >> 3;
+    const int unit = k < run ? x * run + k : of_shared + x * tail_run + (k - run);
+    if (unit < 0 || unit >= (k < run ? of_shared : units) || k - run >= tail_run) return false;  // below 0: row starts that overlap, past 2^31 units
     int before = 0, tiles = 0;
-    for (int i0 = 0; i0 < count; i0 += 64) {
-        if (count > 64) scan(i0, x, parts, upto, upto_tiles);
-        const int own = parts * x.groups * c.heads;
-        const unsigned long long here = __ballot(unit < before + upto && unit >= before + upto - own);
-        if (here) {
-            const int l = __builtin_ctzll(here);
-            p.id = i0 + l;
-            p.s = read_segment(c, b, v, p.id);
-            p.groups = __builtin_amdgcn_readlane(x.groups, l);
-            p.parts = __builtin_amdgcn_readlane(parts, l);
-            p.tile = tiles + __builtin_amdgcn_readlane(upto_tiles - own * x.tiles, l);
-            const int rest = unit - (before + __builtin_amdgcn_readlane(upto - own, l));
-            if (rest < 0 || rest >= __builtin_amdgcn_readlane(own, l)) return false;  // row starts that overlap, past 2^31 units
-            p.part = rest / (p.groups * c.heads);
-            p.h = rest / p.groups % c.heads;
-            p.z = rest % p.groups;
-            p.chunk = chunk;
-            return true;
+    each([&](const UnitLane &x, int i) {
+        const int parts = part_count(even, x), own = parts * x.groups * c.heads;
+        const int upto = wave_upto(own), upto_tiles = wave_upto(own * x.tiles);
+        turn ^= 1;
+        if ((tid & 63) == 63) { s.i[turn][0][wave] = upto; s.i[turn][1][wave] = upto_tiles; }
+        __syncthreads();
+        int first = before + upto - own, tile = tiles + upto_tiles - own * x.tiles;
+#pragma unroll
+        for (int w = 0; w < NW; w++) {
+            const int n = s.i[turn][0][w], m = s.i[turn][1][w];
+            if (w < wave) { first += n; tile += m; }
+            before += n;
+            tiles += m;
         }
-        before += __builtin_amdgcn_readlane(upto, 63);
-        tiles += __builtin_amdgcn_readlane(upto_tiles, 63);
-    }
-    return false;
+        if (unit >= first && unit < first + own) {
+            s.found[0] = i; s.found[1] = x.groups; s.found[2] = x.tiles; s.found[3] = parts; s.found[4] = tile; s.found[5] = unit - first;
+        }
+    });
+    __syncthreads();
+    p.id = __builtin_amdgcn_readfirstlane(s.found[0]);
+    if (p.id < 0) return false;
+    p.s = read_segment(c, b, v, p.id);
+    p.groups = __builtin_amdgcn_readfirstlane(s.found[1]);
+    p.tiles = __builtin_amdgcn_readfirstlane(s.found[2]);
+    p.parts = __builtin_amdgcn_readfirstlane(s.found[3]);
+    p.tile = __builtin_amdgcn_readfirstlane(s.found[4]);
+    const int rest = __builtin_amdgcn_readfirstlane(s.found[5]), of_head = rest / p.groups;
+    p.z = rest - of_head * p.groups;
+    p.part = of_head / c.heads;
+    p.h = of_head - p.part * c.heads;
+    p.chunk = part_keys(even, p.tiles);
+    return true;
 }
 
-template <int TYPE, int D, int RS, int NW>
+template <int TYPE, int D, int MOST, int NW>
 struct PrefixShared {
     typedef Tile<TYPE, D> T;
-    static constexpr int JOIN = NW * 16 * (D + 4) * 4, Q = RS * T::Q_BYTES;
-    __attribute__((aligned(16))) uint8_t mem[Q > JOIN ? Q : JOIN];
-    float m[NW][16 * RS], l[NW][16 * RS], back[16 * RS];
+    static constexpr int JOIN = NW * 16 * (D + 4) * 4, Q = MOST * T::Q_BYTES;  // of one row tile; two are used in turn
+    __attribute__((aligned(16))) uint8_t mem[Q > 2 * JOIN ? Q : 2 * JOIN];
+    float m[NW][16 * MOST], l[NW][16 * MOST], back[16 * MOST];
     unsigned long long seen[QG_MAX_TREE];
+    FindShared<NW> find;
 };
 
 // One unit, as qg_tree_attention takes a part of a sequence: each wave walks tiles of
@@ -401,33 +440,39 @@ QG_DEV void unit_attention(const PrefixArgs &A, const KvView &c, const BatchView
         if (fits && tid < RG) A.part_ml[(size_t)tile0 * 16 + tid] = make_float2(-__builtin_inff(), 0.0f);
         return;
     }
-    float x[RG / (4 * NW)][DL];
-    size_t at_q[RG / (4 * NW)];  // the row and head, or -1
-#pragma unroll
-    for (int i = 0; i < RG / (4 * NW); i++) {
-        const int at = row0 + (i * NW + wave) * 4 + g, t = by_group(A, at);
-        int row = -1;
-        if (at < rows) row = TAIL ? (t < count ? first + t : -1) : kv_clamp(v.row_of[p.s.row0 + t], 0, b.rows - 1);
-        at_q[i] = row >= 0 ? (size_t)row * A.q_heads + p.h * A.group + (at - t * A.group) : (size_t)-1;
-#pragma unroll
-        for (int d = 0; d < DL; d += 4) {
-            const float4 y = row >= 0 ? *(const float4 *)(A.q + at_q[i] * D + n * DL + d) : make_float4(0, 0, 0, 0);
-            x[i][d] = y.x; x[i][d + 1] = y.y; x[i][d + 2] = y.z; x[i][d + 3] = y.w;
-        }
-    }
     const size_t page_bytes = ((size_t)c.heads << c.shift) * D * T::ES;
     const uint8_t *kbase = c.k + (((size_t)A.layer * c.pages * c.heads + p.h) << c.shift) * D * T::ES;
     const uint8_t *vbase = c.v + (((size_t)A.layer * c.pages * c.heads + p.h) << c.shift) * D * T::ES;
     const int slot_mask = (1 << c.shift) - 1;
     // a run of E keys from position pos, aligned to E: inside one page
     auto run = [&](const uint8_t *base, int page, int pos) { return base + (size_t)max(page, 0) * page_bytes + (size_t)((pos & slot_mask) * (D * T::ES)); };
+    // the pages and the places of the rows first, then what lies there: two round trips before the first product
     T tile;
     int t0 = begin + wave * KEYS, kpos = t0 + E * (n >> 2), vpos = t0 + E * g;
     int kpage = kv_page(c, owner, kpos), vpage = kv_page(c, owner, vpos);
     int kpage1 = kv_page(c, owner, kpos + NW * KEYS), vpage1 = kv_page(c, owner, vpos + NW * KEYS);
+    int rows_at[RG / (4 * NW)];
+#pragma unroll
+    for (int i = 0; i < RG / (4 * NW); i++) {
+        const int at = row0 + (i * NW + wave) * 4 + g, t = by_group(A, at);
+        rows_at[i] = -1;
+        if (at < rows) rows_at[i] = TAIL ? (t < count ? first + t : -1) : kv_clamp(v.row_of[p.s.row0 + t], 0, b.rows - 1);
+    }
     if (t0 < end) {
         tile.load_k(run(kbase, kpage, kpos), n, g);
         tile.load_v(run(vbase, vpage, vpos), n);
+    }
+    float x[RG / (4 * NW)][DL];
+    size_t at_q[RG / (4 * NW)];  // the row and head, or -1
+#pragma unroll
+    for (int i = 0; i < RG / (4 * NW); i++) {
+        const int at = row0 + (i * NW + wave) * 4 + g, row = rows_at[i];
+        at_q[i] = row >= 0 ? (size_t)row * A.q_heads + p.h * A.group + (at - by_group(A, at) * A.group) : (size_t)-1;
+#pragma unroll
+        for (int d = 0; d < DL; d += 4) {
+            const float4 y = row >= 0 ? *(const float4 *)(A.q + at_q[i] * D + n * DL + d) : make_float4(0, 0, 0, 0);
+            x[i][d] = y.x; x[i][d + 1] = y.y; x[i][d + 2] = y.z; x[i][d + 3] = y.w;
+        }
     }
 #pragma unroll
     for (int i = 0; i < RG / (4 * NW); i++) {
@@ -559,9 +604,9 @@ QG_DEV void unit_attention(const PrefixArgs &A, const KvView &c, const BatchView
         s.l[0][tid] = sum;
         if (!direct && fits) A.part_ml[(size_t)tile0 * 16 + tid] = make_float2(top, sum);
     }
-    float *join = (float *)s.mem;
 #pragma unroll
     for (int r = 0; r < RT; r++) {
+        float *join = (float *)(s.mem + (r & 1) * SHARED::JOIN);
 #pragma unroll
         for (int i = 0; i < 4; i++)
 #pragma unroll
@@ -594,18 +639,21 @@ QG_DEV void unit_attention(const PrefixArgs &A, const KvView &c, const BatchView
                 *(float4 *)(A.part_o + ((size_t)(tile0 + r) * 16 + row) * D + d) = y;
             }
         }
-        __syncthreads();
     }
 }
 
-// RS row tiles of shared segments, RT of the sequences' own.
-template <int TYPE, int D, int RS, int RT, int NW>
-__global__ __launch_bounds__(64 * NW, (D / 64) * RS <= 6 ? 2 : 1) void prefix_attention_kernel(PrefixArgs A, KvView c, BatchView b, PrefixView v) {
-    __shared__ PrefixShared<TYPE, D, RS, NW> s;
+template <int TYPE, int D, int MOST, bool TAIL, int NW, int RT, typename SHARED>
+QG_DEV void unit_of_tiles(const PrefixArgs &A, const KvView &c, const BatchView &b, const PrefixView &v, const Unit &p, SHARED &s) {
+    if (p.tiles == RT) unit_attention<TYPE, D, RT, TAIL, NW>(A, c, b, v, p, s);
+    else if constexpr (RT < MOST) unit_of_tiles<TYPE, D, MOST, TAIL, NW, RT + 1>(A, c, b, v, p, s);
+}
+template <int TYPE, int D, int MOST, int NW>
+__global__ __launch_bounds__(64 * NW, (D / 64) * MOST <= 6 ? 2 : 1) void prefix_attention_kernel(PrefixArgs A, KvView c, BatchView b, PrefixView v) {
+    __shared__ PrefixShared<TYPE, D, MOST, NW> s;
     Unit p;
-    if (!find_unit<RS, RT>(c, b, A, v, threadIdx.x & 63, blockIdx.x, p)) return;
-    if (p.s.tail) unit_attention<TYPE, D, RT, true, NW>(A, c, b, v, p, s);
-    else unit_attention<TYPE, D, RS, false, NW>(A, c, b, v, p, s);
+    if (!find_unit<MOST, NW>(c, b, A, v, blockIdx.x, s.find, p)) return;
+    if (p.s.tail) unit_of_tiles<TYPE, D, MOST, true, NW, 1>(A, c, b, v, p, s);
+    else unit_of_tiles<TYPE, D, MOST, false, NW, 1>(A, c, b, v, p, s);
 }
 
 // Joins a row's segments.  Few rows and heads: a workgroup each, whose four waves
@@ -714,38 +762,28 @@ __global__ __launch_bounds__(64 * JOIN_WAVES) void prefix_join_kernel(PrefixArgs
     if (odd && (EACH > 1 || wave == 0)) attend_row<TYPE, D>(A, c, b, s, first, n, row, head, lane, s_y[wave]);
 }
 
-// Row groups of all segments, at most (each rounds up), for the segments' own tiles.
-long groups_most(const BatchView &b, int S, int group, int rs, int rt) {
-    return shared_rows_most(b.rows) * group / (16 * rs) + (long)b.rows * group / (16 * rt) + 2L * S;
+// Row groups of all segments, at most (each rounds up), and their row tiles: groups of t tiles have more than t - 1 tiles' rows each.
+long groups_most(const BatchView &b, int S, int group, int dim) {
+    return (shared_rows_most(b.rows) + b.rows) * group / (16 * most_tiles(dim)) + 2L * S;
 }
-// Tiles of partial results that the units can ask for: parts of a segment are at most its keys / chunk + 1.
+// Tiles of partial results that the units can ask for: parts of a segment are at most its share of a round + 1.
 long tiles_most(const BatchView &b, int S, int heads, int group, int dim) {
-    const int rs = most_tiles(dim);
-    return 2L * resident(dim, rs) * rs + heads * (shared_rows_most(b.rows) * group / 16 + (long)b.rows * group / 16 + 2L * S * rs);
+    return 2L * resident(dim, most_tiles(dim)) * most_tiles(dim) +
+           heads * ((shared_rows_most(b.rows) + b.rows) * group / 16 + groups_most(b, S, group, dim) + 2L * S);
 }
-template <int TYPE, int D, int RT>
+template <int TYPE, int D>
 void launch(const PrefixArgs &A, const KvView &c, const BatchView &b, const PrefixView &v, hipStream_t s) {
-    constexpr int RS = most_tiles(D);
-    const long units = 2 * A.resident + groups_most(b, c.sequences, A.group, RS, RT) * c.heads;
-    prefix_attention_kernel<TYPE, D, RS, RT, WAVES><<<(unsigned)((units + 7) / 8 * 8), 64 * WAVES, 0, s>>>(A, c, b, v);
+    const long units = 2 * A.resident + groups_most(b, c.sequences, A.group, D) * c.heads + 16;
+    prefix_attention_kernel<TYPE, D, most_tiles(D), WAVES><<<(unsigned)((units + 7) / 8 * 8), 64 * WAVES, 0, s>>>(A, c, b, v);
     const size_t jobs = (size_t)b.rows * A.q_heads;
     if (jobs > JOIN_FEW) prefix_join_kernel<TYPE, D, 4><<<(unsigned)((jobs + 3) / 4), 256, 0, s>>>(A, c, b, v);
     else prefix_join_kernel<TYPE, D, 1><<<(unsigned)jobs, 256, 0, s>>>(A, c, b, v);
 }
-template <int TYPE, int D>
-void launch_rt(int rt, const PrefixArgs &A, const KvView &c, const BatchView &b, const PrefixView &v, hipStream_t s) {
-    if (rt == 1) launch<TYPE, D, 1>(A, c, b, v, s);
-    else if (rt == 2) launch<TYPE, D, 2>(A, c, b, v, s);
-    else if constexpr (D != 256) {
-        if (rt == 3) launch<TYPE, D, 3>(A, c, b, v, s);
-        else if constexpr (D == 64) launch<TYPE, D, 4>(A, c, b, v, s);
-    }
-}
 template <int TYPE>
-void launch_dim(int rt, const PrefixArgs &A, const KvView &c, const BatchView &b, const PrefixView &v, hipStream_t s) {
-    if (c.dim == 64) launch_rt<TYPE, 64>(rt, A, c, b, v, s);
-    else if (c.dim == 128) launch_rt<TYPE, 128>(rt, A, c, b, v, s);
-    else launch_rt<TYPE, 256>(rt, A, c, b, v, s);
+void launch_dim(const PrefixArgs &A, const KvView &c, const BatchView &b, const PrefixView &v, hipStream_t s) {
+    if (c.dim == 64) launch<TYPE, 64>(A, c, b, v, s);
+    else if (c.dim == 128) launch<TYPE, 128>(A, c, b, v, s);
+    else launch<TYPE, 256>(A, c, b, v, s);
 }
 constexpr long JOBS = 1L << 25;  // rows x heads: of the join kernel, a wave each, within 2^32 threads
 constexpr long TILES = 1L << 27; // of partial results, within an int of rows
@@ -803,17 +841,17 @@ int qg_prefix_attention(float *out, const float *q, int q_heads, float scale, co
     const size_t bytes = 4 * (size_t)b.rows * q_heads * c.dim;
     const QgSpan written[2] = {{out, bytes}, {ws, need}}, read[2] = {{q, bytes}, {prefixes, plan}};
     if (qg_any_overlap(written, read) || qg_overlap(out, bytes, ws, need)) return hipErrorInvalidValue;
-    const int group = q_heads / c.heads, rt = row_tiles(c.dim, (long)b.max_rows * group), rs = most_tiles(c.dim);
+    const int group = q_heads / c.heads;
     const long tiles = tiles_most(b, c.sequences, c.heads, group, c.dim);
     float *part_o = (float *)ws;
     float2 *part_ml = (float2 *)(part_o + (size_t)tiles * 16 * c.dim);
     int4 *joins = (int4 *)(part_ml + (size_t)tiles * 16);
     const PrefixArgs A{attn_rows(out, q, q_heads, group, layer, scale), part_o, part_ml, joins, (int *)(joins + 2 * (size_t)c.sequences),
-                       resident(c.dim, rs), (int)tiles};
+                       resident(c.dim, most_tiles(c.dim)), (int)tiles};
     const PrefixView v = prefix_view(const_cast<void *>(prefixes), c.sequences);
-    if (c.type == QT_F32) launch_dim<QT_F32>(rt, A, c, b, v, qg_stream());
-    else if (c.type == QT_F16) launch_dim<QT_F16>(rt, A, c, b, v, qg_stream());
-    else launch_dim<QT_BF16>(rt, A, c, b, v, qg_stream());
+    if (c.type == QT_F32) launch_dim<QT_F32>(A, c, b, v, qg_stream());
+    else if (c.type == QT_F16) launch_dim<QT_F16>(A, c, b, v, qg_stream());
+    else launch_dim<QT_BF16>(A, c, b, v, qg_stream());
     return hipGetLastError();
 }
 

@@ -12,7 +12,7 @@ struct Segment { int owner, begin, end, row0, rows, up, tail, pad; };
 enum { SEG_INTS = 8, PREFIX_HEAD = 16 };
 
 struct PrefixView {
-    int *head;           // [0] number of segments
+    int *head;           // [0] number of segments, [1] of the shared ones, which come first
     int *segments;       // [2 S] Segment
     int *leaf;           // [S] the last segment of each sequence, -1 without rows
     int *pos;            // [S] a sequence's first row in walking order
