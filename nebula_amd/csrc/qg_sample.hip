@@ -427,16 +427,22 @@ __global__ __launch_bounds__(PIECE_THREADS) void sample_piece_kernel(SampleArgs 
 // ranked (of a bin with too many, those of the 64th part in which the cut is).  What the bins do not
 // hold is left to the search over the whole row.
 // ------------------------------------------------------------------------
-constexpr int SA_LIST = 1024;  // values that are ranked
+constexpr int SA_LIST = 1024, SA_HELD = 2 * SA_LIST;  // values that are ranked; that are held
 template <int WAVES>
 struct GridShared {
     unsigned count[WAVES][SA_GRID];
     unsigned long long excess[WAVES][SA_GRID];
-    unsigned long long put[SA_LIST];  // key, then the complement of the index: of equal keys the lower index is the larger
-    uint32_t sorted_key[SA_LIST];
-    int sorted_index[SA_LIST];
+    union {
+        struct {
+            unsigned long long put[SA_LIST];  // key, then the complement of the index: of equal keys the lower index is the larger
+            uint32_t sorted_key[SA_LIST];
+            int sorted_index[SA_LIST];
+        };
+        double in_order[SA_HELD];             // sums of the held values' weights
+    };
     double upto[SA_LIST], wave_sum[WAVES];
-    int n, hits;
+    uint2 held[SA_HELD];                      // key and index, in the tokens' order
+    int n, hits, of_piece[64];
 };
 template <int WAVES>
 struct SelectShared {
@@ -464,6 +470,7 @@ struct Grid {
     int deepest;                                     // the bin of the cut
     int bin, kept;                                   // the ranked bin (-1: none, or a part of one), and how many of the ranked values stay
     bool part;                                       // the cut is in a part of its bin
+    int held;                                        // values in s.held: all of the bins that any cut can leave; 0: not held
 
     __device__ __forceinline__ double weight(uint32_t key) const { return exp2_d(((double)key_value(key) - (double)m) * a); }
     __device__ __forceinline__ double place_of(uint32_t key) const { return grid_place(key_value(key), a); }
@@ -506,6 +513,58 @@ struct Grid {
         bin = -1;
         kept = 0;
         part = false;
+        held = 0;
+    }
+    // Holds the listed values of bins 0..D, where lists reach that far and they are not too many.
+    __device__ __forceinline__ void hold(int D) {
+        constexpr int EACH = 64 / WAVES, PER = SA_LISTED / 64;
+        const int n = D < 0 || D > reach || pieces > 64 ? 0 : (int)of_lane(count_upto, D);
+        if (n == 0 || n > SA_HELD) return;
+        uint2 y[EACH][PER];
+#pragma unroll
+        for (int k = 0; k < EACH; k++) {
+            const int p = k * WAVES + wave, listed = p < pieces && stats[p].at != GRID_LOW ? stats[p].listed : 0;
+#pragma unroll
+            for (int i = 0; i < PER; i++) y[k][i] = i * 64 + lane < listed ? lists[(size_t)p * SA_LISTED + i * 64 + lane] : make_uint2(0, 0);
+        }
+        unsigned is = 0;
+#pragma unroll
+        for (int k = 0; k < EACH; k++) {
+            int all = 0;
+#pragma unroll
+            for (int i = 0; i < PER; i++) {
+                const bool in = y[k][i].x && (double)place - place_of(y[k][i].x) <= (double)D;
+                is |= (unsigned)in << (k * PER + i);
+                all += (int)__popcll(__ballot(in));
+            }
+            if (lane == 0) s.of_piece[k * WAVES + wave] = all;
+        }
+        __syncthreads();
+        const int own = s.of_piece[lane], before = wave_upto(own) - own;
+#pragma unroll
+        for (int k = 0; k < EACH; k++) {
+            int to = of_lane(before, k * WAVES + wave);
+#pragma unroll
+            for (int i = 0; i < PER; i++) {
+                const bool in = is >> (k * PER + i) & 1;
+                const unsigned long long all = __ballot(in);
+                const int at = to + (int)__popcll(all & ((1ULL << lane) - 1));
+                if (in && at < SA_HELD) s.held[at] = y[k][i];
+                to += (int)__popcll(all);
+            }
+        }
+        held = min(of_lane(before + own, 63), SA_HELD);
+        __syncthreads();
+    }
+    // The bin in which the row's first filter cuts, -1 for none.
+    __device__ __forceinline__ int first_cut(const Request &q, double all, uint32_t least) const {
+        if (q.top_k || q.top_p < 1.0) {
+            const unsigned long long enough =
+                __ballot(lane <= known && count_upto > 0 && (q.top_k ? count_upto >= (unsigned)q.top_k : mass_upto >= q.top_p * all));
+            return enough ? (int)__builtin_ctzll(enough) : -1;
+        }
+        const double d = (double)place - place_of(least);
+        return d <= (double)known ? (int)d : -1;
     }
     __device__ __forceinline__ void put(uint32_t key, int i) {
         const int k = atomicAdd(&s.n, 1);
@@ -514,6 +573,10 @@ struct Grid {
     // f(key, index) of the values in bin D (every lane of some waves each), and of more
     template <typename F>
     __device__ __forceinline__ void each_of_bin(int D, F f) {
+        if (held) {
+            for (int i = tid; i < held; i += THREADS) f(s.held[i].x, (int)s.held[i].y);
+            return;
+        }
         if (D <= reach) {
             for (int e0 = wave; e0 < pieces * (SA_LISTED / 64); e0 += 4 * WAVES) {
                 uint2 y[4];
@@ -566,10 +629,15 @@ struct Grid {
             s.sorted_index[rank] = (int)~(uint32_t)own;
         }
         __syncthreads();
+        sum_up(s.upto, n, [&](int i) { return weight(s.sorted_key[i]); });
+    }
+    // to[i] = w(0) + .. + w(i), i < n
+    template <typename F>
+    __device__ __forceinline__ void sum_up(double *to, int n, F f) {
         double before = 0.0;
         for (int i0 = 0; i0 < n; i0 += THREADS) {
             const int i = i0 + tid;
-            double w = wave_upto(i < n ? weight(s.sorted_key[i]) : 0.0);
+            double w = wave_upto(i < n ? f(i) : 0.0);
             __syncthreads();
             if (lane == 63) s.wave_sum[wave] = w;
             __syncthreads();
@@ -579,7 +647,7 @@ struct Grid {
                 if (k < wave) w += s.wave_sum[k];
                 all += s.wave_sum[k];
             }
-            if (i < n) s.upto[i] = before + w;
+            if (i < n) to[i] = before + w;
             before += all;
         }
         __syncthreads();
@@ -717,16 +785,22 @@ __global__ __launch_bounds__(64 * WAVES) void sample_select_kernel(SampleArgs A,
     __shared__ SelectShared<WAVES> s;
     const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const PieceStat *stats = A.stats + (size_t)row * pieces;
+    // a piece a lane, the same in every wave, or where they are more a piece a thread
+    const bool few = pieces <= 64;
+    const int from = few ? lane : tid, step = few ? 64 : THREADS;
+    const PieceStat none{-__builtin_inff(), GRID_LOW, 0, 0, 0, 0, 0, 0, 0.0, 0.0}, mine = from < pieces ? stats[from] : none;
     const Request q = read_request(A, row);
-    float top = -__builtin_inff();
-    for (int p = tid; p < pieces; p += THREADS) top = larger_or_nan(top, stats[p].top);
+    float top = mine.top;
+    for (int p = from + step; p < pieces; p += step) top = larger_or_nan(top, stats[p].top);
     const bool nan = __any(top != top);
     top = nan ? __builtin_nanf("") : qg_wave_max(top);
-    if (lane == 0) s.top[wave] = top;
-    __syncthreads();
-    top = s.top[0];
+    if (!few) {
+        if (lane == 0) s.top[wave] = top;
+        __syncthreads();
+        top = s.top[0];
 #pragma unroll
-    for (int w = 1; w < WAVES; w++) top = larger_or_nan(top, s.top[w]);
+        for (int w = 1; w < WAVES; w++) top = larger_or_nan(top, s.top[w]);
+    }
     if (!__builtin_isfinite(top)) return no_draw<DRAW>(A, row, tid, top);
     Row<WAVES> r{A, s.row, A.x + (size_t)row * A.cols, tid, lane, wave, q.a, top};
     double *piece = A.kept + (size_t)row * pieces;
@@ -740,8 +814,8 @@ __global__ __launch_bounds__(64 * WAVES) void sample_select_kernel(SampleArgs A,
         int reach = SA_GRID - 1, known = SA_GRID - 1, counted = 0;
         bool below = false;
         double all = 0.0;
-        for (int p = tid; p < pieces; p += THREADS) {
-            const PieceStat y = stats[p];
+        for (int p = from; p < pieces; p += step) {
+            const PieceStat y = p == from ? mine : stats[p];
             const int delta = (int)place - y.at;
             const bool counts = y.at != GRID_LOW && delta < SA_ZERO;
             const double w = counts ? __builtin_amdgcn_ldexp(y.all, -delta) * unit : 0.0;
@@ -759,29 +833,52 @@ __global__ __launch_bounds__(64 * WAVES) void sample_select_kernel(SampleArgs A,
             all = wave_all_add(all);
             reach = -(int)qg_wave_max(-(float)reach);
             known = -(int)qg_wave_max(-(float)known);
-            counted = wave_all_add(counted) + (__any(below) ? 1 << 30 : 0);  // as many as there are, or more
-            if (lane == 0) { s.reach[wave] = reach; s.known[wave] = known; s.flag[wave] = counted; s.grid.wave_sum[wave] = all; }
-            __syncthreads();
-            long in_all = 0;
-            all = 0.0;
+            long in_all = (long)wave_all_add(counted) + (__any(below) ? 1 << 30 : 0);  // as many as there are, or more
+            if (!few) {
+                if (lane == 0) { s.reach[wave] = reach; s.known[wave] = known; s.flag[wave] = (int)min(in_all, 1L << 30); s.grid.wave_sum[wave] = all; }
+                __syncthreads();
+                in_all = 0;
+                all = 0.0;
 #pragma unroll
-            for (int w = 0; w < WAVES; w++) {
-                reach = min(reach, s.reach[w]);
-                known = min(known, s.known[w]);
-                in_all += s.flag[w];
-                all += s.grid.wave_sum[w];
+                for (int w = 0; w < WAVES; w++) {
+                    reach = min(reach, s.reach[w]);
+                    known = min(known, s.known[w]);
+                    in_all += s.flag[w];
+                    all += s.grid.wave_sum[w];
+                }
             }
             Grid<WAVES> g{s.grid, r.x, A.bins + (size_t)row * pieces * SA_GRID, stats, A.listed + (size_t)row * pieces * SA_LISTED, A.cols, pieces,
                           tid, lane, wave, (int)place, top, q.a, unit, reach, known, false};
             g.add_up();
             g.below = in_all > (long)of_lane(g.count_upto, known);
             total = q.weighs_all() ? all : of_lane(g.mass_upto, SA_GRID - 1);
+            const uint32_t least = q.min_p > 0.0 ? r.least_key(q.min_p) : 0;
+            g.hold(g.first_cut(q, all, least));
             found = true;
             if (q.top_k) found = g.template shorten<Grid<WAVES>::BY_COUNT>(q.top_k, 0, cut, total);
             if (found && q.top_p < 1.0) found = g.template shorten<Grid<WAVES>::BY_MASS>(q.top_p * total, 0, cut, total);
-            if (found && q.min_p > 0.0) {
-                const uint32_t t = r.least_key(q.min_p);
-                if (t > cut.t) found = g.template shorten<Grid<WAVES>::BY_KEY>(0.0, t, cut, total);
+            if (found && least > cut.t) found = g.template shorten<Grid<WAVES>::BY_KEY>(0.0, least, cut, total);
+            if (found && DRAW && g.held) {
+                const int n = g.held;
+                __syncthreads();
+                g.sum_up(s.grid.in_order, n, [&](int i) { return cut.keeps(s.grid.held[i].x, (int)s.grid.held[i].y) ? g.weight(s.grid.held[i].x) : 0.0; });
+                for (int d = wave; d < A.draws; d += WAVES) {
+                    // the first sum past the goal, in two steps of 64 and at most 32
+                    const size_t at = (size_t)row * A.draws + d;
+                    const double sum = s.grid.in_order[n - 1], goal = (double)A.u[at] * sum;
+                    const int each = (n + 63) / 64;
+                    unsigned long long hit = __ballot(lane * each < n && s.grid.in_order[min((lane + 1) * each, n) - 1] > goal);
+                    const int i0 = hit ? (int)__builtin_ctzll(hit) * each : 0;
+                    hit = __ballot(hit && lane < each && i0 + lane < n && s.grid.in_order[min(i0 + lane, n - 1)] > goal);
+                    int pick = hit ? i0 + (int)__builtin_ctzll(hit) : n - 1;
+                    while (pick > 0 && !cut.keeps(s.grid.held[pick].x, (int)s.grid.held[pick].y)) pick--;  // past the last one: it is
+                    if (lane == 0) {
+                        const uint2 y = s.grid.held[pick];
+                        A.token[at] = (int)y.y;
+                        if (A.logprob) A.logprob[at] = (float)log(g.weight(y.x) / sum);
+                    }
+                }
+                return;
             }
             if (found && DRAW) {
                 weighed = g.weigh_pieces(cut, piece);
@@ -884,10 +981,10 @@ __global__ __launch_bounds__(64 * WAVES) void sample_select_kernel(SampleArgs A,
         }
     }
 }
-// Workgroups of sixteen waves, or of four where the rows are many.
+// Workgroups of sixteen waves, or of eight where the rows are many.
 template <bool DRAW>
 void select_rows(const SampleArgs &A, int rows, int pieces, hipStream_t s) {
-    if (rows > 256) sample_select_kernel<DRAW, 4><<<rows, 256, 0, s>>>(A, pieces);
+    if (rows > 256) sample_select_kernel<DRAW, 8><<<rows, 512, 0, s>>>(A, pieces);
     else sample_select_kernel<DRAW, 16><<<rows, 1024, 0, s>>>(A, pieces);
 }
 
