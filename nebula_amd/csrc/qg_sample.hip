@@ -458,6 +458,7 @@ struct Grid {
     const float *x;
     const unsigned long long *bins;
     const PieceStat *stats;
+    const PieceStat &mine;                           // of up to 64 pieces the lane's
     const uint2 *lists;
     const int cols, pieces, tid, lane, wave, place;  // place: of the row's largest value
     const float m;
@@ -478,7 +479,7 @@ struct Grid {
     static __device__ __forceinline__ int part_of(double e) { return 63 - min(max((int)((e - __builtin_rint(e) + 0.5) * 64.0), 0), 63); }
     // A piece's bin of a lane, moved to the row's.
     __device__ __forceinline__ int moved_by(int p) const {
-        const int at = stats[p].at;
+        const int at = pieces <= 64 ? of_lane(mine.at, p) : stats[p].at;  // p is the wave's
         return at == GRID_LOW ? SA_GRID : min(place - at, SA_GRID);
     }
     __device__ __forceinline__ unsigned long long row_bin(int p) const {
@@ -516,17 +517,18 @@ struct Grid {
         held = 0;
     }
     // Holds the listed values of bins 0..D, where lists reach that far and they are not too many.
-    __device__ __forceinline__ void hold(int D) {
-        constexpr int EACH = 64 / WAVES, PER = SA_LISTED / 64;
-        const int n = D < 0 || D > reach || pieces > 64 ? 0 : (int)of_lane(count_upto, D);
-        if (n == 0 || n > SA_HELD) return;
-        uint2 y[EACH][PER];
+    static constexpr int EACH = 64 / WAVES, PER = SA_LISTED / 64;  // pieces of a wave, listed values of a lane
+    static __device__ __forceinline__ void read_lists(const uint2 *lists, int pieces, const PieceStat &mine, int wave, int lane, uint2 (&y)[EACH][PER]) {
 #pragma unroll
         for (int k = 0; k < EACH; k++) {
-            const int p = k * WAVES + wave, listed = p < pieces && stats[p].at != GRID_LOW ? stats[p].listed : 0;
+            const int p = k * WAVES + wave, listed = p < pieces ? of_lane(mine.listed, p) : 0;
 #pragma unroll
             for (int i = 0; i < PER; i++) y[k][i] = i * 64 + lane < listed ? lists[(size_t)p * SA_LISTED + i * 64 + lane] : make_uint2(0, 0);
         }
+    }
+    __device__ __forceinline__ void hold(int D, const uint2 (&y)[EACH][PER]) {
+        const int n = D < 0 || D > reach || pieces > 64 ? 0 : (int)of_lane(count_upto, D);
+        if (n == 0 || n > SA_HELD) return;
         unsigned is = 0;
 #pragma unroll
         for (int k = 0; k < EACH; k++) {
@@ -597,7 +599,7 @@ struct Grid {
         if (tid == 0) s.hits = 0;
         __syncthreads();
         for (int p = tid; p < pieces; p += THREADS) {
-            const int delta = moved_by(p);
+            const int at = stats[p].at, delta = at == GRID_LOW ? SA_GRID : min(place - at, SA_GRID);
             if (D >= delta && bins[(size_t)p * SA_GRID + D - delta]) {
                 const int k = atomicAdd(&s.hits, 1);
                 if (k < SA_LIST) hits[k] = p;
@@ -680,7 +682,8 @@ struct Grid {
         if (D != bin) {
             const double b = (double)(place - D);
             int sub = -1;
-            if (n > SA_LIST) {
+            // ranking compares all with all: many held values go by parts too (1000 of them: 22 us for a row)
+            if (n > (held ? SA_LIST / 8 : SA_LIST)) {
                 __syncthreads();
                 if (wave == 0) { s.count[0][lane] = 0; s.excess[0][lane] = 0; }
                 __syncthreads();
@@ -790,6 +793,8 @@ __global__ __launch_bounds__(64 * WAVES) void sample_select_kernel(SampleArgs A,
     const int from = few ? lane : tid, step = few ? 64 : THREADS;
     const PieceStat none{-__builtin_inff(), GRID_LOW, 0, 0, 0, 0, 0, 0, 0.0, 0.0}, mine = from < pieces ? stats[from] : none;
     const Request q = read_request(A, row);
+    uint2 lists[Grid<WAVES>::EACH][Grid<WAVES>::PER];  // on their way from here
+    if (few && q.filters()) Grid<WAVES>::read_lists(A.listed + (size_t)row * pieces * SA_LISTED, pieces, mine, wave, lane, lists);
     float top = mine.top;
     for (int p = from + step; p < pieces; p += step) top = larger_or_nan(top, stats[p].top);
     const bool nan = __any(top != top);
@@ -847,13 +852,13 @@ __global__ __launch_bounds__(64 * WAVES) void sample_select_kernel(SampleArgs A,
                     all += s.grid.wave_sum[w];
                 }
             }
-            Grid<WAVES> g{s.grid, r.x, A.bins + (size_t)row * pieces * SA_GRID, stats, A.listed + (size_t)row * pieces * SA_LISTED, A.cols, pieces,
+            Grid<WAVES> g{s.grid, r.x, A.bins + (size_t)row * pieces * SA_GRID, stats, mine, A.listed + (size_t)row * pieces * SA_LISTED, A.cols, pieces,
                           tid, lane, wave, (int)place, top, q.a, unit, reach, known, false};
             g.add_up();
             g.below = in_all > (long)of_lane(g.count_upto, known);
             total = q.weighs_all() ? all : of_lane(g.mass_upto, SA_GRID - 1);
             const uint32_t least = q.min_p > 0.0 ? r.least_key(q.min_p) : 0;
-            g.hold(g.first_cut(q, all, least));
+            g.hold(g.first_cut(q, all, least), lists);
             found = true;
             if (q.top_k) found = g.template shorten<Grid<WAVES>::BY_COUNT>(q.top_k, 0, cut, total);
             if (found && q.top_p < 1.0) found = g.template shorten<Grid<WAVES>::BY_MASS>(q.top_p * total, 0, cut, total);
