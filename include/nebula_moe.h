@@ -68,6 +68,14 @@ int nm_stack_attend(nm_stack *s, const nm_attention_layer *layers, const nm_atte
  * holds it, runs at a time. */
 int nm_stack_verify(nm_stack *s, const qg_kv_batch *batch, int use_graph);
 
+/* Whether nm_stack_verify reads pages that several sequences hold (qg_kv_fork)
+ * once for all of them: qg_kv_prefixes once a batch and qg_prefix_attention in
+ * every layer, in place of qg_tree_attention.  For batches of forked sequences
+ * over a long common text (off after nm_stack_attend).  Waits for the device,
+ * drops the captured graphs and changes the workspace: not inside a capture, and not
+ * while a caller's graph that holds nm_stack_verify is still to run. */
+int nm_stack_share(nm_stack *s, int on);
+
 /* CPU handoff of one layer's flag-2 tokens (the hybrid path of
  * qwen.c:658-678, narrowed from the whole batch to the flagged tokens).
  * cpu_moe computes the routed part (qc_moe of cpu.c:235-261, through

@@ -47,15 +47,17 @@ struct nm_stack {
     float *x, *qkv, *q, *a;     /* normalised rows, projections, queries, attention rows */
     void *attn_ws;
     size_t attn_ws_bytes;
+    void *prefixes;             /* nm_stack_share: pages that sequences share are read once; NULL: each by itself */
+    size_t prefixes_bytes;
     void *verify_graphs[NM_MAX_TOKENS + 1];
     qg_kv_batch verify_batches[NM_MAX_TOKENS + 1];
 };
 
 static void attend_free(nm_stack *s) {
-    qg_free(s->x); qg_free(s->qkv); qg_free(s->q); qg_free(s->a); qg_free(s->attn_ws);
+    qg_free(s->x); qg_free(s->qkv); qg_free(s->q); qg_free(s->a); qg_free(s->attn_ws); qg_free(s->prefixes);
     free(s->attn_layers);
     s->x = s->qkv = s->q = s->a = NULL;
-    s->attn_ws = NULL;
+    s->attn_ws = s->prefixes = NULL;
     s->attn_layers = NULL;
 }
 
@@ -173,11 +175,40 @@ int nm_stack_attend(nm_stack *s, const nm_attention_layer *layers, const nm_atte
     return 0;
 }
 
+int nm_stack_share(nm_stack *s, int on) {
+    if (!s || !s->attn_layers) return fail("a stack without attention");
+    if (qg_graph_recording()) return fail("nm_stack_share inside a capture");
+    if (!on == !s->prefixes) return 0;
+    const int T = s->max_tokens;
+    int none;
+    const qg_kv_batch most = {.rows = T, .max_rows = T, .start = &none};
+    const size_t ws = on ? qg_prefix_attention_workspace_bytes(&s->cache, &most, s->attn.q_heads)
+                         : qg_tree_attention_workspace_bytes(&s->cache, &most, s->attn.q_heads);
+    const size_t bytes = on ? qg_kv_prefixes_bytes(&s->cache, &most) : 0;
+    void *attn_ws = ws ? qg_alloc(ws) : NULL, *prefixes = bytes ? qg_alloc(bytes) : NULL;
+    if (!attn_ws || (on && !prefixes)) {
+        qg_free(attn_ws); qg_free(prefixes);
+        return fail("attention allocation");
+    }
+    /* graphs hold the old workspace, and may still be running */
+    const int rc = qg_sync();
+    if (rc) { qg_free(attn_ws); qg_free(prefixes); return fail("qg_sync: %s", qg_error(rc)); }
+    for (int i = 0; i <= NM_MAX_TOKENS; i++)
+        if (s->verify_graphs[i]) { qg_graph_destroy(s->verify_graphs[i]); s->verify_graphs[i] = NULL; }
+    qg_free(s->attn_ws); qg_free(s->prefixes);
+    s->attn_ws = attn_ws;
+    s->attn_ws_bytes = ws;
+    s->prefixes = prefixes;
+    s->prefixes_bytes = bytes;
+    return 0;
+}
+
 static int run_verify(nm_stack *s, const qg_kv_batch *batch) {
     const int nt = batch->rows, D = s->width, hd = s->cache.head_dim, Hq = s->attn.q_heads, Hk = s->cache.kv_heads;
     const int qw = Hq * hd, kw = Hk * hd, row = qw + 2 * kw;
     /* rows of no sequence have no attention: zeros, not what the last batch left there */
     GPU(qg_zero(s->a, (size_t)nt * qw * sizeof(float)));
+    if (s->prefixes) GPU(qg_kv_prefixes(NULL, NULL, &s->cache, batch, s->prefixes, s->prefixes_bytes));
     for (int l = 0; l < s->n_layers; l++) {
         const nm_attention_layer *L = &s->attn_layers[l];
         const qg_qk_rows rows = {
@@ -189,7 +220,10 @@ static int run_verify(nm_stack *s, const qg_kv_batch *batch) {
         GPU(qg_norm(s->x, s->h, NULL, D, 1, nt, 0, 0, 1e-6f));
         GPU(qg_matmul(s->qkv, L->qkv, L->qkv_type, row, D, s->x, nt));
         GPU(qg_qk_norm_rope(s->q, NULL, &rows, &s->cache, l, batch));
-        GPU(qg_tree_attention(s->a, s->q, Hq, s->attn.scale, &s->cache, l, batch, s->attn_ws, s->attn_ws_bytes));
+        if (s->prefixes)
+            GPU(qg_prefix_attention(s->a, s->q, Hq, s->attn.scale, &s->cache, l, batch, s->prefixes, s->prefixes_bytes, s->attn_ws, s->attn_ws_bytes));
+        else
+            GPU(qg_tree_attention(s->a, s->q, Hq, s->attn.scale, &s->cache, l, batch, s->attn_ws, s->attn_ws_bytes));
         GPU(qg_matmul(s->x, L->out, L->out_type, D, qw, s->a, nt));
         GPU(qg_binary(s->h, s->h, s->x, nt * D, 0));
         const size_t act = (size_t)s->max_tokens * D, sel = (size_t)s->max_tokens * NM_TOP;

@@ -61,7 +61,7 @@ HOST_SIGNATURES = {
     "handoff_scratch_bytes": ([I, I], Z),
     "moe_handoff": ([P, P, P, P, P, P, I, I, P, Z, CPU_MOE_FN, P, P], I),
     "handoff_reserve": ([I, I], I), "device_reads": ([], C.c_uint64),
-    "stack_attend": ([P, P, P, P], I), "stack_verify": ([P, P, I], I),
+    "stack_attend": ([P, P, P, P], I), "stack_verify": ([P, P, I], I), "stack_share": ([P, I], I),
 }
 
 
