@@ -316,3 +316,111 @@ def test_draws_have_the_probabilities(qgl):
         share = np.bincount(c.token.get().ravel(), minlength=2000) / n
         assert (np.abs(share - p) <= 5 * np.sqrt(p * (1 - p) / n) + 1 / n).all()
         assert (share[p == 0] == 0).all()
+
+
+@pytest.mark.parametrize("cols", [262144, 262145, 300001, 600000, 1 << 20])
+def test_wide_rows(qgl, cols):
+    """Rows of more pieces than waves and lanes hold one each."""
+    rng = np.random.default_rng(cols)
+    x = logits(rng, 9, cols, rounded=True)
+    x[3] = -np.inf
+    x[3, [0, 262143, cols - 1]] = [1.0, 2.0, 3.0]
+    x[4] = np.sort(x[4])                                    # the largest in the last piece
+    x[5] = np.sort(x[5])[::-1]
+    asks = [(1.0, 0, 1.0, 0.0), (0.7, 20, 0.8, 0.0), (1.0, 0, 0.9, 0.0), (1.0, 0, 0.95, 0.0), (0.8, 40, 0.95, 0.05), (1.3, 1000, 0.99, 0.0),
+            (1.0, 0, 1.0, 0.02), (0.0, 0, 1.0, 0.0), (1.0, 100000, 1.0, 0.0)]
+    c = Call(x, asks, 4, rng.random((9, 4)))
+    c.sample()
+    c.check_sample()
+    out = Device(np.full(x.shape, 7, np.float32))
+    qg.call("sampling_softmax", out.p, c.dx.p, c.rows, c.cols, c.ref, c.ws.p, c.bytes)
+    c.check_probs(out.get())
+
+
+@pytest.mark.parametrize("rows,cols", [(256, 12289), (257, 12289), (300, 30000), (1088, 8200)])
+def test_many_rows(qgl, rows, cols):
+    """Enough rows that each takes half the waves, of several pieces."""
+    rng = np.random.default_rng(rows + cols)
+    c = Call(logits(rng, rows, cols, rounded=True), REQUESTS, 2, rng.random((rows, 2)))
+    c.sample()
+    c.check_sample()
+    out = Device(np.full(c.x.shape, 7, np.float32))
+    qg.call("sampling_softmax", out.p, c.dx.p, c.rows, c.cols, c.ref, c.ws.p, c.bytes)
+    c.check_probs(out.get())
+
+
+@pytest.mark.parametrize("rows", [1, 300])
+@pytest.mark.parametrize("above", [5.0, 12.0, 40.0, 400.0, 3e4])
+def test_peaked_rows(qgl, rows, above):
+    """One token far above the others, and cuts that lie deep below it."""
+    rng = np.random.default_rng(int(above))
+    cols = 20011
+    x = logits(rng, rows, cols)
+    for r in range(rows):
+        x[r, rng.integers(cols)] = x[r].max() + above
+    asks = [(1.0, k, p, m) for k in (0, 2, 50, 128, 129, 500, 2000, 9000) for p in (1.0, 0.999999, 0.5) for m in (0.0, 1e-6, 1e-20)]
+    c = Call(np.repeat(x, len(asks), 0) if rows == 1 else x, asks, 2, rng.random((len(asks) if rows == 1 else rows, 2)))
+    c.sample()
+    c.check_sample()
+    out = Device(np.full(c.x.shape, 7, np.float32))
+    qg.call("sampling_softmax", out.p, c.dx.p, c.rows, c.cols, c.ref, c.ws.p, c.bytes)
+    c.check_probs(out.get())
+
+
+@pytest.mark.parametrize("values", [1, 2, 7, 40, 300])
+@pytest.mark.parametrize("cols", [4097, 50021])
+def test_ties(qgl, cols, values):
+    """Few different values: a cut among equal ones keeps the first of them."""
+    rng = np.random.default_rng(values * cols)
+    x = (rng.integers(values, size=(24, cols)) * 0.37).astype(np.float32)
+    x[8:16] = np.sort(x[8:16], 1)
+    x[16:] = -np.sort(-x[16:], 1)
+    asks = [(1.0, 100, 1.0, 0.0), (1.0, 128, 1.0, 0.0), (1.0, 129, 0.9, 0.0), (0.5, 2048, 0.95, 0.0), (1.0, 2049, 1.0, 0.0), (2.0, 4000, 0.6, 0.0), (1.0, 0, 0.3, 0.0),
+            (1.0, 0, 1.0, 0.5)]
+    c = Call(x, asks, 3, rng.random((24, 3)))
+    c.sample()
+    c.check_sample()
+    out = Device(np.full(x.shape, 7, np.float32))
+    qg.call("sampling_softmax", out.p, c.dx.p, c.rows, c.cols, c.ref, c.ws.p, c.bytes)
+    c.check_probs(out.get())
+
+
+def test_falling_rows_and_no_chance(qgl):
+    """u of 0 and just below 1 meet the first and the last token that stays."""
+    rng = np.random.default_rng(14)
+    u = np.tile(np.array([0, 1 - 2.0 ** -24], np.float32), (4, 1))
+    for cols in (100, 9000, 40000):
+        for order in (1, -1):
+            x = np.sort(rng.standard_normal((4, cols)) * 3, 1)[:, ::order].astype(np.float32)
+            c = Call(x, [(1.0, 30, 1.0, 0.0), (1.0, 0, 0.9, 0.0), (1.0, 700, 1.0, 0.0), (0.0, 0, 1.0, 0.0)], 2, u)
+            c.sample()
+            c.check_sample()
+
+
+def test_two_threads(qgl):
+    """Calls and graphs of two threads with workspaces of their own."""
+    import threading
+    rng = np.random.default_rng(15)
+    calls = [Call(logits(rng, rows, cols), REQUESTS, 2, rng.random((rows, 2))) for rows, cols in ((18, 30000), (300, 9000))]
+    outs = [Device(np.zeros(c.x.shape, np.float32)) for c in calls]
+
+    def work(c, out):
+        def both():
+            c.sample()
+            qg.call("sampling_softmax", out.p, c.dx.p, c.rows, c.cols, c.ref, c.ws.p, c.bytes)
+        graph = C.c_void_p()
+        qg.call("graph_begin", C.byref(graph))
+        both()
+        qg.call("graph_end", graph)
+        for _ in range(5):
+            both()
+            qg.call("graph_launch", graph)
+        qg.call("sync")
+        qgl.qg_graph_destroy(graph)
+
+    threads = [threading.Thread(target=work, args=a) for a in zip(calls, outs)]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    for c, out in zip(calls, outs):
+        c.check_sample()
+        c.check_probs(out.get())
