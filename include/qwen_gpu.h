@@ -271,6 +271,13 @@ int qg_tree_attention(float *out, const float *q, int q_heads, float scale, cons
 size_t qg_kv_prefixes_bytes(const qg_kv_cache *cache, const qg_kv_batch *batch);
 int qg_kv_prefixes(int *link, int *shared, const qg_kv_cache *cache, const qg_kv_batch *batch, void *prefixes, size_t prefixes_bytes);
 
+/* How many bytes of keys and values the sequences of a batch must save in each
+ * layer for qg_kv_prefixes to have them shared (what sharing costs is about the
+ * same for all batches): a setting of the calling thread, 48 MiB at first and for
+ * negative values.  link and shared do not depend on it, outputs only within the
+ * attention's error.  Returns the previous setting. */
+int64_t qg_prefix_least_saving(int64_t bytes);
+
 /* qg_tree_attention of a batch in which sequences share pages: the same outputs
  * (within the same error), but a page that several sequences hold is read once
  * for all of them.  `prefixes` as qg_kv_prefixes filled it for this cache and batch;

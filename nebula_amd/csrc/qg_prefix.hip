@@ -81,8 +81,12 @@ __global__ __launch_bounds__(256) void prefix_link_kernel(KvView c, BatchView b,
 // ------------------------------------------------------------------------
 // Common parts count in steps of a quantum: shorter segments would cost more than
 // they save.  It is doubled until the rows of all shared segments together are few
-// enough for the partial results that a workspace holds.
+// enough for the partial results that a workspace holds.  And nothing is shared where all of it together saves less than
+// `least` bytes of reads: joining the segments takes some 5 us (heads of 2 x 128, fp16, each sequence by itself / shared:
+// 8 sequences of 1000 tokens 12.2 / 17.8, of 4000 16.0 / 19.3, of 16000 30.4 / 23.0; 2 of 64000 32.0 / 28.6).
 constexpr int QUANTUM = 256;
+constexpr int64_t LEAST_SAVING = 48 << 20;
+thread_local int64_t tl_least_saving = LEAST_SAVING;
 __host__ __device__ inline long shared_rows_most(long rows) {
     const long most = 16 * rows < 16384 ? 16 * rows : 16384;
     return most > 3 * rows ? most : 3 * rows;
@@ -92,7 +96,7 @@ struct PlanShared {
     unsigned long long key[THREADS];
     int link[THREADS], cut[THREADS], n[THREADS], size[THREADS], off[THREADS], rep[THREADS], next[THREADS], sees[THREADS], top[THREADS], upto[THREADS + 1],
         run[THREADS + 1], first[THREADS + 1], wave[THREADS / 64 + 1];
-    unsigned long long sum;
+    unsigned long long sum, saved;
 };
 template <int THREADS>
 QG_DEV void plan_sync() {
@@ -142,7 +146,7 @@ QG_DEV unsigned long long plan_sort(PlanShared<THREADS> &s, unsigned long long k
     return key;
 }
 template <int THREADS>
-QG_DEV void plan_segments(const KvView &c, const BatchView &b, const PrefixView &v, PlanShared<THREADS> &s, int t) {
+QG_DEV void plan_segments(const KvView &c, const BatchView &b, const PrefixView &v, PlanShared<THREADS> &s, int64_t least_tokens, int t) {
     const int S = c.sequences;
     int first = 0, n = 0, len = 0, link0 = -1, shared0 = 0;
     if (t < S) {
@@ -160,12 +164,14 @@ QG_DEV void plan_segments(const KvView &c, const BatchView &b, const PrefixView 
         s.cut[t] = cut;
         s.size[t] = 0;
         s.top[t] = -1;
-        if (t == 0) s.sum = 0;
+        if (t == 0) { s.sum = 0; s.saved = 0; }
         plan_sync<THREADS>();
+        if (cut) atomicAdd(&s.saved, (unsigned long long)cut);
         link = cut ? link0 : -1;
         while (link >= 0 && s.cut[link] >= cut) link = s.link[link];
-        if (link < 0) cut = 0;
         plan_sync<THREADS>();
+        if ((int64_t)s.saved < least_tokens) link = -1;  // a sequence does not read again what it shares
+        if (link < 0) cut = 0;
         s.link[t] = link;
         s.cut[t] = cut;
         plan_sync<THREADS>();
@@ -220,10 +226,12 @@ QG_DEV void plan_segments(const KvView &c, const BatchView &b, const PrefixView 
     at[t] = pos;
     plan_sync<THREADS>();
     if (t == 0) { v.head[0] = heads + tails; v.head[1] = heads; }
-    if (t < S) {
-        v.leaf[t] = n > 0 ? tail_id : -1;
-        v.pos[t] = pos;
-    }
+    // rows of no sequence: before the first, behind the last, and what one has too many
+    int2 *of_row = (int2 *)v.of_row;
+    for (int r = t, upto = kv_clamp(b.start[0], 0, b.rows); r < upto; r += THREADS) of_row[r] = make_int2(-1, 0);
+    for (int r = kv_clamp(b.start[S], 0, b.rows) + t; r < b.rows; r += THREADS) of_row[r] = make_int2(-1, 0);
+    if (t < S)
+        for (int r = first + n, upto = kv_clamp(b.start[t + 1], 0, b.rows); r < upto; r++) of_row[r] = make_int2(-1, 0);
     auto put = [&](int i, const Segment &x) {
         int4 *to = (int4 *)(v.segments + (size_t)i * SEG_INTS);
         to[0] = make_int4(x.owner, x.begin, x.end, x.row0);
@@ -234,8 +242,10 @@ QG_DEV void plan_segments(const KvView &c, const BatchView &b, const PrefixView 
     if (n > 0) {
         const int top = s.top[t];  // the first of those that leave it last
         put(tail_id, Segment{t, top >= 0 ? s.cut[top] : cut, len + n, pos, n, top >= 0 ? id[top] : above(t), 1, 0});
-        for (int i = 0; i < n; i++)
+        for (int i = 0; i < n; i++) {
             if (pos + i < b.rows) v.row_of[pos + i] = first + i;
+            of_row[first + i] = make_int2(tail_id, pos + i);
+        }
     }
     if (shares) {
         const int next = s.next[t], up = next >= 0 ? id[s.rep[next]] : above(link);
@@ -243,18 +253,18 @@ QG_DEV void plan_segments(const KvView &c, const BatchView &b, const PrefixView 
     }
 }
 template <int THREADS>
-__global__ __launch_bounds__(THREADS) void prefix_plan_kernel(KvView c, BatchView b, PrefixView v) {
+__global__ __launch_bounds__(THREADS) void prefix_plan_kernel(KvView c, BatchView b, PrefixView v, int64_t least_tokens) {
     __shared__ PlanShared<THREADS> s;
-    plan_segments<THREADS>(c, b, v, s, threadIdx.x);
+    plan_segments<THREADS>(c, b, v, s, least_tokens, threadIdx.x);
 }
 // Both for few sequences, a wave each.
 constexpr int SMALL = 16;
-__global__ __launch_bounds__(64 * SMALL) void prefix_small_kernel(KvView c, BatchView b, PrefixView v, int *link, int *shared) {
+__global__ __launch_bounds__(64 * SMALL) void prefix_small_kernel(KvView c, BatchView b, PrefixView v, int64_t least_tokens, int *link, int *shared) {
     __shared__ PlanShared<64> s;
     const int wave = threadIdx.x >> 6;
     if (wave < c.sequences) link_sequence(c, b, v, link, shared, wave, threadIdx.x & 63);
     __syncthreads();
-    if (wave == 0) plan_segments<64>(c, b, v, s, threadIdx.x);
+    if (wave == 0) plan_segments<64>(c, b, v, s, least_tokens, threadIdx.x);
 }
 
 // ------------------------------------------------------------------------
@@ -704,12 +714,10 @@ __global__ __launch_bounds__(64 * JOIN_WAVES) void prefix_join_kernel(PrefixArgs
     const size_t at = EACH == 1 ? blockIdx.x : (size_t)blockIdx.x * EACH + wave;
     if (at >= (size_t)b.rows * A.q_heads) return;
     const int row = (int)(at / A.q_heads), head = (int)(at % A.q_heads), h = by_group(A, head);
-    int first, n;
-    const int s = batch_sequence(b, c.sequences, row, lane, first, n);
-    if (s < 0) return;  // nothing was written for it
-    const int count = segment_count(c, v), pos = v.pos[s] + (row - first);
-    int id = v.leaf[s];
-    if (id < 0 || id >= count) return;
+    const int2 place = ((const int2 *)v.of_row)[row];
+    const int count = segment_count(c, v), pos = __builtin_amdgcn_readfirstlane(place.y);
+    int id = __builtin_amdgcn_readfirstlane(place.x);
+    if (id < 0 || id >= count) return;  // nothing was written for it
     bool odd = false;
     Segment g = read_segment(c, b, v, id);
     int4 j = A.joins[id];
@@ -759,7 +767,10 @@ __global__ __launch_bounds__(64 * JOIN_WAVES) void prefix_join_kernel(PrefixArgs
         }
         odd = __any(odd);
     }
-    if (odd && (EACH > 1 || wave == 0)) attend_row<TYPE, D>(A, c, b, s, first, n, row, head, lane, s_y[wave]);
+    if (!odd || (EACH == 1 && wave)) return;
+    int first, n;
+    const int s = batch_sequence(b, c.sequences, row, lane, first, n);
+    if (s >= 0) attend_row<TYPE, D>(A, c, b, s, first, n, row, head, lane, s_y[wave]);
 }
 
 // Row groups of all segments, at most (each rounds up), and their row tiles: groups of t tiles have more than t - 1 tiles' rows each.
@@ -791,6 +802,12 @@ constexpr long TILES = 1L << 27; // of partial results, within an int of rows
 
 extern "C" {
 
+int64_t qg_prefix_least_saving(int64_t bytes) {
+    const int64_t before = tl_least_saving;
+    tl_least_saving = bytes < 0 ? LEAST_SAVING : bytes < (int64_t)1 << 60 ? bytes : (int64_t)1 << 60;
+    return before;
+}
+
 size_t qg_kv_prefixes_bytes(const qg_kv_cache *cache, const qg_kv_batch *batch) {
     if (qg_kv_check(cache, false, nullptr) || qg_batch_check(batch, false, nullptr)) return 0;
     return prefix_bytes(cache->sequences, batch->rows);
@@ -807,14 +824,15 @@ int qg_kv_prefixes(int *link, int *shared, const qg_kv_cache *cache, const qg_kv
                  in[3] = {{c.table, qg_table_bytes(c)}, {c.length, each}, {b.start, each + 4}};
     if (qg_any_overlap(out, in) || qg_overlap(link, each, shared, each) || qg_overlap(prefixes, need, link, each) || qg_overlap(prefixes, need, shared, each))
         return hipErrorInvalidValue;
-    const PrefixView v = prefix_view(prefixes, c.sequences);
+    const PrefixView v = prefix_view(prefixes, c.sequences, b.rows);
+    const int64_t token = 2LL * c.heads * c.dim * (c.type == QT_F32 ? 4 : 2), least = (tl_least_saving + token - 1) / token;
     if (c.sequences <= SMALL) {
-        prefix_small_kernel<<<1, 64 * SMALL, 0, qg_stream()>>>(c, b, v, link, shared);
+        prefix_small_kernel<<<1, 64 * SMALL, 0, qg_stream()>>>(c, b, v, least, link, shared);
         return hipGetLastError();
     }
     prefix_link_kernel<<<(c.sequences + 3) / 4, 256, 0, qg_stream()>>>(c, b, v, link, shared);
-    if (c.sequences <= 64) prefix_plan_kernel<64><<<1, 64, 0, qg_stream()>>>(c, b, v);
-    else prefix_plan_kernel<QG_MAX_SEQUENCES><<<1, QG_MAX_SEQUENCES, 0, qg_stream()>>>(c, b, v);
+    if (c.sequences <= 64) prefix_plan_kernel<64><<<1, 64, 0, qg_stream()>>>(c, b, v, least);
+    else prefix_plan_kernel<QG_MAX_SEQUENCES><<<1, QG_MAX_SEQUENCES, 0, qg_stream()>>>(c, b, v, least);
     return hipGetLastError();
 }
 
@@ -848,7 +866,7 @@ int qg_prefix_attention(float *out, const float *q, int q_heads, float scale, co
     int4 *joins = (int4 *)(part_ml + (size_t)tiles * 16);
     const PrefixArgs A{attn_rows(out, q, q_heads, group, layer, scale), part_o, part_ml, joins, (int *)(joins + 2 * (size_t)c.sequences),
                        resident(c.dim, most_tiles(c.dim)), (int)tiles};
-    const PrefixView v = prefix_view(const_cast<void *>(prefixes), c.sequences);
+    const PrefixView v = prefix_view(const_cast<void *>(prefixes), c.sequences, b.rows);
     if (c.type == QT_F32) launch_dim<QT_F32>(A, c, b, v, qg_stream());
     else if (c.type == QT_F16) launch_dim<QT_F16>(A, c, b, v, qg_stream());
     else launch_dim<QT_BF16>(A, c, b, v, qg_stream());

@@ -14,16 +14,15 @@ enum { SEG_INTS = 8, PREFIX_HEAD = 16 };
 struct PrefixView {
     int *head;           // [0] number of segments, [1] of the shared ones, which come first
     int *segments;       // [2 S] Segment
-    int *leaf;           // [S] the last segment of each sequence, -1 without rows
-    int *pos;            // [S] a sequence's first row in walking order
     int *link, *shared;  // [S] as found, see qg_kv_prefixes
     int *row_of;         // [rows] in walking order
+    int *of_row;         // [rows][2] the last segment of a row's sequence, -1 for none, and the row's place in walking order
 };
-KV_FN PrefixView prefix_view(void *at, int S) {
-    int *p = (int *)at, *seg = p + PREFIX_HEAD, *leaf = seg + 2 * (size_t)S * SEG_INTS;
-    return PrefixView{p, seg, leaf, leaf + S, leaf + 2 * (size_t)S, leaf + 3 * (size_t)S, leaf + 4 * (size_t)S};
+KV_FN PrefixView prefix_view(void *at, int S, int rows) {
+    int *p = (int *)at, *seg = p + PREFIX_HEAD, *link = seg + 2 * (size_t)S * SEG_INTS, *row_of = link + 2 * (size_t)S;
+    return PrefixView{p, seg, link, link + S, row_of + 2 * (size_t)rows, row_of};
 }
-KV_FN size_t prefix_bytes(int S, int rows) { return 4 * ((size_t)PREFIX_HEAD + 2 * (size_t)S * SEG_INTS + 4 * (size_t)S + rows); }
+KV_FN size_t prefix_bytes(int S, int rows) { return 4 * ((size_t)PREFIX_HEAD + 2 * (size_t)S * SEG_INTS + 2 * (size_t)S + 3 * (size_t)rows); }
 
 KV_FN int segment_count(const KvView &c, const PrefixView &v) { return kv_clamp(v.head[0], 0, 2 * c.sequences); }
 KV_FN Segment segment_inside(const KvView &c, const BatchView &b, Segment s) {

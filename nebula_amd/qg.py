@@ -48,7 +48,7 @@ SIGNATURES = {
     "kv_reserve": ([P, P, P, P, Z], I), "kv_fork": ([P, P, P, I, P, Z], I), "kv_truncate": ([P, P], I),
     "kv_compact": ([P, P, P, P, P], I), "kv_copy_pages": ([P, P, P, I], I),
     "kv_prefixes_bytes": ([P, P], Z), "kv_prefixes": ([P, P, P, P, P, Z], I), "prefix_attention_workspace_bytes": ([P, P, I], Z),
-    "prefix_attention": ([P, P, I, F, P, I, P, P, Z, P, Z], I),
+    "prefix_attention": ([P, P, I, F, P, I, P, P, Z, P, Z], I), "prefix_least_saving": ([C.c_int64], C.c_int64),
     "sample_workspace_bytes": ([I, I], Z), "sample": ([P, P, P, I, I, I, P, P, P, Z], I), "sampling_softmax": ([P, P, I, I, P, P, Z], I),
 }
 

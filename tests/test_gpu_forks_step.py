@@ -20,6 +20,14 @@ pytestmark = pytest.mark.gpu
 ASKS = [(0.8, 40, 0.95, 0.0), (1.0, 0, 0.9, 0.02), (0.0, 0, 1.0, 0.0), (1.2, 0, 1.0, 0.05), (1.0, 0, 1.0, 0.0)]
 
 
+@pytest.fixture(autouse=True)
+def whatever_it_saves(qgl):
+    """Small batches share their pages too."""
+    before = qgl.qg_prefix_least_saving(0)
+    yield
+    qgl.qg_prefix_least_saving(before)
+
+
 class ForkStep(Step):
     """A Step whose attention reads shared pages once and whose probabilities are truncated by each row's request."""
 

@@ -12,6 +12,14 @@ from spec_oracle import BF16, F16, F32, Batch, attention, decode, encode, random
 pytestmark = pytest.mark.gpu
 
 
+@pytest.fixture(autouse=True)
+def whatever_it_saves(qgl):
+    """Small batches share their pages too."""
+    before = qgl.qg_prefix_least_saving(0)
+    yield
+    qgl.qg_prefix_least_saving(before)
+
+
 class Plan:
     """The buffer of a cache and batch, and what was found."""
 
@@ -100,6 +108,22 @@ def test_families(qgl, family, most, tree):
     a = build(rng, f, counts, tree)
     a.check()
     a.plan.check()
+
+
+def test_what_is_worth_sharing(qgl):
+    """Below the least saving each sequence reads for itself: the search's outputs are the same, the attention's within its error."""
+    rng = np.random.default_rng(2)
+    a = build(rng, FAMILIES["two levels"], [1, 3, 1, 2, 1, 1, 1], kv_heads=2, dim=64, typ=F16)
+    outs, heads = [], []
+    saved = sum(int(x) // 256 * 256 for x in prefixes(a.cache.table, a.cache.pages, a.cache.P, a.cache.length, [1] * 7)[1]) * 2 * 2 * 64 * 2
+    for least in (0, saved, saved + 1, 1 << 40, -1):
+        qgl.qg_prefix_least_saving(least)
+        outs.append(a.check())
+        a.plan.check()
+        heads.append(a.plan.buffer.get()[:8].view(np.int32).tolist())  # segments, and those that are shared
+    assert heads[0] == heads[1] and heads[0][1] > 0
+    assert heads[2] == heads[3] == heads[4] == [7, 0]
+    assert np.array_equal(outs[0], outs[1]) and np.array_equal(outs[2], outs[3])
 
 
 @pytest.mark.parametrize("typ", [F32, F16, BF16])
@@ -312,6 +336,22 @@ def test_replayed(qgl, rows):
             assert (np.abs(g - want) <= tol).all(), turn
             assert np.array_equal(a.run(), g)  # eager, the same bits
     qgl.qg_graph_destroy(graph)
+
+
+@pytest.mark.parametrize("fill", [0, 1, 0xFF])
+def test_rows_of_no_sequence_whatever_lay_there(qgl, fill):
+    """Rows before the first sequence, between two and behind the last, with a buffer that an earlier batch filled."""
+    rng = np.random.default_rng(16)
+    for family, counts, most, skip in (("forks", [2, 5, 1, 0, 0, 3, 2], 3, 2), ("two levels", [1, 0, 4, 1, 1, 1, 9], 4, 3), ("strangers", [0, 3, 0], 2, 1)):
+        cache = Forked(rng, FAMILIES[family], counts)
+        batch = Batch(counts, max_rows=most, rows=sum(counts) + skip + 5)
+        batch.start += skip
+        batch.dstart.set(batch.start)
+        fill_rows(rng, cache, batch)
+        a = Attend(cache, batch, rng.standard_normal((batch.rows, 8, cache.D)), cache.D ** -0.5)
+        a.plan.buffer.set(np.full(a.plan.bytes, fill, np.uint8))
+        a.check()
+        a.plan.check()
 
 
 def test_workspace_and_buffer_of_larger_batches(qgl):

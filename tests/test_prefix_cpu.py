@@ -53,6 +53,19 @@ def test_refused_searches(lib):
         assert call(link, shared, ref(c), ref(b), p, size) == INVALID, (link, shared, p, size)
 
 
+def test_least_saving(lib):
+    """A thread's own setting."""
+    import threading
+    first = lib.qg_prefix_least_saving(5)
+    assert first == 48 << 20 and lib.qg_prefix_least_saving(0) == 5 and lib.qg_prefix_least_saving(1 << 62) == 0
+    seen = []
+    t = threading.Thread(target=lambda: seen.append(lib.qg_prefix_least_saving(7)))
+    t.start()
+    t.join()
+    assert seen == [48 << 20]
+    assert lib.qg_prefix_least_saving(-1) == 1 << 60 and lib.qg_prefix_least_saving(-1) == 48 << 20
+
+
 def test_workspaces(lib):
     c = cache(head_dim=128, sequences=64)
     sizes = [lib.qg_prefix_attention_workspace_bytes(ref(c), ref(batch(rows=r, max_rows=m, parent=None)), 16)
@@ -81,7 +94,7 @@ extern "C" int place(const int *p, int heads, int h, int x, int all, long *at) {
 }
 extern "C" long bytes(int S, int rows) {
     int *p = nullptr;
-    const PrefixView v = prefix_view(p, S);
+    const PrefixView v = prefix_view(p, S, rows);
     return (char *)(v.row_of + rows) - (char *)p == (long)prefix_bytes(S, rows) ? (long)prefix_bytes(S, rows) : -1;
 }
 """
