@@ -166,7 +166,8 @@ QG_DEV void plan_segments(const KvView &c, const BatchView &b, const PrefixView 
         s.top[t] = -1;
         if (t == 0) { s.sum = 0; s.saved = 0; }
         plan_sync<THREADS>();
-        if (cut) atomicAdd(&s.saved, (unsigned long long)cut);
+        const unsigned long long saved = wave_all_add((unsigned long long)cut);
+        if ((t & 63) == 0) atomicAdd(&s.saved, saved);
         link = cut ? link0 : -1;
         while (link >= 0 && s.cut[link] >= cut) link = s.link[link];
         plan_sync<THREADS>();
