@@ -17,7 +17,9 @@
 namespace {
 
 // ------------------------------------------------------------------------
-// Which sequences begin with the same pages: a wave per sequence.
+// Which sequences begin with the same pages: a wave per sequence.  Bound by dependent
+// reads (a length, an entry of every earlier sequence, the pages in common): 1024
+// sequences of up to 80 pages 13 us, 64 of 98304 tokens 6.
 // ------------------------------------------------------------------------
 QG_DEV int whole_pages(const KvView &c, int s) { return kv_length(c, s) >> c.shift; }
 QG_DEV int table_page(const KvView &c, int s, int j) {
@@ -80,7 +82,8 @@ __global__ __launch_bounds__(256) void prefix_link_kernel(KvView c, BatchView b,
 // its siblings are sums over runs.
 // ------------------------------------------------------------------------
 // Common parts count in steps of a quantum: shorter segments would cost more than
-// they save.  It is doubled until the rows of all shared segments together are few
+// they save (8 sequences of 2048 tokens, 8 layers: 128 and 256 196 and 198 us, 1024 218;
+// two levels of 8 x 8: 69 and 69, 77).  It is doubled until the rows of all shared segments together are few
 // enough for the partial results that a workspace holds.  And nothing is shared where all of it together saves less than
 // `least` bytes of reads: joining the segments takes some 5 us (heads of 2 x 128, fp16, each sequence by itself / shared:
 // 8 sequences of 1000 tokens 12.2 / 17.8, of 4000 16.0 / 19.3, of 16000 30.4 / 23.0; 2 of 64000 32.0 / 28.6).
@@ -258,7 +261,8 @@ __global__ __launch_bounds__(THREADS) void prefix_plan_kernel(KvView c, BatchVie
     __shared__ PlanShared<THREADS> s;
     plan_segments<THREADS>(c, b, v, s, least_tokens, threadIdx.x);
 }
-// Both for few sequences, a wave each.
+// Both for few sequences, a wave each: 8 sequences 6.3 us, as two kernels 8.5; with more the waves of one
+// workgroup would take several sequences each.
 constexpr int SMALL = 16;
 __global__ __launch_bounds__(64 * SMALL) void prefix_small_kernel(KvView c, BatchView b, PrefixView v, int64_t least_tokens, int *link, int *shared) {
     __shared__ PlanShared<64> s;
@@ -269,7 +273,14 @@ __global__ __launch_bounds__(64 * SMALL) void prefix_small_kernel(KvView c, Batc
 }
 
 // ------------------------------------------------------------------------
-// Attention.
+// Attention: one pass over a segment's keys with the running maximum and sum of a softmax, S^T = K Q^T and O^T = V^T P^T
+// on the 16-bit matrix cores, q and p in two fp16 or three bf16 planes, tiles and planes as qg_tree_attention has them.
+// A unit is a part of a segment's keys for a group of up to 16 MOST of its rows x heads, so that a key that is read
+// serves as many rows as the registers hold.  64 sequences of one row over 98304 tokens in common (heads 16 over 2 of
+// 128, fp16): 155 us where the products alone take 94, the matrix cores busy for a quarter of the cycles and the waves
+// waiting for keys from L2 and behind it for half of theirs; each sequence by itself takes 514.  16 trees of 17 rows over
+// 24576 tokens (bf16) 153 us, 107 and 198.  8 sequences over 2048 tokens 17 us, of which the way to a unit's first key
+// (plan 2.9, pages 2.2, queries 2.5) and the end are more than half.
 // ------------------------------------------------------------------------
 struct PrefixArgs : AttnRows {
     float *part_o;    // [tiles][16][D]
@@ -292,7 +303,8 @@ struct Unit {
 };
 constexpr int CHUNK = 128;  // keys per unit, at least and in steps of
 // What a unit costs, in key x weight: a key weighs 1 more than its row tiles (its reads, and the products and
-// weights of each tile), and to begin and to end takes as long as 1000 do.
+// weights of each tile), and to begin and to end takes as long as 1000 do (two levels of
+// 8 x 8: 69 us, with 100 78 and with 4000 76; 8 x 2048 tokens 198, 200 and 230).
 constexpr float UNIT_COST = 1000.0f;
 __host__ __device__ constexpr int key_weight(int tiles) { return 1 + tiles; }
 
@@ -318,8 +330,9 @@ QG_DEV int part_count(float even, const UnitLane &x) {
 }
 // Every workgroup finds its unit by itself: in one round of resident workgroups (two, where the row groups alone come to
 // half of one) units that cost about the same, of the shared segments first, and of both an eighth to each XCD, in whose
-// L2 the row groups with the same keys meet.  False if there is none.  A thread per segment and nothing unrolled:
-// what runs once is bound by the fetch of its instructions (four segments a lane in every wave: 5 to 13 us, now 2 to 4).
+// L2 the row groups with the same keys meet.  False if there is none.  A thread per segment; a part's size is formed anew
+// where it is needed, since an array that is picked from by a variable would be moved to shared memory under a size that
+// is read from the launch's packet in the host's memory (8 us; this takes 2.9).
 template <int NW>
 struct FindShared { float f[2][2][NW]; int i[2][2][NW], found[8]; };
 template <int MOST, int NW>
@@ -668,7 +681,8 @@ __global__ __launch_bounds__(64 * NW, (D / 64) * MOST <= 6 ? 2 : 1) void prefix_
 }
 
 // Joins a row's segments.  Few rows and heads: a workgroup each, whose four waves
-// share the parts; many: a wave each.
+// share the parts (8 rows, 8 layers: 198 us, by a wave each 203); many: a wave each
+// (272 rows of 20 heads 156 us, by workgroups 164).  Bound by four dependent reads: 6 to 11 us.
 constexpr int JOIN_WAVES = 4;
 constexpr size_t JOIN_FEW = 1024;
 

@@ -265,6 +265,10 @@ struct Row {
 // added up as a whole number under the count, in one 64-bit atomic whose order does not
 // matter.  The values of the first bins, up to SA_LISTED of them, are listed: few tokens
 // stay of most rows, and then nothing is read again.
+// 1088 rows x 131072 (570 MB): requests whose first filter is a small top-k 150 us (3.8 TB/s), one
+// weight per value in 64 bits 200, nearly all values in bins (top-p alone, top-k 1000) 330, the ten kinds mixed
+// 215 to 240.  Of 4096 values in a workgroup's registers: 16 loads of a thread on their way, eight
+// workgroups on a CU; with the next piece on its way in as many registers again 474 us, 16-byte loads 264.
 // ------------------------------------------------------------------------
 constexpr int PIECE_THREADS = 256, PIECE_WAVES = PIECE_THREADS / 64, PIECE_VALUES = SA_PIECE / PIECE_THREADS, BIN_COUNT = 49, BIN_BITS = 36;
 constexpr double GRID_FAR = (double)(1 << 19);  // places further out are left to the search over the row
@@ -425,7 +429,9 @@ __global__ __launch_bounds__(PIECE_THREADS) void sample_piece_kernel(SampleArgs 
 // A row's cut, and its draws, by one workgroup.  The bins of all pieces say in which one a filter cuts; its
 // values, from the lists where these reach and else read again from the pieces that have some, are
 // ranked (of a bin with too many, those of the 64th part in which the cut is).  What the bins do not
-// hold is left to the search over the whole row.
+// hold is left to the search over the whole row.  Bound by dependent steps (statistics, bins, the cut's bin, its values in
+// order, sums, draws): a row 14 us, 1088 rows of the ten kinds 58, two of them on a CU (105 registers a lane; three with
+// 80 spill and gain nothing).
 // ------------------------------------------------------------------------
 constexpr int SA_LIST = 1024, SA_HELD = 2 * SA_LIST;  // values that are ranked; that are held
 template <int WAVES>
@@ -682,7 +688,8 @@ struct Grid {
         if (D != bin) {
             const double b = (double)(place - D);
             int sub = -1;
-            // ranking compares all with all: many held values go by parts too (1000 of them: 22 us for a row)
+            // ranking compares all with all: many held values go by parts too (1088 rows x 131072 251 us, all ranked 267; sorted in
+            // 55 steps 270); where they are not held, a part would cost another reading of the pieces (45 us for a row, ranked 38)
             if (n > (held ? SA_LIST / 8 : SA_LIST)) {
                 __syncthreads();
                 if (wave == 0) { s.count[0][lane] = 0; s.excess[0][lane] = 0; }
@@ -986,14 +993,16 @@ __global__ __launch_bounds__(64 * WAVES) void sample_select_kernel(SampleArgs A,
         }
     }
 }
-// Workgroups of sixteen waves, or of eight where the rows are many.
+// Workgroups of sixteen waves, or of eight where the rows are more than the CUs: 68 rows x 50000 59 us (eight 63), 300 rows x
+// 151936 65 (sixteen 75), 1088 rows x 131072 251 (280).
 template <bool DRAW>
 void select_rows(const SampleArgs &A, int rows, int pieces, hipStream_t s) {
     if (rows > 256) sample_select_kernel<DRAW, 8><<<rows, 512, 0, s>>>(A, pieces);
     else sample_select_kernel<DRAW, 16><<<rows, 1024, 0, s>>>(A, pieces);
 }
 
-// Probabilities of a piece; one that lies below the cut is not read.
+// Probabilities of a piece; one that lies below the cut is not read.  Bound by memory: 1088 rows x 131072 140 us, 570 MB
+// written at 4.1 TB/s.
 __global__ __launch_bounds__(PIECE_THREADS) void sample_probs_kernel(SampleArgs A, int pieces) {
     const int row = blockIdx.x / pieces, piece = blockIdx.x % pieces, tid = threadIdx.x;
     const RowResult q = A.results[row];
