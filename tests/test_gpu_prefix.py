@@ -381,3 +381,65 @@ def test_buffer_of_another_batch(qgl):
         qg.call("sync")
     a.check()
     other.check()
+
+
+def test_starts_outside_the_rows(qgl):
+    """Row starts below the first row and behind the last are cut to what there is; starts that run backwards, lengths that are none:
+    nothing outside is touched, and the next right call is right."""
+    rng = np.random.default_rng(17)
+    counts = [2, 0, 5, 5]
+    cache = Forked(rng, [(-1, 0, 700), (0, 600, 3), (0, 530, 60), (2, 580, 9)], counts)
+    batch = Batch(counts, rows=14, max_rows=5)
+    batch.start = np.array([-7, 2, 2, 9, 1 << 30], np.int32)
+    batch.places = lambda: [(0, 0, 0), (1, 0, 1)] + [(2 + i, 2, i) for i in range(5)] + [(9 + i, 3, i) for i in range(5)]
+    batch.dstart.set(batch.start)
+    fill_rows(rng, cache, batch)
+    a = Attend(cache, batch, rng.standard_normal((14, 8, 64)), 0.125)
+    a.check()
+    for starts in ([5, -3, 900, 2, 1 << 30], [14, 9, 3, 1, 0], [1 << 30] * 5, [-(1 << 31)] * 5, [0, 14, 0, 14, 0]):
+        batch.dstart.set(np.array(starts, np.int32))
+        for lengths in ([1 << 30, -5, -(1 << 31), cache.width * cache.P + 1], list(cache.length)):
+            cache.dlength.set(np.array(lengths, np.int32))
+            a.run()
+    batch.dstart.set(batch.start)
+    a.out.set(np.full(a.q.shape, 7, np.float32))
+    a.check()
+
+
+@pytest.mark.parametrize("sequences", [300, 700, 1024])
+def test_hundreds_of_segments(qgl, sequences):
+    """As many segments as a workgroup of the attention has threads, and more, shared ones among them."""
+    rng = np.random.default_rng(18)
+    family = [(-1, 0, 600)]
+    for i in range(1, sequences):
+        family.append((int(rng.integers(0, i)), int(rng.integers(200, 900)), int(rng.integers(0, 400))))
+    a = build(rng, family, [int(rng.integers(0, 4)) for _ in family], heads=4, kv_heads=1)
+    a.check()
+    a.plan.check()
+    count, shared = a.plan.buffer.get()[:8].view(np.int32)
+    assert count >= 256 and shared > 16
+
+
+def test_far_layers(qgl):
+    """A layer behind more than 4 GiB of others, and pages at the end of the pools: offsets beyond 32 bits."""
+    rng = np.random.default_rng(19)
+    layers, heads, dim, page, pages = 40, 8, 128, 64, 1024
+    cache = Forked(rng, [(-1, 0, 700), (0, 640, 3), (0, 600, 70)], [2, 1, 3], kv_heads=heads, page=page, dim=dim)
+    bytes_layer = pages * heads * page * dim * 2
+    big = [Device.__new__(Device) for _ in range(2)]
+    for d in big:
+        d.x, d.p = np.zeros(1, np.uint8), qgl.qg_alloc(layers * bytes_layer)
+        assert d.p
+    batch = Batch([2, 1, 3])
+    fill_rows(rng, cache, batch)
+    layer, first = layers - 1, pages - cache.pages
+    for d, host in zip(big, (cache.k, cache.v)):
+        qg.call("write", d.p + layer * bytes_layer + first * heads * page * dim * 2, np.ascontiguousarray(host).ctypes.data, host.nbytes)
+    desc = qg.KvCache.from_buffer_copy(cache.desc)
+    table = Device(np.where(cache.table >= 0, cache.table + first, -1).astype(np.int32))
+    desc.k, desc.v, desc.layers, desc.pages, desc.table = big[0].p, big[1].p, layers, pages, table.p
+    q = rng.standard_normal((6, heads * 2, dim)).astype(np.float32)
+    want, tol, _ = attention(cache, batch, q, dim ** -0.5)
+    cache.ref = C.byref(desc)
+    got = Attend(cache, batch, q, dim ** -0.5, layer).run()
+    assert np.all(np.abs(got - want) <= tol)
