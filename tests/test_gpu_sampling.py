@@ -424,3 +424,45 @@ def test_two_threads(qgl):
     for c, out in zip(calls, outs):
         c.check_sample()
         c.check_probs(out.get())
+
+
+def test_rows_behind_two_thousand_million_values(qgl):
+    """Offsets beyond 32 bits: the last rows of a large array come out as the same rows by themselves."""
+    rng = np.random.default_rng(16)
+    rows, cols, few = 33000, 65538, 18
+    big = Device.__new__(Device)
+    big.x, big.p = np.zeros(1, np.uint8), qgl.qg_alloc(rows * cols * 4)
+    assert big.p
+    c = Call(logits(rng, few, cols), REQUESTS, 1, rng.random((few, 1)))
+    c.sample()
+    qg.call("sync")
+    want, wlog = c.token.get().ravel().copy(), c.logprob.get().ravel().copy()
+    probs = Device(np.zeros(c.x.shape, np.float32))
+    qg.call("sampling_softmax", probs.p, c.dx.p, few, cols, c.ref, c.ws.p, c.bytes)
+    wprobs = probs.get().copy()
+    qg.call("zero", big.p, rows * cols * 4)
+    for at in (0, rows - few):
+        qg.call("write", big.p + at * cols * 4, c.x.ctypes.data, c.x.nbytes)
+    arrays = []
+    for a in c.arrays:
+        v = a.get()
+        whole = np.full(rows, v[0], v.dtype)
+        whole[:few] = whole[-few:] = v
+        arrays.append(Device(whole))
+    sampling = qg.Sampling(*[a.p for a in arrays])
+    u = np.full(rows, 0.5, np.float32)
+    u[:few] = u[-few:] = c.u.ravel()
+    du, token, logprob = Device(u), Device(np.full(rows, -7, np.int32)), Device(np.zeros(rows, np.float32))
+    n = qgl.qg_sample_workspace_bytes(rows, cols)
+    ws = Device.__new__(Device)
+    ws.x, ws.p = np.zeros(1, np.uint8), qgl.qg_alloc(n)
+    assert ws.p
+    qg.call("sample", token.p, logprob.p, big.p, rows, cols, 1, C.byref(sampling), du.p, ws.p, n)
+    qg.call("sync")
+    for part in (slice(0, few), slice(rows - few, rows)):
+        assert np.array_equal(token.get()[part], want) and np.array_equal(logprob.get()[part], wlog)
+    qg.call("sampling_softmax", big.p, big.p, rows, cols, C.byref(sampling), ws.p, n)
+    got = np.zeros_like(c.x)
+    for at in (0, rows - few):
+        qg.call("read", got.ctypes.data, big.p + at * cols * 4, got.nbytes)
+        assert np.array_equal(got, wprobs)
