@@ -16,7 +16,7 @@ namespace {
 
 constexpr int SA_DIGIT = 11, SA_BINS = 1 << SA_DIGIT, SA_PIECE = 4096;
 constexpr int SA_MAX_COLS = 1 << 24, SA_MAX_DRAWS = 64;
-constexpr int SA_GRID = 64, SA_LISTED = 128;
+constexpr int SA_GRID = 64, SA_LISTED = 192, SA_LISTS = 128;  // listed values of a piece: at most, and where that suffices
 
 // What the pass over a piece of a row leaves: its largest value (NaN if there is one) and that
 // value's bin, whether weights lie below the bins it keeps, the last of these, the last whose values
@@ -379,7 +379,10 @@ __global__ __launch_bounds__(PIECE_THREADS) void sample_piece_kernel(SampleArgs 
     if (lane == 0) { s_rest[wave] = rest; s_below[wave] = below; }
     __syncthreads();
     if (wave == 0) {
-        const int most = q.top_k ? min(max(2 * q.top_k, 32), SA_LISTED) : SA_LISTED;  // a piece may hold all top_k, of a bin's about half
+        // a piece may hold all top_k, of a bin's about half; the full length only where the row's top_k may fill most of the usual one
+        // (68 rows x 50000 with top-k 1000 56 -> 40 us; the full length for all: 1088 rows x 131072 247 -> 253; room for it, which
+        // 1088 rows of top-k 1000 do not use, costs them 372 -> 388)
+        const int most = q.top_k > 48 * pieces ? SA_LISTED : q.top_k ? min(max(2 * q.top_k, 32), SA_LISTS) : SA_LISTS;
         const unsigned long long b = s_bin[lane];
         const unsigned upto = wave_upto(bin_count(b));
         const int cover = min((int)__popcll(__ballot(upto <= (unsigned)most)) - 1, known), listed = cover < 0 ? 0 : (int)of_lane(upto, cover);
@@ -430,7 +433,7 @@ __global__ __launch_bounds__(PIECE_THREADS) void sample_piece_kernel(SampleArgs 
 // values, from the lists where these reach and else read again from the pieces that have some, are
 // ranked (of a bin with too many, those of the 64th part in which the cut is).  What the bins do not
 // hold is left to the search over the whole row.  Bound by dependent steps (statistics, bins, the cut's bin, its values in
-// order, sums, draws): a row 14 us, 1088 rows of the ten kinds 58, two of them on a CU (105 registers a lane; three with
+// order, sums, draws): a row 14 us, 1088 rows of the ten kinds 58, two of them on a CU (114 registers a lane; three with
 // 80 spill and gain nothing).
 // ------------------------------------------------------------------------
 constexpr int SA_LIST = 1024, SA_HELD = 2 * SA_LIST;  // values that are ranked; that are held
@@ -525,22 +528,25 @@ struct Grid {
     // Holds the listed values of bins 0..D, where lists reach that far and they are not too many.
     static constexpr int EACH = 64 / WAVES, PER = SA_LISTED / 64;  // pieces of a wave, listed values of a lane
     static __device__ __forceinline__ void read_lists(const uint2 *lists, int pieces, const PieceStat &mine, int wave, int lane, uint2 (&y)[EACH][PER]) {
+        const bool longer = __any(mine.listed > SA_LISTS);
 #pragma unroll
         for (int k = 0; k < EACH; k++) {
             const int p = k * WAVES + wave, listed = p < pieces ? of_lane(mine.listed, p) : 0;
 #pragma unroll
-            for (int i = 0; i < PER; i++) y[k][i] = i * 64 + lane < listed ? lists[(size_t)p * SA_LISTED + i * 64 + lane] : make_uint2(0, 0);
+            for (int i = 0; i < PER; i++) y[k][i] = (i * 64 < SA_LISTS || longer) && i * 64 + lane < listed ? lists[(size_t)p * SA_LISTED + i * 64 + lane] : make_uint2(0, 0);
         }
     }
     __device__ __forceinline__ void hold(int D, const uint2 (&y)[EACH][PER]) {
         const int n = D < 0 || D > reach || pieces > 64 ? 0 : (int)of_lane(count_upto, D);
         if (n == 0 || n > SA_HELD) return;
         unsigned is = 0;
+        const bool longer = __any(mine.listed > SA_LISTS);
 #pragma unroll
         for (int k = 0; k < EACH; k++) {
             int all = 0;
 #pragma unroll
             for (int i = 0; i < PER; i++) {
+                if (i * 64 >= SA_LISTS && !longer) continue;
                 const bool in = y[k][i].x && (double)place - place_of(y[k][i].x) <= (double)D;
                 is |= (unsigned)in << (k * PER + i);
                 all += (int)__popcll(__ballot(in));
@@ -554,6 +560,7 @@ struct Grid {
             int to = of_lane(before, k * WAVES + wave);
 #pragma unroll
             for (int i = 0; i < PER; i++) {
+                if (i * 64 >= SA_LISTS && !longer) continue;
                 const bool in = is >> (k * PER + i) & 1;
                 const unsigned long long all = __ballot(in);
                 const int at = to + (int)__popcll(all & ((1ULL << lane) - 1));
