@@ -471,7 +471,7 @@ struct Grid {
     const uint2 *lists;
     const int cols, pieces, tid, lane, wave, place;  // place: of the row's largest value
     const float m;
-    const double a, unit;                            // unit: of a weight at place's lower end, the largest value's being 1
+    const double a, unit;                            // unit: what the largest value, whose weight is 1, adds to its bin
     int reach, known;                                // bins 0..reach are in the lists, 0..known in the bins
     bool below;                                      // whether the row has weights below the known bins
     // lane D of each wave: values in bin D from the top and with the bins above, and their weight
@@ -516,7 +516,7 @@ struct Grid {
             for (int k = 0; k < 4; k++) { n += bin_count(b[k]); e += bin_excess(b[k]); }
         }
         all_waves(n, e, count, e);
-        mass = bin_mass(count, e, lane) * unit;
+        mass = bin_mass(count, e, lane) / unit;
         count_upto = wave_upto(count);
         mass_upto = wave_upto(mass);
         deepest = SA_GRID - 1;
@@ -710,7 +710,7 @@ struct Grid {
                 });
                 __syncthreads();
                 const unsigned c = s.count[0][lane], c_upto = wave_upto(c);
-                const double w = bin_mass(c, s.excess[0][lane], D) * unit, w_upto = wave_upto(w);
+                const double w = bin_mass(c, s.excess[0][lane], D) / unit, w_upto = wave_upto(w);
                 if (BY == BY_KEY) {
                     sub = part_of((double)key_value(t) * a);
                 } else {
@@ -771,7 +771,7 @@ struct Grid {
                 }
             } else {
                 const unsigned long long b = row_bin(p);
-                if (lane < whole) sum = bin_mass(bin_count(b), bin_excess(b), lane) * unit;
+                if (lane < whole) sum = bin_mass(bin_count(b), bin_excess(b), lane) / unit;
                 if (whole == deepest)
                     for (int k = lane; k < kept; k += 64)
                         if (s.sorted_index[k] / SA_PIECE == p) sum += weight(s.sorted_key[k]);
@@ -828,7 +828,8 @@ __global__ __launch_bounds__(64 * WAVES) void sample_select_kernel(SampleArgs A,
     const double place = grid_place(top, q.a);
     bool found = false, weighed = false, listed = false;  // listed: the pieces' lists hold what stays
     if (__builtin_fabs(place) < 0.5 * GRID_FAR) {
-        const double unit = 1.0 / power_of<true>((double)top * q.a).p;
+        // as bins have it, and a quotient: values that equal the largest weigh whole numbers, of which a top-p may be one
+        const double p_top = power_of<true>((double)top * q.a).p, unit = q.filters() ? bin_mass(1, bin_excess(bin_entry(p_top)), 0) : p_top;
         // the bins that every piece's list and bins cover, and the weight of all
         int reach = SA_GRID - 1, known = SA_GRID - 1, counted = 0;
         bool below = false;
@@ -837,7 +838,7 @@ __global__ __launch_bounds__(64 * WAVES) void sample_select_kernel(SampleArgs A,
             const PieceStat y = p == from ? mine : stats[p];
             const int delta = (int)place - y.at;
             const bool counts = y.at != GRID_LOW && delta < SA_ZERO;
-            const double w = counts ? __builtin_amdgcn_ldexp(y.all, -delta) * unit : 0.0;
+            const double w = counts ? __builtin_amdgcn_ldexp(y.all, -delta) / unit : 0.0;
             if (!q.filters()) piece[p] = w;
             all += w;
             if (!counts) continue;

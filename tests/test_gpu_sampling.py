@@ -466,3 +466,25 @@ def test_rows_behind_two_thousand_million_values(qgl):
     for at in (0, rows - few):
         qg.call("read", got.ctypes.data, big.p + at * cols * 4, got.nbytes)
         assert np.array_equal(got, wprobs)
+
+
+@pytest.mark.parametrize("value", [0.0, 3.25, -2000.0, 0.7])
+@pytest.mark.parametrize("n", [4, 84, 134, 366, 1020, 2044, 4288, 40000, 100000])
+def test_shares_that_whole_numbers_meet(qgl, n, value):
+    """n equal values, of which top-p keeps an exact part: weights of 1 have sums without a rounding, and no border is unclear."""
+    cols = n + n // 3 + 5
+    x = np.full((12, cols), -np.inf, np.float32)
+    rng = np.random.default_rng(n)
+    for row in x:
+        row[rng.choice(cols, n, replace=False)] = value
+    asks = [(T, k, p, 0.0) for T in (1.0, 0.7, 3.0) for k, p in ((0, 0.5), (0, 0.25), (0, 0.75), (n // 2, 0.5))]
+    c = Call(x, asks, 2, np.tile(np.array([0, 1 - 2.0 ** -24], np.float32), (12, 1)))
+    c.sample()
+    out = Device(np.full(x.shape, 7, np.float32))
+    qg.call("sampling_softmax", out.p, c.dx.p, c.rows, c.cols, c.ref, c.ws.p, c.bytes)
+    token, probs = c.token.get(), out.get()
+    for r, (T, k, p, _) in enumerate(asks):
+        kept = np.nonzero(x[r] == np.float32(value))[0][:math.ceil((k or n) * p)]  # the fewest that weigh p of all
+        assert np.array_equal(np.nonzero(probs[r])[0], kept), (r, asks[r], np.count_nonzero(probs[r]), len(kept))
+        assert (probs[r, kept] == np.float32(1 / len(kept))).all()
+        assert token[r].tolist() == [kept[0], kept[-1]], (r, asks[r])
