@@ -261,7 +261,7 @@ struct Row {
 // One pass over the values, in pieces.  A bin holds the weights whose exponents x a round to one whole
 // number, the same for all pieces of a row, so that those of all pieces can be added; a piece keeps the
 // SA_GRID bins from its largest value down, of these only as many as the row's filters
-// may cut in.  A weight is 1..2 times its bin's lower end: what it has above that, to 2^-36, is
+// may cut in.  A weight is 1..2 times its bin's lower end: what it has above that, to 2^-38, is
 // added up as a whole number under the count, in one 64-bit atomic whose order does not
 // matter.  The values of the first bins, up to SA_LISTED of them, are listed: few tokens
 // stay of most rows, and then nothing is read again.
@@ -270,7 +270,7 @@ struct Row {
 // 215 to 240.  Of 4096 values in a workgroup's registers: 16 loads of a thread on their way, eight
 // workgroups on a CU; with the next piece on its way in as many registers again 474 us, 16-byte loads 264.
 // ------------------------------------------------------------------------
-constexpr int PIECE_THREADS = 256, PIECE_WAVES = PIECE_THREADS / 64, PIECE_VALUES = SA_PIECE / PIECE_THREADS, BIN_COUNT = 49, BIN_BITS = 36;
+constexpr int PIECE_THREADS = 256, PIECE_WAVES = PIECE_THREADS / 64, PIECE_VALUES = SA_PIECE / PIECE_THREADS, BIN_COUNT = 51, BIN_BITS = 38;
 constexpr double GRID_FAR = (double)(1 << 19);  // places further out are left to the search over the row
 constexpr int GRID_LOW = -(1 << 30);            // in place of one: the piece's weights are 0 beside a row's largest within half of that
 
@@ -705,7 +705,7 @@ struct Grid {
                     const double e = (double)key_value(key) * a;
                     if (__builtin_rint(e) != b || !cut.keeps(key, i)) return;
                     atomicAdd(&s.count[0][part_of(e)], 1u);
-                    // up to 2^24 values of less than 2^37 above their count
+                    // up to 2^24 values of at most 2^38 beside their count
                     atomicAdd(&s.excess[0][part_of(e)], bin_excess(bin_entry(power_of<true>(e).p)));
                 });
                 __syncthreads();
