@@ -969,7 +969,12 @@ __global__ __launch_bounds__(64 * WAVES) void sample_select_kernel(SampleArgs A,
                 before = of_lane(upto, 63);
             }
         }
-        for (int i0 = p * SA_PIECE; !listed && i0 < min((p + 1) * SA_PIECE, A.cols) && !past; i0 += 16 * 64) {
+        // Read again, the piece may weigh less than what was recorded of it, and the goal lie between the two: bins round, and powers
+        // of x a differ from those of (x - max) a by what the products were rounded.  Then it is the last token that stays.
+        const int end = min((p + 1) * SA_PIECE, A.cols);
+        int full = -1;  // the last chunk that holds something, if it was passed over
+        bool take = last;
+        for (int i0 = listed ? end : p * SA_PIECE; i0 < end && !past; i0 += 16 * 64) {
             float v[16];
             double sum = 0.0;
 #pragma unroll
@@ -980,19 +985,27 @@ __global__ __launch_bounds__(64 * WAVES) void sample_select_kernel(SampleArgs A,
                 if (v[k] > -__builtin_inff() && cut.keeps(order_key(v[k]), i0 + k * 64 + lane)) { stays |= 1u << k; sum += r.weight(v[k]); }
             }
             sum = wave_all_add(sum);
-            if (sum == 0.0) continue;
-            if (!last && !(before + sum * (1.0 + 1e-12) > goal)) { before += sum; continue; }
+            if (sum > 0.0 && !take && !(before + sum * (1.0 + 1e-12) > goal)) {
+                before += sum;
+                full = i0;
+            } else if (sum > 0.0) {
+                full = -1;
 #pragma unroll
-            for (int k = 0; k < 16; k++) {
-                if (past || !__any(stays >> k & 1)) continue;
-                const double w = stays >> k & 1 ? r.weight(v[k]) : 0.0, upto = wave_upto(w) + before;
-                const unsigned long long hit = __ballot(!last && w > 0.0 && upto > goal), any = __ballot(w > 0.0);
-                if (!any) continue;
-                const int l = hit ? __builtin_ctzll(hit) : 63 - __builtin_clzll(any);
-                pick = i0 + k * 64 + l;
-                won = of_lane(w, l);
-                past = hit != 0;
-                before = of_lane(upto, 63);
+                for (int k = 0; k < 16; k++) {
+                    if (past || !__any(stays >> k & 1)) continue;
+                    const double w = stays >> k & 1 ? r.weight(v[k]) : 0.0, upto = wave_upto(w) + before;
+                    const unsigned long long hit = __ballot(!take && w > 0.0 && upto > goal), any = __ballot(w > 0.0);
+                    if (!any) continue;
+                    const int l = hit ? __builtin_ctzll(hit) : 63 - __builtin_clzll(any);
+                    pick = i0 + k * 64 + l;
+                    won = of_lane(w, l);
+                    past = hit != 0;
+                    before = of_lane(upto, 63);
+                }
+            }
+            if (full >= 0 && i0 + 16 * 64 >= end) {  // no token passed, and the last one has not been looked at
+                take = true;
+                i0 = full - 16 * 64;
             }
         }
         if (lane == 0) {
