@@ -575,7 +575,7 @@ struct Grid {
     __device__ __forceinline__ int first_cut(const Request &q, double all, uint32_t least) const {
         if (q.top_k || q.top_p < 1.0) {
             const unsigned long long enough =
-                __ballot(lane <= known && count_upto > 0 && (q.top_k ? count_upto >= (unsigned)q.top_k : mass_upto >= q.top_p * all));
+                __ballot(lane <= known && count > 0 && (q.top_k ? count_upto >= (unsigned)q.top_k : mass_upto >= q.top_p * all));
             return enough ? (int)__builtin_ctzll(enough) : -1;
         }
         const double d = (double)place - place_of(least);
@@ -678,10 +678,10 @@ struct Grid {
             if (!(d <= (double)known)) return !below;  // nothing that weighs lies below
             D = (int)d;
         } else {
-            const unsigned long long enough = __ballot(lane <= known && count_upto > 0 && (BY == BY_MASS ? mass_upto >= target : (double)count_upto >= target));
-            if (!enough) return !below;
+            // a bin that holds something: the sums up to an empty one may be larger than those before it by their last bits
+            const unsigned long long enough = __ballot(lane <= known && count > 0 && (BY == BY_MASS ? mass_upto >= target : (double)count_upto >= target));
+            if (!enough) return BY == BY_COUNT && !below;
             D = __builtin_ctzll(enough);
-            if (D > deepest) return true;  // sums that differ in their last bits
         }
         const int n = (int)of_lane(count, D);
         int first = (int)of_lane(count_upto, D) - n;
@@ -716,7 +716,7 @@ struct Grid {
                 } else {
                     const unsigned long long enough = __ballot(c > 0 && (BY == BY_MASS ? before + w_upto >= target : (double)first + c_upto >= target));
                     const unsigned long long some = __ballot(c > 0);
-                    if (!some) return true;
+                    if (!some) return false;
                     sub = enough ? __builtin_ctzll(enough) : 63 - __builtin_clzll(some);
                 }
                 if (of_lane(c, sub) > SA_LIST) return false;
@@ -748,7 +748,7 @@ struct Grid {
             __syncthreads();
             stay = BY == BY_MASS ? min(s.n + 1, kept) : s.n;
         }
-        if (BY != BY_KEY && stay <= 0) return true;
+        if (BY != BY_KEY && stay <= 0) return false;  // a filter that would not be applied
         kept = stay;
         deepest = D;
         cut = BY == BY_KEY ? Cut{t, 0x7fffffff} : Cut{s.sorted_key[kept - 1], s.sorted_index[kept - 1]};

@@ -146,6 +146,32 @@ def test_draws_at_the_end_of_a_piece_of_all_tokens(qgl, case):
     check(rows[:300], [(T, 0, 1.0, 0.0)], np.tile(np.float32([[u]]), (300, 1)))
 
 
+# T, top-p, the largest values, how many copies of each lie `off` lower: where the sums of the bins reach top-p is, but for
+# the last bits of a sum, the end of the largest; the bin behind them is empty
+EMPTY = [(1.051647424697876, 0.5, (-0.15683889389038086, -0.9144611358642578, -1.5316662788391113), 16, 2.915785789489746),
+         (F("0x1.19ddeap+0"), 0.5, (F("0x1.a88afp-1"), F("-0x1.7d0cp-4"), F("-0x1.6715ep-1")), 16, F("0x1.86c01cp+1")),
+         (F("0x1.5a8006p+0"), 0.25, (F("0x1.2f16p-5"), F("-0x1.48fefp-1"), F("-0x1.b632e8p+0"), F("-0x1.990b2p+1")), 96, F("0x1.2c382ep+2")),
+         (F("0x1.26831p-1"), 0.25, (F("0x1.04a64p-2"), F("-0x1.171a4p-3"), F("-0x1.ee166p-2")), 48, F("0x1.9847cp+0")),
+         (F("0x1.56d988p+0"), 0.25, (F("0x1.eadcp-1"), F("-0x1.cc6bp-4"), F("-0x1.0b069p+0")), 48, F("0x1.db4a68p+1")),
+         (F("0x1.1247ap-1"), 0.5, (F("-0x1.a1ae4p-3"), F("-0x1.479d5p-1"), F("-0x1.298648p+0"), F("-0x1.8aa64p+0")), 32, F("0x1.db4a68p+0")),
+         (F("0x1.1247ap+0"), 0.5, (F("-0x1.63c89p-1"), F("-0x1.cfc05p+0"), F("-0x1.2e959cp+1"), F("-0x1.7ec048p+1")), 32, F("0x1.db4a68p+1")),
+         (F("0x1.3d8f3cp-1"), 0.25, (F("0x1.69f69p-1"), F("0x1.b84d8p-3"), F("-0x1.5d38cp-3")), 96, F("0x1.1324f4p+1"))]
+
+
+@pytest.mark.parametrize("cols", [0, 4096, 9000])
+@pytest.mark.parametrize("case", range(len(EMPTY)))
+def test_top_p_that_ends_before_an_empty_bin(qgl, case, cols):
+    T, p, top, copies, off = EMPTY[case]
+    top = np.float32(top)
+    x = np.concatenate([top, np.repeat(top - np.float32(off), copies)])
+    if cols:
+        x = np.concatenate([x, np.full(cols - len(x), -np.inf, np.float32)])
+    share = np.cumsum(np.exp((top.astype(np.float64) - float(top[0])) / T))
+    u = [0.0, 1 - 2.0 ** -24] + [v for s in share for v in around(s / share[-1])]
+    check([x], [(T, 0, p, 0.0)], [u])
+    check([x, np.roll(x, 3)], [(T, 0, p, 0.0), (T, 0, p, 1e-6)], [u, u])
+
+
 @pytest.mark.parametrize("ask", [(1.0, 0, 1.0, 0.0), (0.01, 0, 1.0, 0.0), (1e-3, 0, 1.0, 0.0), (1.0, 0, 0.9, 0.0), (1.0, 0, 0.999, 0.0), (2.0, 0, 1.0, 1e-3), (1.0, 5000, 1.0, 0.0),
                                  (1.0, 3000, 0.9, 1e-3), (1.0, 40, 0.95, 0.0)])
 @pytest.mark.parametrize("cols", [4096, 12289, 30000])
