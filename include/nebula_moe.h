@@ -62,7 +62,8 @@ int nm_stack_attend(nm_stack *s, const nm_attention_layer *layers, const nm_atte
  * weight); rows of no sequence take the MoE alone.  Keys and values of the rows are stored behind the cached tokens;
  * lengths do not change (qg_kv_compact does that once drafts are accepted).
  * use_graph: captured on first use per number of rows and replayed while the
- * batch's arrays stay where they are; what they hold may change.  Inside a capture
+ * batch's arrays stay where they are (and, with nm_stack_share, the calling thread's
+ * qg_prefix_least_saving is what it was); what they hold may change.  Inside a capture
  * of the caller's (qg_graph_begin) the calls join that graph, whatever use_graph
  * says.  A stack has one hidden state and one workspace: one call, or one graph that
  * holds it, runs at a time. */

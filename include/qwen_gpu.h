@@ -275,7 +275,8 @@ int qg_kv_prefixes(int *link, int *shared, const qg_kv_cache *cache, const qg_kv
  * layer for qg_kv_prefixes to have them shared (what sharing costs is about the
  * same for all batches): a setting of the calling thread, 48 MiB at first and for
  * negative values.  link and shared do not depend on it, outputs only within the
- * attention's error.  Returns the previous setting. */
+ * attention's error.  A captured qg_kv_prefixes keeps the setting of its capture.
+ * Returns the previous setting. */
 int64_t qg_prefix_least_saving(int64_t bytes);
 
 /* qg_tree_attention of a batch in which sequences share pages: the same outputs

@@ -51,6 +51,7 @@ struct nm_stack {
     size_t prefixes_bytes;
     void *verify_graphs[NM_MAX_TOKENS + 1];
     qg_kv_batch verify_batches[NM_MAX_TOKENS + 1];
+    int64_t verify_saving[NM_MAX_TOKENS + 1];   /* qg_prefix_least_saving as captured (0: pages are not shared) */
 };
 
 static void attend_free(nm_stack *s) {
@@ -241,8 +242,10 @@ int nm_stack_verify(nm_stack *s, const qg_kv_batch *batch, int use_graph) {
     if (!use_graph || qg_graph_recording()) return run_verify(s, batch);
     void **g = &s->verify_graphs[batch->rows];
     qg_kv_batch *b = &s->verify_batches[batch->rows];
-    if (*g && (b->max_rows != batch->max_rows || b->start != batch->start || b->parent != batch->parent)) {
-        /* the graph reads other arrays; it may still be running */
+    int64_t saving = 0;
+    if (s->prefixes) { saving = qg_prefix_least_saving(0); qg_prefix_least_saving(saving); }
+    if (*g && (b->max_rows != batch->max_rows || b->start != batch->start || b->parent != batch->parent || s->verify_saving[batch->rows] != saving)) {
+        /* the graph reads other arrays, or shares pages by another setting; it may still be running */
         GPU(qg_sync());
         qg_graph_destroy(*g);
         *g = NULL;
@@ -253,6 +256,7 @@ int nm_stack_verify(nm_stack *s, const qg_kv_batch *batch, int use_graph) {
         const int end = qg_graph_end(*g);
         if (end) { qg_graph_destroy(*g); *g = NULL; return fail("capture verify step: %s", qg_error(end)); }
         *b = *batch;
+        s->verify_saving[batch->rows] = saving;
     }
     GPU(qg_graph_launch(*g));
     return 0;
