@@ -343,10 +343,11 @@ typedef struct {
 /* token[rows][draws]: the first i with sum_{j<=i} w_j > u[r][d] sum_j w_j over
  * what stays of row r of x [rows][cols], u [rows][draws] in [0, 1);
  * logprob[rows][draws] (or NULL): log(w_i / sum_j w_j).  Weights and sums in 64
- * bits; the sums that top-p is held against to 2^-37 of themselves, or to
- * 2^(2 b - 63), 2^b >= cols, in a row that is searched as a whole (over 1024 values
- * within a 64th of a bit of weight where a filter cuts, cuts further than 2^-62 below the
- * largest weight, |x / T| past 2^17).  -infinity is never drawn; a row of nothing else, or with NaN or
+ * bits; the sums that draws and top-p are held against to 2^-35 of themselves (2^-37
+ * where |x / T| is at most 2^14), or to 2^(2 b - 63), 2^b >= cols, those of top-p in a
+ * row that is searched as a whole (over 1024 values within a 64th of a bit of weight
+ * where a filter cuts, cuts further than 2^-62 below the largest weight, |x / T| past
+ * 2^17).  -infinity is never drawn; a row of nothing else, or with NaN or
  * +infinity, gives -1 and NaN.  draws 1..64 of each row, independent of each
  * other (drafted siblings, several answers' first tokens).
  * qg_sampling_softmax: out = w_i / sum_j w_j, 0 where a token does not stay,

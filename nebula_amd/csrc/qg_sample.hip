@@ -271,7 +271,10 @@ struct Row {
 // workgroups on a CU; with the next piece on its way in as many registers again 474 us, 16-byte loads 264.
 // ------------------------------------------------------------------------
 constexpr int PIECE_THREADS = 256, PIECE_WAVES = PIECE_THREADS / 64, PIECE_VALUES = SA_PIECE / PIECE_THREADS, BIN_COUNT = 51, BIN_BITS = 38;
-constexpr double GRID_FAR = (double)(1 << 19);  // places further out are left to the search over the row
+// Places further out are left to the search over the row.  A row's largest place is below half of it: exponents of up to 2^18 are
+// off by 2^-36, weights and the largest's with them and by the bins' 2^-39 each: sums to 2^-35 of themselves (exponents up to
+// 2^15: to 2^-37), which the weights of (x - max) a that follow within a piece are held against.
+constexpr double GRID_FAR = (double)(1 << 19);
 constexpr int GRID_LOW = -(1 << 30);            // in place of one: the piece's weights are 0 beside a row's largest within half of that
 
 QG_DEV double grid_place(float x, double a) { return __builtin_rint((double)x * a); }
