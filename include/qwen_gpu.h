@@ -272,11 +272,12 @@ size_t qg_kv_prefixes_bytes(const qg_kv_cache *cache, const qg_kv_batch *batch);
 int qg_kv_prefixes(int *link, int *shared, const qg_kv_cache *cache, const qg_kv_batch *batch, void *prefixes, size_t prefixes_bytes);
 
 /* How many bytes of keys and values the sequences of a batch must save in each
- * layer for qg_kv_prefixes to have them shared (what sharing costs is about the
- * same for all batches): a setting of the calling thread, 48 MiB at first and for
- * negative values.  link and shared do not depend on it, outputs only within the
- * attention's error.  A captured qg_kv_prefixes keeps the setting of its capture.
- * Returns the previous setting. */
+ * layer for qg_kv_prefixes to have them shared (sharing costs 2 to 10 us a layer
+ * whatever is saved; prompt chunks, sequences of more than 64 rows, gain nothing and
+ * do not count): a setting of the calling thread, 48 MiB at first and for negative
+ * values; 0 shares whatever there is.  link and shared do not depend on it, outputs
+ * only within the attention's error.  A captured qg_kv_prefixes keeps the setting of
+ * its capture.  Returns the previous setting. */
 int64_t qg_prefix_least_saving(int64_t bytes);
 
 /* qg_tree_attention of a batch in which sequences share pages: the same outputs

@@ -84,9 +84,19 @@ __global__ __launch_bounds__(256) void prefix_link_kernel(KvView c, BatchView b,
 // Common parts count in steps of a quantum: shorter segments would cost more than
 // they save (8 sequences of 2048 tokens, 8 layers: 128 and 256 196 and 198 us, 1024 218;
 // two levels of 8 x 8: 69 and 69, 77).  It is doubled until the rows of all shared segments together are few
-// enough for the partial results that a workspace holds.  And nothing is shared where all of it together saves less than
-// `least` bytes of reads: joining the segments takes some 5 us (heads of 2 x 128, fp16, each sequence by itself / shared:
-// 8 sequences of 1000 tokens 12.2 / 17.8, of 4000 16.0 / 19.3, of 16000 30.4 / 23.0; 2 of 64000 32.0 / 28.6).
+// enough for the partial results that a workspace holds.
+//
+// Nothing is shared where all of it together saves less than `least` bytes of reads.  One row a sequence, us of a layer, the pages
+// shared / each sequence by itself / in qg_tree_attention (heads, cache, sequences, MiB saved):
+//   2 x 128 fp16 8, 10: 17.2 / 14.5 / 13.3    8, 23: 17.7 / 17.8 / 15.6    8, 47: 19.1 / 20.6 / 19.2    8, 95: 24.2 / 27.8 / 28.8
+//   2 x 128 fp16 2, 48: 24.5 / 28.2 / 29.2    32, 47: 21.5 / 21.2 / 17.3   32, 93: 25.8 / 26.2 / 23.0   32, 155: 26.0 / 31.0 / 27.1
+//   4 x 256 fp16 8, 42: 23.5 / 25.6 / 20.3    8, 91: 24.5 / 33.9 / 27.5    1 x 64 fp16 8, 96: 30.0 / 29.1 / 28.7, 160: 30.7 / 39.0 / 38.5
+//   8 x 128 F32 8, 42: 22.1 / 23.3 / 20.2     32 (of 256 tokens), 62: 31.3 / 25.1 / 23.8
+// the two sides cross between 20 and 95; the limit costs at most 2.1 us in what was timed but for the last, 6.
+// What a prompt chunk's rows (more than a tree has) share does not count: their products take longer than their reads, and the row
+// groups fill the registers with one sequence's rows as well.  8 chunks of 128 rows over 8000 common tokens: 2 x 128 fp16 229 / 212
+// / 212, 4 x 128 with groups of five 330 / 219 / 253, 8 x 128 466 / 371 / 365; of 30 such batches of 96 and 128 rows one gained.
+// Of 17 rows most gain (8 x 128 bf16 85 / 109 / 88), of 33 and 64 some lose.
 constexpr int QUANTUM = 256;
 constexpr int64_t LEAST_SAVING = 48 << 20;
 thread_local int64_t tl_least_saving = LEAST_SAVING;
@@ -169,7 +179,7 @@ QG_DEV void plan_segments(const KvView &c, const BatchView &b, const PrefixView 
         s.top[t] = -1;
         if (t == 0) { s.sum = 0; s.saved = 0; }
         plan_sync<THREADS>();
-        const unsigned long long saved = wave_all_add((unsigned long long)cut);
+        const unsigned long long saved = wave_all_add((unsigned long long)(n > QG_MAX_TREE ? 0 : cut));
         if ((t & 63) == 0) atomicAdd(&s.saved, saved);
         link = cut ? link0 : -1;
         while (link >= 0 && s.cut[link] >= cut) link = s.link[link];
