@@ -19,7 +19,9 @@ namespace {
 // ------------------------------------------------------------------------
 // Which sequences begin with the same pages: a wave per sequence.  Bound by dependent
 // reads (a length, an entry of every earlier sequence, the pages in common): 1024
-// sequences of up to 80 pages 13 us, 64 of 98304 tokens 6.
+// sequences of up to 80 pages 13 us, 64 of 98304 tokens 6.  Each earlier sequence that has more in common than those
+// before it is one more such round: where every sequence branches from the one before it at a later page, this and the plan
+// take 51 us for 64 sequences, 233 for 256 and 1360 for 1024 (from one text, at one place, 9, 19 and 27).
 // ------------------------------------------------------------------------
 QG_DEV int whole_pages(const KvView &c, int s) { return kv_length(c, s) >> c.shift; }
 QG_DEV int table_page(const KvView &c, int s, int j) {
@@ -92,7 +94,7 @@ __global__ __launch_bounds__(256) void prefix_link_kernel(KvView c, BatchView b,
 //   2 x 128 fp16 2, 48: 24.5 / 28.2 / 29.2    32, 47: 21.5 / 21.2 / 17.3   32, 93: 25.8 / 26.2 / 23.0   32, 155: 26.0 / 31.0 / 27.1
 //   4 x 256 fp16 8, 42: 23.5 / 25.6 / 20.3    8, 91: 24.5 / 33.9 / 27.5    1 x 64 fp16 8, 96: 30.0 / 29.1 / 28.7, 160: 30.7 / 39.0 / 38.5
 //   8 x 128 F32 8, 42: 22.1 / 23.3 / 20.2     32 (of 256 tokens), 62: 31.3 / 25.1 / 23.8
-// the two sides cross between 20 and 95; the limit costs at most 2.1 us in what was timed but for the last, 6.
+// the two sides cross between 20 and 95; the limit costs at most 2.5 us in what was timed but for the last, 6.
 // What a prompt chunk's rows (more than a tree has) share does not count: their products take longer than their reads, and the row
 // groups fill the registers with one sequence's rows as well.  8 chunks of 128 rows over 8000 common tokens: 2 x 128 fp16 229 / 212
 // / 212, 4 x 128 with groups of five 330 / 219 / 253, 8 x 128 466 / 371 / 365; of 30 such batches of 96 and 128 rows one gained.
@@ -288,7 +290,7 @@ __global__ __launch_bounds__(64 * SMALL) void prefix_small_kernel(KvView c, Batc
 // A unit is a part of a segment's keys for a group of up to 16 MOST of its rows x heads, so that a key that is read
 // serves as many rows as the registers hold.  64 sequences of one row over 98304 tokens in common (heads 16 over 2 of
 // 128, fp16): 155 us where the products alone take 94, the matrix cores busy for a quarter of the cycles and the waves
-// waiting for keys from L2 and behind it for half of theirs; each sequence by itself takes 514.  16 trees of 17 rows over
+// waiting for keys from L2 and behind it for half of theirs; qg_tree_attention takes 507.  16 trees of 17 rows over
 // 24576 tokens (bf16) 153 us, 107 and 198.  8 sequences over 2048 tokens 17 us, of which the way to a unit's first key
 // (plan 2.9, pages 2.2, queries 2.5) and the end are more than half.
 // ------------------------------------------------------------------------

@@ -136,7 +136,9 @@ struct RowShared {
     int found_bin;
 };
 
-// A row of any shape by one workgroup, which reads it again for every step.
+// A row of any shape by one workgroup, which reads it again for every step, at what a CU reads and adds to shared memory.  The
+// whole call: 1 row x 151936 175 us (|x / T| past 2^17, top-p or top-k) and 320 to 390 (flat, all in one 64th of a bit), 68 x 50000
+// 78 to 166, 1088 x 131072 770 to 1860; rows that the bins serve 20 to 35, 20 to 40 and 330 at most.
 template <int WAVES>
 struct Row {
     static constexpr int THREADS = 64 * WAVES, OWN = SA_BINS / THREADS;  // bins of a thread
@@ -383,8 +385,9 @@ __global__ __launch_bounds__(PIECE_THREADS) void sample_piece_kernel(SampleArgs 
     __syncthreads();
     if (wave == 0) {
         // a piece may hold all top_k, of a bin's about half; the full length only where the row's top_k may fill most of the usual one
-        // (68 rows x 50000 with top-k 1000 56 -> 40 us; the full length for all: 1088 rows x 131072 247 -> 253; room for it, which
-        // 1088 rows of top-k 1000 do not use, costs them 372 -> 388)
+        // (us, usual / full length: 68 rows x 24576 with top-k 500 40 / 34, x 50000 with 500 38 / 39, 1000 52 / 40, x 131072 with 1000
+        // 51 / 52, 1500 80 / 83, 2500 117 / 101; next to the limit, 68 x 80000 with 1000, 43 / 44; 1088 x 131072 with 1000 352 / 362.
+        // Room for it costs the rows that do not use it 4 %)
         const int most = q.top_k > 48 * pieces ? SA_LISTED : q.top_k ? min(max(2 * q.top_k, 32), SA_LISTS) : SA_LISTS;
         const unsigned long long b = s_bin[lane];
         const unsigned upto = wave_upto(bin_count(b));
@@ -437,7 +440,8 @@ __global__ __launch_bounds__(PIECE_THREADS) void sample_piece_kernel(SampleArgs 
 // ranked (of a bin with too many, those of the 64th part in which the cut is).  What the bins do not
 // hold is left to the search over the whole row.  Bound by dependent steps (statistics, bins, the cut's bin, its values in
 // order, sums, draws): a row 14 us, 1088 rows of the ten kinds 58, two of them on a CU (114 registers a lane; three with
-// 80 spill and gain nothing).
+// 80 spill and gain nothing).  Past 64 pieces nothing is held, and lists are read once more: 4 rows x 262145 with top-k 20 33 us,
+// x 262144 22.
 // ------------------------------------------------------------------------
 constexpr int SA_LIST = 1024, SA_HELD = 2 * SA_LIST;  // values that are ranked; that are held
 template <int WAVES>
@@ -1017,8 +1021,10 @@ __global__ __launch_bounds__(64 * WAVES) void sample_select_kernel(SampleArgs A,
         }
     }
 }
-// Workgroups of sixteen waves, or of eight where the rows are more than the CUs: 68 rows x 50000 59 us (eight 63), 300 rows x
-// 151936 65 (sixteen 75), 1088 rows x 131072 251 (280).
+// Workgroups of sixteen waves, or of eight where the rows are more than the CUs: 300 rows x 151936 97 us (sixteen 105), 512 x 50000
+// 70 (89), 1088 x 131072 243 (274).  Up to 256 rows eight take 1 us less where the bins and lists serve (68 x 50000 35.3 and 36.4),
+// but much longer where rows are read again: a flat row of 151936 442 (sixteen 386), top-k 5000 of 17 such rows 68 (54), 4 rows x
+// 2^20 114 (76).
 template <bool DRAW>
 void select_rows(const SampleArgs &A, int rows, int pieces, hipStream_t s) {
     if (rows > 256) sample_select_kernel<DRAW, 8><<<rows, 512, 0, s>>>(A, pieces);
