@@ -284,7 +284,7 @@ int64_t qg_prefix_least_saving(int64_t bytes);
  * (within the same error), but a page that several sequences hold is read once
  * for all of them.  `prefixes` as qg_kv_prefixes filled it for this cache and batch;
  * other arguments, refusals and special values as there.  For few rows a sequence
- * over a long common text.  Where nothing is shared it takes longer: 1 to 2 us for up to
+ * over a long common text.  Where nothing is shared it takes longer: 1 to 4 us for up to
  * 8 sequences of one row and few heads, up to half as long again for many rows and wide
  * heads.  Finding what is shared takes 5 to 30 us, once for all layers, and about 1 us
  * for each sequence of a line where every one branches from the one before it.
